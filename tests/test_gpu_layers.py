@@ -1,0 +1,672 @@
+"""GPU parity of the layer operators against their 64-bit restatement
+(oracle/layers_oracle.py).
+
+Tolerances.  u(t) = finfo(t).eps / 2 bounds one rounding to type t, relative.
+
+  dropout        32-bit scale (1/(1-p) rounded: u32) and one product (u32),
+                 then the rounding to the output's type: u(t) + 3 u32 relative.
+                 The mask is exact.
+  quantize_rows  exact: both sides are IEEE 32-bit division and rounding.
+  int8_linear    the sum is exact; its conversion, two products and the bias's
+                 sum round in 32 bits: 4 u32 of the terms' magnitudes, then u(t).
+  gated_ffn      a sum of K products in 32 bits, in any order, is off by at most
+                 K u32 sum|x w|; measured sums stay below sqrt(K) u32 times the
+                 2-norm by far, so rows are checked against
+                   E = 4 sqrt(K + 8) u32 * sqrt(sum x^2 w^2)     (a sum's own error)
+                 propagated to h by the derivative's bound, plus u(t) |h|.
+                 Gradients: dg and du are rounded to t before the products, so
+                 their relative 2-norm error is at most u(t) (that rounding)
+                 + u(t) (the output's) + 32-bit terms; checked in the 2-norm at
+                 2 u(t) + 64 u32, and no element off by more than 16 times that
+                 of the larger of itself and the output's root mean square
+                 (an element is a sum of many independently rounded terms).
+"""
+
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import ppo_amd
+from oracle import layers_oracle as ref
+from ppo_amd import _lib
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def u_of(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rn(g, dtype, *shape, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def at_offset(t, dev, offset):
+    """A contiguous device copy of t whose storage starts `offset` elements in."""
+    buf = torch.empty(t.numel() + offset, dtype=t.dtype, device=dev)
+    v = buf[offset:].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+def assert_within(got, want, bound, what=""):
+    """|got - want| <= bound elementwise (fp64 tensors or numbers)."""
+    err = (got.double().cpu() - want).abs()
+    over = err - bound
+    assert bool((over <= 0).all()), f"{what}: {float(over.max()):.3g} over the bound, " \
+                                    f"error {float(err.max()):.3g}"
+
+
+# --- dropout ---------------------------------------------------------------------------------
+
+DROP_SHAPES = [(1, 1), (3, 5), (1, 4099), (128, 128), (37, 72), (300, 17), (2, 70000), (70000, 3),
+               (257, 1024)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", DROP_SHAPES)
+def test_dropout_matches_oracle(dev, shape, dtype):
+    M, C = shape
+    g = torch.Generator().manual_seed(M * 31 + C)
+    t = TYPES[dtype]
+    p, seed = (0.1, 0.5, 0.37)[(M + C) % 3], 0x9876543210ABCDEF + M
+    rows = torch.randint(0, 1 << 40, (M,), generator=g) if C % 2 else None
+    x, dy = rn(g, t, M, C), rn(g, t, M, C)
+    xd = at_offset(x, dev, C % 3).requires_grad_()
+    y = ppo_amd.dropout(xd, p, seed, rows=None if rows is None else rows.to(dev))
+    (dx,) = torch.autograd.grad(y, [xd], dy.to(dev))
+    for got, src in ((y.detach(), x), (dx, dy)):
+        want = ref.dropout(src.double(), p, seed, None if rows is None else rows.numpy())
+        assert torch.equal((got.cpu() != 0) | (src == 0), (want != 0) | (src == 0))
+        # (2^-24: half the distance of fp16's subnormals)
+        assert_within(got, want, want.abs() * (u_of(t) + 3 * U32)
+                      + (2.0 ** -25 if t == torch.float16 else 0.0))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_dropout_edges(dev, dtype):
+    t = TYPES[dtype]
+    x = torch.randn(33, 40, device=dev).to(t)
+    assert torch.equal(ppo_amd.dropout(x, 0.0, 1), x)
+    assert torch.equal(ppo_amd.dropout(x, 1e-12, 1), x)
+    assert torch.equal(ppo_amd.dropout(x, 1.0, 1), torch.zeros_like(x))
+    for empty in (x[:0], torch.empty(4, 0, dtype=t, device=dev), torch.empty(0, dtype=t, device=dev)):
+        assert ppo_amd.dropout(empty, 0.5, 1).shape == empty.shape
+    # infinities and NaN that are dropped are gone, and the kept ones stay
+    bad = torch.full((64, 64), float("nan"), dtype=t, device=dev)
+    bad[::2] = float("inf")
+    y = ppo_amd.dropout(bad, 0.5, 77)
+    keep = torch.from_numpy(ref.keep_mask(0.5, 77, np.arange(64), 64)).to(dev)
+    assert bool((y[~keep] == 0).all()) and not bool(torch.isfinite(y[keep]).any())
+
+
+def test_dropout_shapes_share_the_mask(dev):
+    """The last dimension is the columns, the others together the rows."""
+    x = torch.randn(6, 5, 24, device=dev)
+    y = ppo_amd.dropout(x, 0.4, 5)
+    assert torch.equal(y.view(30, 24), ppo_amd.dropout(x.view(30, 24), 0.4, 5))
+    one = ppo_amd.dropout(x[0, 0], 0.4, 5)
+    assert torch.equal(one, y[0, 0])
+    rows = torch.tensor([7, 7, 2, 7, 29], device=dev)  # the same row again
+    z = ppo_amd.dropout(x.view(30, 24)[rows], 0.4, 5, rows=rows)
+    assert torch.equal(z, y.view(30, 24)[rows])
+
+
+def test_dropout_seeds(dev):
+    x = torch.ones(50, 50, device=dev)
+    for seed in (0, 3, -1, 1 << 62, (1 << 63) - 1):
+        by_tensor = ppo_amd.dropout(x, 0.5, torch.tensor([seed], dtype=torch.int64, device=dev))
+        assert torch.equal(by_tensor, ppo_amd.dropout(x, 0.5, seed))
+    assert not torch.equal(ppo_amd.dropout(x, 0.5, 1), ppo_amd.dropout(x, 0.5, 2))
+    assert torch.equal(ppo_amd.dropout(x, 0.5, -1), ppo_amd.dropout(x, 0.5, 2**64 - 1))
+
+
+def test_dropout_refusals(dev):
+    x = torch.ones(4, 6, device=dev)
+    for p in (-0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError):
+            ppo_amd.dropout(x, p, 1)
+    with pytest.raises(TypeError):
+        ppo_amd.dropout(x, 0.5, 1.5)
+    with pytest.raises(TypeError):
+        ppo_amd.dropout(x, 0.5, torch.tensor([1.0], device=dev))
+    with pytest.raises(RuntimeError):
+        ppo_amd.dropout(x, 0.5, torch.tensor([1]))
+    with pytest.raises(ValueError):
+        ppo_amd.dropout(x, 0.5, torch.tensor([1, 2], device=dev))
+    with pytest.raises(ValueError):
+        ppo_amd.dropout(x, 0.5, 1, rows=torch.arange(5, device=dev))
+    with pytest.raises(TypeError):
+        ppo_amd.dropout(x, 0.5, 1, rows=torch.arange(4, device=dev, dtype=torch.int32))
+    with pytest.raises(ValueError, match="contiguous"):
+        ppo_amd.dropout(x.t(), 0.5, 1)
+    with pytest.raises(TypeError):
+        ppo_amd.dropout(x.double(), 0.5, 1)
+    with pytest.raises(ValueError):
+        ppo_amd.dropout(torch.ones((), device=dev), 0.5, 1)
+
+
+def test_dropout_second_derivative_is_refused(dev):
+    x = torch.ones(4, 6, device=dev, requires_grad=True)
+    y = ppo_amd.dropout(x, 0.5, 1)
+    (dx,) = torch.autograd.grad((y * y).sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+# --- 8 bits ------------------------------------------------------------------------------------
+
+QUANT_SHAPES = [(1, 1), (3, 5), (7, 64), (130, 127), (5, 1000), (9, 4096), (3, 10007), (2, 70001),
+                (4100, 16)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", QUANT_SHAPES)
+def test_quantize_rows_is_exact(dev, shape, dtype):
+    M, K = shape
+    g = torch.Generator().manual_seed(M + 7 * K)
+    x = rn(g, TYPES[dtype], M, K)
+    if M > 2:
+        x[1] = 0
+        x[2] *= 1e-3
+        x[2, K // 2] = 3.0
+    q, s = ppo_amd.quantize_rows(at_offset(x, dev, K % 3))
+    wq, ws = ref.quantize_rows(x.float().numpy())
+    assert q.dtype == torch.int8 and s.dtype == torch.float32 and s.shape == (M,)
+    assert np.array_equal(s.cpu().numpy(), ws)
+    assert np.array_equal(q.cpu().numpy(), wq)
+
+
+def test_quantize_rows_edges(dev):
+    x = torch.zeros(8, 70)
+    x[0, 3] = float("inf")
+    x[1, 69] = float("nan")
+    x[2, 5] = -float("inf")
+    x[3] = torch.arange(70) * 1e-44        # subnormal: the scale is coarse
+    x[4] = 3e38
+    x[5, 69] = -0.0
+    x[6] = torch.arange(70) - 35.0
+    x[7, 0] = 1e-45                        # a scale that rounds to 0
+    q, s = ppo_amd.quantize_rows(x.to(dev))
+    wq, ws = ref.quantize_rows(x.numpy())
+    assert np.array_equal(s.cpu().numpy(), ws, equal_nan=True)
+    assert np.array_equal(q.cpu().numpy(), wq)
+    assert not q[:3].any() and torch.isnan(s[:3]).all() and s[7] == 0
+    q, s = ppo_amd.quantize_rows(torch.empty(0, 5, device=dev))
+    assert q.shape == (0, 5) and s.shape == (0,)
+    q, s = ppo_amd.quantize_rows(x.to(dev).view(2, 4, 70))
+    assert q.shape == (2, 4, 70) and s.shape == (2, 4)
+    with pytest.raises(ValueError):
+        ppo_amd.quantize_rows(torch.empty(5, 0, device=dev))
+
+
+INT8_SHAPES = [(1, 1, 1), (1, 4, 16), (2, 3, 33), (16, 65, 128), (17, 48, 1000), (33, 17, 130),
+               (64, 130, 515), (65, 64, 64), (100, 127, 96), (129, 200, 2049), (300, 513, 64),
+               (70, 64, 8192), (1, 4096, 512), (2048, 2048, 160), (3300, 4200, 48), (257, 31, 77)]
+
+
+def _int8_case(dtype, M, N, K, bias):
+    g = torch.Generator().manual_seed(M * 3 + N * 5 + K)
+    x = rn(g, TYPES[dtype], M, K)
+    w = rn(g, torch.float32, N, K, scale=K ** -0.5)
+    b = rn(g, TYPES[dtype], N) if bias else None
+    xq, xs = ref.quantize_rows(x.float().numpy())
+    wq, ws = ref.quantize_rows(w.numpy())
+    return x, xq, xs, wq, ws, b
+
+
+def _int8_bound(want, b, t):
+    mag = want.abs() if b is None else (want - b.double()).abs() + b.double().abs() + want.abs()
+    tiny = 2.0 ** -25 if t == torch.float16 else 0.0
+    return 4 * U32 * mag + u_of(t) * want.abs() * (1 + 4 * U32) + tiny
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", INT8_SHAPES)
+def test_int8_linear_matches_oracle(dev, shape, dtype):
+    M, N, K = shape
+    t, bias = TYPES[dtype], (M + N) % 2 == 1
+    x, xq, xs, wq, ws, b = _int8_case(dtype, M, N, K, bias)
+    want = torch.from_numpy(ref.int8_linear(xq, xs, wq, ws,
+                                            None if b is None else b.double().numpy()))
+    bound = _int8_bound(want, b, t)
+    bd = None if b is None else b.to(dev)
+    wqd, wsd = torch.from_numpy(wq).to(dev), torch.from_numpy(ws).to(dev)
+    got = ppo_amd.int8_linear(x.to(dev), wqd, wsd, bd)
+    assert got.dtype == t and got.shape == (M, N)
+    assert_within(got, want, bound, "float x")
+    # the same from an 8-bit x, from rows that start at odd addresses
+    xqd, xsd = at_offset(torch.from_numpy(xq), dev, 3), torch.from_numpy(xs).to(dev)
+    again = ppo_amd.int8_linear(xqd, at_offset(torch.from_numpy(wq), dev, 1), wsd, bd,
+                                x_scale=xsd, out_dtype=t)
+    assert torch.equal(again, got)
+
+
+def test_int8_linear_extremes(dev):
+    """The largest sums stay exact; rows that are not finite give NaN and touch
+    no other row."""
+    K = 1 << 17
+    x = torch.full((3, K), 127, dtype=torch.int8, device=dev)
+    x[1] = -127
+    w = torch.full((5, K), 127, dtype=torch.int8, device=dev)
+    one = torch.ones(5, device=dev)
+    y = ppo_amd.int8_linear(x, w, one, x_scale=one[:3], out_dtype=torch.float32)
+    assert y[0].tolist() == [float(np.float32(127 * 127 * K))] * 5
+    assert torch.equal(y[1], -y[0])
+    with pytest.raises(_lib.PPOLibraryError):
+        ppo_amd.int8_linear(torch.ones(1, K + 1, device=dev), torch.ones(2, K + 1, dtype=torch.int8,
+                                                                         device=dev), one[:2])
+    for M in (5, 100):
+        x = torch.randn(M, 40, device=dev)
+        wq, ws = ppo_amd.quantize_rows(torch.randn(6, 40, device=dev))
+        clean = ppo_amd.int8_linear(x, wq, ws)
+        x[2, 7], x[3, 0] = float("nan"), float("inf")
+        y = ppo_amd.int8_linear(x, wq, ws)
+        assert torch.isnan(y[2:4]).all()
+        ok = [m for m in range(M) if m not in (2, 3)]
+        assert torch.equal(y[ok], clean[ok])
+    assert ppo_amd.int8_linear(torch.empty(0, 40, device=dev), wq, ws).shape == (0, 6)
+    assert ppo_amd.int8_linear(torch.randn(2, 3, 40, device=dev), wq, ws).shape == (2, 3, 6)
+
+
+def test_int8_linear_refusals(dev):
+    x = torch.randn(4, 8, device=dev)
+    wq, ws = ppo_amd.quantize_rows(torch.randn(6, 8, device=dev))
+    q, s = ppo_amd.quantize_rows(x)
+    f = ppo_amd.int8_linear
+    for bad in (lambda: f(x, wq[:, :4].contiguous(), ws), lambda: f(x, wq, ws[:5]),
+                lambda: f(x, wq, ws, bias=torch.zeros(5, device=dev)), lambda: f(q, wq, ws),
+                lambda: f(x, wq, ws, x_scale=s), lambda: f(q, wq, ws, x_scale=s),
+                lambda: f(q, wq, ws, x_scale=s[:3], out_dtype=torch.float32),
+                lambda: f(x.t(), wq, ws)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f(x, wq.float(), ws), lambda: f(x.double(), wq, ws),
+                lambda: f(x, wq, ws, out_dtype=torch.bfloat16),
+                lambda: f(x, wq, ws, bias=torch.zeros(6, dtype=torch.float16, device=dev)),
+                lambda: f(q, wq, ws, x_scale=s, out_dtype=torch.int8)):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        f(x.requires_grad_(), wq, ws)
+
+
+# --- gated feed-forward block --------------------------------------------------------------
+
+def gated_case(dtype, M, D, F, bias, seed=0):
+    g = torch.Generator().manual_seed(seed + M * 3 + D * 5 + F * 7)
+    t = TYPES[dtype]
+    x = rn(g, t, M, D)
+    wg, wu = (rn(g, t, F, D, scale=D ** -0.5) for _ in range(2))
+    bg, bu = (rn(g, t, F, scale=0.1) for _ in range(2)) if bias else (None, None)
+    return x, wg, wu, bg, bu, rn(g, t, M, F, scale=0.1)
+
+
+def d64(*ts):
+    return [None if t is None else t.double() for t in ts]
+
+
+def check_grad(got, want, t, what):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all(), what
+    tol = 2 * u_of(t) + 64 * U32
+    diff, norm = (got - want).norm(), want.norm()
+    tiny = 2.0 ** -25 * math.sqrt(want.numel()) if t == torch.float16 else 0.0
+    assert diff <= tol * norm + tiny, f"{what}: {float(diff / norm):.3g} of {tol:.3g}"
+    rms = norm / math.sqrt(want.numel())
+    worst = ((got - want).abs() / want.abs().clamp(min=float(rms) + 1e-30)).max()
+    assert worst <= 16 * tol + 1e-4 * (t == torch.float16), f"{what}: {float(worst):.3g} max"
+
+
+def check_forward(got, x, wg, wu, bg, bu, act, t, keep=None, p=0.0):
+    x, wg, wu, bg, bu = d64(x, wg, wu, bg, bu)
+    want, g, u = ref.gated_ffn(x, wg, wu, bg, bu, act, keep, p)
+    K, up = x.shape[1], (1 / (1 - p) if p < 1 else 1.0)
+    eg = 4 * math.sqrt(K + 8) * U32 * ((x * x) @ (wg * wg).T).sqrt() + 2 * U32 * g.abs()
+    eu = 4 * math.sqrt(K + 8) * U32 * ((x * x) @ (wu * wu).T).sqrt() + 2 * U32 * u.abs()
+    a, da = ref.activation(g, act)
+    # the activation's own arithmetic: a few roundings of |g|; |act'| <= 1.13
+    ea = 1.13 * eg + 8 * U32 * g.abs() + 8 * U32
+    bound = (ea * (u.abs() + eu) + a.abs() * eu) * up + 4 * U32 * want.abs()
+    tiny = 2.0 ** -25 if t == torch.float16 else 0.0
+    bound = bound + u_of(t) * (want.abs() + bound) + tiny
+    if keep is not None:
+        assert bool((got.cpu()[~keep] == 0).all())
+        bound = torch.where(keep, bound, torch.zeros_like(bound))
+    assert_within(got, want, bound, "h")
+    return g, u
+
+
+ACTS = ["silu", "gelu", "tanh", "relu"]
+GATED_SHAPES = [(1, 1, 1), (1, 8, 4), (3, 5, 7), (2, 64, 33), (16, 31, 17), (17, 128, 96),
+                (33, 72, 50), (64, 200, 65), (65, 64, 64), (128, 128, 256), (100, 333, 127),
+                (257, 129, 31), (300, 96, 520), (70, 2100, 24), (1000, 40, 1030),
+                (2200, 136, 1600)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", GATED_SHAPES)
+def test_gated_matches_oracle(dev, shape, dtype):
+    M, D, F = shape
+    t, act = TYPES[dtype], ACTS[(M + D + F) % 4]
+    bias, p = (M + F) % 2 == 0, (0.0, 0.3)[D % 2]
+    print(f"gated {dtype} {shape} {act} bias={bias} p={p}", flush=True)
+    x, wg, wu, bg, bu, dh = gated_case(dtype, M, D, F, bias)
+    seed = 11 + M
+    rows = torch.randint(0, 1 << 34, (M,), generator=torch.Generator().manual_seed(M))
+    keep = None
+    if p:
+        keep = torch.from_numpy(ref.keep_mask(p, seed, rows.numpy(), F))
+    offset = (M + D) % 3 % 2
+    leaves = [None if v is None else at_offset(v, dev, offset).requires_grad_()
+              for v in (x, wg, wu, bg, bu)]
+    kw = dict(activation=act, dropout_p=p, seed=seed, rows=rows.to(dev))
+    with torch.no_grad():
+        acting = ppo_amd.gated_ffn(*leaves, **kw)
+    h = ppo_amd.gated_ffn(*leaves, **kw)
+    assert h.dtype == t and h.shape == (M, F)
+    assert torch.equal(acting, h.detach())  # saving g and u changes no bit
+    g, u = check_forward(h.detach(), x, wg, wu, bg, bu, act, t, keep, p)
+    if act == "relu":
+        # the kink: rows where the sums' last bits decide the side are not compared
+        dh[(g.abs() < 1e-5)] = 0
+    grads = torch.autograd.grad(h, [v for v in leaves if v is not None], dh.to(dev))
+    want = ref.gated_ffn_grads(*d64(x, wg, wu), g, u, act, dh.double(), keep, p)
+    for name, got, w in zip(("dx", "dwg", "dwu", "dbg", "dbu"), grads, want):
+        check_grad(got, w, t, name)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,D,F", [(8, 16, 12), (90, 48, 40)])
+def test_gated_gradients_against_differences(dev, act, M, D, F):
+    """Directional derivatives of the 64-bit forward by central differences:
+    step 1e-5, so off by about 1e-10 (the third derivative) + 1e-11 (cancellation)
+    of unit-scale values, far below the 32-bit gradients' own 2 u32 K-ish error,
+    taken as 1e-5 of the sum of the absolute terms."""
+    x, wg, wu, bg, bu, dh = gated_case("fp32", M, D, F, True, seed=4)
+    base = d64(x, wg, wu, bg, bu)
+    if act == "relu":
+        _, g, _ = ref.gated_ffn(*base, act)
+        dh[g.abs() < 1e-2] = 0  # the step must not cross the kink
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+    grads = torch.autograd.grad(ppo_amd.gated_ffn(*leaves, activation=act), leaves, dh.to(dev))
+    gen = torch.Generator().manual_seed(9)
+    for k in range(5):
+        v = torch.randn(base[k].shape, generator=gen, dtype=torch.float64)
+        eps = 1e-5
+        side = []
+        for s in (eps, -eps):
+            moved = list(base)
+            moved[k] = base[k] + s * v
+            side.append((ref.gated_ffn(*moved, act)[0] * dh.double()).sum())
+        slope = (side[0] - side[1]) / (2 * eps)
+        got = (grads[k].double().cpu() * v)
+        assert abs(got.sum() - slope) <= 1e-5 * got.abs().sum() + 1e-8
+
+
+def test_gated_large_grid(dev):
+    """Tiles of every size, ragged in both directions, bf16, against 64-bit
+    products on the GPU."""
+    for M, D, F in ((4100, 264, 3000), (1500, 520, 1100), (515, 1032, 392)):
+        x, wg, wu, bg, bu, dh = gated_case("bf16", M, D, F, False)
+        leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu)]
+        h = ppo_amd.gated_ffn(*leaves, activation="gelu")
+        grads = torch.autograd.grad(h, leaves, dh.to(dev))
+        x6, g6, u6, d6 = (v.to(dev).double() for v in (x, wg, wu, dh))
+        want, g, u = ref.gated_ffn(x6, g6, u6, None, None, "gelu")
+        check_grad(h.detach(), want.cpu(), torch.bfloat16, "h")
+        for got, w in zip(grads, ref.gated_ffn_grads(x6, g6, u6, g, u, "gelu", d6)):
+            check_grad(got, w.cpu(), torch.bfloat16, f"{M} {D} {F}")
+
+
+def test_gated_dropout_is_dropouts(dev):
+    x, wg, wu, bg, bu, _ = gated_case("fp32", 70, 24, 37, True)
+    args = [v.to(dev) for v in (x, wg, wu, bg, bu)]
+    rows = torch.randperm(70, device=dev) * 12345
+    fused = ppo_amd.gated_ffn(*args, dropout_p=0.25, seed=99, rows=rows)
+    apart = ppo_amd.dropout(ppo_amd.gated_ffn(*args), 0.25, 99, rows=rows)
+    assert torch.equal(fused, apart)
+    assert not bool(ppo_amd.gated_ffn(*args, dropout_p=1.0).any())
+
+
+def test_gated_subsets_and_empties(dev):
+    x, wg, wu, bg, bu, dh = gated_case("bf16", 40, 24, 56, True)
+    args = [v.to(dev) for v in (x, wg, wu, bg, bu)]
+    full = [v.clone().requires_grad_() for v in args]
+    want = torch.autograd.grad(ppo_amd.gated_ffn(*full), full, dh.to(dev))
+    for pick in itertools.chain(([k] for k in range(5)), ([0, 1], [1, 4], [2, 3])):
+        some = [v.clone().requires_grad_(k in pick) for k, v in enumerate(args)]
+        h = ppo_amd.gated_ffn(*some)
+        got = torch.autograd.grad(h, [some[k] for k in pick], dh.to(dev))
+        for k, t in zip(pick, got):
+            assert torch.equal(t, want[k])
+    # no rows: an empty result, and gradients that are zeros
+    none = [args[0][:0].requires_grad_()] + [v.clone().requires_grad_() for v in args[1:]]
+    h = ppo_amd.gated_ffn(*none, dropout_p=0.5)
+    assert h.shape == (0, 56)
+    grads = torch.autograd.grad(h.sum(), none)
+    assert grads[0].shape == (0, 24) and all(not t.any() for t in grads[1:])
+    # leading dimensions, and an incoming gradient that is not contiguous
+    x3 = args[0].view(4, 10, 24).clone().requires_grad_()
+    h = ppo_amd.gated_ffn(x3, *args[1:])
+    assert h.shape == (4, 10, 56)
+    strided = dh.to(dev).view(4, 10, 56).permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    (dx,) = torch.autograd.grad(h, [x3], strided)
+    assert torch.equal(dx.view(40, 24), want[0])
+
+
+def test_gated_same_bits_again(dev):
+    """Split sums are joined in a fixed order."""
+    for M, D, F in ((96, 2048, 64), (300, 200, 72)):
+        x, wg, wu, bg, bu, dh = gated_case("bf16", M, D, F, True)
+        leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+        runs = []
+        for _ in range(3):
+            h = ppo_amd.gated_ffn(*leaves, dropout_p=0.1, seed=3)
+            runs.append([h.detach(), *torch.autograd.grad(h, leaves, dh.to(dev))])
+        for again in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(runs[0], again))
+
+
+@pytest.mark.parametrize("M", [3, 100])
+def test_gated_values_that_are_not_finite(dev, M):
+    """A NaN or an infinity stays in its row."""
+    x, wg, wu, _, _, _ = gated_case("bf16", M, 40, 24, False)
+    args = [v.to(dev) for v in (x, wg, wu)]
+    clean = ppo_amd.gated_ffn(*args)
+    args[0][1, 39] = float("nan")
+    args[0][2, 0] = float("inf")
+    h = ppo_amd.gated_ffn(*args)
+    assert torch.isnan(h[1]).all() and not torch.isfinite(h[2]).any()
+    ok = [m for m in range(M) if m not in (1, 2)]
+    assert torch.equal(h[ok], clean[ok])
+
+
+def test_gated_refusals(dev):
+    x, w, b = torch.randn(4, 8, device=dev), torch.randn(6, 8, device=dev), torch.randn(6, device=dev)
+    f = ppo_amd.gated_ffn
+    for bad in (lambda: f(x, w[:, :4].contiguous(), w), lambda: f(x, w, w[:5]),
+                lambda: f(x, w, w, b), lambda: f(x, w, w, b, b[:5]), lambda: f(x.t(), w, w),
+                lambda: f(x, w, w, activation="swish"), lambda: f(x, w, w, dropout_p=2.0),
+                lambda: f(x, w, w, dropout_p=0.1, rows=torch.arange(3, device=dev)),
+                lambda: f(x[:, :0], w[:, :0].contiguous(), w[:, :0].contiguous()),
+                lambda: f(torch.ones((), device=dev), w, w)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f(x.double(), w, w), lambda: f(x, w.half(), w),
+                lambda: f(x, w, w, b.half(), b), lambda: f(x, w, w, seed=0.5)):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(RuntimeError):
+        f(x, w.cpu(), w)
+    y = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad((f(y, w, w) ** 2).sum(), [y], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    # a row-id tensor changed before the backward pass is noticed
+    rows = torch.arange(4, device=dev)
+    h = f(y, w, w, dropout_p=0.5, rows=rows)
+    rows += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+
+
+# --- streams, graphs ---------------------------------------------------------------------------
+
+def test_layers_on_a_side_stream(dev):
+    x, wg, wu, bg, bu, dh = gated_case("bf16", 300, 136, 264, True)
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+    wq, ws = ppo_amd.quantize_rows(leaves[1].detach())
+
+    def step():
+        h = ppo_amd.gated_ffn(*leaves, dropout_p=0.2, seed=8)
+        z = ppo_amd.dropout(h, 0.2, 9)
+        return [z.detach(), *torch.autograd.grad(z, leaves, dh.to(dev)),
+                ppo_amd.int8_linear(leaves[0].detach(), wq, ws)]
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for s in streams:  # two at once
+        s.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(s):
+            got.append(step())
+    torch.cuda.synchronize()
+    for run in got:
+        assert all(torch.equal(a, b) for a, b in zip(want, run))
+
+
+def test_layers_captured(dev):
+    """Forward and backward in two graphs captured on one stream, replayed side
+    by side on two: each has its own scratch.  The seed and the row ids are read
+    at replay, so every replay is checked against an eager call on the values
+    that it saw."""
+    x, wg, wu, bg, bu, dh = gated_case("bf16", 200, 2056, 72, True)
+    xs = [x.to(dev), (x * 0.5).to(dev)]
+    dh = dh.to(dev)
+    seed = torch.tensor([1], dtype=torch.int64, device=dev)
+    rows = torch.arange(200, device=dev)
+
+    def step(xin, leaves):
+        h = ppo_amd.gated_ffn(xin, *leaves, dropout_p=0.3, seed=seed, rows=rows)
+        q = ppo_amd.int8_linear(h.detach(), *pair)
+        return [h.detach(), q, *torch.autograd.grad(h, leaves, dh)]
+
+    pair = ppo_amd.quantize_rows(torch.randn(40, 72, device=dev))
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    leaves = [v.to(dev).requires_grad_() for v in (wg, wu, bg, bu)]
+    with torch.cuda.stream(side):
+        step(xs[0], leaves)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for xin in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(step(xin, leaves))
+        graphs.append(g)
+    lanes = [torch.cuda.Stream(dev) for _ in range(2)]
+    for k in range(4):
+        seed.fill_(100 + k)
+        rows.add_(17)
+        torch.cuda.synchronize()
+        for g, lane in zip(graphs, lanes):
+            with torch.cuda.stream(lane):
+                g.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in outs]
+        for xin, run in zip(xs, got):
+            assert all(torch.equal(a, b) for a, b in zip(step(xin, leaves), run)), k
+
+
+# --- together -------------------------------------------------------------------------------
+
+def test_rows_give_an_update_its_acting_masks(dev):
+    """A policy with dropout acts on a rollout row by row; its update meets the
+    samples in another order.  With rollout indices as row ids the masks are the
+    acting ones: the log-probs agree to rounding and the loss's ratio is 1."""
+    torch.manual_seed(1)
+    T, N, A = 12, 20, 5
+    policy = ppo_amd.GatedMLP(6, 64, A, dropout=0.3, seed=3).to(dev)
+    value = ppo_amd.GatedMLP(6, 64, 1).to(dev)
+    obs = torch.randn(T, N, 6, device=dev)
+    ids = torch.arange(T * N, device=dev).view(T, N)
+    logp = torch.empty(T, N, device=dev)
+    acts = torch.empty(T, N, dtype=torch.int32, device=dev)
+    with torch.no_grad():
+        for t in range(T):
+            ppo_amd.sample_categorical(policy(obs[t], rows=ids[t]), actions_out=acts[t],
+                                       log_probs_out=logp[t])
+    perm = torch.randperm(T * N, device=dev)[:100]
+    take = lambda a: a.reshape(T * N, *a.shape[2:])[perm]  # noqa: E731
+    o, i = take(obs).contiguous(), take(ids)
+    zeros = torch.zeros(100, device=dev)
+    loss, stats = ppo_amd.ppo_loss_discrete(policy(o, rows=i), take(acts), take(logp),
+                                            torch.randn(100, device=dev), zeros,
+                                            value(o).squeeze(1))
+    loss.backward()
+    # kl = mean(old - new) of log-probs equal to 32-bit rounding
+    assert abs(float(stats["approx_kl"])) < 1e-5 and float(stats["clipfrac"]) == 0
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all())
+               for p in policy.parameters())
+    ppo_amd.check_waits(dev)
+    # without them the masks are others'
+    other = torch.log_softmax(policy(o), 1).gather(1, take(acts).long()[:, None]).squeeze(1)
+    assert float((other - take(logp)).abs().max()) > 1e-2
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_gated_policy_in_vec_ppo(dev, graphs):
+    """GatedMLP networks through VecPPO: rollout, updates (eager and replayed
+    from graphs), and acting with 8-bit copies."""
+    torch.manual_seed(2)
+    T, N, A = 16, 8, 4
+    policy, value = ppo_amd.GatedMLP(6, 64, A).to(dev), ppo_amd.GatedMLP(6, 64, 1).to(dev)
+    vec = ppo_amd.VecPPO(policy, value, batch_size=32, graphs=graphs, check_waits="sync")
+    buf = ppo_amd.RolloutBuffer(T, N, (6,), device=dev)
+    before = [p.detach().clone() for p in policy.parameters()]
+    for _ in range(3):
+        buf.reset()
+        for _ in range(T):
+            vec.act(torch.randn(N, 6, device=dev), buffer=buf)
+            buf.add_outcome(torch.randn(N, device=dev), (torch.rand(N, device=dev) < 0.1))
+        buf.finish()
+        vec.update(buf)
+    assert all(bool(torch.isfinite(p).all()) for p in policy.parameters())
+    assert all(not torch.equal(a, b) for a, b in zip(before, policy.parameters()))
+    eight = ppo_amd.int8_copy(policy)
+    obs = torch.randn(300, 6, device=dev)
+    with torch.no_grad():
+        want, got = policy(obs), eight(obs)
+    # 8-bit rows: each product is off by at most 1/254 of its row's and channel's maximum
+    # per factor; together well inside a tenth of the logits' spread
+    assert got.shape == want.shape
+    assert float((got - want).abs().max()) < 0.1 * float(want.std()) + 0.05
+    acts, logp = ppo_amd.sample_categorical(got)
+    assert acts.shape == (300,) and bool(torch.isfinite(logp).all())
+
+
+def test_int8_copy_of_the_reference_networks(dev):
+    torch.manual_seed(3)
+    mlp = ppo_amd.MLP(4, 128, 2).to(dev)
+    eight = ppo_amd.int8_copy(mlp)
+    assert isinstance(eight.net[0], ppo_amd.Int8Linear) and isinstance(mlp.net[0], torch.nn.Linear)
+    obs = torch.randn(50, 4, device=dev)
+    # by hand, through the oracle
+    x = obs.cpu()
+    for k in (0, 2, 4):
+        w, b = mlp.net[k].weight.detach().cpu(), mlp.net[k].bias.detach().cpu()
+        xq, xs = ref.quantize_rows(x.numpy())
+        wq, ws = ref.quantize_rows(w.numpy())
+        x = torch.from_numpy(ref.int8_linear(xq, xs, wq, ws, b.double().numpy())).float()
+        if k < 4:
+            x = x.clamp(min=0)
+    # (a last-bit difference may move a hidden value to the next 8-bit step: 1/127 of its row)
+    torch.testing.assert_close(eight(obs).cpu(), x, rtol=0, atol=5e-3)

@@ -1,0 +1,188 @@
+"""The layer operators without a GPU: the C ABI of include/ppo_layers.h, its
+argument checks (which return before any device work), the Python refusals,
+and the oracle they are tested against."""
+
+import ctypes
+import os
+import re
+
+import numpy as np
+import pytest
+import torch
+
+import ppo_amd
+from oracle import layers_oracle as ref
+from ppo_amd import _lib, layers
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "ppo_layers.h")
+P = ctypes.c_void_p(4096)  # non-null, aligned, never dereferenced
+
+
+def declared_functions():
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    return sorted(set(re.findall(r"\b(ppo_layer_[a-z0-9_]+)\s*\(", text)))
+
+
+def test_exports_match_the_header():
+    lib = _lib.load_layers()
+    names = declared_functions()
+    assert names and set(names) == set(_lib.LAYER_SIGNATURES)
+    for name in names:
+        assert hasattr(lib, name)
+    syms = os.popen(f"nm -D --defined-only {_lib.LAYERS_PATH}").read()
+    assert set(re.findall(r"\bT (\S+)$", syms, flags=re.M)) == set(names)
+
+
+def drop(p, seed=1):
+    return ctypes.byref(_lib.Dropout(p, seed, None, None))
+
+
+def test_dropout_arguments():
+    f = _lib.load_layers().ppo_layer_dropout
+    assert f(P, P, 3, 4, 4, drop(0.1), None) == 1          # type
+    assert f(P, P, 0, -1, 4, drop(0.1), None) == 1
+    assert f(P, P, 0, 4, 4, None, None) == 1
+    for p in (-0.1, 1.1, float("nan")):
+        assert f(P, P, 0, 4, 4, drop(p), None) == 1
+    assert f(None, P, 0, 4, 4, drop(0.1), None) == 1
+    assert f(None, None, 0, 0, 4, drop(0.1), None) == 0    # nothing to do
+    assert f(None, None, 0, 4, 0, drop(0.1), None) == 0
+    assert f(P, P, 0, 1, (1 << 33) + 1, drop(0.1), None) == 3
+
+
+def test_quantize_arguments():
+    f = _lib.load_layers().ppo_layer_quantize_rows
+    assert f(P, 5, 4, 4, P, P, None) == 1
+    assert f(P, 0, 4, 0, P, P, None) == 1
+    assert f(P, 0, 4, 4, None, P, None) == 1
+    assert f(None, 0, 0, 4, None, None, None) == 0
+    assert f(P, 0, 1 << 31, 4, P, P, None) == 3
+
+
+def test_int8_linear_arguments():
+    lib = _lib.load_layers()
+    f = lib.ppo_layer_int8_linear
+
+    def call(x=P, xq=None, xs=None, wq=P, ws=P, dtype=0, M=200, N=64, K=64, out=P, work=P,
+             nbytes=1 << 40):
+        return f(x, xq, xs, wq, ws, None, dtype, M, N, K, out, work, nbytes, None)
+
+    assert call(dtype=-1) == 1 and call(M=-1) == 1 and call(N=0) == 1 and call(K=0) == 1
+    assert call(wq=None) == 1 and call(ws=None) == 1 and call(out=None) == 1
+    assert call(x=None) == 1 and call(x=None, xq=P) == 1
+    assert call(M=0, x=None, wq=None, out=None, work=None) == 0
+    assert call(K=(1 << 17) + 1) == 3
+    need = lib.ppo_layer_int8_linear_workspace_bytes(200, 64, 64, 1)
+    assert need >= 200 * 64 + 200 * 4
+    assert call(nbytes=need - 1) == 2 and call(work=None) == 2
+    assert call(work=ctypes.c_void_p(4097)) == 2
+    assert lib.ppo_layer_int8_linear_workspace_bytes(0, 64, 64, 1) == 0
+
+
+def test_gated_arguments():
+    lib = _lib.load_layers()
+
+    def fwd(x=P, wg=P, wu=P, bg=None, bu=None, dtype=0, M=200, D=33, F=64, act=2, d=None, h=P,
+            work=P, nbytes=1 << 40):
+        return lib.ppo_layer_gated_forward(x, wg, wu, bg, bu, dtype, M, D, F, act, d, h, None,
+                                           work, nbytes, None)
+
+    assert fwd(dtype=3) == 1 and fwd(M=-1) == 1 and fwd(D=0) == 1 and fwd(F=0) == 1
+    assert fwd(act=-1) == 1 and fwd(act=4) == 1 and fwd(d=drop(2.0)) == 1
+    assert fwd(bg=P) == 1 and fwd(bu=P) == 1
+    assert fwd(x=None) == 1 and fwd(wg=None) == 1 and fwd(wu=None) == 1 and fwd(h=None) == 1
+    assert fwd(M=0, x=None, wg=None, wu=None, h=None) == 0
+    assert fwd(M=1 << 28) == 3 and fwd(D=1 << 22) == 3
+    need = lib.ppo_layer_gated_workspace_bytes(0, 200, 33, 64)
+    assert need > 0 and fwd(nbytes=need - 1) == 2 and fwd(work=None) == 2
+    assert lib.ppo_layer_gated_workspace_bytes(0, 0, 33, 64) == 0
+
+    def bwd(dh=P, x=P, wg=P, wu=P, saved=P, dtype=0, M=200, D=33, F=64, act=2, d=None, dx=P,
+            dwg=P, dwu=P, dbg=None, dbu=None, work=P, nbytes=1 << 40):
+        return lib.ppo_layer_gated_backward(dh, x, wg, wu, saved, dtype, M, D, F, act, d, dx, dwg,
+                                            dwu, dbg, dbu, work, nbytes, None)
+
+    assert bwd(dtype=3) == 1 and bwd(M=0) == 1 and bwd(D=0) == 1 and bwd(F=-2) == 1
+    assert bwd(act=7) == 1 and bwd(d=drop(-1.0)) == 1
+    assert bwd(dwu=None) == 1 and bwd(dwg=None) == 1 and bwd(dbg=P) == 1 and bwd(dbu=P) == 1
+    assert bwd(dh=None) == 1 and bwd(saved=None) == 1 and bwd(x=None) == 1 and bwd(wu=None) == 1
+    need = lib.ppo_layer_gated_backward_workspace_bytes(0, 200, 33, 64)
+    assert need > 0 and bwd(nbytes=need - 1) == 2 and bwd(work=None) == 2
+    assert bwd(work=ctypes.c_void_p(4097)) == 2
+
+
+def test_cpu_tensors_and_types_are_refused():
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    for call in (lambda: ppo_amd.dropout(x, 0.1, 1), lambda: ppo_amd.gated_ffn(x, w, w),
+                 lambda: ppo_amd.quantize_rows(x),
+                 lambda: ppo_amd.int8_linear(x, w.to(torch.int8), torch.ones(6))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+    with pytest.raises(TypeError):
+        ppo_amd.dropout([1.0], 0.1, 1)
+
+
+def test_module_arguments():
+    with pytest.raises(ValueError):
+        ppo_amd.GatedLinear(4, 4, activation="swish")
+    with pytest.raises(ValueError):
+        ppo_amd.GatedLinear(4, 4, dropout=1.5)
+    m = ppo_amd.GatedMLP(6, 16, 3, dropout=0.1, seed=5)
+    assert [tuple(p.shape) for p in m.parameters()] == [
+        (16, 6), (16,), (16, 6), (16,), (16, 16), (16,), (16, 16), (16,), (3, 16), (3,)]
+    assert [int(l.seed) for l in m.hidden] == [10, 11]
+    m.reseed(7)
+    assert [int(l.seed) for l in m.hidden] == [14, 15]
+    assert layers.ACTIVATIONS.keys() == {"relu", "tanh", "silu", "gelu"}
+
+
+# --- the oracle -------------------------------------------------------------------------
+
+def test_philox_known_answers():
+    """Vectors published with the generator's paper: counter and key all
+    zeros, all ones, for 7 and 10 rounds."""
+    zero, ones = [np.uint64(0)] * 4, [np.uint64(0xFFFFFFFF)] * 4
+    hexes = lambda words: " ".join(f"{int(w):08x}" for w in words)  # noqa: E731
+    assert hexes(ref.philox4x32(zero, (0, 0), 7)) == "5f6fb709 0d893f64 4f121f81 4f730a48"
+    assert hexes(ref.philox4x32(zero, (0, 0), 10)) == "6627e8d5 e169c58d bc57ac4c 9b00dbd8"
+    assert hexes(ref.philox4x32(ones, (0xFFFFFFFF, 0xFFFFFFFF), 10)) == \
+        "408f276d 41c83b0e a20bc7c6 6d5451fd"
+
+
+def test_keep_mask_statistics():
+    n = 1 << 20
+    for p in (0.1, 0.5):
+        keep = ref.keep_mask(p, 1234567890123, np.arange(1024), 1024)
+        assert abs(keep.mean() - (1 - p)) < 5 * np.sqrt(p * (1 - p) / n)
+    assert ref.keep_mask(0.0, 9, [3], 40).all() and not ref.keep_mask(1.0, 9, [3], 40).any()
+    # a row's mask goes by its id alone
+    a, b = ref.keep_mask(0.5, 7, [5, 1 << 33, 2], 37), ref.keep_mask(0.5, 7, [1 << 33], 50)
+    assert (a[1] == b[0, :37]).all() and (a[0] != a[2]).any()
+
+
+@pytest.mark.parametrize("act", ["relu", "tanh", "silu", "gelu"])
+def test_oracle_gradients_are_autograds(act):
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    x, wg, wu, bg, bu, dh = r(7, 5), r(6, 5), r(6, 5), r(6), r(6), r(7, 6)
+    keep = torch.rand(7, 6, generator=g) < 0.7
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, bg, bu)]
+    f = {"relu": torch.relu, "tanh": torch.tanh, "silu": torch.nn.functional.silu,
+         "gelu": torch.nn.functional.gelu}[act]
+    lx, lwg, lwu, lbg, lbu = leaves
+    h = f(lx @ lwg.T + lbg) * (lx @ lwu.T + lbu) * keep / 0.7
+    h.backward(dh)
+    want, gg, uu = ref.gated_ffn(x, wg, wu, bg, bu, act, keep, 0.3)
+    torch.testing.assert_close(want, h.detach(), rtol=1e-12, atol=1e-12)
+    got = ref.gated_ffn_grads(x, wg, wu, gg, uu, act, dh, keep, 0.3)
+    for a, leaf in zip(got, leaves):
+        torch.testing.assert_close(a, leaf.grad, rtol=1e-11, atol=1e-12)
+
+
+def test_oracle_quantize():
+    x = np.array([[127.0, -63.5, 0.5, 1.5], [0, 0, 0, 0], [1, np.inf, 0, 0], [np.nan, 1, 2, 3]],
+                 dtype=np.float32)
+    q, s = ref.quantize_rows(x)
+    assert s[0] == 1 and s[1] == 0 and np.isnan(s[2:]).all()
+    assert q.tolist() == [[127, -64, 0, 2], [0] * 4, [0] * 4, [0] * 4]

@@ -1,0 +1,170 @@
+// Shared pieces of the layer operators (libppo_layers.so): element types,
+// activations, the dropout generator and the host-side launch helpers.
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ppo_amd.h"
+#include "ppo_layers.h"
+
+namespace ppo {
+
+using bf16 = __hip_bfloat16;
+using fp16 = __half;
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+// Sixteen bytes at any address: rows of an odd width start anywhere.
+typedef v4i v4i_any __attribute__((aligned(1)));
+
+inline int hip_status(hipError_t e) { return e == hipSuccess ? PPO_OK : PPO_ERR_HIP_BASE + (int)e; }
+inline int last_launch_status() { return hip_status(hipGetLastError()); }
+
+__host__ __device__ constexpr int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+__host__ __device__ constexpr int64_t div_up(int64_t x, int64_t a) { return (x + a - 1) / a; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+inline int dtype_size(int dtype) { return dtype == PPO_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype >= PPO_DTYPE_F32 && dtype <= PPO_DTYPE_F16; }
+
+// Elements that 16 bytes hold.
+template <class T>
+constexpr int kPer16 = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(fp16 x) { return __half2float(x); }
+// Rounds to nearest even, as torch's casts do.
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16(x); }
+template <>
+__device__ __forceinline__ fp16 from_f32<fp16>(float x) { return __float2half_rn(x); }
+
+// Calls f with a value of the C++ type of `dtype` (checked by the caller).
+template <class F>
+int with_dtype(int dtype, F&& f) {
+  if (dtype == PPO_DTYPE_F32) return f(float{});
+  if (dtype == PPO_DTYPE_BF16) return f(bf16{});
+  return f(fp16{});
+}
+
+// Four consecutive elements, stored together where p allows it (`vec`: the
+// row's start and pitch are multiples of four elements), else those in range.
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4], int count, bool vec) {
+  struct __attribute__((aligned(4 * sizeof(T)))) Four { T x[4]; } q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q.x[i] = from_f32<T>(v[i]);
+  if (vec && count >= 4) {
+    *reinterpret_cast<Four*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < count) p[i] = q.x[i];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Activations: act(g), and its derivative for the backward pass.  32 bits
+// throughout; the gelu is x * Phi(x) with the error function.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+
+__device__ __forceinline__ float activate(int act, float g) {
+  if (act == PPO_LAYER_SILU) return g / (1.0f + expf(-g));
+  if (act == PPO_LAYER_GELU) return g * (0.5f * (1.0f + erff(g * 0.70710678f)));
+  if (act == PPO_LAYER_TANH) return tanhf(g);
+  return g > 0.0f ? g : (g != g ? g : 0.0f);
+}
+
+__device__ __forceinline__ void activate_grad(int act, float g, float& a, float& da) {
+  if (act == PPO_LAYER_SILU) {
+    const float s = sigmoid(g);
+    a = g * s;
+    da = s * (1.0f + g * (1.0f - s));
+  } else if (act == PPO_LAYER_GELU) {
+    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678f));
+    a = g * cdf;
+    da = cdf + g * expf(-0.5f * g * g) * 0.39894228f;
+  } else if (act == PPO_LAYER_TANH) {
+    a = tanhf(g);
+    da = 1.0f - a * a;
+  } else {
+    a = g > 0.0f ? g : (g != g ? g : 0.0f);
+    da = g > 0.0f ? 1.0f : 0.0f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Dropout.  Element (row, column) is kept if word (column mod 4) of
+// Philox4x32 at the counter (column / 4, row id, 0) under the 64-bit seed is
+// below keep = round((1 - p) 2^32), and is then multiplied by 1 / (1 - p).
+// The mask is a function of (seed, row id, column) alone, so the backward
+// pass, or an update that meets the row again in another minibatch, forms it
+// anew instead of reading it.  Seven rounds: the fewest that its authors
+// (Salmon, Moraes, Dror, Shaw, SC 2011) found to pass every test of
+// BigCrush; each round is two 32x32-bit products.
+// ---------------------------------------------------------------------------
+struct Dropout {
+  const int64_t* rows;      // row ids, or null: 0, 1, ...
+  const uint64_t* seed_at;  // seed in device memory, or null: `seed`
+  uint64_t seed;
+  uint32_t keep;            // kept: word < keep (all: every word)
+  int mode;                 // 0 no dropout, 1 a random mask, 2 nothing is kept
+  float scale;              // 1 / (1 - p)
+};
+
+inline Dropout make_dropout(double p, uint64_t seed, const uint64_t* seed_at, const int64_t* rows) {
+  Dropout d = {rows, seed_at, seed, 0, 0, 1.0f};
+  if (!(p > 0.0)) return d;
+  d.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+  // nearbyint rounds ties to even; 2^32 (p below 2^-33) keeps every word
+  const double keep = nearbyint((1.0 - p) * 4294967296.0);
+  if (keep >= 4294967296.0) return d;  // (and then scale rounds to 1)
+  d.keep = (uint32_t)keep;
+  d.mode = d.keep ? 1 : 2;
+  return d;
+}
+
+__device__ __forceinline__ uint4 philox(uint64_t seed, uint32_t c0, uint64_t row) {
+  uint32_t x0 = c0, x1 = (uint32_t)row, x2 = (uint32_t)(row >> 32), x3 = 0;
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const uint64_t p0 = (uint64_t)x0 * 0xD2511F53u, p1 = (uint64_t)x2 * 0xCD9E8D57u;
+    x0 = (uint32_t)(p1 >> 32) ^ x1 ^ k0;
+    x1 = (uint32_t)p1;
+    x2 = (uint32_t)(p0 >> 32) ^ x3 ^ k1;
+    x3 = (uint32_t)p0;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(x0, x1, x2, x3);
+}
+
+__device__ __forceinline__ uint64_t dropout_seed(const Dropout& d) {
+  return d.seed_at ? *d.seed_at : d.seed;
+}
+
+// Multipliers of four columns from 4 * group on: dropped elements are
+// selected away, not multiplied by zero, so an infinity or a NaN there goes.
+__device__ __forceinline__ void drop4(const Dropout& d, uint64_t seed, uint64_t row,
+                                      uint32_t group, float (&v)[4]) {
+  if (d.mode == 0) return;
+  uint4 w = make_uint4(0, 0, 0, 0);
+  if (d.mode == 1) w = philox(seed, group, row);
+  v[0] = w.x < d.keep ? v[0] * d.scale : 0.0f;
+  v[1] = w.y < d.keep ? v[1] * d.scale : 0.0f;
+  v[2] = w.z < d.keep ? v[2] * d.scale : 0.0f;
+  v[3] = w.w < d.keep ? v[3] * d.scale : 0.0f;
+}
+
+}  // namespace ppo

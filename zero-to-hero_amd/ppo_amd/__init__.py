@@ -13,6 +13,9 @@ include/ppo_amd.h) behind the reference's own PPO surface:
   optim     ClippedAdam (clip_grad_norm_ + Adam, two launches)
   reference_patch  _advantages / _update_batch for the reference's own
             PPOAgent class (reference_patch.apply(PPOAgent))
+  layers    gated_ffn, dropout, quantize_rows, int8_linear and the modules
+            GatedLinear, GatedMLP, Int8Linear, int8_copy: the feed-forward
+            layers of larger policies (libppo_layers.so)
   torch_ops the hot path as registered operators, torch.ops.ppo_amd.*
             (gae, gae_normalize, normalize_advantages, ppo_loss_discrete,
             ppo_loss_gaussian), visible to torch.compile and the dispatcher
@@ -28,6 +31,16 @@ from .agent import (
     TrainingConfig,
     Transition,
     cartpole_sizes,
+)
+from .layers import (
+    GatedLinear,
+    GatedMLP,
+    Int8Linear,
+    dropout,
+    gated_ffn,
+    int8_copy,
+    int8_linear,
+    quantize_rows,
 )
 from .ops import (
     LossStats,
@@ -65,6 +78,9 @@ def load_library():
 __all__ = [
     "CartPoleVec",
     "ClippedAdam",
+    "GatedLinear",
+    "GatedMLP",
+    "Int8Linear",
     "LIB_PATH",
     "LossStats",
     "MLP",
@@ -79,9 +95,13 @@ __all__ = [
     "cartpole_sizes",
     "check_waits",
     "discounted_returns",
+    "dropout",
     "gae",
     "gae_normalize",
+    "gated_ffn",
     "gather_rows",
+    "int8_copy",
+    "int8_linear",
     "load_library",
     "mlp_act_categorical",
     "mlp_forward_categorical",
@@ -94,6 +114,7 @@ __all__ = [
     "ppo_loss_gaussian_fused",
     "ppo_mlp_cat_grads",
     "ppo_mlp_cat_step",
+    "quantize_rows",
     "sample_categorical",
     "sample_gaussian",
 ]

@@ -156,6 +156,69 @@ SIGNATURES = {
     ),
 }
 
+# ---------------------------------------------------------------------------
+# libppo_layers.so (include/ppo_layers.h)
+# ---------------------------------------------------------------------------
+LAYERS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libppo_layers.so")
+
+
+class Dropout(ctypes.Structure):
+    """struct ppo_dropout (include/ppo_layers.h)."""
+
+    _fields_ = [
+        ("p", ctypes.c_double),
+        ("seed", ctypes.c_uint64),
+        ("seed_at", ctypes.c_void_p),
+        ("row_ids", ctypes.c_void_p),
+    ]
+
+
+_drop = ctypes.POINTER(Dropout)
+
+# name -> (restype, argtypes); one entry per function in include/ppo_layers.h
+LAYER_SIGNATURES = {
+    "ppo_layer_dropout": (_int, [_vp, _vp, _int, _i64, _i64, _drop, _vp]),
+    "ppo_layer_quantize_rows": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
+    "ppo_layer_int8_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "ppo_layer_int8_linear": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _sz, _vp],
+    ),
+    "ppo_layer_gated_workspace_bytes": (_sz, [_int, _i64, _i64, _i64]),
+    "ppo_layer_gated_forward": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int, _drop, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "ppo_layer_gated_backward_workspace_bytes": (_sz, [_int, _i64, _i64, _i64]),
+    "ppo_layer_gated_backward": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _int, _drop, _vp, _vp, _vp, _vp, _vp,
+         _vp, _sz, _vp],
+    ),
+}
+
+_layers = None
+
+
+def load_layers() -> ctypes.CDLL:
+    """Load libppo_layers.so once and attach the prototypes; raise if absent."""
+    global _layers
+    if _layers is None:
+        load()
+        if not os.path.exists(LAYERS_PATH):
+            raise RuntimeError(
+                f"{LAYERS_PATH} is not built. Build it with `python -m ppo_amd.build` "
+                "(or __graft_entry__.build()); ppo_amd has no CPU fallback."
+            )
+        lib = ctypes.CDLL(LAYERS_PATH)
+        for name, (res, args) in LAYER_SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+        _layers = lib
+    return _layers
+
+
 _lib = None
 
 
