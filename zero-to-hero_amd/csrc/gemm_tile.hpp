@@ -12,11 +12,11 @@
 // with four consecutive columns n of one row m: a vector store, and one call
 // of the dropout generator.
 //
-// A workgroup computes a BM x BN tile over K steps of 128 bytes.  Both tiles
+// A workgroup computes a BM x BN tile over stages of 64 bytes of K.  The tiles
 // go from memory to LDS without passing through registers (buffer loads with
-// the LDS bit: 64 lanes, 16 bytes each, to consecutive LDS addresses), two
-// buffers in turn.  A row's chunk c sits in slot c ^ (row % 8), which spreads
-// the sixteen rows that a fragment read touches over all banks; since the LDS
+// the LDS bit: 64 lanes, 16 bytes each, to consecutive LDS addresses) into a
+// ring of four stages.  A row's chunk c sits in slot c ^ (row / 4 % 4), which
+// spreads the rows that a fragment read touches over all banks; since the LDS
 // side of the load is fixed, the lanes permute the addresses they load from
 // instead.  The buffer descriptor ends with the operand's last row and lanes
 // past the end of a row ask for an offset behind it: the hardware gives zero
@@ -37,37 +37,70 @@ struct GemmArgs {
   int64_t kbytes;   // of a row, a multiple of 16
   int M, N;         // N: output columns
   int tiles_m, tiles_n;
-  int steps_per_split;     // K steps of 128 bytes that one split takes
+  int stages_per_split;    // stages of kStageBytes that one split takes
   char* partial;    // [splits][1 or 2][M][N4] 32-bit sums, or null: no split
 };
 
-constexpr int kStepBytes = 128;
+constexpr int kStageBytes = 64;  // of a row, in one stage of the ring
+constexpr int kRing = 4;
 
+// Sums of one matrix instruction: kEdge x kEdge outputs over 64 lanes, 4 or
+// 16 a lane, in groups of four consecutive columns n of one row m.
+template <class T, int kEdge>
+struct AccOf;
 template <class T>
-struct AccOf { using type = v4f; };
+struct AccOf<T, 16> { typedef float type __attribute__((ext_vector_type(4))); };
+template <class T>
+struct AccOf<T, 32> { typedef float type __attribute__((ext_vector_type(16))); };
 template <>
-struct AccOf<int8_t> { using type = v4i; };
-template <class T>
-using Acc = typename AccOf<T>::type;
+struct AccOf<int8_t, 16> { typedef int type __attribute__((ext_vector_type(4))); };
+template <>
+struct AccOf<int8_t, 32> { typedef int type __attribute__((ext_vector_type(16))); };
+template <class T, int kEdge = 16>
+using Acc = typename AccOf<T, kEdge>::type;
 
-template <class T>
-__device__ __forceinline__ Acc<T> mfma16(v4i w, v4i x, Acc<T> c) {
+// c += w x over the k of one chunk per lane: row lane % kEdge of W and of X,
+// chunk lane / kEdge of a run.
+template <class T, int kEdge>
+__device__ __forceinline__ Acc<T, kEdge> mfma(v4i w, v4i x, Acc<T, kEdge> c) {
   if constexpr (sizeof(T) == 4) {
     const v4f a = __builtin_bit_cast(v4f, w), b = __builtin_bit_cast(v4f, x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    for (int i = 0; i < 4; ++i)
+      if constexpr (kEdge == 16)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+      else
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
     return c;
   } else if constexpr (sizeof(T) == 1) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0);
+    if constexpr (kEdge == 16)
+      return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_i32_32x32x32_i8(w, x, c, 0, 0, 0);
   } else if constexpr (__is_same(T, fp16)) {
-    typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w),
-                                                  __builtin_bit_cast(v8h, x), c, 0, 0, 0);
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    const v8 a = __builtin_bit_cast(v8, w), b = __builtin_bit_cast(v8, x);
+    if constexpr (kEdge == 16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   } else {
-    typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, w),
-                                                   __builtin_bit_cast(v8b, x), c, 0, 0, 0);
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    const v8 a = __builtin_bit_cast(v8, w), b = __builtin_bit_cast(v8, x);
+    if constexpr (kEdge == 16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+}
+
+// Four consecutive columns of a lane's sums.
+template <class T, int kEdge>
+__device__ __forceinline__ Acc<T> four(const Acc<T, kEdge>& c, int group) {
+  Acc<T> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = c[4 * group + i];
+  return r;
 }
 
 // Descriptor of `bytes` (below 2^31) from p on; loads behind it give zero.
@@ -91,10 +124,12 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, v4i buffer, uint32_t o
       "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer));
 }
 
-// Waits for this wave's loads (to LDS too) and LDS reads, then for the whole
-// workgroup: what every wave loaded may be read, what it read overwritten.
-__device__ __forceinline__ void lds_loads_wait_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// Waits until at most kLeft of this wave's loads are under way, and for its
+// LDS reads, then for the whole workgroup: what every wave had loaded until
+// then may be read, what it has read overwritten.
+template <int kLeft>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
 constexpr uint32_t kBehind = 0x80000000u;  // an offset that no descriptor reaches
@@ -126,16 +161,29 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 // Epi: kGated (two W matrices, one output), and
 //   void operator()(int m, int n, Acc<T> c [, Acc<T> second]) for columns
 // n..n+3 of row m < M, n < N (columns past N - 1 are the callee's to skip).
+//
+// A stage is two phases, each one 16-byte chunk per lane of every fragment.
+// While the matrix cores work on one phase, the fragments of the next are read
+// from LDS, one read to every few matrix instructions.  The workgroup meets
+// once a stage, when its second phase has been read: the stage's place in the
+// ring is then free for the loads of the stage four later, which are spread
+// over the following stage (issued together they would hold up the matrix
+// instructions behind them), three stages ahead of their use.
 template <class T, int BM, int BN, int kWavesM, int kWavesN, class Epi>
 __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     gemm_tile_kernel(const GemmArgs a, const Epi epi) {
   constexpr int kWaves = kWavesM * kWavesN;
-  constexpr int TM = BM / kWavesM / 16, TN = BN / kWavesN / 16;
-  constexpr int XL = BM / 8 / kWaves, WL = BN / 8 / kWaves;  // loads of a wave per step
+  constexpr int kEdge = 32;  // of a matrix instruction's block
+  constexpr int TM = BM / kWavesM / kEdge, TN = BN / kWavesN / kEdge;
+  constexpr int XL = BM / 16 / kWaves, WL = BN / 16 / kWaves;  // loads of a wave per stage
+  constexpr int kLoads = XL + WL;
+  constexpr int kFrags = TM + TN, kMfmas = TM * TN;
   constexpr bool kGated = Epi::kGated;
   constexpr int kCols = kGated ? BN / 2 : BN;  // output columns of a tile
-  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && (!kGated || TN % 2 == 0), "");
-  __shared__ __align__(1024) char lds[2][(BM + BN) * kStepBytes];
+  constexpr int kStage = (BM + BN) * kStageBytes;
+  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && kLoads % 2 == 0, "");
+  static_assert(!kGated || TN % 2 == 0, "");
+  __shared__ __align__(1024) char lds[kRing][kStage];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -143,105 +191,146 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   int tm, tn;
   tile_of(a, tm, tn);
   const int m0 = tm * BM, n0 = tn * kCols;
-  const int steps = (int)div_up(a.kbytes, kStepBytes);
-  const int first = blockIdx.y * a.steps_per_split;
-  const int last = min(steps, first + a.steps_per_split);
+  const int stages = (int)div_up(a.kbytes, kStageBytes);
+  const int first = blockIdx.y * a.stages_per_split;
+  const int last = min(stages, first + a.stages_per_split);
 
-  // --- addresses of this wave's loads -----------------------------------------------
-  const int row8 = lane >> 3;
-  const uint32_t chunk = ((lane & 7) ^ row8) * 16;
-  const v4i bx = buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * (uint32_t)a.xpitch);
-  const uint32_t w_bytes = (uint32_t)min(kCols, a.N - n0) * (uint32_t)a.wpitch;
+  // --- loads ------------------------------------------------------------------------
+  const int row16 = lane >> 2;
+  const uint32_t chunk = ((lane & 3) ^ (row16 >> 2)) * 16;
+  const uint32_t xp = (uint32_t)a.xpitch, wp = (uint32_t)a.wpitch;
+  const v4i bx = buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
+  const uint32_t w_bytes = (uint32_t)min(kCols, a.N - n0) * wp;
   const v4i bw0 = buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
   const v4i bw1 = kGated ? buffer_of(a.w1 + n0 * a.wpitch, w_bytes) : bw0;
-  uint32_t x_off[XL], w_off[WL];
-  bool second[WL];  // of the gated pair, the same in all lanes
-#pragma unroll
-  for (int i = 0; i < XL; ++i)
-    x_off[i] = (uint32_t)((wave * XL + i) * 8 + row8) * (uint32_t)a.xpitch;
-#pragma unroll
-  for (int i = 0; i < WL; ++i) {
-    const int j = (wave * WL + i) * 8;  // first of the eight LDS rows
-    int col = j;
-    second[i] = false;
-    if (kGated) {  // a wave's columns: half from the first matrix, half from the second
-      constexpr int kSpan = TN * 16, kHalf = kSpan / 2;
-      second[i] = j % kSpan >= kHalf;
-      col = j / kSpan * kHalf + j % kHalf;
-    }
-    w_off[i] = (uint32_t)(col + row8) * (uint32_t)a.wpitch;
-  }
+  const uint32_t x_off = (uint32_t)(wave * XL * 16 + row16) * xp, w_off = (uint32_t)row16 * wp;
   const uint32_t lds0 =
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
-  auto load_step = [&](int step, int buf) {
-    const uint32_t kb = (uint32_t)step * kStepBytes + chunk;
-    const uint32_t k_off = kb < (uint32_t)a.kbytes ? kb : kBehind;
-    const uint32_t to = lds0 + buf * (BM + BN) * kStepBytes;
-#pragma unroll
-    for (int i = 0; i < XL; ++i) load_to_lds(to + (wave * XL + i) * 1024, bx, x_off[i] + k_off);
-#pragma unroll
-    for (int i = 0; i < WL; ++i)
-      load_to_lds(to + BM * kStepBytes + (wave * WL + i) * 1024, second[i] ? bw1 : bw0,
-                  w_off[i] + k_off);
+  // load i of a stage (X's first): sixteen rows
+  auto load = [&](int i, uint32_t to, uint32_t k_off) {
+    if (i < XL) {
+      load_to_lds(to + (wave * XL + i) * 1024, bx, x_off + (uint32_t)(i * 16) * xp + k_off);
+    } else {
+      const int j = (wave * WL + i - XL) * 16;  // first of the sixteen LDS rows
+      int col = j;
+      bool second = false;
+      if (kGated) {  // a wave's columns: half from the first matrix, half from the second
+        constexpr int kSpan = TN * kEdge, kHalf = kSpan / 2;
+        second = j % kSpan >= kHalf;
+        col = j / kSpan * kHalf + j % kHalf;
+      }
+      load_to_lds(to + BM * kStageBytes + (wave * WL + i - XL) * 1024, second ? bw1 : bw0,
+                  w_off + (uint32_t)col * wp + k_off);
+    }
+  };
+  // (stages past the last ask for nothing and get zeros, so that every stage
+  // has the same number of loads under way)
+  auto k_offset = [&](int stage) {
+    const uint32_t kb = (uint32_t)stage * kStageBytes + chunk;
+    return stage < last && kb < (uint32_t)a.kbytes ? kb : kBehind;
   };
 
-  // --- sums -------------------------------------------------------------------------
-  Acc<T> acc[TM][TN];
+  // --- fragments --------------------------------------------------------------------
+  const int r = lane & (kEdge - 1), kq = lane / kEdge;
+  const int x_at = (wm * TM * kEdge + r) * kStageBytes;
+  const int w_at = (BM + wn * TN * kEdge + r) * kStageBytes;
+  const int slot[2] = {(kq ^ (r >> 2 & 3)) * 16, ((2 + kq) ^ (r >> 2 & 3)) * 16};
+  struct Frags { v4i w[TN], x[TM]; };
+  Frags f[2];
+  // fragment g of a phase: W's first
+  auto read = [&](Frags& to, int g, const char* stage, int phase) {
+    if (g < TN)
+      to.w[g] =
+          *reinterpret_cast<const v4i*>(stage + w_at + g * kEdge * kStageBytes + slot[phase]);
+    else
+      to.x[g - TN] = *reinterpret_cast<const v4i*>(stage + x_at + (g - TN) * kEdge * kStageBytes +
+                                                   slot[phase]);
+  };
+
+  Acc<T, kEdge> acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = Acc<T>{0, 0, 0, 0};
-
-  const int r16 = lane & 15, kq = lane >> 4;
-  const int x_at = (wm * TM * 16 + r16) * kStepBytes;
-  const int w_at = (BM + wn * TN * 16 + r16) * kStepBytes;
-  if (first < last) load_step(first, 0);
-  lds_loads_wait_barrier();
-  for (int step = first; step < last; ++step) {
-    const int buf = (step - first) & 1;
-    if (step + 1 < last) load_step(step + 1, buf ^ 1);
-    const char* s = lds[buf];
+    for (int j = 0; j < TN; ++j) acc[i][j] = Acc<T, kEdge>(0);
+  // one phase: group g is a read of the next phase's fragments, the loads that
+  // are due (half of a stage's, from `from` on) and the matrix instructions
+  auto phase = [&](Frags& next, const char* stage, int p, const Frags& cur, int from, uint32_t to,
+                   uint32_t k_off) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int slot = ((ks * 4 + kq) ^ (r16 & 7)) * 16;
-      v4i xf[TM], wf[TN];
+    for (int g = 0; g < kFrags; ++g) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-        wf[j] = *reinterpret_cast<const v4i*>(s + w_at + j * 16 * kStepBytes + slot);
+      for (int i = g * (kLoads / 2) / kFrags; i < (g + 1) * (kLoads / 2) / kFrags; ++i)
+        load(from + i, to, k_off);
+      read(next, g, stage, p);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-        xf[i] = *reinterpret_cast<const v4i*>(s + x_at + i * 16 * kStepBytes + slot);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<T>(wf[j], xf[i], acc[i][j]);
+      for (int e = g * kMfmas / kFrags; e < (g + 1) * kMfmas / kFrags; ++e)
+        acc[e / TN][e % TN] =
+            mfma<T, kEdge>(cur.w[e % TN], cur.x[e / TN], acc[e / TN][e % TN]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    lds_loads_wait_barrier();
+  };
+
+  // three stages and the first half of the fourth's loads under way
+#pragma unroll
+  for (int t = 0; t < kRing; ++t) {
+    const uint32_t k_off = k_offset(first + t);
+#pragma unroll
+    for (int i = 0; i < (t < kRing - 1 ? kLoads : kLoads / 2); ++i) load(i, lds0 + t * kStage, k_off);
   }
+  stage_barrier<2 * kLoads + kLoads / 2>();
+#pragma unroll
+  for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[0], 0);
+  for (int t = first; t < last; ++t) {
+    const int at = (t - first) % kRing, next = (at + 1) % kRing, ahead = (at + 3) % kRing;
+    phase(f[1], lds[at], 1, f[0], kLoads / 2, lds0 + ahead * kStage, k_offset(t + 3));
+    stage_barrier<2 * kLoads>();
+    phase(f[0], lds[next], 0, f[1], 0, lds0 + at * kStage, k_offset(t + 4));
+  }
+  // (the last loads wrote zeros: nothing may reach LDS after the workgroup has ended)
+  stage_barrier<0>();
 
   // --- epilogue ---------------------------------------------------------------------
+  // Through LDS, 32 rows of the wave's block at a time: a lane then holds
+  // columns next to its neighbours' (whole lines are stored), and the
+  // operator's arithmetic is a loop whose code is there once, not once for
+  // every register.  A wave reads only what it wrote.
+  constexpr int kSpan = TN * kEdge, kPitch = kSpan + 4;  // (16 bytes spread the banks)
+  constexpr int kOut = kGated ? kSpan / 2 : kSpan, kLanes = kOut / 4, kRows = 64 / kLanes;
+  static_assert(kWaves * kEdge * kPitch * 4 <= kRing * kStage, "");
+  typedef Acc<T> A4;
+  A4* mine = reinterpret_cast<A4*>(&lds[0][0] + wave * kEdge * kPitch * 4);
+  const int n = n0 + wn * kOut + lane % kLanes * 4;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int m = m0 + (wm * TM + i) * 16 + r16;
-    if (m >= a.M) continue;
 #pragma unroll
-    for (int j = 0; j < (kGated ? TN / 2 : TN); ++j) {
-      const int n = n0 + wn * (kGated ? TN * 8 : TN * 16) + j * 16 + kq * 4;
-      if (n >= a.N) continue;
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        mine[(r * kPitch + j * kEdge + g * 8 + kq * 4) / 4] = four<T, kEdge>(acc[i][j], g);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int row = lane / kLanes; row < kEdge; row += kRows) {
+      const int m = m0 + (wm * TM + i) * kEdge + row;
+      if (m >= a.M || n >= a.N) continue;
+      const A4 c = mine[row * kPitch / 4 + lane % kLanes];
       if constexpr (kGated) {
+        const A4 c2 = mine[row * kPitch / 4 + kLanes + lane % kLanes];
         if (a.partial) {
-          store_partial(a, blockIdx.y, 0, 2, m, n, acc[i][j]);
-          store_partial(a, blockIdx.y, 1, 2, m, n, acc[i][j + TN / 2]);
+          store_partial(a, blockIdx.y, 0, 2, m, n, c);
+          store_partial(a, blockIdx.y, 1, 2, m, n, c2);
         } else {
-          epi(m, n, acc[i][j], acc[i][j + TN / 2]);
+          epi(m, n, c, c2);
         }
       } else {
         if (a.partial)
-          store_partial(a, blockIdx.y, 0, 1, m, n, acc[i][j]);
+          store_partial(a, blockIdx.y, 0, 1, m, n, c);
         else
-          epi(m, n, acc[i][j]);
+          epi(m, n, c);
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -267,6 +356,8 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a, const 
   else
     epi(m, n, sum[0]);
 }
+
+constexpr int kRunBytes = 128;  // of K that a wave of the rows kernel takes at a time
 
 // Sixteen bytes of a row that ends `left` bytes from p on; zeros behind.
 __device__ __forceinline__ v4i load16_upto(const char* p, int left) {
@@ -305,7 +396,7 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
     for (int h = 0; h < kHalves; ++h) acc[i][h] = Acc<T>{0, 0, 0, 0};
 
   const int kbytes = (int)a.kbytes;
-  const int full = kbytes / kStepBytes;  // whole runs
+  const int full = kbytes / kRunBytes;  // whole runs
   // kRuns runs' loads are under way before the first is used
   constexpr int kRuns = MT == 1 ? 4 : MT == 2 ? 3 : 2;
   auto take = [&](int s, auto runs) {
@@ -313,7 +404,7 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
     v4i wf[R][kHalves][2], xf[R][MT][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t k = (int64_t)(s + r * kWaves) * kStepBytes;
+      const int64_t k = (int64_t)(s + r * kWaves) * kRunBytes;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
@@ -332,14 +423,14 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int h = 0; h < kHalves; ++h)
-            acc[i][h] = mfma16<T>(wf[r][h][ks], xf[r][i][ks], acc[i][h]);
+            acc[i][h] = mfma<T, 16>(wf[r][h][ks], xf[r][i][ks], acc[i][h]);
   };
   int s = wave;
   for (; s + (kRuns - 1) * kWaves < full; s += kRuns * kWaves)
     take(s, std::integral_constant<int, kRuns>{});
   for (; s < full; s += kWaves) take(s, std::integral_constant<int, 1>{});
-  if (full * kStepBytes < kbytes && wave == full % kWaves) {  // the run that ends inside
-    const int64_t k = (int64_t)full * kStepBytes;
+  if (full * kRunBytes < kbytes && wave == full % kWaves) {  // the run that ends inside
+    const int64_t k = (int64_t)full * kRunBytes;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const int left = kbytes - (int)k - ks * 64 - kq * 16;
@@ -348,7 +439,7 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
         const v4i xf = load16_upto(x[i] + k + ks * 64, left);
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
-          acc[i][h] = mfma16<T>(load16_upto(w[h] + k + ks * 64, left), xf, acc[i][h]);
+          acc[i][h] = mfma<T, 16>(load16_upto(w[h] + k + ks * 64, left), xf, acc[i][h]);
       }
     }
   }
@@ -393,7 +484,7 @@ constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay belo
 inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes) {
   GemmPlan p = {0, 1, 0};
   if (M <= kRowsMax) return p;
-  const int64_t steps = div_up(kbytes, kStepBytes);
+  const int64_t stages = div_up(kbytes, kStageBytes);
   auto tiles = [&](int64_t b) { return div_up(M, b) * div_up(wrows, b); };
   if (tiles(256) >= 200) {
     p.tile = 256;
@@ -401,7 +492,7 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes) {
     p.tile = 128;
   } else {
     p.tile = 64;
-    while (tiles(64) * p.splits < 512 && steps / (p.splits * 2) >= 8 && p.splits < 16)
+    while (tiles(64) * p.splits < 512 && stages / (p.splits * 2) >= 16 && p.splits < 16)
       p.splits *= 2;
   }
   if (p.splits > 1) p.partial_bytes = (size_t)p.splits * M * round_up(wrows, 8) * 4;
@@ -429,20 +520,19 @@ int launch_gemm(GemmArgs a, const Epi& epi, char* partial, hipStream_t stream) {
       hipLaunchKernelGGL((gemm_rows_kernel<T, 4, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
     return last_launch_status();
   }
-  const int steps = (int)div_up(a.kbytes, kStepBytes);
-  a.steps_per_split = (int)div_up(steps, p.splits);
+  a.stages_per_split = (int)div_up(div_up(a.kbytes, kStageBytes), p.splits);
   const int cols = Epi::kGated ? p.tile / 2 : p.tile;
   a.tiles_m = (int)div_up(a.M, p.tile);
   a.tiles_n = (int)div_up(a.N, cols);
   const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)p.splits);
   if (p.tile == 256)
-    hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 4, Epi>), grid, dim3(512), 0, stream, a,
+    hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 2, Epi>), grid, dim3(256), 0, stream, a,
                        epi);
   else if (p.tile == 128)
     hipLaunchKernelGGL((gemm_tile_kernel<T, 128, 128, 2, 2, Epi>), grid, dim3(256), 0, stream, a,
                        epi);
   else
-    hipLaunchKernelGGL((gemm_tile_kernel<T, 64, 64, 2, 2, Epi>), grid, dim3(256), 0, stream, a,
+    hipLaunchKernelGGL((gemm_tile_kernel<T, 64, 64, 2, 1, Epi>), grid, dim3(128), 0, stream, a,
                        epi);
   if (p.splits > 1) {
     const int64_t n = (int64_t)a.M * div_up(a.N, 4);
