@@ -14,6 +14,7 @@ namespace {
 template <class T>
 struct GatedEpi {
   static constexpr bool kGated = true;
+  static constexpr int kBatch = 1;
   const T* bg;
   const T* bu;
   T* h;
@@ -22,15 +23,28 @@ struct GatedEpi {
   int F, F4, act;
   Dropout drop;
 
-  __device__ __forceinline__ void operator()(int m, int n, v4f g, v4f u) const {
-    const int count = F - n;
-    if (bg) {
+  struct Cols { float g[4], u[4]; };
+  typedef int64_t Row;
+  __device__ __forceinline__ Cols columns(int n) const {
+    Cols c;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < count) {
-          g[i] += to_f32(bg[n + i]);
-          u[i] += to_f32(bu[n + i]);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int at = min(n + i, F - 1);
+      c.g[i] = bg ? to_f32(bg[at]) : 0.0f;
+      c.u[i] = bg ? to_f32(bu[at]) : 0.0f;
+    }
+    return c;
+  }
+  __device__ __forceinline__ Row row(int m) const {
+    return drop.mode && drop.rows ? drop.rows[m] : m;
+  }
+  __device__ __forceinline__ void operator()(int m, int n, const Cols& cols, Row id, v4f g,
+                                             v4f u) const {
+    const int count = F - n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      g[i] += cols.g[i];
+      u[i] += cols.u[i];
     }
     if (saved) {
       float* s = saved + (int64_t)m * F4 + n;
@@ -41,7 +55,7 @@ struct GatedEpi {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = activate(act, g[i]) * u[i];
     if (drop.mode)
-      drop4(drop, dropout_seed(drop), drop.rows ? drop.rows[m] : m, (uint32_t)n >> 2, v);
+      drop4(drop, dropout_seed(drop), (uint64_t)id, (uint32_t)n >> 2, v);
     store4(h + (int64_t)m * F + n, v, count, (F & 3) == 0);
   }
 };
@@ -50,10 +64,15 @@ struct GatedEpi {
 template <class T>
 struct StoreEpi {
   static constexpr bool kGated = false;
+  static constexpr int kBatch = 4;
   T* out0;
   T* out1;
   int split, N;
-  __device__ __forceinline__ void operator()(int m, int n, v4f c) const {
+  struct Cols {};
+  struct Row {};
+  __device__ __forceinline__ Cols columns(int) const { return {}; }
+  __device__ __forceinline__ Row row(int) const { return {}; }
+  __device__ __forceinline__ void operator()(int m, int n, Cols, Row, v4f c) const {
     T* row = m < split ? out0 + (int64_t)m * N : out1 + (int64_t)(m - split) * N;
     const float v[4] = {c[0], c[1], c[2], c[3]};
     store4(row + n, v, N - n, (N & 3) == 0);

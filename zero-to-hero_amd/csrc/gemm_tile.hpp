@@ -158,9 +158,13 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
   *reinterpret_cast<A*>(a.partial + at) = v;
 }
 
-// Epi: kGated (two W matrices, one output), and
-//   void operator()(int m, int n, Acc<T> c [, Acc<T> second]) for columns
-// n..n+3 of row m < M, n < N (columns past N - 1 are the callee's to skip).
+// Epi, the operator's epilogue: kGated (two W matrices, one output), kBatch
+// (rows that a lane takes at once: more where it waits for loads, one where
+// its code is long),
+//   Cols columns(int n), what columns n..n+3 bring along (a bias, scales),
+//   Row row(int m), what row m does,
+//   void operator()(int m, int n, const Cols&, const Row&, Acc<T> c [, Acc<T> second])
+// for columns n..n+3 of row m < M, n < N (those past N - 1 are its to skip).
 //
 // A stage is two phases, each one 16-byte chunk per lane of every fragment.
 // While the matrix cores work on one phase, the fragments of the next are read
@@ -299,7 +303,10 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   static_assert(kWaves * kEdge * kPitch * 4 <= kRing * kStage, "");
   typedef Acc<T> A4;
   A4* mine = reinterpret_cast<A4*>(&lds[0][0] + wave * kEdge * kPitch * 4);
+  constexpr int kBatch = Epi::kBatch;
+  static_assert(kEdge % (kRows * kBatch) == 0, "");
   const int n = n0 + wn * kOut + lane % kLanes * 4;
+  const typename Epi::Cols cols = epi.columns(min(n, a.N - 1));
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -310,23 +317,32 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-    for (int row = lane / kLanes; row < kEdge; row += kRows) {
-      const int m = m0 + (wm * TM + i) * kEdge + row;
-      if (m >= a.M || n >= a.N) continue;
-      const A4 c = mine[row * kPitch / 4 + lane % kLanes];
-      if constexpr (kGated) {
-        const A4 c2 = mine[row * kPitch / 4 + kLanes + lane % kLanes];
-        if (a.partial) {
-          store_partial(a, blockIdx.y, 0, 2, m, n, c);
-          store_partial(a, blockIdx.y, 1, 2, m, n, c2);
+    for (int row0 = 0; row0 < kEdge; row0 += kRows * kBatch) {
+      typename Epi::Row rows[kBatch];  // (their loads are under way together)
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        rows[b] = epi.row(min(m0 + (wm * TM + i) * kEdge + row0 + b * kRows + lane / kLanes,
+                              a.M - 1));
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int row = row0 + b * kRows + lane / kLanes;
+        const int m = m0 + (wm * TM + i) * kEdge + row;
+        if (m >= a.M || n >= a.N) continue;
+        const A4 c = mine[row * kPitch / 4 + lane % kLanes];
+        if constexpr (kGated) {
+          const A4 c2 = mine[row * kPitch / 4 + kLanes + lane % kLanes];
+          if (a.partial) {
+            store_partial(a, blockIdx.y, 0, 2, m, n, c);
+            store_partial(a, blockIdx.y, 1, 2, m, n, c2);
+          } else {
+            epi(m, n, cols, rows[b], c, c2);
+          }
         } else {
-          epi(m, n, c, c2);
+          if (a.partial)
+            store_partial(a, blockIdx.y, 0, 1, m, n, c);
+          else
+            epi(m, n, cols, rows[b], c);
         }
-      } else {
-        if (a.partial)
-          store_partial(a, blockIdx.y, 0, 1, m, n, c);
-        else
-          epi(m, n, c);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -352,9 +368,9 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a, const 
       sum[h] = s ? sum[h] + v : v;
     }
   if constexpr (kHalves == 2)
-    epi(m, n, sum[0], sum[1]);
+    epi(m, n, epi.columns(n), epi.row(m), sum[0], sum[1]);
   else
-    epi(m, n, sum[0]);
+    epi(m, n, epi.columns(n), epi.row(m), sum[0]);
 }
 
 constexpr int kRunBytes = 128;  // of K that a wave of the rows kernel takes at a time
@@ -389,6 +405,7 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
   const char* x[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) x[i] = a.x + (int64_t)min(i * 16 + r16, a.M - 1) * a.xpitch + kq * 16;
+  const typename Epi::Cols cols = epi.columns(min(n0 + kq * 4, a.N - 1));
   Acc<T> acc[MT][kHalves];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -461,9 +478,9 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
     const int m = i * 16 + r16, n = n0 + kq * 4;
     if (m >= a.M || n >= a.N) continue;
     if constexpr (kHalves == 2)
-      epi(m, n, sum[0], sum[1]);
+      epi(m, n, cols, epi.row(m), sum[0], sum[1]);
     else
-      epi(m, n, sum[0]);
+      epi(m, n, cols, epi.row(m), sum[0]);
   }
 }
 

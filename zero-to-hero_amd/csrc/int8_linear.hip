@@ -9,21 +9,31 @@ namespace {
 template <class T>
 struct Int8Epi {
   static constexpr bool kGated = false;
+  static constexpr int kBatch = 4;
   const float* xs;
   const float* ws;
   const T* bias;
   T* out;
   int N;
-  __device__ __forceinline__ void operator()(int m, int n, v4i c) const {
-    const float s = xs[m];
+  struct Cols { float scale[4], bias[4]; };
+  typedef float Row;
+  __device__ __forceinline__ Cols columns(int n) const {
+    Cols c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = min(n + i, N - 1);
+      c.scale[i] = ws[at];
+      c.bias[i] = bias ? to_f32(bias[at]) : 0.0f;
+    }
+    return c;
+  }
+  __device__ __forceinline__ Row row(int m) const { return xs[m]; }
+  __device__ __forceinline__ void operator()(int m, int n, const Cols& cols, Row s, v4i c) const {
     float v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[i] = 0.0f;
-      if (n + i < N) {
-        v[i] = (float)c[i] * s * ws[n + i];
-        if (bias) v[i] += to_f32(bias[n + i]);
-      }
+      v[i] = (float)c[i] * s * cols.scale[i];
+      if (bias) v[i] += cols.bias[i];  // (without one, a zero keeps its sign)
     }
     store4(out + (int64_t)m * N + n, v, N - n, (N & 3) == 0);
   }
