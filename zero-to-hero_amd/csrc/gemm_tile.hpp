@@ -12,15 +12,14 @@
 // with four consecutive columns n of one row m: a vector store, and one call
 // of the dropout generator.
 //
-// A workgroup computes a BM x BN tile over stages of 64 bytes of K.  The tiles
-// go from memory to LDS without passing through registers (buffer loads with
-// the LDS bit: 64 lanes, 16 bytes each, to consecutive LDS addresses) into a
-// ring of four stages.  A row's chunk c sits in slot c ^ (row / 4 % 4), which
-// spreads the rows that a fragment read touches over all banks; since the LDS
-// side of the load is fixed, the lanes permute the addresses they load from
-// instead.  The buffer descriptor ends with the operand's last row and lanes
-// past the end of a row ask for an offset behind it: the hardware gives zero
-// for both, so partial tiles need no other path.
+// A workgroup computes a BM x BN tile over K steps of 128 bytes, a whole line
+// of memory per row (half lines were fetched twice: 1127 against 988 us for
+// 8192 x 4096 x 16384 in bf16).  The tiles pass through registers into one of
+// two LDS buffers.  A row's chunk c sits in slot c ^ (row % 8), which spreads
+// the rows that a fragment read touches over all banks.  The buffer
+// descriptor ends with the operand's last row and lanes past the end of a row
+// ask for an offset behind it: the hardware gives zero for both, so partial
+// tiles need no other path.
 #pragma once
 
 #include <type_traits>
@@ -37,12 +36,11 @@ struct GemmArgs {
   int64_t kbytes;   // of a row, a multiple of 16
   int M, N;         // N: output columns
   int tiles_m, tiles_n;
-  int stages_per_split;    // stages of kStageBytes that one split takes
+  int steps_per_split;     // K steps that one split takes
   char* partial;    // [splits][1 or 2][M][N4] 32-bit sums, or null: no split
 };
 
-constexpr int kStageBytes = 64;  // of a row, in one stage of the ring
-constexpr int kRing = 4;
+constexpr int kStepBytes = 128;  // of a row, in one step
 
 // Sums of one matrix instruction: kEdge x kEdge outputs over 64 lanes, 4 or
 // 16 a lane, in groups of four consecutive columns n of one row m.
@@ -104,32 +102,18 @@ __device__ __forceinline__ Acc<T> four(const Acc<T, kEdge>& c, int group) {
 }
 
 // Descriptor of `bytes` (below 2^31) from p on; loads behind it give zero.
-__device__ __forceinline__ v4i buffer_of(const char* p, uint32_t bytes) {
-  const uint64_t a = (uint64_t)p;
-  v4i r;
-  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
-  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff);
-  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
-  r[3] = 0x00020000;
-  return r;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const char* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)bytes, 0x00020000);
 }
 
-// 64 lanes, 16 bytes each from buffer + offset, to LDS at lds + 16 * lane
-// (`lds` is the same in all lanes).  Nothing in registers is written; the
-// data has arrived after lds_loads_wait_barrier().
-__device__ __forceinline__ void load_to_lds(uint32_t lds, v4i buffer, uint32_t offset) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer));
+__device__ __forceinline__ v4i load16(__amdgpu_buffer_rsrc_t buffer, uint32_t offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(buffer, (int)offset, 0, 0);
 }
 
-// Waits until at most kLeft of this wave's loads are under way, and for its
-// LDS reads, then for the whole workgroup: what every wave had loaded until
-// then may be read, what it has read overwritten.
-template <int kLeft>
-__device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+// Waits for this wave's LDS reads and writes, then for the whole workgroup;
+// loads from memory stay under way.
+__device__ __forceinline__ void lds_only_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 constexpr uint32_t kBehind = 0x80000000u;  // an offset that no descriptor reaches
@@ -166,28 +150,29 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 //   void operator()(int m, int n, const Cols&, const Row&, Acc<T> c [, Acc<T> second])
 // for columns n..n+3 of row m < M, n < N (those past N - 1 are its to skip).
 //
-// A stage is two phases, each one 16-byte chunk per lane of every fragment.
+// A step is four phases, each one 16-byte chunk per lane of every fragment.
 // While the matrix cores work on one phase, the fragments of the next are read
-// from LDS, one read to every few matrix instructions.  The workgroup meets
-// once a stage, when its second phase has been read: the stage's place in the
-// ring is then free for the loads of the stage four later, which are spread
-// over the following stage (issued together they would hold up the matrix
-// instructions behind them), three stages ahead of their use.
+// from LDS, one read to every few matrix instructions; between them the next
+// step's data goes from registers to the other buffer and the loads of the
+// step after it take its place in the registers, a whole step ahead of their
+// use.  The workgroup meets once a step, before the last phase: by then every
+// wave has read the buffer to its end and written the other one.
 template <class T, int BM, int BN, int kWavesM, int kWavesN, class Epi>
 __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     gemm_tile_kernel(const GemmArgs a, const Epi epi) {
   constexpr int kWaves = kWavesM * kWavesN;
   constexpr int kEdge = 32;  // of a matrix instruction's block
   constexpr int TM = BM / kWavesM / kEdge, TN = BN / kWavesN / kEdge;
-  constexpr int XL = BM / 16 / kWaves, WL = BN / 16 / kWaves;  // loads of a wave per stage
+  constexpr int kPhases = 4;
+  constexpr int XL = BM / 8 / kWaves, WL = BN / 8 / kWaves;  // loads of a wave per step
   constexpr int kLoads = XL + WL;
   constexpr int kFrags = TM + TN, kMfmas = TM * TN;
   constexpr bool kGated = Epi::kGated;
   constexpr int kCols = kGated ? BN / 2 : BN;  // output columns of a tile
-  constexpr int kStage = (BM + BN) * kStageBytes;
-  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && kLoads % 2 == 0, "");
+  constexpr int kBuffer = (BM + BN) * kStepBytes;
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "");
   static_assert(!kGated || TN % 2 == 0, "");
-  __shared__ __align__(1024) char lds[kRing][kStage];
+  __shared__ __align__(1024) char lds[2][kBuffer];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -195,60 +180,56 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   int tm, tn;
   tile_of(a, tm, tn);
   const int m0 = tm * BM, n0 = tn * kCols;
-  const int stages = (int)div_up(a.kbytes, kStageBytes);
-  const int first = blockIdx.y * a.stages_per_split;
-  const int last = min(stages, first + a.stages_per_split);
+  const int steps = (int)div_up(a.kbytes, kStepBytes);
+  const int first = blockIdx.y * a.steps_per_split;
+  const int count = max(0, min(steps - first, a.steps_per_split));
 
   // --- loads ------------------------------------------------------------------------
-  const int row16 = lane >> 2;
-  const uint32_t chunk = ((lane & 3) ^ (row16 >> 2)) * 16;
+  const int row8 = lane >> 3;
   const uint32_t xp = (uint32_t)a.xpitch, wp = (uint32_t)a.wpitch;
-  const v4i bx = buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
+  const auto bx = buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
   const uint32_t w_bytes = (uint32_t)min(kCols, a.N - n0) * wp;
-  const v4i bw0 = buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
-  const v4i bw1 = kGated ? buffer_of(a.w1 + n0 * a.wpitch, w_bytes) : bw0;
-  const uint32_t x_off = (uint32_t)(wave * XL * 16 + row16) * xp, w_off = (uint32_t)row16 * wp;
-  const uint32_t lds0 =
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
-  // load i of a stage (X's first): sixteen rows
-  auto load = [&](int i, uint32_t to, uint32_t k_off) {
-    if (i < XL) {
-      load_to_lds(to + (wave * XL + i) * 1024, bx, x_off + (uint32_t)(i * 16) * xp + k_off);
-    } else {
-      const int j = (wave * WL + i - XL) * 16;  // first of the sixteen LDS rows
-      int col = j;
-      bool second = false;
-      if (kGated) {  // a wave's columns: half from the first matrix, half from the second
-        constexpr int kSpan = TN * kEdge, kHalf = kSpan / 2;
-        second = j % kSpan >= kHalf;
-        col = j / kSpan * kHalf + j % kHalf;
-      }
-      load_to_lds(to + BM * kStageBytes + (wave * WL + i - XL) * 1024, second ? bw1 : bw0,
-                  w_off + (uint32_t)col * wp + k_off);
+  const auto bw0 = buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
+  const auto bw1 = buffer_of((kGated ? a.w1 : a.w0) + n0 * a.wpitch, w_bytes);
+  const uint32_t x_off = (uint32_t)(wave * XL * 8 + row8) * xp, w_off = (uint32_t)row8 * wp;
+  // load i of a step (X's first): eight rows
+  auto load = [&](int i, uint32_t k_off) -> v4i {
+    if (i < XL) return load16(bx, x_off + (uint32_t)(i * 8) * xp + k_off);
+    const int j = (wave * WL + i - XL) * 8;  // first of the eight LDS rows
+    int col = j;
+    bool second = false;
+    if (kGated) {  // a wave's columns: half from the first matrix, half from the second
+      constexpr int kSpan = TN * kEdge, kHalf = kSpan / 2;
+      second = j % kSpan >= kHalf;
+      col = j / kSpan * kHalf + j % kHalf;
     }
+    return load16(second ? bw1 : bw0, w_off + (uint32_t)col * wp + k_off);
   };
-  // (stages past the last ask for nothing and get zeros, so that every stage
-  // has the same number of loads under way)
-  auto k_offset = [&](int stage) {
-    const uint32_t kb = (uint32_t)stage * kStageBytes + chunk;
-    return stage < last && kb < (uint32_t)a.kbytes ? kb : kBehind;
+  // steps past the last ask for nothing
+  auto k_offset = [&](int step) {
+    const uint32_t kb = (uint32_t)(first + step) * kStepBytes + (lane & 7) * 16;
+    return step < count && kb < (uint32_t)a.kbytes ? kb : kBehind;
+  };
+  const int put_at = row8 * kStepBytes + ((lane & 7) ^ row8) * 16;
+  auto put = [&](int i, v4i v, char* buf) {
+    const int row = i < XL ? (wave * XL + i) * 8 : BM + (wave * WL + i - XL) * 8;
+    *reinterpret_cast<v4i*>(buf + row * kStepBytes + put_at) = v;
   };
 
   // --- fragments --------------------------------------------------------------------
   const int r = lane & (kEdge - 1), kq = lane / kEdge;
-  const int x_at = (wm * TM * kEdge + r) * kStageBytes;
-  const int w_at = (BM + wn * TN * kEdge + r) * kStageBytes;
-  const int slot[2] = {(kq ^ (r >> 2 & 3)) * 16, ((2 + kq) ^ (r >> 2 & 3)) * 16};
+  const int x_at = (wm * TM * kEdge + r) * kStepBytes;
+  const int w_at = (BM + wn * TN * kEdge + r) * kStepBytes;
   struct Frags { v4i w[TN], x[TM]; };
   Frags f[2];
   // fragment g of a phase: W's first
-  auto read = [&](Frags& to, int g, const char* stage, int phase) {
+  auto read = [&](Frags& to, int g, const char* buf, int phase) {
+    const int slot = ((phase * 2 + kq) ^ (r & 7)) * 16;
     if (g < TN)
-      to.w[g] =
-          *reinterpret_cast<const v4i*>(stage + w_at + g * kEdge * kStageBytes + slot[phase]);
+      to.w[g] = *reinterpret_cast<const v4i*>(buf + w_at + g * kEdge * kStepBytes + slot);
     else
-      to.x[g - TN] = *reinterpret_cast<const v4i*>(stage + x_at + (g - TN) * kEdge * kStageBytes +
-                                                   slot[phase]);
+      to.x[g - TN] =
+          *reinterpret_cast<const v4i*>(buf + x_at + (g - TN) * kEdge * kStepBytes + slot);
   };
 
   Acc<T, kEdge> acc[TM][TN];
@@ -256,42 +237,51 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = Acc<T, kEdge>(0);
-  // one phase: group g is a read of the next phase's fragments, the loads that
-  // are due (half of a stage's, from `from` on) and the matrix instructions
-  auto phase = [&](Frags& next, const char* stage, int p, const Frags& cur, int from, uint32_t to,
-                   uint32_t k_off) {
+  auto multiply = [&](const Frags& from, int g) {
 #pragma unroll
-    for (int g = 0; g < kFrags; ++g) {
-#pragma unroll
-      for (int i = g * (kLoads / 2) / kFrags; i < (g + 1) * (kLoads / 2) / kFrags; ++i)
-        load(from + i, to, k_off);
-      read(next, g, stage, p);
-#pragma unroll
-      for (int e = g * kMfmas / kFrags; e < (g + 1) * kMfmas / kFrags; ++e)
-        acc[e / TN][e % TN] =
-            mfma<T, kEdge>(cur.w[e % TN], cur.x[e / TN], acc[e / TN][e % TN]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int e = g * kMfmas / kFrags; e < (g + 1) * kMfmas / kFrags; ++e)
+      acc[e / TN][e % TN] = mfma<T, kEdge>(from.w[e % TN], from.x[e / TN], acc[e / TN][e % TN]);
   };
 
-  // three stages and the first half of the fourth's loads under way
+  v4i staged[kLoads];  // the step that goes to LDS next
+  {
+    const uint32_t k0 = k_offset(0), k1 = k_offset(1);
 #pragma unroll
-  for (int t = 0; t < kRing; ++t) {
-    const uint32_t k_off = k_offset(first + t);
+    for (int i = 0; i < kLoads; ++i) staged[i] = load(i, k0);
 #pragma unroll
-    for (int i = 0; i < (t < kRing - 1 ? kLoads : kLoads / 2); ++i) load(i, lds0 + t * kStage, k_off);
+    for (int i = 0; i < kLoads; ++i) put(i, staged[i], lds[0]);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) staged[i] = load(i, k1);
+    lds_only_barrier();
+#pragma unroll
+    for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[0], 0);
   }
-  stage_barrier<2 * kLoads + kLoads / 2>();
+  for (int step = 0; step < count; ++step) {
+    char* cur = lds[step & 1];
+    char* other = lds[step & 1 ^ 1];
+    const uint32_t k_off = k_offset(step + 2);
+    constexpr int kGroups = (kPhases - 1) * kFrags;
 #pragma unroll
-  for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[0], 0);
-  for (int t = first; t < last; ++t) {
-    const int at = (t - first) % kRing, next = (at + 1) % kRing, ahead = (at + 3) % kRing;
-    phase(f[1], lds[at], 1, f[0], kLoads / 2, lds0 + ahead * kStage, k_offset(t + 3));
-    stage_barrier<2 * kLoads>();
-    phase(f[0], lds[next], 0, f[1], 0, lds0 + at * kStage, k_offset(t + 4));
+    for (int q = 0; q < kGroups; ++q) {
+      const int p = q / kFrags, g = q % kFrags;
+      read(f[(p + 1) & 1], g, cur, p + 1);
+#pragma unroll
+      for (int i = q * kLoads / kGroups; i < (q + 1) * kLoads / kGroups; ++i) {
+        put(i, staged[i], other);
+        staged[i] = load(i, k_off);
+      }
+      multiply(f[p & 1], g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    lds_only_barrier();
+#pragma unroll
+    for (int g = 0; g < kFrags; ++g) {
+      read(f[0], g, other, 0);
+      multiply(f[1], g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
-  // (the last loads wrote zeros: nothing may reach LDS after the workgroup has ended)
-  stage_barrier<0>();
+  lds_only_barrier();  // (the last phase has read ahead in what the epilogue overwrites)
 
   // --- epilogue ---------------------------------------------------------------------
   // Through LDS, 32 rows of the wave's block at a time: a lane then holds
@@ -300,7 +290,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   // every register.  A wave reads only what it wrote.
   constexpr int kSpan = TN * kEdge, kPitch = kSpan + 4;  // (16 bytes spread the banks)
   constexpr int kOut = kGated ? kSpan / 2 : kSpan, kLanes = kOut / 4, kRows = 64 / kLanes;
-  static_assert(kWaves * kEdge * kPitch * 4 <= kRing * kStage, "");
+  static_assert(kWaves * kEdge * kPitch * 4 <= 2 * kBuffer, "");
   typedef Acc<T> A4;
   A4* mine = reinterpret_cast<A4*>(&lds[0][0] + wave * kEdge * kPitch * 4);
   constexpr int kBatch = Epi::kBatch;
@@ -501,7 +491,7 @@ constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay belo
 inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes) {
   GemmPlan p = {0, 1, 0};
   if (M <= kRowsMax) return p;
-  const int64_t stages = div_up(kbytes, kStageBytes);
+  const int64_t steps = div_up(kbytes, kStepBytes);
   auto tiles = [&](int64_t b) { return div_up(M, b) * div_up(wrows, b); };
   if (tiles(256) >= 200) {
     p.tile = 256;
@@ -509,7 +499,7 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes) {
     p.tile = 128;
   } else {
     p.tile = 64;
-    while (tiles(64) * p.splits < 512 && stages / (p.splits * 2) >= 16 && p.splits < 16)
+    while (tiles(64) * p.splits < 512 && steps / (p.splits * 2) >= 8 && p.splits < 16)
       p.splits *= 2;
   }
   if (p.splits > 1) p.partial_bytes = (size_t)p.splits * M * round_up(wrows, 8) * 4;
@@ -537,7 +527,7 @@ int launch_gemm(GemmArgs a, const Epi& epi, char* partial, hipStream_t stream) {
       hipLaunchKernelGGL((gemm_rows_kernel<T, 4, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
     return last_launch_status();
   }
-  a.stages_per_split = (int)div_up(div_up(a.kbytes, kStageBytes), p.splits);
+  a.steps_per_split = (int)div_up(div_up(a.kbytes, kStepBytes), p.splits);
   const int cols = Epi::kGated ? p.tile / 2 : p.tile;
   a.tiles_m = (int)div_up(a.M, p.tile);
   a.tiles_n = (int)div_up(a.N, cols);
