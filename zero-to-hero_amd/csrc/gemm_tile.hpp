@@ -167,6 +167,8 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   constexpr int XL = BM / 8 / kWaves, WL = BN / 8 / kWaves;  // loads of a wave per step
   constexpr int kLoads = XL + WL;
   constexpr int kFrags = TM + TN, kMfmas = TM * TN;
+  // steps that are on their way through registers: two where they fit
+  constexpr int kAhead = BM * BN >= 256 * 256 ? 1 : 2;
   constexpr bool kGated = Epi::kGated;
   constexpr int kCols = kGated ? BN / 2 : BN;  // output columns of a tile
   constexpr int kBuffer = (BM + BN) * kStepBytes;
@@ -237,49 +239,67 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = Acc<T, kEdge>(0);
-  auto multiply = [&](const Frags& from, int g) {
+  auto multiply = [&](const Frags& from, int e) {
+    acc[e / TN][e % TN] = mfma<T, kEdge>(from.w[e % TN], from.x[e / TN], acc[e / TN][e % TN]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The matrix instructions of a phase in their order; behind each goes what it
+  // is to cover: the reads behind the first of every pair, the rest (`other`,
+  // called with the share of the phase that is over) behind the second.
+  auto phase = [&](const Frags& from, Frags& to, const char* buf, int p, auto&& other) {
 #pragma unroll
-    for (int e = g * kMfmas / kFrags; e < (g + 1) * kMfmas / kFrags; ++e)
-      acc[e / TN][e % TN] = mfma<T, kEdge>(from.w[e % TN], from.x[e / TN], acc[e / TN][e % TN]);
+    for (int e = 0; e < kMfmas; ++e) {
+      multiply(from, e);
+      // reads: evenly over the even slots (all slots if there are too few)
+      constexpr int kEven = (kMfmas + 1) / 2;
+      if (e % 2 == 0) {
+#pragma unroll
+        for (int g = e / 2 * kFrags / kEven; g < (e / 2 + 1) * kFrags / kEven; ++g)
+          read(to, g, buf, p);
+      }
+      if (e % 2 == 1 || kMfmas == 1) other(e / 2, kMfmas / 2 > 0 ? kMfmas / 2 : 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
-  v4i staged[kLoads];  // the step that goes to LDS next
+  v4i staged[kAhead][kLoads];  // the steps that go to LDS next
   {
-    const uint32_t k0 = k_offset(0), k1 = k_offset(1);
+    const uint32_t k0 = k_offset(0);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) staged[i] = load(i, k0);
+    for (int i = 0; i < kLoads; ++i) staged[0][i] = load(i, k0);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) put(i, staged[i], lds[0]);
+    for (int i = 0; i < kLoads; ++i) put(i, staged[0][i], lds[0]);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) staged[i] = load(i, k1);
+    for (int h = 0; h < kAhead; ++h) {
+      const uint32_t k_off = k_offset(h + 1);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) staged[h][i] = load(i, k_off);
+    }
     lds_only_barrier();
 #pragma unroll
     for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[0], 0);
   }
-  for (int step = 0; step < count; ++step) {
+  auto one_step = [&](int step, v4i (&next)[kLoads]) {
     char* cur = lds[step & 1];
     char* other = lds[step & 1 ^ 1];
-    const uint32_t k_off = k_offset(step + 2);
-    constexpr int kGroups = (kPhases - 1) * kFrags;
+    const uint32_t k_off = k_offset(step + 1 + kAhead);
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
-      const int p = q / kFrags, g = q % kFrags;
-      read(f[(p + 1) & 1], g, cur, p + 1);
+    for (int p = 0; p < kPhases - 1; ++p)
+      phase(f[p & 1], f[(p + 1) & 1], cur, p + 1, [&](int slot, int slots) {
+        const int at = p * slots + slot, all = (kPhases - 1) * slots;
 #pragma unroll
-      for (int i = q * kLoads / kGroups; i < (q + 1) * kLoads / kGroups; ++i) {
-        put(i, staged[i], other);
-        staged[i] = load(i, k_off);
-      }
-      multiply(f[p & 1], g);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+        for (int i = at * kLoads / all; i < (at + 1) * kLoads / all; ++i) {
+          put(i, next[i], other);
+          next[i] = load(i, k_off);
+        }
+      });
     lds_only_barrier();
+    phase(f[1], f[0], other, 0, [](int, int) {});
+  };
+  for (int step = 0; step < count; step += kAhead) {
 #pragma unroll
-    for (int g = 0; g < kFrags; ++g) {
-      read(f[0], g, other, 0);
-      multiply(f[1], g);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int h = 0; h < kAhead; ++h)
+      if (h == 0 || step + h < count) one_step(step + h, staged[h]);
   }
   lds_only_barrier();  // (the last phase has read ahead in what the epilogue overwrites)
 
