@@ -5,7 +5,8 @@
 // Forward: one product over both weight matrices (gemm_tile.hpp; a wave holds
 // the gate's and the up projection's sums of the same elements, so g and u
 // never leave registers unless the backward pass wants them).  Backward: one
-// elementwise pass forms dg and du in both orders, then two products.
+// elementwise pass forms dg and du, then two products read them, x and the
+// weights as they lie.
 #include "gemm_tile.hpp"
 
 namespace ppo {
@@ -60,20 +61,24 @@ struct GatedEpi {
   }
 };
 
-// Plain store of the sums, rows from `split` on to a second output.
+// Plain store of the sums.  Rows from `second` on go to a second output;
+// `rows` of each are stored (the rest belongs to padding).
 template <class T>
 struct StoreEpi {
   static constexpr bool kGated = false;
   static constexpr int kBatch = 4;
   T* out0;
   T* out1;
-  int split, N;
+  int rows, second, N;
   struct Cols {};
   struct Row {};
   __device__ __forceinline__ Cols columns(int) const { return {}; }
   __device__ __forceinline__ Row row(int) const { return {}; }
   __device__ __forceinline__ void operator()(int m, int n, Cols, Row, v4f c) const {
-    T* row = m < split ? out0 + (int64_t)m * N : out1 + (int64_t)(m - split) * N;
+    T* out = out0;
+    if (m >= second) m -= second, out = out1;
+    if (m >= rows) return;
+    T* row = out + (int64_t)m * N;
     const float v[4] = {c[0], c[1], c[2], c[3]};
     store4(row + n, v, N - n, (N & 3) == 0);
   }
@@ -88,51 +93,45 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T* in, int64_t rows
       out[r * pitch + c] = c < cols ? in[r * cols + c] : from_f32<T>(0.0f);
 }
 
-constexpr int kTr = 64;  // edge of the tiles that are transposed through LDS
+constexpr int kTileM = 64;  // rows and columns that a workgroup of the next kernel takes
+constexpr int kTileF = 64;
 
-// in [rows][cols] -> out[c][r] at out + c * pitch + r, zeros for r in
-// [rows, rows4): the k-contiguous form of an operand whose rows are k.
-template <class T>
-__global__ void __launch_bounds__(256) transpose_kernel(const T* in, int64_t rows, int cols, T* out,
-                                                        int64_t pitch, int64_t padded) {
-  __shared__ T tile[kTr][kTr + 16 / sizeof(T) / 2 + 1];
-  const int64_t r0 = (int64_t)blockIdx.x * kTr;
-  const int c0 = blockIdx.y * kTr;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  for (int i = ty; i < kTr; i += 4)
-    tile[i][tx] = r0 + i < rows && c0 + tx < cols ? in[(r0 + i) * cols + c0 + tx] : from_f32<T>(0.0f);
-  __syncthreads();
-  for (int i = ty; i < kTr; i += 4)
-    if (c0 + i < cols && r0 + tx < padded) out[(c0 + i) * pitch + r0 + tx] = tile[tx][i];
-}
-
-// dg and du of a 64 x 64 tile, from dh and the saved g and u: rows for dx
-// (dgu [M][2 Fp], dg then du) and, transposed, rows for the weights' gradients
-// (dgu_t [2 F][Mp]); with `sums`, the tile's column sums for the biases
-// ([row tiles][2 F], joined in order by bias_join_kernel).
+// dg and du from dh and the saved g and u, as rows [dg | du] of pitch 2 fp (fp:
+// F rounded up to 16 bytes, zeros behind F), the operand of both products;
+// with `sums`, a tile's column sums for the biases ([row tiles][2 F], joined
+// in order by bias_join_kernel).
 template <class T>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const float* saved, int64_t M,
                                                          int F, int F4, int act, Dropout drop,
-                                                         T* dgu, int64_t fp, T* dgu_t, int64_t mp,
-                                                         float* sums) {
-  __shared__ float tile[2][kTr][kTr + 1];
-  const int64_t r0 = (int64_t)blockIdx.x * kTr;
-  const int c0 = blockIdx.y * kTr;
+                                                         T* dgu, int64_t fp, float* sums) {
+  __shared__ float part[16][2 * kTileF + 4];
+  const int64_t r0 = (int64_t)blockIdx.x * kTileM;
+  const int c0 = blockIdx.y * kTileF;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;  // four columns, rows ty + 16 i
   const int n = c0 + tx * 4;
   const uint64_t seed = drop.mode ? dropout_seed(drop) : 0;
+  const bool vec = (F & 3) == 0 && ((uintptr_t)dh & (4 * sizeof(T) - 1)) == 0;
+  float sg[4] = {0, 0, 0, 0}, su[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = ty + 16 * i;
-    const int64_t m = r0 + r;
+  for (int i = 0; i < kTileM / 16; ++i) {
+    const int64_t m = r0 + ty + 16 * i;
+    if (m >= M || n >= fp) continue;
     float dg[4] = {0, 0, 0, 0}, du[4] = {0, 0, 0, 0};
-    if (m < M && n < F) {
+    if (n < F) {
       const v4f g = *reinterpret_cast<const v4f*>(saved + m * F4 + n);
       const v4f u = *reinterpret_cast<const v4f*>(saved + (M + m) * F4 + n);
       float d[4] = {0, 0, 0, 0};
+      const T* dp = dh + m * F + n;
+      struct __attribute__((aligned(4 * sizeof(T)))) Four { T x[4]; } four;
+      if (vec) {
+        four = *reinterpret_cast<const Four*>(dp);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n + k < F) d[k] = to_f32(dh[m * F + n + k]);
+        for (int k = 0; k < 4; ++k) d[k] = to_f32(four.x[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n + k < F) d[k] = to_f32(dp[k]);
+      }
       if (drop.mode) drop4(drop, seed, drop.rows ? drop.rows[m] : m, (uint32_t)n >> 2, d);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -141,35 +140,25 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
           activate_grad(act, g[k], a, da);
           du[k] = d[k] * a;
           dg[k] = d[k] * u[k] * da;
+          su[k] += du[k];
+          sg[k] += dg[k];
         }
     }
+    store4(dgu + m * 2 * fp + n, dg, 4, true);
+    store4(dgu + m * 2 * fp + fp + n, du, 4, true);
+  }
+  if (!sums) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      tile[0][r][tx * 4 + k] = dg[k];
-      tile[1][r][tx * 4 + k] = du[k];
-    }
-    if (dgu && m < M && n < fp) {  // (columns F..fp are zeros)
-      store4(dgu + m * 2 * fp + n, dg, 4, true);
-      store4(dgu + m * 2 * fp + fp + n, du, 4, true);
-    }
+  for (int k = 0; k < 4; ++k) {
+    part[ty][tx * 4 + k] = sg[k];
+    part[ty][kTileF + tx * 4 + k] = su[k];
   }
   __syncthreads();
-  if (dgu_t) {
-    const int cx = threadIdx.x & 15, cy = threadIdx.x >> 4;  // four rows m, columns cy + 16 i
-    const int64_t m = r0 + cx * 4;
-    for (int i = 0; i < 8; ++i) {
-      const int half = i >> 2, c = cy + 16 * (i & 3);
-      if (c0 + c >= F || m >= mp) continue;
-      const float v[4] = {tile[half][cx * 4][c], tile[half][cx * 4 + 1][c],
-                          tile[half][cx * 4 + 2][c], tile[half][cx * 4 + 3][c]};
-      store4(dgu_t + ((int64_t)half * F + c0 + c) * mp + m, v, 4, true);
-    }
-  }
-  if (sums && threadIdx.x < 2 * kTr) {
-    const int half = threadIdx.x / kTr, c = threadIdx.x % kTr;
+  if (threadIdx.x < 2 * kTileF) {
+    const int half = threadIdx.x / kTileF, c = threadIdx.x % kTileF;
     if (c0 + c < F) {
       float s = 0.0f;
-      for (int r = 0; r < kTr; ++r) s += tile[half][r][c];
+      for (int r = 0; r < 16; ++r) s += part[r][threadIdx.x];
       sums[(int64_t)blockIdx.x * 2 * F + half * F + c0 + c] = s;
     }
   }
@@ -230,23 +219,29 @@ ForwardPlan plan_forward(int dtype, int64_t M, int64_t D, int64_t F, bool aligne
 }
 
 struct BackwardPlan {
-  int64_t fp, mp;  // F and M rounded up to 16 bytes of elements
-  char *dgu, *dgu_t, *w_t, *x_t, *sums, *partial;
+  int64_t fp;     // F rounded up to 16 bytes of elements
+  int64_t pitch;  // bytes of a row of x and the weights
+  bool pad;
+  char *dgu, *x, *wg, *wu, *sums, *partial;
   size_t bytes;
 };
 
-BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, char* ws) {
+BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool aligned, char* ws) {
   const int64_t size = dtype_size(dtype);
   BackwardPlan b = {};
   b.fp = round_up(F, 16 / size);
-  b.mp = round_up(M, 16 / size);
+  b.pitch = round_up(D * size, 16);
+  b.pad = !aligned || b.pitch != D * size;
   Scratch s{ws};
   b.dgu = s.take(M * 2 * b.fp * size);
-  b.dgu_t = s.take(2 * F * b.mp * size);
-  b.w_t = s.take(D * 2 * b.fp * size);
-  b.x_t = s.take(D * b.mp * size);
-  b.sums = s.take(div_up(M, kTr) * 2 * F * 4);
-  const GemmPlan gx = plan_gemm(M, D, 2 * b.fp * size), gw = plan_gemm(2 * F, D, b.mp * size);
+  if (b.pad) {
+    b.x = s.take(M * b.pitch);
+    b.wg = s.take(F * b.pitch);
+    b.wu = s.take(F * b.pitch);
+  }
+  b.sums = s.take(div_up(M, kTileM) * 2 * F * 4);
+  const GemmPlan gx = plan_gemm(M, D, 2 * b.fp * size, true),
+                 gw = plan_gemm(2 * b.fp, D, M * size, true);
   b.partial = s.take((int64_t)(gx.partial_bytes > gw.partial_bytes ? gx.partial_bytes
                                                                    : gw.partial_bytes));
   b.bytes = s.used;
@@ -260,9 +255,8 @@ bool forward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
   return M < lim && D < lim && F < lim && gemm_fits(M, 2 * F, round_up(D * dtype_size(dtype), 16));
 }
 bool backward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
-  const int64_t size = dtype_size(dtype);
-  return forward_fits(dtype, M, D, F) && gemm_fits(M, D, 2 * round_up(F, 16) * size) &&
-         gemm_fits(2 * F, D, round_up(M, 16) * size);
+  const int64_t size = dtype_size(dtype), pitch = 2 * round_up(F, 16) * size;
+  return forward_fits(dtype, M, D, F) && gemm_fits(M, D, pitch) && gemm_fits(2 * F, D, pitch);
 }
 
 template <class T>
@@ -270,14 +264,6 @@ void pad_rows(const void* in, int64_t rows, int64_t cols, char* out, int64_t pit
               hipStream_t stream) {
   hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256),
                      0, stream, (const T*)in, rows, (int)cols, (T*)out, (int)(pitch / sizeof(T)));
-}
-
-template <class T>
-void transpose(const void* in, int64_t rows, int64_t cols, char* out, int64_t pitch,
-               int64_t padded, hipStream_t stream) {
-  hipLaunchKernelGGL((transpose_kernel<T>),
-                     dim3((unsigned)div_up(padded, kTr), (unsigned)div_up(cols, kTr)), dim3(256), 0,
-                     stream, (const T*)in, rows, (int)cols, (T*)out, pitch, padded);
 }
 
 bool drop_ok(const ppo_dropout* d) { return !d || (d->p >= 0.0 && d->p <= 1.0); }
@@ -341,7 +327,7 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
 extern "C" size_t ppo_layer_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t D,
                                                            int64_t F) {
   if (!dtype_ok(dtype) || !sizes_ok(M, D, F) || !backward_fits(dtype, M, D, F)) return 0;
-  return plan_backward(dtype, M, D, F, nullptr).bytes;
+  return plan_backward(dtype, M, D, F, false, nullptr).bytes;
 }
 
 extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const void* wg,
@@ -356,8 +342,11 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
   if (M == 0) return PPO_ERR_INVALID_ARG;  // (the sums over no rows are the caller's zeros)
   if (!dh || !saved || (dwg && !x) || (dx && (!wg || !wu))) return PPO_ERR_INVALID_ARG;
   if (!backward_fits(dtype, M, D, F)) return PPO_ERR_TOO_LARGE;
-  const BackwardPlan b = plan_backward(dtype, M, D, F, (char*)workspace);
-  if (!workspace || workspace_bytes < b.bytes || !aligned16(workspace)) return PPO_ERR_WORKSPACE;
+  const bool aligned = aligned16(x) && aligned16(wg) && aligned16(wu);
+  const BackwardPlan b = plan_backward(dtype, M, D, F, aligned, (char*)workspace);
+  if (!workspace || workspace_bytes < ppo_layer_gated_backward_workspace_bytes(dtype, M, D, F) ||
+      !aligned16(workspace))
+    return PPO_ERR_WORKSPACE;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   return with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
@@ -365,38 +354,43 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
     int st;
     if (!dx && !dwg && !dbg) return (int)PPO_OK;
     hipLaunchKernelGGL((gated_grad_kernel<T>),
-                       dim3((unsigned)div_up(M, kTr), (unsigned)div_up(F, kTr)), dim3(256), 0,
-                       stream, (const T*)dh, saved, M, (int)F, (int)F4, activation, drop_of(drop),
-                       dx ? (T*)b.dgu : nullptr, b.fp, dwg ? (T*)b.dgu_t : nullptr, b.mp,
-                       dbg ? (float*)b.sums : nullptr);
+                       dim3((unsigned)div_up(M, kTileM), (unsigned)div_up(b.fp, kTileF)), dim3(256),
+                       0, stream, (const T*)dh, saved, M, (int)F, (int)F4, activation,
+                       drop_of(drop), (T*)b.dgu, b.fp, dbg ? (float*)b.sums : nullptr);
     if ((st = last_launch_status())) return st;
     if (dbg) {
       hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)div_up(2 * F, 64)), dim3(256), 0,
-                         stream, (const float*)b.sums, div_up(M, kTr), (int)F, (T*)dbg, (T*)dbu);
+                         stream, (const float*)b.sums, div_up(M, kTileM), (int)F, (T*)dbg, (T*)dbu);
       if ((st = last_launch_status())) return st;
     }
-    if (dx) {
-      transpose<T>(wg, F, D, b.w_t, 2 * b.fp, b.fp, stream);
-      transpose<T>(wu, F, D, b.w_t + b.fp * size, 2 * b.fp, b.fp, stream);
-      GemmArgs a = {};
-      a.x = b.dgu;
-      a.w0 = b.w_t;
-      a.xpitch = a.wpitch = a.kbytes = 2 * b.fp * size;
-      a.M = (int)M;
-      a.N = (int)D;
-      const StoreEpi<T> epi = {(T*)dx, nullptr, (int)M, (int)D};
-      if ((st = launch_gemm<T>(a, epi, b.partial, stream))) return st;
+    GemmArgs a = {};
+    a.N = (int)D;
+    a.wpitch = D * size;
+    if (b.pad) {
+      if (dwg) pad_rows<T>(x, M, D, b.x, b.pitch, stream);
+      if (dx) pad_rows<T>(wg, F, D, b.wg, b.pitch, stream);
+      if (dx) pad_rows<T>(wu, F, D, b.wu, b.pitch, stream);
+      a.wpitch = b.pitch;
     }
-    if (dwg) {
-      transpose<T>(x, M, D, b.x_t, b.mp, b.mp, stream);
-      GemmArgs a = {};
-      a.x = b.dgu_t;
-      a.w0 = b.x_t;
-      a.xpitch = a.wpitch = a.kbytes = b.mp * size;
-      a.M = (int)(2 * F);
-      a.N = (int)D;
-      const StoreEpi<T> epi = {(T*)dwg, (T*)dwu, (int)F, (int)D};
-      if ((st = launch_gemm<T>(a, epi, b.partial, stream))) return st;
+    a.x = b.dgu;
+    a.xpitch = 2 * b.fp * size;
+    if (dx) {  // [dg | du] [wg; wu], the weights as they lie: k-rows of D columns
+      a.w0 = b.pad ? b.wg : (const char*)wg;
+      a.w1 = b.pad ? b.wu : (const char*)wu;
+      a.M = (int)M;
+      a.kbytes = a.x_range = b.fp * size;
+      a.k = F;
+      a.ranges = 2;
+      const StoreEpi<T> epi = {(T*)dx, nullptr, (int)M, (int)M, (int)D};
+      if ((st = launch_gemm<T, false, true>(a, epi, b.partial, stream))) return st;
+    }
+    if (dwg) {  // [dg | du]^T x: both operands by their rows m
+      a.w0 = b.pad ? b.x : (const char*)x;
+      a.M = (int)(2 * b.fp);
+      a.k = M;
+      a.ranges = 1;
+      const StoreEpi<T> epi = {(T*)dwg, (T*)dwu, (int)F, (int)b.fp, (int)D};
+      if ((st = launch_gemm<T, true, true>(a, epi, b.partial, stream))) return st;
     }
     return (int)PPO_OK;
   });

@@ -1,7 +1,8 @@
 // The matrix product under the layer operators: C[m,n] = sum_k X[m,k] W[n,k]
-// on the matrix cores, for rows of fp32, bf16, fp16 or int8 that are
-// contiguous along k, with the operator's epilogue applied to the sums while
-// they are still in registers.
+// on the matrix cores, with the operator's epilogue applied to the sums.  Each
+// operand's rows are contiguous along k (fp32, bf16, fp16 or int8), or, for
+// the products of a backward pass, it is stored the other way about, k-rows of
+// consecutive m or n (not for int8).
 //
 // Everything is laid out in 16-byte chunks of a row: 4 fp32, 8 16-bit or 16
 // int8 elements.  A lane of the matrix instructions below holds one chunk of
@@ -20,6 +21,11 @@
 // descriptor ends with the operand's last row and lanes past the end of a row
 // ask for an offset behind it: the hardware gives zero for both, so partial
 // tiles need no other path.
+//
+// An operand stored by k-rows is kept that way in LDS (nothing is transposed
+// in memory) and turned while it is read: 16-bit fragments by the transposing
+// LDS read, in which sixteen lanes fetch four k-rows of sixteen columns and
+// each receives one column's four values; fp32 by single words.
 #pragma once
 
 #include <type_traits>
@@ -34,6 +40,9 @@ struct GemmArgs {
   const char* w1;   // second matrix of a gated product, [N] rows
   int64_t xpitch, wpitch;  // bytes, multiples of 16
   int64_t kbytes;   // of a row, a multiple of 16
+  int64_t k;        // k-rows of an operand that is stored by them
+  int ranges;       // 2: K is two ranges of kbytes and k; W's second is w1, X's
+  int64_t x_range;  //    x_range bytes behind its first
   int M, N;         // N: output columns
   int tiles_m, tiles_n;
   int steps_per_split;     // K steps that one split takes
@@ -116,6 +125,68 @@ __device__ __forceinline__ void lds_only_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// How one operand's tile of kRows rows of C (or columns) goes to LDS and from
+// there to fragments.  kT: stored by k-rows.
+template <class T, int kRows, int kWaves, bool kT>
+struct Side {
+  static constexpr int kSize = (int)sizeof(T);
+  static constexpr int kLoads = kRows / 8 / kWaves;       // of a wave per step
+  static constexpr int kPerLine = kRows * kSize / 16;     // chunks of a k-row (kT)
+  static constexpr int kLines = 64 / kPerLine;            // k-rows that one load covers (kT)
+  static constexpr int kSwing = kSize == 2 ? 64 : 128;    // bytes that 32 columns take (kT)
+  static_assert(!kT || (kSize >= 2 && kPerLine <= 64), "");
+
+  // where a lane's chunk of load 0 lies in memory, relative to the tile's start
+  static __device__ __forceinline__ uint32_t offset(int wave, int lane, uint32_t pitch) {
+    if (kT) return (uint32_t)(wave * kLoads * kLines + lane / kPerLine) * pitch + lane % kPerLine * 16;
+    return (uint32_t)(wave * kLoads * 8 + (lane >> 3)) * pitch;
+  }
+  static __device__ __forceinline__ uint32_t stride(uint32_t pitch) {  // from load to load
+    return (uint32_t)(kT ? kLines : 8) * pitch;
+  }
+  // k-rows k..k+3 of a fragment's columns lie 32 columns apart, so that they
+  // do not meet in one bank
+  static __device__ __forceinline__ int swing(int k) {
+    return kSize == 4 ? k >> 2 & 1 : kRows >= 128 ? k & 3 : k >> 1 & 1;
+  }
+  static __device__ __forceinline__ void put(char* tile, int wave, int lane, int i, v4i v) {
+    if (kT) {
+      const int k = (wave * kLoads + i) * kLines + lane / kPerLine, c = lane % kPerLine * 16;
+      tile += k * kRows * kSize + (c / kSwing ^ swing(k)) * kSwing + c % kSwing;
+    } else {
+      const int row8 = lane >> 3;
+      tile += (wave * kLoads + i) * 8 * kStepBytes + row8 * kStepBytes + ((lane & 7) ^ row8) * 16;
+    }
+    *reinterpret_cast<v4i*>(tile) = v;
+  }
+  // one chunk of rows (columns) 32 * block .. + 31 in phase 0..3: row lane % 32,
+  // chunk 2 * phase + lane / 32
+  static __device__ __forceinline__ v4i read(char* tile, int lane, int block, int phase) {
+    const int kq = lane >> 5;
+    if constexpr (!kT) {
+      const int r = lane & 31;
+      return *reinterpret_cast<const v4i*>(tile + (block * 32 + r) * kStepBytes +
+                                           ((phase * 2 + kq) ^ (r & 7)) * 16);
+    } else if constexpr (kSize == 2) {
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) v4s lds_v4s;
+      const int i = lane & 15, k = phase * 16 + kq * 8 + i / 4;
+      char* at = tile + k * kRows * 2 + (block ^ swing(k)) * kSwing + (lane >> 4 & 1) * 32 + i % 4 * 8;
+      struct { v4s lo, hi; } r;
+      r.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+      r.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 4 * kRows * 2));
+      return __builtin_bit_cast(v4i, r);
+    } else {
+      const int k = (phase * 2 + kq) * 4;
+      const char* at = tile + k * kRows * 4 + (block ^ swing(k)) * kSwing + (lane & 31) * 4;
+      v4i r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const int*>(at + j * kRows * 4);
+      return r;
+    }
+  }
+};
+
 constexpr uint32_t kBehind = 0x80000000u;  // an offset that no descriptor reaches
 
 // Workgroup -> tile.  Workgroups go round-robin over the eight XCDs, each
@@ -157,15 +228,16 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 // step after it take its place in the registers, a whole step ahead of their
 // use.  The workgroup meets once a step, before the last phase: by then every
 // wave has read the buffer to its end and written the other one.
-template <class T, int BM, int BN, int kWavesM, int kWavesN, class Epi>
+template <class T, int BM, int BN, int kWavesM, int kWavesN, bool kXT, bool kWT, class Epi>
 __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     gemm_tile_kernel(const GemmArgs a, const Epi epi) {
   constexpr int kWaves = kWavesM * kWavesN;
   constexpr int kEdge = 32;  // of a matrix instruction's block
   constexpr int TM = BM / kWavesM / kEdge, TN = BN / kWavesN / kEdge;
   constexpr int kPhases = 4;
-  constexpr int XL = BM / 8 / kWaves, WL = BN / 8 / kWaves;  // loads of a wave per step
-  constexpr int kLoads = XL + WL;
+  typedef Side<T, BM, kWaves, kXT> X;
+  typedef Side<T, BN, kWaves, kWT> W;
+  constexpr int kLoads = X::kLoads + W::kLoads;
   constexpr int kFrags = TM + TN, kMfmas = TM * TN;
   // steps that are on their way through registers: two where they fit
   constexpr int kAhead = BM * BN >= 256 * 256 ? 1 : 2;
@@ -173,7 +245,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   constexpr int kCols = kGated ? BN / 2 : BN;  // output columns of a tile
   constexpr int kBuffer = (BM + BN) * kStepBytes;
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "");
-  static_assert(!kGated || TN % 2 == 0, "");
+  static_assert(!kGated || (TN % 2 == 0 && !kWT), "");
   __shared__ __align__(1024) char lds[2][kBuffer];
 
   const int lane = threadIdx.x & 63;
@@ -182,56 +254,73 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   int tm, tn;
   tile_of(a, tm, tn);
   const int m0 = tm * BM, n0 = tn * kCols;
-  const int steps = (int)div_up(a.kbytes, kStepBytes);
+  constexpr int kStepK = kStepBytes / (int)sizeof(T);
+  const int per_range = (int)(kXT ? div_up(a.k, kStepK) : div_up(a.kbytes, kStepBytes));
+  const int steps = per_range * a.ranges;
   const int first = blockIdx.y * a.steps_per_split;
   const int count = max(0, min(steps - first, a.steps_per_split));
 
   // --- loads ------------------------------------------------------------------------
-  const int row8 = lane >> 3;
   const uint32_t xp = (uint32_t)a.xpitch, wp = (uint32_t)a.wpitch;
-  const auto bx = buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
+  const uint32_t x_off = X::offset(wave, lane, xp);
+  const uint32_t w_off = kWT || !kGated ? W::offset(wave, lane, wp) : (uint32_t)(lane >> 3) * wp;
+  typedef __amdgpu_buffer_rsrc_t Buffer;
+  // one operand's source for a step: an operand of k-contiguous rows has one
+  // descriptor and a moving offset, one of k-rows a descriptor per step
+  struct Source { Buffer b0, b1; uint32_t off; };
   const uint32_t w_bytes = (uint32_t)min(kCols, a.N - n0) * wp;
-  const auto bw0 = buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
-  const auto bw1 = buffer_of((kGated ? a.w1 : a.w0) + n0 * a.wpitch, w_bytes);
-  const uint32_t x_off = (uint32_t)(wave * XL * 8 + row8) * xp, w_off = (uint32_t)row8 * wp;
-  // load i of a step (X's first): eight rows
-  auto load = [&](int i, uint32_t k_off) -> v4i {
-    if (i < XL) return load16(bx, x_off + (uint32_t)(i * 8) * xp + k_off);
-    const int j = (wave * WL + i - XL) * 8;  // first of the eight LDS rows
-    int col = j;
-    bool second = false;
-    if (kGated) {  // a wave's columns: half from the first matrix, half from the second
-      constexpr int kSpan = TN * kEdge, kHalf = kSpan / 2;
-      second = j % kSpan >= kHalf;
-      col = j / kSpan * kHalf + j % kHalf;
-    }
-    return load16(second ? bw1 : bw0, w_off + (uint32_t)col * wp + k_off);
+  const Buffer bx = kXT ? buffer_of(a.x, 0)
+                        : buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
+  const Buffer bw0 = kWT ? bx : buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
+  const Buffer bw1 = kGated ? buffer_of(a.w1 + n0 * a.wpitch, w_bytes) : bw0;
+  auto by_rows = [&](const char* base, int64_t pitch, int64_t col_bytes, int local, bool live) {
+    const int64_t k0 = (int64_t)local * kStepK;
+    const int64_t left = live ? (a.k - k0) * pitch - col_bytes : 0;
+    return buffer_of(base + k0 * pitch + col_bytes,
+                     (uint32_t)max((int64_t)0, min(left, (int64_t)0x7fffffff)));
   };
   // steps past the last ask for nothing
-  auto k_offset = [&](int step) {
-    const uint32_t kb = (uint32_t)(first + step) * kStepBytes + (lane & 7) * 16;
-    return step < count && kb < (uint32_t)a.kbytes ? kb : kBehind;
+  auto source = [&](int step, Source& x, Source& w) {
+    const bool live = step < count;
+    const int at = first + step;
+    const int range = at >= per_range && a.ranges > 1, local = at - (range ? per_range : 0);
+    const uint32_t kb = (uint32_t)local * kStepBytes + (lane & 7) * 16;
+    const uint32_t k_off = live && kb < (uint32_t)a.kbytes ? kb : kBehind;
+    x = {bx, bx, k_off + (uint32_t)(range ? a.x_range : 0)};
+    w = {bw0, bw1, k_off};
+    if (kXT) x.off = 0, x.b0 = by_rows(a.x, a.xpitch, (int64_t)m0 * (int)sizeof(T), local, live);
+    if (kWT)
+      w.off = 0, w.b0 = by_rows(range ? a.w1 : a.w0, a.wpitch, (int64_t)n0 * (int)sizeof(T), local,
+                                live);
   };
-  const int put_at = row8 * kStepBytes + ((lane & 7) ^ row8) * 16;
+  // load i of a step (X's first)
+  auto load = [&](int i, const Source& x, const Source& w) -> v4i {
+    if (i < X::kLoads) return load16(x.b0, x_off + (uint32_t)i * X::stride(xp) + x.off);
+    const int iw = i - X::kLoads;
+    if (!kGated) return load16(w.b0, w_off + (uint32_t)iw * W::stride(wp) + w.off);
+    // a wave's columns: half from the first matrix, half from the second
+    constexpr int kSpan = TN * kEdge, kHalf = kSpan / 2;
+    const int j = (wave * W::kLoads + iw) * 8;  // first of the eight LDS rows
+    const int col = j / kSpan * kHalf + j % kHalf;
+    return load16(j % kSpan >= kHalf ? w.b1 : w.b0, w_off + (uint32_t)col * wp + w.off);
+  };
   auto put = [&](int i, v4i v, char* buf) {
-    const int row = i < XL ? (wave * XL + i) * 8 : BM + (wave * WL + i - XL) * 8;
-    *reinterpret_cast<v4i*>(buf + row * kStepBytes + put_at) = v;
+    if (i < X::kLoads)
+      X::put(buf, wave, lane, i, v);
+    else
+      W::put(buf + BM * kStepBytes, wave, lane, i - X::kLoads, v);
   };
 
   // --- fragments --------------------------------------------------------------------
   const int r = lane & (kEdge - 1), kq = lane / kEdge;
-  const int x_at = (wm * TM * kEdge + r) * kStepBytes;
-  const int w_at = (BM + wn * TN * kEdge + r) * kStepBytes;
   struct Frags { v4i w[TN], x[TM]; };
   Frags f[2];
   // fragment g of a phase: W's first
-  auto read = [&](Frags& to, int g, const char* buf, int phase) {
-    const int slot = ((phase * 2 + kq) ^ (r & 7)) * 16;
+  auto read = [&](Frags& to, int g, char* buf, int phase) {
     if (g < TN)
-      to.w[g] = *reinterpret_cast<const v4i*>(buf + w_at + g * kEdge * kStepBytes + slot);
+      to.w[g] = W::read(buf + BM * kStepBytes, lane, wn * TN + g, phase);
     else
-      to.x[g - TN] =
-          *reinterpret_cast<const v4i*>(buf + x_at + (g - TN) * kEdge * kStepBytes + slot);
+      to.x[g - TN] = X::read(buf, lane, wm * TM + g - TN, phase);
   };
 
   Acc<T, kEdge> acc[TM][TN];
@@ -246,7 +335,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   // The matrix instructions of a phase in their order; behind each goes what it
   // is to cover: the reads behind the first of every pair, the rest (`other`,
   // called with the share of the phase that is over) behind the second.
-  auto phase = [&](const Frags& from, Frags& to, const char* buf, int p, auto&& other) {
+  auto phase = [&](const Frags& from, Frags& to, char* buf, int p, auto&& other) {
 #pragma unroll
     for (int e = 0; e < kMfmas; ++e) {
       multiply(from, e);
@@ -264,16 +353,17 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
 
   v4i staged[kAhead][kLoads];  // the steps that go to LDS next
   {
-    const uint32_t k0 = k_offset(0);
+    Source x, w;
+    source(0, x, w);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) staged[0][i] = load(i, k0);
+    for (int i = 0; i < kLoads; ++i) staged[0][i] = load(i, x, w);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) put(i, staged[0][i], lds[0]);
 #pragma unroll
     for (int h = 0; h < kAhead; ++h) {
-      const uint32_t k_off = k_offset(h + 1);
+      source(h + 1, x, w);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) staged[h][i] = load(i, k_off);
+      for (int i = 0; i < kLoads; ++i) staged[h][i] = load(i, x, w);
     }
     lds_only_barrier();
 #pragma unroll
@@ -282,7 +372,8 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   auto one_step = [&](int step, v4i (&next)[kLoads]) {
     char* cur = lds[step & 1];
     char* other = lds[step & 1 ^ 1];
-    const uint32_t k_off = k_offset(step + 1 + kAhead);
+    Source x, w;
+    source(step + 1 + kAhead, x, w);
 #pragma unroll
     for (int p = 0; p < kPhases - 1; ++p)
       phase(f[p & 1], f[(p + 1) & 1], cur, p + 1, [&](int slot, int slots) {
@@ -290,7 +381,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
 #pragma unroll
         for (int i = at * kLoads / all; i < (at + 1) * kLoads / all; ++i) {
           put(i, next[i], other);
-          next[i] = load(i, k_off);
+          next[i] = load(i, x, w);
         }
       });
     lds_only_barrier();
@@ -508,9 +599,9 @@ constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay belo
 
 // How a product of M rows and `wrows` rows of W (both matrices of a gated one
 // together) over `kbytes` is cut.
-inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes) {
+inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool by_k_rows = false) {
   GemmPlan p = {0, 1, 0};
-  if (M <= kRowsMax) return p;
+  if (M <= kRowsMax && !by_k_rows) return p;
   const int64_t steps = div_up(kbytes, kStepBytes);
   auto tiles = [&](int64_t b) { return div_up(M, b) * div_up(wrows, b); };
   if (tiles(256) >= 200) {
@@ -532,35 +623,41 @@ inline bool gemm_fits(int64_t M, int64_t N, int64_t pitch_bytes) {
          div_up(M, 64) * div_up(N, 32) < ((int64_t)1 << 30);
 }
 
-template <class T, class Epi>
+template <class T, bool kXT = false, bool kWT = false, class Epi>
 int launch_gemm(GemmArgs a, const Epi& epi, char* partial, hipStream_t stream) {
   const int64_t wrows = (int64_t)a.N * (Epi::kGated ? 2 : 1);
-  const GemmPlan p = plan_gemm(a.M, wrows, a.kbytes);
+  if (a.ranges == 0) a.ranges = 1;
+  const int64_t kbytes = a.ranges * (kXT ? a.k * (int64_t)sizeof(T) : a.kbytes);
+  const GemmPlan p = plan_gemm(a.M, wrows, kbytes, kXT || kWT);
   a.partial = p.splits > 1 ? partial : nullptr;
-  if (p.tile == 0) {
-    const dim3 grid((unsigned)div_up(a.N, 16));
-    if (a.M <= 16)
-      hipLaunchKernelGGL((gemm_rows_kernel<T, 1, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
-    else if (a.M <= 32)
-      hipLaunchKernelGGL((gemm_rows_kernel<T, 2, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
-    else
-      hipLaunchKernelGGL((gemm_rows_kernel<T, 4, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
-    return last_launch_status();
+  if constexpr (!kXT && !kWT) {
+    if (p.tile == 0) {
+      const dim3 grid((unsigned)div_up(a.N, 16));
+      if (a.M <= 16)
+        hipLaunchKernelGGL((gemm_rows_kernel<T, 1, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
+      else if (a.M <= 32)
+        hipLaunchKernelGGL((gemm_rows_kernel<T, 2, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
+      else
+        hipLaunchKernelGGL((gemm_rows_kernel<T, 4, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
+      return last_launch_status();
+    }
   }
-  a.steps_per_split = (int)div_up(div_up(a.kbytes, kStepBytes), p.splits);
+  const int64_t range_steps = kXT ? div_up(a.k, kStepBytes / (int)sizeof(T))
+                                  : div_up(a.kbytes, kStepBytes);
+  a.steps_per_split = (int)div_up(range_steps * a.ranges, p.splits);
   const int cols = Epi::kGated ? p.tile / 2 : p.tile;
   a.tiles_m = (int)div_up(a.M, p.tile);
   a.tiles_n = (int)div_up(a.N, cols);
   const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)p.splits);
   if (p.tile == 256)
-    hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 2, Epi>), grid, dim3(256), 0, stream, a,
-                       epi);
+    hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 2, kXT, kWT, Epi>), grid, dim3(256), 0,
+                       stream, a, epi);
   else if (p.tile == 128)
-    hipLaunchKernelGGL((gemm_tile_kernel<T, 128, 128, 2, 2, Epi>), grid, dim3(256), 0, stream, a,
-                       epi);
+    hipLaunchKernelGGL((gemm_tile_kernel<T, 128, 128, 2, 2, kXT, kWT, Epi>), grid, dim3(256), 0,
+                       stream, a, epi);
   else
-    hipLaunchKernelGGL((gemm_tile_kernel<T, 64, 64, 2, 1, Epi>), grid, dim3(128), 0, stream, a,
-                       epi);
+    hipLaunchKernelGGL((gemm_tile_kernel<T, 64, 64, 2, 1, kXT, kWT, Epi>), grid, dim3(128), 0,
+                       stream, a, epi);
   if (p.splits > 1) {
     const int64_t n = (int64_t)a.M * div_up(a.N, 4);
     hipLaunchKernelGGL((gemm_join_kernel<T, Epi>), dim3((unsigned)div_up(n, 256)), dim3(256), 0,
