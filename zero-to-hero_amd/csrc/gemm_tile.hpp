@@ -15,12 +15,15 @@
 //
 // A workgroup computes a BM x BN tile over K steps of 128 bytes, a whole line
 // of memory per row (half lines were fetched twice: 1127 against 988 us for
-// 8192 x 4096 x 16384 in bf16).  The tiles pass through registers into one of
-// two LDS buffers.  A row's chunk c sits in slot c ^ (row % 8), which spreads
-// the rows that a fragment read touches over all banks.  The buffer
-// descriptor ends with the operand's last row and lanes past the end of a row
-// ask for an offset behind it: the hardware gives zero for both, so partial
-// tiles need no other path.
+// 8192 x 4096 x 16384 in bf16).  The tiles go from memory to one of two LDS
+// buffers without passing through registers (buffer loads with the LDS bit: 64
+// lanes, 16 bytes each, to consecutive LDS addresses; through registers the
+// LDS writes cost 5 to 8% of 8192 x 8192 x 4096).  A row's chunk c sits in slot
+// c ^ (row % 8), which spreads the rows that a fragment read touches over all
+// banks; since the LDS side of the load is fixed, the lanes permute the
+// addresses they load from instead.  The buffer descriptor ends with the
+// operand's last row and lanes past the end of a row ask for an offset behind
+// it: the hardware gives zero for both, so partial tiles need no other path.
 //
 // An operand stored by k-rows is kept that way in LDS (nothing is transposed
 // in memory) and turned while it is read: 16-bit fragments by the transposing
@@ -111,18 +114,31 @@ __device__ __forceinline__ Acc<T> four(const Acc<T, kEdge>& c, int group) {
 }
 
 // Descriptor of `bytes` (below 2^31) from p on; loads behind it give zero.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const char* p, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)bytes, 0x00020000);
+__device__ __forceinline__ v4i buffer_of(const char* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  v4i r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff);
+  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
+  r[3] = 0x00020000;
+  return r;
 }
 
-__device__ __forceinline__ v4i load16(__amdgpu_buffer_rsrc_t buffer, uint32_t offset) {
-  return __builtin_amdgcn_raw_buffer_load_b128(buffer, (int)offset, 0, 0);
+// 64 lanes, 16 bytes each from buffer + offset, to LDS at lds + 16 * lane
+// (`lds` is the same in all lanes).  Nothing in registers is written; the
+// data has arrived after a barrier below that waits for it.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, v4i buffer, uint32_t offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer));
 }
 
-// Waits for this wave's LDS reads and writes, then for the whole workgroup;
-// loads from memory stay under way.
-__device__ __forceinline__ void lds_only_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// Waits until at most kLeft of this wave's loads are under way, and for its
+// LDS reads, then for the whole workgroup.
+template <int kLeft>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
 // How one operand's tile of kRows rows of C (or columns) goes to LDS and from
@@ -136,11 +152,6 @@ struct Side {
   static constexpr int kSwing = kSize == 2 ? 64 : 128;    // bytes that 32 columns take (kT)
   static_assert(!kT || (kSize >= 2 && kPerLine <= 64), "");
 
-  // where a lane's chunk of load 0 lies in memory, relative to the tile's start
-  static __device__ __forceinline__ uint32_t offset(int wave, int lane, uint32_t pitch) {
-    if (kT) return (uint32_t)(wave * kLoads * kLines + lane / kPerLine) * pitch + lane % kPerLine * 16;
-    return (uint32_t)(wave * kLoads * 8 + (lane >> 3)) * pitch;
-  }
   static __device__ __forceinline__ uint32_t stride(uint32_t pitch) {  // from load to load
     return (uint32_t)(kT ? kLines : 8) * pitch;
   }
@@ -149,15 +160,17 @@ struct Side {
   static __device__ __forceinline__ int swing(int k) {
     return kSize == 4 ? k >> 2 & 1 : kRows >= 128 ? k & 3 : k >> 1 & 1;
   }
-  static __device__ __forceinline__ void put(char* tile, int wave, int lane, int i, v4i v) {
+  // what a lane fetches with load i, relative to the tile's start: its place
+  // in LDS is fixed (16 * lane), so the lanes permute what they ask for
+  static __device__ __forceinline__ uint32_t offset(int wave, int lane, int i, uint32_t pitch) {
     if (kT) {
       const int k = (wave * kLoads + i) * kLines + lane / kPerLine, c = lane % kPerLine * 16;
-      tile += k * kRows * kSize + (c / kSwing ^ swing(k)) * kSwing + c % kSwing;
-    } else {
-      const int row8 = lane >> 3;
-      tile += (wave * kLoads + i) * 8 * kStepBytes + row8 * kStepBytes + ((lane & 7) ^ row8) * 16;
+      return (uint32_t)k * pitch + (uint32_t)((c / kSwing ^ swing(k)) * kSwing + c % kSwing);
     }
-    *reinterpret_cast<v4i*>(tile) = v;
+    return (uint32_t)((wave * kLoads + i) * 8 + (lane >> 3)) * pitch;
+  }
+  static __device__ __forceinline__ uint32_t chunk(int lane) {  // (not kT) within a step
+    return (uint32_t)((lane & 7) ^ (lane >> 3)) * 16;
   }
   // one chunk of rows (columns) 32 * block .. + 31 in phase 0..3: row lane % 32,
   // chunk 2 * phase + lane / 32
@@ -223,11 +236,12 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 //
 // A step is four phases, each one 16-byte chunk per lane of every fragment.
 // While the matrix cores work on one phase, the fragments of the next are read
-// from LDS, one read to every few matrix instructions; between them the next
-// step's data goes from registers to the other buffer and the loads of the
-// step after it take its place in the registers, a whole step ahead of their
-// use.  The workgroup meets once a step, before the last phase: by then every
-// wave has read the buffer to its end and written the other one.
+// from LDS, a read or a load in the shadow of each matrix instruction.  The
+// workgroup meets once a step, before the last phase: every wave has then read
+// the buffer to its end and the other buffer's loads have arrived.  The loads
+// of the step after next go into the freed buffer during the last phase and
+// the first of the next step (issued at once they hold up the instructions
+// behind them; later they arrive late).
 template <class T, int BM, int BN, int kWavesM, int kWavesN, bool kXT, bool kWT, class Epi>
 __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     gemm_tile_kernel(const GemmArgs a, const Epi epi) {
@@ -239,8 +253,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   typedef Side<T, BN, kWaves, kWT> W;
   constexpr int kLoads = X::kLoads + W::kLoads;
   constexpr int kFrags = TM + TN, kMfmas = TM * TN;
-  // steps that are on their way through registers: two where they fit
-  constexpr int kAhead = BM * BN >= 256 * 256 ? 1 : 2;
+  constexpr int kEarly = kLoads / 2;  // loads of a step in the last phase before it
   constexpr bool kGated = Epi::kGated;
   constexpr int kCols = kGated ? BN / 2 : BN;  // output columns of a tile
   constexpr int kBuffer = (BM + BN) * kStepBytes;
@@ -262,9 +275,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
 
   // --- loads ------------------------------------------------------------------------
   const uint32_t xp = (uint32_t)a.xpitch, wp = (uint32_t)a.wpitch;
-  const uint32_t x_off = X::offset(wave, lane, xp);
-  const uint32_t w_off = kWT || !kGated ? W::offset(wave, lane, wp) : (uint32_t)(lane >> 3) * wp;
-  typedef __amdgpu_buffer_rsrc_t Buffer;
+  typedef v4i Buffer;
   // one operand's source for a step: an operand of k-contiguous rows has one
   // descriptor and a moving offset, one of k-rows a descriptor per step
   struct Source { Buffer b0, b1; uint32_t off; };
@@ -284,7 +295,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     const bool live = step < count;
     const int at = first + step;
     const int range = at >= per_range && a.ranges > 1, local = at - (range ? per_range : 0);
-    const uint32_t kb = (uint32_t)local * kStepBytes + (lane & 7) * 16;
+    const uint32_t kb = (uint32_t)local * kStepBytes + X::chunk(lane);
     const uint32_t k_off = live && kb < (uint32_t)a.kbytes ? kb : kBehind;
     x = {bx, bx, k_off + (uint32_t)(range ? a.x_range : 0)};
     w = {bw0, bw1, k_off};
@@ -293,22 +304,21 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
       w.off = 0, w.b0 = by_rows(range ? a.w1 : a.w0, a.wpitch, (int64_t)n0 * (int)sizeof(T), local,
                                 live);
   };
+  const uint32_t lds0 =
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
   // load i of a step (X's first)
-  auto load = [&](int i, const Source& x, const Source& w) -> v4i {
-    if (i < X::kLoads) return load16(x.b0, x_off + (uint32_t)i * X::stride(xp) + x.off);
+  auto load = [&](int i, int buf, const Source& x, const Source& w) {
+    const uint32_t to = lds0 + buf * kBuffer + (i < X::kLoads ? (wave * X::kLoads + i) * 1024
+                        : BM * kStepBytes + (wave * W::kLoads + i - X::kLoads) * 1024);
+    if (i < X::kLoads) return load_to_lds(to, x.b0, X::offset(wave, lane, i, xp) + x.off);
     const int iw = i - X::kLoads;
-    if (!kGated) return load16(w.b0, w_off + (uint32_t)iw * W::stride(wp) + w.off);
+    if (!kGated) return load_to_lds(to, w.b0, W::offset(wave, lane, iw, wp) + w.off);
     // a wave's columns: half from the first matrix, half from the second
     constexpr int kSpan = TN * kEdge, kHalf = kSpan / 2;
     const int j = (wave * W::kLoads + iw) * 8;  // first of the eight LDS rows
     const int col = j / kSpan * kHalf + j % kHalf;
-    return load16(j % kSpan >= kHalf ? w.b1 : w.b0, w_off + (uint32_t)col * wp + w.off);
-  };
-  auto put = [&](int i, v4i v, char* buf) {
-    if (i < X::kLoads)
-      X::put(buf, wave, lane, i, v);
-    else
-      W::put(buf + BM * kStepBytes, wave, lane, i - X::kLoads, v);
+    load_to_lds(to, j % kSpan >= kHalf ? w.b1 : w.b0,
+                (uint32_t)(col + (lane >> 3)) * wp + w.off);
   };
 
   // --- fragments --------------------------------------------------------------------
@@ -351,48 +361,39 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     }
   };
 
-  v4i staged[kAhead][kLoads];  // the steps that go to LDS next
+  Source x, w;
   {
-    Source x, w;
     source(0, x, w);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) staged[0][i] = load(i, x, w);
+    for (int i = 0; i < kLoads; ++i) load(i, 0, x, w);
+    source(1, x, w);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) put(i, staged[0][i], lds[0]);
-#pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
-      source(h + 1, x, w);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) staged[h][i] = load(i, x, w);
-    }
-    lds_only_barrier();
+    for (int i = 0; i < kEarly; ++i) load(i, 1, x, w);
+    stage_barrier<kEarly>();
 #pragma unroll
     for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[0], 0);
   }
-  auto one_step = [&](int step, v4i (&next)[kLoads]) {
-    char* cur = lds[step & 1];
-    char* other = lds[step & 1 ^ 1];
-    Source x, w;
-    source(step + 1 + kAhead, x, w);
+  for (int step = 0; step < count; ++step) {
+    const int b = step & 1;
+    char* cur = lds[b];
+    char* other = lds[b ^ 1];
 #pragma unroll
     for (int p = 0; p < kPhases - 1; ++p)
       phase(f[p & 1], f[(p + 1) & 1], cur, p + 1, [&](int slot, int slots) {
-        const int at = p * slots + slot, all = (kPhases - 1) * slots;
+        if (p > 0) return;
+        constexpr int kRest = kLoads - kEarly;
 #pragma unroll
-        for (int i = at * kLoads / all; i < (at + 1) * kLoads / all; ++i) {
-          put(i, next[i], other);
-          next[i] = load(i, x, w);
-        }
+        for (int i = slot * kRest / slots; i < (slot + 1) * kRest / slots; ++i)
+          load(kEarly + i, b ^ 1, x, w);
       });
-    lds_only_barrier();
-    phase(f[1], f[0], other, 0, [](int, int) {});
-  };
-  for (int step = 0; step < count; step += kAhead) {
+    stage_barrier<0>();
+    source(step + 2, x, w);
+    phase(f[1], f[0], other, 0, [&](int slot, int slots) {
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h)
-      if (h == 0 || step + h < count) one_step(step + h, staged[h]);
+      for (int i = slot * kEarly / slots; i < (slot + 1) * kEarly / slots; ++i) load(i, b, x, w);
+    });
   }
-  lds_only_barrier();  // (the last phase has read ahead in what the epilogue overwrites)
+  stage_barrier<0>();  // (the last loads and reads are ahead in what the epilogue overwrites)
 
   // --- epilogue ---------------------------------------------------------------------
   // Through LDS, 32 rows of the wave's block at a time: a lane then holds
