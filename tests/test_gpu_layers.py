@@ -28,6 +28,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import ppo_amd
 from oracle import layers_oracle as ref
@@ -152,12 +153,14 @@ def test_dropout_refusals(dev):
         ppo_amd.dropout(torch.ones((), device=dev), 0.5, 1)
 
 
-def test_dropout_second_derivative_is_refused(dev):
-    x = torch.ones(4, 6, device=dev, requires_grad=True)
+def test_dropout_second_derivative(dev):
+    """d/dx of sum(y^2) is 2 up mask y; its own derivative 2 (up mask)^2."""
+    x = torch.randn(40, 6, device=dev, requires_grad=True)
     y = ppo_amd.dropout(x, 0.5, 1)
     (dx,) = torch.autograd.grad((y * y).sum(), [x], create_graph=True)
-    with pytest.raises(RuntimeError):
-        dx.sum().backward()
+    (ddx,) = torch.autograd.grad(dx.sum(), [x])
+    keep = torch.from_numpy(ref.keep_mask(0.5, 1, np.arange(40), 6)).to(dev)
+    assert torch.equal(ddx, torch.where(keep, 8.0, 0.0))
 
 
 # --- 8 bits ------------------------------------------------------------------------------------
@@ -506,15 +509,102 @@ def test_gated_refusals(dev):
     with pytest.raises(RuntimeError):
         f(x, w.cpu(), w)
     y = x.clone().requires_grad_()
-    (dx,) = torch.autograd.grad((f(y, w, w) ** 2).sum(), [y], create_graph=True)
-    with pytest.raises(RuntimeError):
-        dx.sum().backward()
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad((f(y, w, w) ** 2).sum(), [y], create_graph=True)
     # a row-id tensor changed before the backward pass is noticed
     rows = torch.arange(4, device=dev)
     h = f(y, w, w, dropout_p=0.5, rows=rows)
     rows += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+# --- the native host path ----------------------------------------------------------------
+
+class _Declines:
+    """A native host path that takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_python_path_gives_the_same_bits(dev, monkeypatch):
+    """Calls that the native host path declines run through Python's checks and
+    autograd functions: the same launches, the same bits."""
+    x, wg, wu, bg, bu, dh = gated_case("bf16", 50, 24, 37, True)
+    dh, rows = dh.to(dev), torch.randperm(50, device=dev)
+    seeds = (5, torch.tensor([5], dtype=torch.int64, device=dev))
+
+    def run():
+        out = []
+        for seed in seeds:
+            leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+            h = ppo_amd.gated_ffn(*leaves, dropout_p=0.2, seed=seed, rows=rows)
+            z = ppo_amd.dropout(h, 0.3, seed)
+            out += [z.detach(), *torch.autograd.grad(z, leaves, dh)]
+            q, s = ppo_amd.quantize_rows(leaves[1].detach())
+            out += [q, s, ppo_amd.int8_linear(leaves[0].detach(), q, s)]
+            xq, xs = ppo_amd.quantize_rows(leaves[0].detach())
+            out.append(ppo_amd.int8_linear(xq, q, s, leaves[3].detach(), xs, torch.bfloat16))
+            with torch.no_grad():
+                out += [ppo_amd.gated_ffn(*leaves), ppo_amd.dropout(h, 0.3, seed)]
+        y = x[:0].to(dev).requires_grad_()
+        out += [ppo_amd.dropout(y, 0.5, 1).detach(), ppo_amd.gated_ffn(y, *leaves[1:3]).detach()]
+        return out
+
+    native = run()
+    monkeypatch.setattr(ppo_amd.layers, "_native", _Declines)
+    python = run()
+    assert len(native) == len(python)
+    assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(native, python))
+    # and the Python path's own second derivatives
+    t = torch.randn(40, 6, device=dev, requires_grad=True)
+    y = ppo_amd.dropout(t, 0.5, 1)
+    (dt,) = torch.autograd.grad((y * y).sum(), [t], create_graph=True)
+    (ddt,) = torch.autograd.grad(dt.sum(), [t])
+    assert set(ddt.unique().tolist()) == {0.0, 8.0}
+    w = torch.randn(5, 6, device=dev)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad((ppo_amd.gated_ffn(t, w, w) ** 2).sum(), [t], create_graph=True)
+
+
+def test_saved_tensor_hooks_and_checkpoints(dev):
+    """Saved tensors that come back from the host, and a recomputed forward."""
+    x, wg, wu, bg, bu, dh = gated_case("fp32", 30, 24, 36, True)
+    dh = dh.to(dev)
+
+    def grads(wrap):
+        leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+        rows = torch.arange(30, device=dev)
+        f = lambda *a: ppo_amd.dropout(  # noqa: E731
+            ppo_amd.gated_ffn(*a, dropout_p=0.2, seed=4, rows=rows), 0.1, 9)
+        return torch.autograd.grad(wrap(f, leaves), leaves, dh)
+
+    def on_host(f, leaves):
+        with torch.autograd.graph.save_on_cpu():
+            return f(*leaves)
+
+    def again(f, leaves):
+        return torch.utils.checkpoint.checkpoint(f, *leaves, use_reentrant=False)
+
+    want = grads(lambda f, leaves: f(*leaves))
+    for wrap in (on_host, again):
+        assert all(torch.equal(a, b) for a, b in zip(want, grads(wrap)))
+
+
+def test_forward_mode_and_batched_gradients_are_refused(dev):
+    """No silent zeros for what the operators do not offer."""
+    import torch.autograd.forward_ad as fwad
+
+    x, w = torch.randn(4, 8, device=dev), torch.randn(6, 8, device=dev)
+    for f in (lambda t: ppo_amd.dropout(t, 0.5, 1), lambda t: ppo_amd.gated_ffn(t, w, w)):
+        with fwad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+            f(fwad.make_dual(x.clone().requires_grad_(), torch.ones_like(x)))
+        y = x.clone().requires_grad_()
+        out = f(y)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out, [y], torch.ones(2, *out.shape, device=dev),
+                                is_grads_batched=True)
 
 
 # --- streams, graphs ---------------------------------------------------------------------------
@@ -619,7 +709,7 @@ def test_rows_give_an_update_its_acting_masks(dev):
     ppo_amd.check_waits(dev)
     # without them the masks are others'
     other = torch.log_softmax(policy(o), 1).gather(1, take(acts).long()[:, None]).squeeze(1)
-    assert float((other - take(logp)).abs().max()) > 1e-2
+    assert float((other.detach() - take(logp)).abs().max()) > 1e-2
 
 
 @pytest.mark.parametrize("graphs", [False, True])

@@ -13,112 +13,17 @@
 // gae_normalize T x N = 128 x 8 25.3 and 16.5; the categorical loss with its
 // backward, B = 100,003, A = 4, 94 and 52; the Gaussian one, B = 2,097,152, D = 6,
 // 102 and 56; action selection for 4096 environments 42.4 and 7.5.
-#include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/SavedTensorHooks.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Device.h>
-#include <torch/csrc/Generator.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/graph_task.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include "ppo_amd.h"
+#include "native.hpp"
 #include "scale.hpp"
+
+namespace ppo_native {
+Python P;
+extern PyMethodDef kLayerMethods[];  // native_layers.cpp
+}  // namespace ppo_native
 
 namespace {
 
-namespace py = pybind11;
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// What init() hands over: the workspace pool, the LossStats class, the function
-// that raises for a library error code, and torch.nn's classes.
-struct Python {
-  PyObject* pool = nullptr;
-  PyObject* stats = nullptr;
-  PyObject* fail = nullptr;
-  PyObject *sequential = nullptr, *linear = nullptr, *relu = nullptr, *tanh = nullptr;
-  PyObject* scalar_names[PPO_NUM_SCALARS] = {};
-  PyObject *get = nullptr, *modules = nullptr, *parameters = nullptr, *net = nullptr,
-           *weight = nullptr, *bias = nullptr, *in_features = nullptr, *out_features = nullptr;
-} P;
-
-// Thrown for a call that is not the ordinary one (entry clears a Python error that
-// a look at its arguments has set).
-struct NotPlain {};
-
-void need(bool ok) {
-  if (!ok) throw NotPlain{};
-}
-
-// Modes, transforms and traces that want to see torch operators or autograd
-// functions: not for this path.
-bool plain_mode() {
-  return !torch::jit::tracer::isTracing() && !at::impl::torch_function_mode_enabled() &&
-         !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
-         !c10::impl::tls_is_dispatch_key_included(
-             c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
-}
-
-void need_plain_mode() { need(plain_mode()); }
-
-// Keys of tensors that stand for another tensor, or for none: no storage of
-// their own to read.
-constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Python, c10::DispatchKey::Batched,
-                                        c10::DispatchKey::FuncTorchBatched,
-                                        c10::DispatchKey::FuncTorchGradWrapper,
-                                        c10::DispatchKey::Functionalize,
-                                        c10::DispatchKey::Negative, c10::DispatchKey::Conjugate,
-                                        c10::DispatchKey::ZeroTensor});
-
-// A torch.Tensor (or Parameter) itself: no subclass, no wrapper, dense GPU
-// storage, contiguous.
-const Tensor& plain(PyObject* o, at::ScalarType type) {
-  need(THPVariable_CheckExact(o));
-  const Tensor& t = THPVariable_Unpack(o);
-  need(t.defined() && t.is_cuda() && t.layout() == at::kStrided &&
-       !t.key_set().has_any(kWrapped) && t.scalar_type() == type && t.is_contiguous());
-  return t;
-}
-
-const Tensor& plain(PyObject* o, at::ScalarType type, const at::Device& device) {
-  const Tensor& t = plain(o, type);
-  need(t.device() == device);
-  return t;
-}
-
-const Tensor& plain_rows(PyObject* o, const at::Device& device, int64_t n) {
-  const Tensor& t = plain(o, at::kFloat, device);
-  need(t.dim() == 1 && t.size(0) == n);
-  return t;
-}
-
-double number(PyObject* o) {
-  need(PyFloat_CheckExact(o) || PyLong_CheckExact(o));
-  const double x = PyFloat_AsDouble(o);
-  need(x != -1.0 || !PyErr_Occurred());
-  return x;
-}
-
-int64_t integer(PyObject* o) {
-  const int64_t x = PyLong_AsLongLong(o);
-  need(x != -1 || !PyErr_Occurred());
-  return x;
-}
-
-const float* in(const Tensor& t) { return t.const_data_ptr<float>(); }
-float* out(const Tensor& t) { return t.data_ptr<float>(); }
-
-void* current_stream(const at::Device& device) {
-  return c10::hip::getCurrentHIPStream(device.index()).stream();
-}
+using namespace ppo_native;
 
 // The pool's buffer for (device, stream): ops._WorkspacePool.get.
 Tensor workspace(const at::Device& device, void* stream, size_t nbytes) {
@@ -131,22 +36,6 @@ Tensor workspace(const at::Device& device, void* stream, size_t nbytes) {
   return THPVariable_Unpack(r);
 }
 
-// Allocations and the library call, outside the GIL: other Python threads run
-// while this one waits for memory or for room in a full hardware queue.
-template <typename F>
-int unlocked(F f) {
-  py::gil_scoped_release no_gil;
-  return f();
-}
-
-// Raises PPOLibraryError (ops._native_failed) for a non-zero status.
-void check(const char* name, int code, const at::Device& device, void* stream) {
-  if (code == PPO_OK) return;
-  py::object dev = py::reinterpret_steal<py::object>(THPDevice_New(device));
-  py::reinterpret_borrow<py::object>(P.fail)(name, code, dev,
-                                             reinterpret_cast<uintptr_t>(stream));
-}
-
 // Element i of a 1-D fp32 tensor as a 0-d tensor on the same storage (no
 // autograd view).
 Tensor element(const Tensor& t, int64_t i) {
@@ -155,19 +44,6 @@ Tensor element(const Tensor& t, int64_t i) {
   impl->set_sizes_contiguous(at::IntArrayRef{});
   impl->set_storage_offset(t.storage_offset() + i);
   return Tensor(std::move(impl));
-}
-
-PyObject* wrap(const Tensor& t) {
-  PyObject* o = THPVariable_Wrap(t);
-  if (!o) throw py::error_already_set();
-  return o;
-}
-
-PyObject* tuple_of(std::initializer_list<Tensor> ts) {
-  py::tuple r(ts.size());
-  size_t k = 0;
-  for (const Tensor& t : ts) PyTuple_SET_ITEM(r.ptr(), k++, wrap(t));
-  return r.release().ptr();
 }
 
 // LossStats of a [6] tensor.
@@ -640,30 +516,6 @@ PyObject* mlp_grads(PyObject* const* a) {
 
 // --- module ----------------------------------------------------------------------------
 
-template <PyObject* (*kFn)(PyObject* const*), int kArgs>
-PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != kArgs) {
-    PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
-    return nullptr;
-  }
-  try {
-    need(P.pool != nullptr);
-    need_plain_mode();
-    return kFn(args);
-  } catch (const NotPlain&) {
-    PyErr_Clear();
-    Py_RETURN_NONE;
-  } catch (py::error_already_set& e) {
-    e.restore();
-    return nullptr;
-  } catch (const std::exception&) {
-    torch::translate_exception_to_python(std::current_exception());
-    return nullptr;
-  }
-}
-
-#define PPO_ENTRY(name, fn, nargs) \
-  {name, (PyCFunction)(void (*)(void))(&entry<fn, nargs>), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     PPO_ENTRY("gae", gae, 6),
     PPO_ENTRY("gae_normalize", gae_normalize, 7),
@@ -674,7 +526,6 @@ PyMethodDef kMethods[] = {
     PPO_ENTRY("mlp_act", mlp_act, 9),
     PPO_ENTRY("mlp_grads", mlp_grads, 14),
     {nullptr, nullptr, 0, nullptr}};
-#undef PPO_ENTRY
 
 // The reference counts of a tensor with one owner in C++ (as a saved variable is)
 // and one reference to its Python object (as the tuple of saved tensors holds),
@@ -741,5 +592,6 @@ void init(py::object pool, py::object stats, py::object fail, const std::vector<
 PYBIND11_MODULE(_native, m) {
   m.def("init", &init);
   m.def("scale_grads", &scale_grads);
-  if (PyModule_AddFunctions(m.ptr(), kMethods)) throw py::error_already_set();
+  if (PyModule_AddFunctions(m.ptr(), kMethods) || PyModule_AddFunctions(m.ptr(), kLayerMethods))
+    throw py::error_already_set();
 }

@@ -27,10 +27,9 @@ from typing import Optional, Union
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _ptr, _require, _stream
+from .ops import _native, _ptr, _require, _stream
 
 __all__ = ["gated_ffn", "dropout", "quantize_rows", "int8_linear", "GatedLinear", "GatedMLP",
            "Int8Linear", "int8_copy"]
@@ -99,11 +98,11 @@ class _Dropout(torch.autograd.Function):
         return _dropout_into(x, _drop(p, seed, rows))
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         seed, rows = ctx.saved_tensors
-        drop = _drop(ctx.p, ctx.seed if seed is None else seed, rows)
-        return _dropout_into(dy.contiguous(), drop), None, None, None
+        # linear in x: its derivative is the same mask (create_graph comes again)
+        return (_Dropout.apply(dy.contiguous(), ctx.p, ctx.seed if seed is None else seed, rows),
+                None, None, None)
 
 
 def dropout(x: torch.Tensor, p: float, seed: Seed, rows: Optional[torch.Tensor] = None
@@ -120,10 +119,13 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, rows: Optional[torch.Tensor] 
     bits), or an int64 tensor of one value on x's device that is read when the
     kernel runs, so that a captured graph takes a new one per replay.
 
-    Differentiable once in x; the backward pass forms the mask again, from
-    `seed` and `rows` as they were (neither may be changed in place in
-    between).  Other than torch's, it drops infinities and NaN to 0.
+    Differentiable in x; the backward pass forms the mask again, from `seed`
+    and `rows` as they were (neither may be changed in place in between).
+    Other than torch's, it drops infinities and NaN to 0.
     """
+    got = _native().layer_dropout(x, p, seed, rows)
+    if got is not None:
+        return got
     _require(x, "x", tuple(DTYPES))
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
@@ -163,8 +165,10 @@ class _GatedFFN(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh):
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_ffn can be differentiated once: its backward pass has no "
+                               "create_graph")
         x, wg, wu, saved, seed, rows = ctx.saved_tensors
         D, F = x.shape[-1], wg.shape[0]
         M, device, dtype = x.numel() // D, x.device, DTYPES[x.dtype]
@@ -208,9 +212,14 @@ def gated_ffn(
     neither), all fp32, bf16 or fp16 alike; returns [..., F].  `activation` is
     "relu", "tanh", "silu" or "gelu" (with the error function).  The dropout
     arguments are those of dropout(), whose mask over [M, F] it applies.
-    Differentiable once in x, the weights and the biases: g and u are kept for
-    the backward pass in 32 bits (8 M F bytes), the mask is formed again.
+    Differentiable once in x, the weights and the biases (create_graph raises):
+    g and u are kept for the backward pass in 32 bits (8 M F bytes), the mask
+    is formed again.
     """
+    got = _native().layer_gated_ffn(x, w_gate, w_up, b_gate, b_up,
+                                    ACTIVATIONS.get(activation), dropout_p, seed, rows)
+    if got is not None:
+        return got
     _require(x, "x", tuple(DTYPES))
     device, dtype = x.device, (x.dtype,)
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -250,6 +259,9 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     and weight_scale.  A row of zeros has scale 0; one that holds an infinity
     or a NaN has scale NaN and q = 0, so products with it are NaN.  Not
     differentiable."""
+    got = _native().layer_quantize_rows(x)
+    if got is not None:
+        return got
     _require(x, "x", tuple(DTYPES))
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., K] with K > 0, got {tuple(x.shape)}")
@@ -280,6 +292,9 @@ def int8_linear(
     in fp32, the result rounded once to out_dtype (default: x's type; needed
     for an int8 x).  bias [N] has the result's type.  For acting: not
     differentiable, and refused for an x that requires a gradient."""
+    got = _native().layer_int8_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
+    if got is not None:
+        return got
     _require(x, "x", (*DTYPES, torch.int8))
     device = x.device
     if x.dim() < 1 or x.shape[-1] == 0:
