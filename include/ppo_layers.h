@@ -61,8 +61,8 @@ int ppo_layer_dropout(const void* x, void* y, int dtype, int64_t rows, int64_t c
                       const ppo_dropout* drop, void* stream);
 
 /*
- * 8-bit rows: scale[r] = max_c |x[r,c]| / 127 (fp32, correctly rounded) and
- * q[r,c] = x[r,c] / scale[r] rounded to the nearest integer, ties to even,
+ * 8-bit rows: scale[r] = max_c |x[r,c]| times 1/127, both in fp32, and
+ * q[r,c] = x[r,c] / scale[r] (in fp32) to the nearest integer, ties to even,
  * within [-127, 127].  A row of zeros has scale 0 and q = 0; a row that holds
  * an infinity or a NaN has scale NaN and q = 0, so that products with it are
  * NaN.

@@ -48,7 +48,8 @@ def quantize_rows(x):
     """fp32-valued x [M,K] -> (q int8, scale fp32), in 32-bit IEEE arithmetic."""
     x = np.asarray(x, dtype=np.float32)
     top = np.abs(x).max(1)
-    scale = np.where(np.isfinite(top), top / np.float32(127), np.float32(np.nan)).astype(np.float32)
+    scale = np.where(np.isfinite(top), top * (np.float32(1) / np.float32(127)),
+                     np.float32(np.nan)).astype(np.float32)
     live = scale > 0
     with np.errstate(all="ignore"):
         q = np.clip(np.rint(x / scale[:, None]), -127, 127)

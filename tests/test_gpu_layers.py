@@ -186,6 +186,19 @@ def test_quantize_rows_is_exact(dev, shape, dtype):
     assert np.array_equal(q.cpu().numpy(), wq)
 
 
+def test_quantize_rows_ties(dev):
+    """Quotients at ties and a few units in the last place to either side."""
+    k = torch.arange(-126, 127).float() + 0.5
+    rows = [torch.cat([k, torch.tensor([127.0])])]
+    for n in range(1, 4):
+        rows += [torch.nextafter(rows[-1], torch.full_like(rows[-1], 200.0)).clamp(max=127.0)]
+    rows += [r * s for r in rows for s in (0.37, 1e-3, 3e4, 1e-38, 1e30)]
+    x = torch.stack(rows)
+    q, s = ppo_amd.quantize_rows(x.to(dev))
+    wq, ws = ref.quantize_rows(x.numpy())
+    assert np.array_equal(s.cpu().numpy(), ws) and np.array_equal(q.cpu().numpy(), wq)
+
+
 def test_quantize_rows_edges(dev):
     x = torch.zeros(8, 70)
     x[0, 3] = float("inf")

@@ -254,8 +254,8 @@ def gated_ffn(
 # ---------------------------------------------------------------------------
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q int8 like x, scale fp32 [...]) of x [..., K] (fp32, bf16 or fp16):
-    scale = max |x| / 127 of each row and q = x / scale to the nearest
-    integer, ties to even.  For a weight [N, K] these are int8_linear's weight
+    scale = max |x| times 1/127 (in fp32) of each row and q = x / scale to the
+    nearest integer, ties to even.  For a weight [N, K] these are int8_linear's weight
     and weight_scale.  A row of zeros has scale 0; one that holds an infinity
     or a NaN has scale NaN and q = 0, so products with it are NaN.  Not
     differentiable."""
