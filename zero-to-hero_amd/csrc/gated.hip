@@ -15,7 +15,7 @@ namespace {
 template <class T>
 struct GatedEpi {
   static constexpr bool kGated = true;
-  static constexpr int kBatch = 1;
+  static constexpr int kBatch = 2;
   const T* bg;
   const T* bu;
   T* h;
@@ -39,25 +39,37 @@ struct GatedEpi {
   __device__ __forceinline__ Row row(int m) const {
     return drop.mode && drop.rows ? drop.rows[m] : m;
   }
-  __device__ __forceinline__ void operator()(int m, int n, const Cols& cols, Row id, v4f g,
-                                             v4f u) const {
-    const int count = F - n;
+  template <int B>
+  __device__ __forceinline__ void apply(int n, const Cols& cols, const int (&m)[B],
+                                        const bool (&live)[B], const Row (&id)[B],
+                                        const v4f (&cg)[B], const v4f (&cu)[B]) const {
+    float g[4 * B], u[4 * B], a[4 * B];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      g[i] += cols.g[i];
-      u[i] += cols.u[i];
+    for (int k = 0; k < 4 * B; ++k) {
+      g[k] = cg[k / 4][k % 4] + cols.g[k % 4];
+      u[k] = cu[k / 4][k % 4] + cols.u[k % 4];
     }
     if (saved) {
-      float* s = saved + (int64_t)m * F4 + n;
-      *reinterpret_cast<v4f*>(s) = g;
-      *reinterpret_cast<v4f*>(s + half) = u;
-    }
-    float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = activate(act, g[i]) * u[i];
-    if (drop.mode)
-      drop4(drop, dropout_seed(drop), (uint64_t)id, (uint32_t)n >> 2, v);
-    store4(h + (int64_t)m * F + n, v, count, (F & 3) == 0);
+      for (int b = 0; b < B; ++b) {
+        float* s = saved + (int64_t)m[b] * F4 + n;
+        const v4f vg = {g[4 * b], g[4 * b + 1], g[4 * b + 2], g[4 * b + 3]};
+        const v4f vu = {u[4 * b], u[4 * b + 1], u[4 * b + 2], u[4 * b + 3]};
+        if (live[b]) {
+          *reinterpret_cast<v4f*>(s) = vg;
+          *reinterpret_cast<v4f*>(s + half) = vu;
+        }
+      }
+    }
+    activate<T>(act, g, a);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[4 * b + i] * u[4 * b + i];
+      if (drop.mode) drop4(drop, dropout_seed(drop), (uint64_t)id[b], (uint32_t)n >> 2, v);
+      if (live[b]) store4(h + (int64_t)m[b] * F + n, v, F - n, (F & 3) == 0);
+    }
   }
 };
 
@@ -74,13 +86,17 @@ struct StoreEpi {
   struct Row {};
   __device__ __forceinline__ Cols columns(int) const { return {}; }
   __device__ __forceinline__ Row row(int) const { return {}; }
-  __device__ __forceinline__ void operator()(int m, int n, Cols, Row, v4f c) const {
-    T* out = out0;
-    if (m >= second) m -= second, out = out1;
-    if (m >= rows) return;
-    T* row = out + (int64_t)m * N;
-    const float v[4] = {c[0], c[1], c[2], c[3]};
-    store4(row + n, v, N - n, (N & 3) == 0);
+  template <int B>
+  __device__ __forceinline__ void apply(int n, Cols, const int (&m)[B], const bool (&live)[B],
+                                        const Row (&)[B], const v4f (&c)[B]) const {
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const bool other = m[b] >= second;
+      const int at = other ? m[b] - second : m[b];
+      const float v[4] = {c[b][0], c[b][1], c[b][2], c[b][3]};
+      if (live[b] && at < rows)
+        store4((other ? out1 : out0) + (int64_t)at * N + n, v, N - n, (N & 3) == 0);
+    }
   }
 };
 
@@ -133,13 +149,14 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
           if (n + k < F) d[k] = to_f32(dp[k]);
       }
       if (drop.mode) drop4(drop, seed, drop.rows ? drop.rows[m] : m, (uint32_t)n >> 2, d);
+      const float gs[4] = {g[0], g[1], g[2], g[3]};
+      float a[4], da[4];
+      activate_grad<T>(act, gs, a, da);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (n + k < F) {
-          float a, da;
-          activate_grad(act, g[k], a, da);
-          du[k] = d[k] * a;
-          dg[k] = d[k] * u[k] * da;
+          du[k] = d[k] * a[k];
+          dg[k] = d[k] * u[k] * da[k];
           su[k] += du[k];
           sg[k] += dg[k];
         }

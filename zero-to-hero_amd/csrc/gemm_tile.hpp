@@ -231,8 +231,10 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 // its code is long),
 //   Cols columns(int n), what columns n..n+3 bring along (a bias, scales),
 //   Row row(int m), what row m does,
-//   void operator()(int m, int n, const Cols&, const Row&, Acc<T> c [, Acc<T> second])
-// for columns n..n+3 of row m < M, n < N (those past N - 1 are its to skip).
+//   void apply(n, const Cols&, const int (&m)[B], const bool (&live)[B],
+//              const Row (&)[B], const Acc<T> (&c)[B] [, const Acc<T> (&second)[B]])
+// for columns n..n+3 of B rows m, of which the live ones are stored (n < N for
+// those; columns past N - 1 are its to skip).
 //
 // A step is four phases, each one 16-byte chunk per lane of every fragment.
 // While the matrix cores work on one phase, the fragments of the next are read
@@ -421,34 +423,50 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
 #pragma unroll 1
     for (int row0 = 0; row0 < kEdge; row0 += kRows * kBatch) {
       typename Epi::Row rows[kBatch];  // (their loads are under way together)
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        rows[b] = epi.row(min(m0 + (wm * TM + i) * kEdge + row0 + b * kRows + lane / kLanes,
-                              a.M - 1));
+      int m[kBatch];
+      bool live[kBatch];
+      A4 c[kBatch], c2[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const int row = row0 + b * kRows + lane / kLanes;
-        const int m = m0 + (wm * TM + i) * kEdge + row;
-        if (m >= a.M || n >= a.N) continue;
-        const A4 c = mine[row * kPitch / 4 + lane % kLanes];
-        if constexpr (kGated) {
-          const A4 c2 = mine[row * kPitch / 4 + kLanes + lane % kLanes];
-          if (a.partial) {
-            store_partial(a, blockIdx.y, 0, 2, m, n, c);
-            store_partial(a, blockIdx.y, 1, 2, m, n, c2);
-          } else {
-            epi(m, n, cols, rows[b], c, c2);
+        m[b] = m0 + (wm * TM + i) * kEdge + row;
+        live[b] = m[b] < a.M && n < a.N;
+        rows[b] = epi.row(min(m[b], a.M - 1));
+        c[b] = mine[row * kPitch / 4 + lane % kLanes];
+        if constexpr (kGated) c2[b] = mine[row * kPitch / 4 + kLanes + lane % kLanes];
+      }
+      if (a.partial) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+          if (live[b]) {
+            store_partial(a, blockIdx.y, 0, kGated ? 2 : 1, m[b], n, c[b]);
+            if constexpr (kGated) store_partial(a, blockIdx.y, 1, 2, m[b], n, c2[b]);
           }
-        } else {
-          if (a.partial)
-            store_partial(a, blockIdx.y, 0, 1, m, n, c);
-          else
-            epi(m, n, cols, rows[b], c);
-        }
+      } else if constexpr (kGated) {
+        epi.apply(n, cols, m, live, rows, c, c2);
+      } else {
+        epi.apply(n, cols, m, live, rows, c);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The epilogue of one row's four columns.
+template <class T, class Epi, int kHalves>
+__device__ __forceinline__ void apply_one(const Epi& epi, int m, int n,
+                                          const typename Epi::Cols& cols, bool live,
+                                          const Acc<T> (&sum)[kHalves]) {
+  const int ms[1] = {m};
+  const bool lives[1] = {live};
+  const typename Epi::Row rows[1] = {epi.row(m)};
+  const Acc<T> c[1] = {sum[0]};
+  if constexpr (kHalves == 2) {
+    const Acc<T> c2[1] = {sum[1]};
+    epi.apply(n, cols, ms, lives, rows, c, c2);
+  } else {
+    epi.apply(n, cols, ms, lives, rows, c);
   }
 }
 
@@ -469,10 +487,7 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a, const 
       const Acc<T> v = *reinterpret_cast<const Acc<T>*>(a.partial + at);
       sum[h] = s ? sum[h] + v : v;
     }
-  if constexpr (kHalves == 2)
-    epi(m, n, epi.columns(n), epi.row(m), sum[0], sum[1]);
-  else
-    epi(m, n, epi.columns(n), epi.row(m), sum[0]);
+  apply_one<T>(epi, m, n, epi.columns(n), true, sum);
 }
 
 constexpr int kRunBytes = 128;  // of K that a wave of the rows kernel takes at a time
@@ -578,11 +593,7 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
       for (int v = 1; v < kWaves; ++v) sum[h] += red[v][i * kHalves + h][lane];
     }
     const int m = i * 16 + r16, n = n0 + kq * 4;
-    if (m >= a.M || n >= a.N) continue;
-    if constexpr (kHalves == 2)
-      epi(m, n, cols, epi.row(m), sum[0], sum[1]);
-    else
-      epi(m, n, cols, epi.row(m), sum[0]);
+    if (m < a.M && n < a.N) apply_one<T>(epi, m, n, cols, true, sum);
   }
 }
 

@@ -28,14 +28,20 @@ struct Int8Epi {
     return c;
   }
   __device__ __forceinline__ Row row(int m) const { return xs[m]; }
-  __device__ __forceinline__ void operator()(int m, int n, const Cols& cols, Row s, v4i c) const {
-    float v[4];
+  template <int B>
+  __device__ __forceinline__ void apply(int n, const Cols& cols, const int (&m)[B],
+                                        const bool (&live)[B], const Row (&s)[B],
+                                        const v4i (&c)[B]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = (float)c[i] * s * cols.scale[i];
-      if (bias) v[i] += cols.bias[i];  // (without one, a zero keeps its sign)
+    for (int b = 0; b < B; ++b) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = (float)c[b][i] * s[b] * cols.scale[i];
+        if (bias) v[i] += cols.bias[i];  // (without one, a zero keeps its sign)
+      }
+      if (live[b]) store4(out + (int64_t)m[b] * N + n, v, N - n, (N & 3) == 0);
     }
-    store4(out + (int64_t)m * N + n, v, N - n, (N & 3) == 0);
   }
 };
 
