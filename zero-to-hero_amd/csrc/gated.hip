@@ -109,8 +109,11 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T* in, int64_t rows
       out[r * pitch + c] = c < cols ? in[r * cols + c] : from_f32<T>(0.0f);
 }
 
-constexpr int kTileM = 64;  // rows and columns that a workgroup of the next kernel takes
-constexpr int kTileF = 64;
+// Rows and columns that a workgroup of the next kernel takes: whole kilobytes
+// of the saved rows (tiles of 64 x 64 took 291 us for 8192 x 8192 in bf16, whose
+// 0.94 GB need 178 at a large copy's rate).
+constexpr int kTileM = 16;
+constexpr int kTileF = 256;
 
 // dg and du from dh and the saved g and u, as rows [dg | du] of pitch 2 fp (fp:
 // F rounded up to 16 bytes, zeros behind F), the operand of both products;
@@ -120,49 +123,59 @@ template <class T>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const float* saved, int64_t M,
                                                          int F, int F4, int act, Dropout drop,
                                                          T* dgu, int64_t fp, float* sums) {
-  __shared__ float part[16][2 * kTileF + 4];
-  const int64_t r0 = (int64_t)blockIdx.x * kTileM;
-  const int c0 = blockIdx.y * kTileF;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;  // four columns, rows ty + 16 i
+  __shared__ float part[4][2 * kTileF];
+  // neighbouring workgroups take neighbouring columns
+  const uint32_t across = (uint32_t)((fp + kTileF - 1) / kTileF);
+  const uint32_t row_tile = blockIdx.x / across;
+  const int64_t r0 = (int64_t)row_tile * kTileM;
+  const int c0 = (int)(blockIdx.x % across) * kTileF;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;  // four columns, rows ty + 4 i
   const int n = c0 + tx * 4;
   const uint64_t seed = drop.mode ? dropout_seed(drop) : 0;
   const bool vec = (F & 3) == 0 && ((uintptr_t)dh & (4 * sizeof(T) - 1)) == 0;
+  constexpr int kRows = kTileM / 4;
+  struct __attribute__((aligned(4 * sizeof(T)))) Four { T x[4]; };
+  v4f g[kRows], u[kRows];
+  Four d[kRows];
+  int64_t id[kRows];
+  // (every row's loads are under way before the first is used)
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t m = min(r0 + ty + 4 * i, M - 1);
+    const int c = min(n, F4 - 4);
+    g[i] = *reinterpret_cast<const v4f*>(saved + m * F4 + c);
+    u[i] = *reinterpret_cast<const v4f*>(saved + (M + m) * F4 + c);
+    id[i] = drop.mode && drop.rows ? drop.rows[m] : m;
+    const T* dp = dh + m * F;
+    if (vec) {
+      d[i] = *reinterpret_cast<const Four*>(dp + c);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[i].x[k] = dp[min(n + k, F - 1)];
+    }
+  }
   float sg[4] = {0, 0, 0, 0}, su[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < kTileM / 16; ++i) {
-    const int64_t m = r0 + ty + 16 * i;
-    if (m >= M || n >= fp) continue;
-    float dg[4] = {0, 0, 0, 0}, du[4] = {0, 0, 0, 0};
-    if (n < F) {
-      const v4f g = *reinterpret_cast<const v4f*>(saved + m * F4 + n);
-      const v4f u = *reinterpret_cast<const v4f*>(saved + (M + m) * F4 + n);
-      float d[4] = {0, 0, 0, 0};
-      const T* dp = dh + m * F + n;
-      struct __attribute__((aligned(4 * sizeof(T)))) Four { T x[4]; } four;
-      if (vec) {
-        four = *reinterpret_cast<const Four*>(dp);
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t m = r0 + ty + 4 * i;
+    float v[4], dg[4], du[4], a[4], da[4];
+    const float gs[4] = {g[i][0], g[i][1], g[i][2], g[i][3]};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d[k] = to_f32(four.x[k]);
-      } else {
+    for (int k = 0; k < 4; ++k) v[k] = to_f32(d[i].x[k]);
+    if (drop.mode) drop4(drop, seed, (uint64_t)id[i], (uint32_t)n >> 2, v);
+    activate_grad<T>(act, gs, a, da);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (n + k < F) d[k] = to_f32(dp[k]);
-      }
-      if (drop.mode) drop4(drop, seed, drop.rows ? drop.rows[m] : m, (uint32_t)n >> 2, d);
-      const float gs[4] = {g[0], g[1], g[2], g[3]};
-      float a[4], da[4];
-      activate_grad<T>(act, gs, a, da);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n + k < F) {
-          du[k] = d[k] * a[k];
-          dg[k] = d[k] * u[k] * da[k];
-          su[k] += du[k];
-          sg[k] += dg[k];
-        }
+    for (int k = 0; k < 4; ++k) {
+      const bool live = m < M && n + k < F;  // (what is behind F is not the saved values')
+      du[k] = live ? v[k] * a[k] : 0.0f;
+      dg[k] = live ? v[k] * u[i][k] * da[k] : 0.0f;
+      su[k] += du[k];
+      sg[k] += dg[k];
     }
-    store4(dgu + m * 2 * fp + n, dg, 4, true);
-    store4(dgu + m * 2 * fp + fp + n, du, 4, true);
+    if (m < M && n < fp) {
+      store4(dgu + m * 2 * fp + n, dg, 4, true);
+      store4(dgu + m * 2 * fp + fp + n, du, 4, true);
+    }
   }
   if (!sums) return;
 #pragma unroll
@@ -171,31 +184,33 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
     part[ty][kTileF + tx * 4 + k] = su[k];
   }
   __syncthreads();
-  if (threadIdx.x < 2 * kTileF) {
-    const int half = threadIdx.x / kTileF, c = threadIdx.x % kTileF;
-    if (c0 + c < F) {
-      float s = 0.0f;
-      for (int r = 0; r < 16; ++r) s += part[r][threadIdx.x];
-      sums[(int64_t)blockIdx.x * 2 * F + half * F + c0 + c] = s;
-    }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int c = threadIdx.x;
+    if (c0 + c >= F) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s += part[r][half * kTileF + c];
+    sums[(int64_t)row_tile * 2 * F + half * F + c0 + c] = s;
   }
 }
 
 // Column sums over the row tiles, in order.
+constexpr int kJoinRows = 16;
 template <class T>
-__global__ void __launch_bounds__(256) bias_join_kernel(const float* sums, int64_t parts, int F,
-                                                        T* dbg, T* dbu) {
-  __shared__ double part[4][64];
+__global__ void __launch_bounds__(64 * kJoinRows) bias_join_kernel(const float* sums, int64_t parts,
+                                                                   int F, T* dbg, T* dbu) {
+  __shared__ double part[kJoinRows][64];
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + tx;
   double s = 0.0;
   if (c < 2 * F)
-    for (int64_t k = ty; k < parts; k += 4) s += sums[k * 2 * F + c];
+    for (int64_t k = ty; k < parts; k += kJoinRows) s += sums[k * 2 * F + c];
   part[ty][tx] = s;
   __syncthreads();
   if (ty || c >= 2 * F) return;
-  const float v = (float)((part[0][tx] + part[1][tx]) + (part[2][tx] + part[3][tx]));
-  (c < F ? dbg[c] : dbu[c - F]) = from_f32<T>(v);
+  for (int r = 1; r < kJoinRows; ++r) s += part[r][tx];
+  (c < F ? dbg[c] : dbu[c - F]) = from_f32<T>((float)s);
 }
 
 // A bump allocator over the caller's workspace (or, with a null base, its size).
@@ -222,7 +237,7 @@ ForwardPlan plan_forward(int dtype, int64_t M, int64_t D, int64_t F, bool aligne
   const int64_t size = dtype_size(dtype);
   ForwardPlan f = {};
   f.pitch = round_up(D * size, 16);
-  const GemmPlan g = plan_gemm(M, 2 * F, f.pitch);
+  const GemmPlan g = plan_gemm(M, 2 * F, f.pitch, size == 4);
   f.pad = g.tile != 0 && (!aligned || f.pitch != D * size);
   Scratch s{ws};
   if (f.pad) {
@@ -257,8 +272,8 @@ BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool alig
     b.wu = s.take(F * b.pitch);
   }
   b.sums = s.take(div_up(M, kTileM) * 2 * F * 4);
-  const GemmPlan gx = plan_gemm(M, D, 2 * b.fp * size, true),
-                 gw = plan_gemm(2 * b.fp, D, M * size, true);
+  const GemmPlan gx = plan_gemm(M, D, 2 * b.fp * size, size == 4, true),
+                 gw = plan_gemm(2 * b.fp, D, M * size, size == 4, true);
   b.partial = s.take((int64_t)(gx.partial_bytes > gw.partial_bytes ? gx.partial_bytes
                                                                    : gw.partial_bytes));
   b.bytes = s.used;
@@ -273,7 +288,8 @@ bool forward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
 }
 bool backward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
   const int64_t size = dtype_size(dtype), pitch = 2 * round_up(F, 16) * size;
-  return forward_fits(dtype, M, D, F) && gemm_fits(M, D, pitch) && gemm_fits(2 * F, D, pitch);
+  return forward_fits(dtype, M, D, F) && gemm_fits(M, D, pitch) && gemm_fits(2 * F, D, pitch) &&
+         div_up(M, kTileM) * div_up(F + 8, kTileF) < ((int64_t)1 << 31);
 }
 
 template <class T>
@@ -371,13 +387,14 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
     int st;
     if (!dx && !dwg && !dbg) return (int)PPO_OK;
     hipLaunchKernelGGL((gated_grad_kernel<T>),
-                       dim3((unsigned)div_up(M, kTileM), (unsigned)div_up(b.fp, kTileF)), dim3(256),
-                       0, stream, (const T*)dh, saved, M, (int)F, (int)F4, activation,
+                       dim3((unsigned)(div_up(M, kTileM) * div_up(b.fp, kTileF))), dim3(256), 0,
+                       stream, (const T*)dh, saved, M, (int)F, (int)F4, activation,
                        drop_of(drop), (T*)b.dgu, b.fp, dbg ? (float*)b.sums : nullptr);
     if ((st = last_launch_status())) return st;
     if (dbg) {
-      hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)div_up(2 * F, 64)), dim3(256), 0,
-                         stream, (const float*)b.sums, div_up(M, kTileM), (int)F, (T*)dbg, (T*)dbu);
+      hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)div_up(2 * F, 64)),
+                         dim3(64 * kJoinRows), 0, stream, (const float*)b.sums,
+                         div_up(M, kTileM), (int)F, (T*)dbg, (T*)dbu);
       if ((st = last_launch_status())) return st;
     }
     GemmArgs a = {};

@@ -610,20 +610,52 @@ constexpr int kRowsMax = 64;       // rows that the rows kernel takes
 constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay below 2^31 bytes
 
 // How a product of M rows and `wrows` rows of W (both matrices of a gated one
-// together) over `kbytes` is cut.
-inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool by_k_rows = false) {
-  GemmPlan p = {0, 1, 0};
-  if (M <= kRowsMax && !by_k_rows) return p;
-  const int64_t steps = div_up(kbytes, kStepBytes);
-  auto tiles = [&](int64_t b) { return div_up(M, b) * div_up(wrows, b); };
-  if (tiles(256) >= 200) {
-    p.tile = 256;
-  } else if (tiles(128) >= 200) {
-    p.tile = 128;
-  } else {
-    p.tile = 64;
-    while (tiles(64) * p.splits < 512 && steps / (p.splits * 2) >= 8 && p.splits < 16)
-      p.splits *= 2;
+// together) over `kbytes` is cut: the tile and the number of splits of K with
+// the least expected time in us.  A workgroup takes `step` a K step and `fixed`
+// for its start and epilogue while it shares its CU (what the CU gets done),
+// and at least `alone` a step and `lone` where it waits for memory; a split
+// adds a second launch, and its partial sums are written and read again.
+// Measured on MI355X (us, bf16 unless said), tile 256 / 128 / 64 without split:
+// gated 4096 x 1024 -> 2048 41.5 / 41.7 / 59.6, 1024 x 2048 -> 2048 49 / 28 / 26,
+// fp32 4096 x 512 -> 1024 134 / 74 / 102; 128 in two splits 79, 33 and 90;
+// fp32 1024 x 1024 -> 512 in 64s and one, two or four splits 40 / 43 / 31.  The
+// rows kernel's time is that of reading W, more for the second to fourth
+// sixteen rows: 16, 32 and 64 rows of 4096 -> 8192 gated 26, 31 and 46, against
+// 25, 26 and 27 for tiles of 64 in two splits; fp32 4096 -> 4096 25, 33 and 52
+// against 44, 44 and 47.
+inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
+                          bool by_k_rows = false) {
+  GemmPlan p = {-1, 1, 0};
+  double best = 0.0;
+  if (M <= kRowsMax && !by_k_rows) {
+    p.tile = 0;
+    const int sets = M <= 16 ? 1 : M <= 32 ? 2 : 4;  // the kernel's MT
+    best = 2.0 + (double)wrows * kbytes / 5.5e6 * (0.8 + 0.2 * sets);
+  }
+  struct Cost { int tile, per_cu; double step[2], alone[2], fixed, lone; };
+  static const Cost kCosts[] = {
+      {256, 1, {1.05, 7.4}, {1.15, 7.4}, 12.0, 12.0},
+      {128, 2, {0.29, 1.9}, {0.65, 1.95}, 5.0, 8.0},
+      {64, 5, {0.10, 0.62}, {0.55, 1.0}, 1.9, 6.0},
+  };
+  constexpr int kCus = 256;
+  const double steps = (double)div_up(kbytes, kStepBytes);
+  for (const Cost& c : kCosts) {
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && steps < 4.0 * splits) break;
+      const double groups = (double)(div_up(M, c.tile) * div_up(wrows, c.tile)) * splits;
+      const double each = ceil(steps / splits);
+      const double busy = ceil(groups / kCus) * (each * c.step[fp32] + c.fixed);
+      const double waits = ceil(groups / (kCus * c.per_cu)) * (each * c.alone[fp32] + c.lone);
+      // 6 us for the launch, and the sums at 7 TB/s (they stay in the caches)
+      const double join = splits > 1 ? 6.0 + splits * 8.0 * M * wrows / 7e6 : 0.0;
+      const double time = fmax(busy, waits) + join;
+      if (p.tile < 0 || time < best) {
+        best = time;
+        p.tile = c.tile;
+        p.splits = splits;
+      }
+    }
   }
   if (p.splits > 1) p.partial_bytes = (size_t)p.splits * M * round_up(wrows, 8) * 4;
   return p;
@@ -640,7 +672,7 @@ int launch_gemm(GemmArgs a, const Epi& epi, char* partial, hipStream_t stream) {
   const int64_t wrows = (int64_t)a.N * (Epi::kGated ? 2 : 1);
   if (a.ranges == 0) a.ranges = 1;
   const int64_t kbytes = a.ranges * (kXT ? a.k * (int64_t)sizeof(T) : a.kbytes);
-  const GemmPlan p = plan_gemm(a.M, wrows, kbytes, kXT || kWT);
+  const GemmPlan p = plan_gemm(a.M, wrows, kbytes, sizeof(T) == 4, kXT || kWT);
   a.partial = p.splits > 1 ? partial : nullptr;
   if constexpr (!kXT && !kWT) {
     if (p.tile == 0) {

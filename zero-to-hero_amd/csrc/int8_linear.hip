@@ -218,7 +218,7 @@ struct Int8Plan {
 Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, bool quantize, bool ax, bool aw, char* ws) {
   Int8Plan p = {};
   p.pitch = round_up(K, 16);
-  const GemmPlan g = plan_gemm(M, N, p.pitch);
+  const GemmPlan g = plan_gemm(M, N, p.pitch, false);
   const bool odd = p.pitch != K;
   p.pad_x = !quantize && g.tile != 0 && (odd || !ax);
   p.pad_w = g.tile != 0 && (odd || !aw);
@@ -304,7 +304,7 @@ extern "C" int ppo_layer_int8_linear(const void* x, const int8_t* xq, const floa
       if ((st = last_launch_status())) return st;
     }
     // the tile kernel's rows end on 16 bytes (zeros behind K), the rows kernel's on K
-    if (plan_gemm(M, N, p.pitch).tile) a.kbytes = p.pitch;
+    if (plan_gemm(M, N, p.pitch, false).tile) a.kbytes = p.pitch;
     const Int8Epi<T> epi = {x ? (const float*)p.xs : xs, ws, (const T*)bias, (T*)out, (int)N};
     return launch_gemm<int8_t>(a, epi, p.partial, stream);
   });
