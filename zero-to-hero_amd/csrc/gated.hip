@@ -100,13 +100,39 @@ struct StoreEpi {
   }
 };
 
-// [rows][cols] -> the same rows at a pitch, zeros behind each row.
+// Up to three matrices of `cols` columns to rows at a pitch, zeros behind each
+// row, in one launch (blockIdx.y).
 template <class T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const T* in, int64_t rows, int cols, T* out,
-                                                       int pitch) {
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < pitch; c += 256)
-      out[r * pitch + c] = c < cols ? in[r * cols + c] : from_f32<T>(0.0f);
+struct PadArgs {
+  const T* in[3];
+  T* out[3];
+  int64_t rows[3];
+};
+template <class T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const PadArgs<T> a, int cols, int pitch) {
+  const T* in = a.in[blockIdx.y];
+  T* out = a.out[blockIdx.y];
+  constexpr int kN = kPer16<T>;
+  // a workgroup takes as many rows at once as 256 threads of 16 bytes cover
+  const int chunks = pitch / kN;
+  int per_row = 256;
+  while (per_row / 2 >= chunks && per_row > 1) per_row >>= 1;
+  const int at = threadIdx.x & (per_row - 1), lanes = 256 / per_row;
+  for (int64_t r = (int64_t)blockIdx.x * lanes + threadIdx.x / per_row; r < a.rows[blockIdx.y];
+       r += (int64_t)gridDim.x * lanes)
+    for (int c = at * kN; c < pitch; c += per_row * kN) {
+      struct __attribute__((aligned(16))) { T e[kN]; } x;
+      v4i v = {0, 0, 0, 0};
+      if (c + kN <= cols) {
+        v = *reinterpret_cast<const v4i_any*>(in + r * cols + c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          x.e[i] = c + i < cols ? in[r * cols + c + i] : from_f32<T>(0.0f);
+        v = __builtin_bit_cast(v4i, x);
+      }
+      *reinterpret_cast<v4i*>(out + r * pitch + c) = v;
+    }
 }
 
 // Rows and columns that a workgroup of the next kernel takes: whole kilobytes
@@ -292,11 +318,17 @@ bool backward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
          div_up(M, kTileM) * div_up(F + 8, kTileF) < ((int64_t)1 << 31);
 }
 
+// Padded copies of x [M,D] and of the weights [F,D] (those that are not NULL).
 template <class T>
-void pad_rows(const void* in, int64_t rows, int64_t cols, char* out, int64_t pitch,
-              hipStream_t stream) {
-  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256),
-                     0, stream, (const T*)in, rows, (int)cols, (T*)out, (int)(pitch / sizeof(T)));
+int pad_rows(const void* x, const void* wg, const void* wu, char* xp, char* wgp, char* wup,
+             int64_t M, int64_t D, int64_t F, int64_t pitch, hipStream_t stream) {
+  const PadArgs<T> a = {{(const T*)x, (const T*)wg, (const T*)wu},
+                        {(T*)xp, (T*)wgp, (T*)wup},
+                        {x ? M : 0, wg ? F : 0, wu ? F : 0}};
+  const int64_t rows = M > F ? M : F;
+  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(rows < 4096 ? rows : 4096), 3),
+                     dim3(256), 0, stream, a, (int)D, (int)(pitch / sizeof(T)));
+  return last_launch_status();
 }
 
 bool drop_ok(const ppo_dropout* d) { return !d || (d->p >= 0.0 && d->p <= 1.0); }
@@ -342,9 +374,8 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
     a.M = (int)M;
     a.N = (int)F;
     if (f.pad) {
-      pad_rows<T>(x, M, D, f.x, f.pitch, stream);
-      pad_rows<T>(wg, F, D, f.wg, f.pitch, stream);
-      pad_rows<T>(wu, F, D, f.wu, f.pitch, stream);
+      const int st = pad_rows<T>(x, wg, wu, f.x, f.wg, f.wu, M, D, F, f.pitch, stream);
+      if (st) return st;
       a.x = f.x;
       a.w0 = f.wg;
       a.w1 = f.wu;
@@ -401,9 +432,9 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
     a.N = (int)D;
     a.wpitch = D * size;
     if (b.pad) {
-      if (dwg) pad_rows<T>(x, M, D, b.x, b.pitch, stream);
-      if (dx) pad_rows<T>(wg, F, D, b.wg, b.pitch, stream);
-      if (dx) pad_rows<T>(wu, F, D, b.wu, b.pitch, stream);
+      st = pad_rows<T>(dwg ? x : nullptr, dx ? wg : nullptr, dx ? wu : nullptr, b.x, b.wg, b.wu, M,
+                       D, F, b.pitch, stream);
+      if (st) return st;
       a.wpitch = b.pitch;
     }
     a.x = b.dgu;
