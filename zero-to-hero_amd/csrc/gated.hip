@@ -24,8 +24,15 @@ struct GatedEpi {
   int F, F4, act;
   Dropout drop;
 
-  struct Cols { float g[4], u[4]; };
-  typedef int64_t Row;
+  static constexpr bool kRows = true;
+  struct Cols {
+    float g[4], u[4];
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(g[i]), "+v"(u[i]));
+    }
+  };
+  typedef long Row;
   __device__ __forceinline__ Cols columns(int n) const {
     Cols c;
 #pragma unroll
@@ -82,7 +89,10 @@ struct StoreEpi {
   T* out0;
   T* out1;
   int rows, second, N;
-  struct Cols {};
+  static constexpr bool kRows = false;
+  struct Cols {
+    __device__ __forceinline__ void arrived() {}
+  };
   struct Row {};
   __device__ __forceinline__ Cols columns(int) const { return {}; }
   __device__ __forceinline__ Row row(int) const { return {}; }

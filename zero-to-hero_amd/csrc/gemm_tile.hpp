@@ -200,15 +200,20 @@ struct Side {
   }
 };
 
+// Waits for this wave's LDS reads and writes, then for the workgroup.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 constexpr uint32_t kBehind = 0x80000000u;  // an offset that no descriptor reaches
 
 // Workgroup -> tile.  Workgroups go round-robin over the eight XCDs, each
 // with an L2 of its own: an XCD takes a run of consecutive tiles, and a run
 // walks blocks of kGroup row tiles by columns, so that the tiles in flight on
 // one XCD share rows and columns.
-__device__ __forceinline__ void tile_of(const GemmArgs& a, int& tm, int& tn) {
+__device__ __forceinline__ void tile_of(const GemmArgs& a, int id, int& tm, int& tn) {
   constexpr int kXcds = 8, kGroup = 8;
-  const int n = a.tiles_m * a.tiles_n, id = blockIdx.x;
+  const int n = a.tiles_m * a.tiles_n;
   const int xcd = id % kXcds, q = n / kXcds, r = n % kXcds;
   const int t = xcd * q + min(xcd, r) + id / kXcds;
   const int per = kGroup * a.tiles_n, first = t / per * kGroup;
@@ -227,10 +232,10 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 }
 
 // Epi, the operator's epilogue: kGated (two W matrices, one output), kBatch
-// (rows that a lane takes at once: more where it waits for loads, one where
-// its code is long),
+// (rows that a lane takes at once),
 //   Cols columns(int n), what columns n..n+3 bring along (a bias, scales),
-//   Row row(int m), what row m does,
+//   Row row(int m), what row m does (kRows: whether that is anything),
+// both plain 32-bit or 64-bit values that are fetched before the stores begin,
 //   void apply(n, const Cols&, const int (&m)[B], const bool (&live)[B],
 //              const Row (&)[B], const Acc<T> (&c)[B] [, const Acc<T> (&second)[B]])
 // for columns n..n+3 of B rows m, of which the live ones are stored (n < N for
@@ -266,9 +271,6 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / kWavesN, wn = wave % kWavesN;
-  int tm, tn;
-  tile_of(a, tm, tn);
-  const int m0 = tm * BM, n0 = tn * kCols;
   constexpr int kStepK = kStepBytes / (int)sizeof(T);
   const int per_range = (int)(kXT ? div_up(a.k, kStepK) : div_up(a.kbytes, kStepBytes));
   const int steps = per_range * a.ranges;
@@ -281,11 +283,19 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   // one operand's source for a step: an operand of k-contiguous rows has one
   // descriptor and a moving offset, one of k-rows a descriptor per step
   struct Source { Buffer b0, b1; uint32_t off; };
-  const uint32_t w_bytes = (uint32_t)min(kCols, a.N - n0) * wp;
-  const Buffer bx = kXT ? buffer_of(a.x, 0)
-                        : buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
-  const Buffer bw0 = kWT ? bx : buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
-  const Buffer bw1 = kGated ? buffer_of(a.w1 + n0 * a.wpitch, w_bytes) : bw0;
+  int m0, n0;  // of the tile that is loaded
+  Buffer bx, bw0, bw1;
+  auto locate = [&](int id) {
+    int tm, tn;
+    tile_of(a, id, tm, tn);
+    m0 = tm * BM;
+    n0 = tn * kCols;
+    const uint32_t w_bytes = (uint32_t)min(kCols, a.N - n0) * wp;
+    bx = kXT ? buffer_of(a.x, 0)
+             : buffer_of(a.x + m0 * a.xpitch, (uint32_t)min(BM, a.M - m0) * xp);
+    bw0 = kWT ? bx : buffer_of(a.w0 + n0 * a.wpitch, w_bytes);
+    bw1 = kGated ? buffer_of(a.w1 + n0 * a.wpitch, w_bytes) : bw0;
+  };
   auto by_rows = [&](const char* base, int64_t pitch, int64_t col_bytes, int local, bool live) {
     const int64_t k0 = (int64_t)local * kStepK;
     const int64_t left = live ? (a.k - k0) * pitch - col_bytes : 0;
@@ -336,10 +346,6 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   };
 
   Acc<T, kEdge> acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = Acc<T, kEdge>(0);
   auto multiply = [&](const Frags& from, int e) {
     acc[e / TN][e % TN] = mfma<T, kEdge>(from.w[e % TN], from.x[e / TN], acc[e / TN][e % TN]);
     __builtin_amdgcn_sched_barrier(0);
@@ -363,93 +369,136 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     }
   };
 
-  Source x, w;
-  {
-    source(0, x, w);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) load(i, 0, x, w);
-    source(1, x, w);
-#pragma unroll
-    for (int i = 0; i < kEarly; ++i) load(i, 1, x, w);
-    stage_barrier<kEarly>();
-#pragma unroll
-    for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[0], 0);
-  }
-  for (int step = 0; step < count; ++step) {
-    const int b = step & 1;
-    char* cur = lds[b];
-    char* other = lds[b ^ 1];
-#pragma unroll
-    for (int p = 0; p < kPhases - 1; ++p)
-      phase(f[p & 1], f[(p + 1) & 1], cur, p + 1, [&](int slot, int slots) {
-        if (p > 0) return;
-        constexpr int kRest = kLoads - kEarly;
-#pragma unroll
-        for (int i = slot * kRest / slots; i < (slot + 1) * kRest / slots; ++i)
-          load(kEarly + i, b ^ 1, x, w);
-      });
-    stage_barrier<0>();
-    source(step + 2, x, w);
-    phase(f[1], f[0], other, 0, [&](int slot, int slots) {
-#pragma unroll
-      for (int i = slot * kEarly / slots; i < (slot + 1) * kEarly / slots; ++i) load(i, b, x, w);
-    });
-  }
-  stage_barrier<0>();  // (the last loads and reads are ahead in what the epilogue overwrites)
-
   // --- epilogue ---------------------------------------------------------------------
   // Through LDS, 32 rows of the wave's block at a time: a lane then holds
   // columns next to its neighbours' (whole lines are stored), and the
   // operator's arithmetic is a loop whose code is there once, not once for
-  // every register.  A wave reads only what it wrote.
-  constexpr int kSpan = TN * kEdge, kPitch = kSpan + 4;  // (16 bytes spread the banks)
-  constexpr int kOut = kGated ? kSpan / 2 : kSpan, kLanes = kOut / 4, kRows = 64 / kLanes;
-  static_assert(kWaves * kEdge * kPitch * 4 <= 2 * kBuffer, "");
+  // every register.  A wave reads only what it wrote.  Row r's chunks (16
+  // bytes) are permuted by r % 16 to spread the banks.
+  constexpr int kSpan = TN * kEdge, kOut = kGated ? kSpan / 2 : kSpan;
+  constexpr int kLanes = kOut / 4, kRows = 64 / kLanes, kBatch = Epi::kBatch;
+  static_assert(kWaves * kEdge * kSpan * 4 <= kBuffer && kEdge % (kRows * kBatch) == 0, "");
   typedef Acc<T> A4;
-  A4* mine = reinterpret_cast<A4*>(&lds[0][0] + wave * kEdge * kPitch * 4);
-  constexpr int kBatch = Epi::kBatch;
-  static_assert(kEdge % (kRows * kBatch) == 0, "");
-  const int n = n0 + wn * kOut + lane % kLanes * 4;
-  const typename Epi::Cols cols = epi.columns(min(n, a.N - 1));
+  A4* mine = reinterpret_cast<A4*>(&lds[0][0] + wave * kEdge * kSpan * 4);
+  constexpr int kRowSets = (TM * kEdge + 63) / 64;
+  auto finish = [&](int em0, int en0, const typename Epi::Cols& cols,
+                    const typename Epi::Row (&states)[kRowSets], bool more) {
+    const int n = en0 + wn * kOut + lane % kLanes * 4;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        mine[(r * kPitch + j * kEdge + g * 8 + kq * 4) / 4] = four<T, kEdge>(acc[i][j], g);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+        for (int g = 0; g < 4; ++g)
+          mine[r * (kSpan / 4) + ((j * 8 + g * 2 + kq) ^ (r & 15))] =
+              four<T, kEdge>(acc[i][j], g);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      // (the next tile's first loads have then arrived, with most of the stores)
+      if (i == TM - 1 && more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll 1
-    for (int row0 = 0; row0 < kEdge; row0 += kRows * kBatch) {
-      typename Epi::Row rows[kBatch];  // (their loads are under way together)
-      int m[kBatch];
-      bool live[kBatch];
-      A4 c[kBatch], c2[kBatch];
+      for (int row0 = 0; row0 < kEdge; row0 += kRows * kBatch) {
+        typename Epi::Row rows[kBatch];
+        int m[kBatch];
+        bool live[kBatch];
+        A4 c[kBatch], c2[kBatch];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int row = row0 + b * kRows + lane / kLanes;
-        m[b] = m0 + (wm * TM + i) * kEdge + row;
-        live[b] = m[b] < a.M && n < a.N;
-        rows[b] = epi.row(min(m[b], a.M - 1));
-        c[b] = mine[row * kPitch / 4 + lane % kLanes];
-        if constexpr (kGated) c2[b] = mine[row * kPitch / 4 + kLanes + lane % kLanes];
-      }
-      if (a.partial) {
+        for (int b = 0; b < kBatch; ++b) {
+          const int row = row0 + b * kRows + lane / kLanes, at = i * kEdge + row;
+          m[b] = em0 + wm * TM * kEdge + at;
+          live[b] = m[b] < a.M && n < a.N;
+          if constexpr (Epi::kRows) rows[b] = __shfl(states[i * kEdge / 64], at & 63, 64);
+          c[b] = mine[row * (kSpan / 4) + ((lane % kLanes) ^ (row & 15))];
+          if constexpr (kGated) c2[b] = mine[row * (kSpan / 4) + ((kLanes + lane % kLanes) ^ (row & 15))];
+        }
+        if (a.partial) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-          if (live[b]) {
-            store_partial(a, blockIdx.y, 0, kGated ? 2 : 1, m[b], n, c[b]);
-            if constexpr (kGated) store_partial(a, blockIdx.y, 1, 2, m[b], n, c2[b]);
-          }
-      } else if constexpr (kGated) {
-        epi.apply(n, cols, m, live, rows, c, c2);
-      } else {
-        epi.apply(n, cols, m, live, rows, c);
+          for (int b = 0; b < kBatch; ++b)
+            if (live[b]) {
+              store_partial(a, blockIdx.y, 0, kGated ? 2 : 1, m[b], n, c[b]);
+              if constexpr (kGated) store_partial(a, blockIdx.y, 1, 2, m[b], n, c2[b]);
+            }
+        } else if constexpr (kGated) {
+          epi.apply(n, cols, m, live, rows, c, c2);
+        } else {
+          epi.apply(n, cols, m, live, rows, c);
+        }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+  };
+
+  // --- tiles ------------------------------------------------------------------------
+  // Where the grid is smaller than the tiles, a workgroup takes several, and
+  // the first step of the next is loaded (into the second buffer) while the
+  // epilogue of the last uses the first.  A tile's steps go to the buffers in
+  // turn, the second first.
+  constexpr bool kLoop = BM * BN >= 256 * 256;
+  const int tiles = a.tiles_m * a.tiles_n;
+  Source x, w;
+  locate(blockIdx.x);
+  source(0, x, w);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) load(i, 1, x, w);
+  for (int id = blockIdx.x;; id += gridDim.x) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = Acc<T, kEdge>(0);
+    source(1, x, w);
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i) load(i, 0, x, w);
+    if (id == (int)blockIdx.x) stage_barrier<kEarly>();
+#pragma unroll
+    for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[1], 0);
+    for (int step = 0; step < count; ++step) {
+      const int b = step & 1 ^ 1;
+      char* cur = lds[b];
+      char* other = lds[b ^ 1];
+#pragma unroll
+      for (int p = 0; p < kPhases - 1; ++p)
+        phase(f[p & 1], f[(p + 1) & 1], cur, p + 1, [&](int slot, int slots) {
+          if (p > 0) return;
+          constexpr int kRest = kLoads - kEarly;
+#pragma unroll
+          for (int i = slot * kRest / slots; i < (slot + 1) * kRest / slots; ++i)
+            load(kEarly + i, b ^ 1, x, w);
+        });
+      stage_barrier<0>();
+      source(step + 2, x, w);
+      phase(f[1], f[0], other, 0, [&](int slot, int slots) {
+#pragma unroll
+        for (int i = slot * kEarly / slots; i < (slot + 1) * kEarly / slots; ++i) load(i, b, x, w);
+      });
+    }
+    // what the epilogue needs beside the sums is fetched before its LDS is free
+    // and the next tile's loads are under way: waiting for it later would wait
+    // for those
+    const int em0 = m0, en0 = n0;
+    const bool more = kLoop && id + (int)gridDim.x < tiles;
+    typename Epi::Cols cols = epi.columns(min(en0 + wn * kOut + lane % kLanes * 4, a.N - 1));
+    typename Epi::Row states[kRowSets];
+    if constexpr (Epi::kRows) {
+#pragma unroll
+      for (int i = 0; i < kRowSets; ++i)
+        states[i] = epi.row(min(em0 + wm * TM * kEdge + i * 64 + lane, a.M - 1));
+    }
+    stage_barrier<0>();
+    if constexpr (Epi::kRows) {
+#pragma unroll
+      for (int i = 0; i < kRowSets; ++i) asm volatile("" : "+v"(states[i]));
+    }
+    cols.arrived();
+    if (more) {
+      locate(id + gridDim.x);
+      source(0, x, w);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load(i, 1, x, w);
+    }
+    finish(em0, en0, cols, states, more);
+    if (!more) break;
+    lds_barrier();
   }
 }
 
@@ -460,7 +509,8 @@ __device__ __forceinline__ void apply_one(const Epi& epi, int m, int n,
                                           const Acc<T> (&sum)[kHalves]) {
   const int ms[1] = {m};
   const bool lives[1] = {live};
-  const typename Epi::Row rows[1] = {epi.row(m)};
+  typename Epi::Row rows[1];
+  if constexpr (Epi::kRows) rows[0] = epi.row(m);
   const Acc<T> c[1] = {sum[0]};
   if constexpr (kHalves == 2) {
     const Acc<T> c2[1] = {sum[1]};
@@ -606,6 +656,7 @@ struct GemmPlan {
   size_t partial_bytes;
 };
 
+constexpr int kCus = 256;
 constexpr int kRowsMax = 64;       // rows that the rows kernel takes
 constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay below 2^31 bytes
 
@@ -638,7 +689,6 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
       {128, 2, {0.29, 1.9}, {0.65, 1.95}, 5.0, 8.0},
       {64, 5, {0.10, 0.62}, {0.55, 1.0}, 1.9, 6.0},
   };
-  constexpr int kCus = 256;
   const double steps = (double)div_up(kbytes, kStepBytes);
   for (const Cost& c : kCosts) {
     for (int splits = 1; splits <= 16; splits *= 2) {
@@ -692,7 +742,9 @@ int launch_gemm(GemmArgs a, const Epi& epi, char* partial, hipStream_t stream) {
   const int cols = Epi::kGated ? p.tile / 2 : p.tile;
   a.tiles_m = (int)div_up(a.M, p.tile);
   a.tiles_n = (int)div_up(a.N, cols);
-  const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)p.splits);
+  // (256: a workgroup of the largest tile has a CU to itself and takes tile after tile)
+  const int tiles = a.tiles_m * a.tiles_n;
+  const dim3 grid((unsigned)(p.tile == 256 && tiles > kCus ? kCus : tiles), (unsigned)p.splits);
   if (p.tile == 256)
     hipLaunchKernelGGL((gemm_tile_kernel<T, 256, 256, 2, 2, kXT, kWT, Epi>), grid, dim3(256), 0,
                        stream, a, epi);

@@ -15,7 +15,14 @@ struct Int8Epi {
   const T* bias;
   T* out;
   int N;
-  struct Cols { float scale[4], bias[4]; };
+  static constexpr bool kRows = true;
+  struct Cols {
+    float scale[4], bias[4];
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(scale[i]), "+v"(bias[i]));
+    }
+  };
   typedef float Row;
   __device__ __forceinline__ Cols columns(int n) const {
     Cols c;
