@@ -441,6 +441,24 @@ def test_gated_large_grid(dev):
             check_grad(got, w.cpu(), torch.bfloat16, f"{M} {D} {F}")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,D,F", [(1, 40, 24), (2, 64, 128), (4, 33, 1000), (60, 24, 68)])
+def test_gated_gradients_of_few_rows(dev, dtype, M, D, F):
+    """Few dg and du: their rounding must not show.  The gradients are within
+    their own rounding u(t), the 32-bit terms and the square of u(t) (what is
+    left of dg twice rounded)."""
+    t = TYPES[dtype]
+    x, wg, wu, bg, bu, dh = gated_case(dtype, M, D, F, True, seed=6)
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+    grads = torch.autograd.grad(ppo_amd.gated_ffn(*leaves), leaves, dh.to(dev))
+    _, g, u = ref.gated_ffn(*d64(x, wg, wu, bg, bu), "silu")
+    want = ref.gated_ffn_grads(*d64(x, wg, wu), g, u, "silu", dh.double())
+    for name, got, w in zip(("dx", "dwg", "dwu", "dbg", "dbu"), grads, want):
+        diff, norm = (got.double().cpu() - w).norm(), w.norm()
+        tiny = 2.0 ** -25 * math.sqrt(w.numel()) if t == torch.float16 else 0.0
+        assert diff <= (u_of(t) + u_of(t) ** 2 + 64 * U32) * norm + tiny, name
+
+
 def test_gated_dropout_is_dropouts(dev):
     x, wg, wu, bg, bu, _ = gated_case("fp32", 70, 24, 37, True)
     args = [v.to(dev) for v in (x, wg, wu, bg, bu)]

@@ -145,20 +145,29 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const PadArgs<T> a, int c
     }
 }
 
+// What rounding x to T leaves (nothing where the rounded value is not finite).
+template <class T>
+__device__ __forceinline__ float rounding_rest(float x) {
+  const float left = x - to_f32(from_f32<T>(x));
+  return fabsf(left) <= fabsf(x) ? left : 0.0f;
+}
+
 // Rows and columns that a workgroup of the next kernel takes: whole kilobytes
 // of the saved rows (tiles of 64 x 64 took 291 us for 8192 x 8192 in bf16, whose
 // 0.94 GB need 178 at a large copy's rate).
 constexpr int kTileM = 16;
 constexpr int kTileF = 256;
 
-// dg and du from dh and the saved g and u, as rows [dg | du] of pitch 2 fp (fp:
-// F rounded up to 16 bytes, zeros behind F), the operand of both products;
-// with `sums`, a tile's column sums for the biases ([row tiles][2 F], joined
-// in order by bias_join_kernel).
+// dg and du from dh and the saved g and u, as rows [dg | du] of `pitch` elements
+// (each of fp: F rounded up to 16 bytes, zeros behind F), the operand of both
+// products; with `rest`, what their rounding to T left follows in the row.
+// With `sums`, a tile's column sums for the biases ([row tiles][2 F], joined in
+// order by bias_join_kernel).
 template <class T>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const float* saved, int64_t M,
                                                          int F, int F4, int act, Dropout drop,
-                                                         T* dgu, int64_t fp, float* sums) {
+                                                         T* dgu, int64_t fp, int64_t pitch,
+                                                         bool rest, float* sums) {
   __shared__ float part[4][2 * kTileF];
   // neighbouring workgroups take neighbouring columns
   const uint32_t across = (uint32_t)((fp + kTileF - 1) / kTileF);
@@ -209,8 +218,18 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
       sg[k] += dg[k];
     }
     if (m < M && n < fp) {
-      store4(dgu + m * 2 * fp + n, dg, 4, true);
-      store4(dgu + m * 2 * fp + fp + n, du, 4, true);
+      T* row = dgu + m * pitch + n;
+      store4(row, dg, 4, true);
+      store4(row + fp, du, 4, true);
+      if (rest) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          dg[k] = rounding_rest<T>(dg[k]);
+          du[k] = rounding_rest<T>(du[k]);
+        }
+        store4(row + 2 * fp, dg, 4, true);
+        store4(row + 3 * fp, du, 4, true);
+      }
     }
   }
   if (!sums) return;
@@ -286,8 +305,16 @@ ForwardPlan plan_forward(int dtype, int64_t M, int64_t D, int64_t F, bool aligne
   return f;
 }
 
+// A 16-bit dg or du is off by up to half a step, which averages out in the sums
+// of both products, except where there are few of them: with 2 x 128 of them,
+// bf16 weight gradients were off by 2.6e-3 in the 2-norm where their own rounding
+// makes 1.7e-3.  Up to this many elements the products take what the rounding
+// left as well, as further ranges of K (their time is that of a launch).
+constexpr int64_t kRestElements = 4096;
+
 struct BackwardPlan {
   int64_t fp;     // F rounded up to 16 bytes of elements
+  bool rest;      // dg and du in two parts each
   int64_t pitch;  // bytes of a row of x and the weights
   bool pad;
   char *dgu, *x, *wg, *wu, *sums, *partial;
@@ -301,15 +328,17 @@ BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool alig
   b.pitch = round_up(D * size, 16);
   b.pad = !aligned || b.pitch != D * size;
   Scratch s{ws};
-  b.dgu = s.take(M * 2 * b.fp * size);
+  b.rest = size == 2 && M * F <= kRestElements;
+  const int64_t parts = b.rest ? 4 : 2;
+  b.dgu = s.take(M * parts * b.fp * size);
   if (b.pad) {
     b.x = s.take(M * b.pitch);
     b.wg = s.take(F * b.pitch);
     b.wu = s.take(F * b.pitch);
   }
   b.sums = s.take(div_up(M, kTileM) * 2 * F * 4);
-  const GemmPlan gx = plan_gemm(M, D, 2 * b.fp * size, size == 4, true),
-                 gw = plan_gemm(2 * b.fp, D, M * size, size == 4, true);
+  const GemmPlan gx = plan_gemm(M, D, parts * b.fp * size, size == 4, true),
+                 gw = plan_gemm(2 * b.fp, D, parts / 2 * M * size, size == 4, true);
   b.partial = s.take((int64_t)(gx.partial_bytes > gw.partial_bytes ? gx.partial_bytes
                                                                    : gw.partial_bytes));
   b.bytes = s.used;
@@ -430,7 +459,8 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
     hipLaunchKernelGGL((gated_grad_kernel<T>),
                        dim3((unsigned)(div_up(M, kTileM) * div_up(b.fp, kTileF))), dim3(256), 0,
                        stream, (const T*)dh, saved, M, (int)F, (int)F4, activation,
-                       drop_of(drop), (T*)b.dgu, b.fp, dbg ? (float*)b.sums : nullptr);
+                       drop_of(drop), (T*)b.dgu, b.fp, (b.rest ? 4 : 2) * b.fp, b.rest,
+                       dbg ? (float*)b.sums : nullptr);
     if ((st = last_launch_status())) return st;
     if (dbg) {
       hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)div_up(2 * F, 64)),
@@ -448,22 +478,23 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
       a.wpitch = b.pitch;
     }
     a.x = b.dgu;
-    a.xpitch = 2 * b.fp * size;
+    a.xpitch = (b.rest ? 4 : 2) * b.fp * size;
     if (dx) {  // [dg | du] [wg; wu], the weights as they lie: k-rows of D columns
       a.w0 = b.pad ? b.wg : (const char*)wg;
       a.w1 = b.pad ? b.wu : (const char*)wu;
       a.M = (int)M;
       a.kbytes = a.x_range = b.fp * size;
       a.k = F;
-      a.ranges = 2;
+      a.ranges = b.rest ? 4 : 2;
       const StoreEpi<T> epi = {(T*)dx, nullptr, (int)M, (int)M, (int)D};
       if ((st = launch_gemm<T, false, true>(a, epi, b.partial, stream))) return st;
     }
     if (dwg) {  // [dg | du]^T x: both operands by their rows m
-      a.w0 = b.pad ? b.x : (const char*)x;
+      a.w0 = a.w1 = b.pad ? b.x : (const char*)x;
       a.M = (int)(2 * b.fp);
       a.k = M;
-      a.ranges = 1;
+      a.ranges = b.rest ? 2 : 1;
+      a.x_range = 2 * b.fp * size;
       const StoreEpi<T> epi = {(T*)dwg, (T*)dwu, (int)F, (int)b.fp, (int)D};
       if ((st = launch_gemm<T, true, true>(a, epi, b.partial, stream))) return st;
     }

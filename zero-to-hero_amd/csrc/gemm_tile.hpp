@@ -44,8 +44,8 @@ struct GemmArgs {
   int64_t xpitch, wpitch;  // bytes, multiples of 16
   int64_t kbytes;   // of a row, a multiple of 16
   int64_t k;        // k-rows of an operand that is stored by them
-  int ranges;       // 2: K is two ranges of kbytes and k; W's second is w1, X's
-  int64_t x_range;  //    x_range bytes behind its first
+  int ranges;       // K is so many ranges of kbytes and k: W's are w0 and w1 in turn,
+  int64_t x_range;  //    X's lie x_range bytes apart in its rows
   int M, N;         // N: output columns
   int tiles_m, tiles_n;
   int steps_per_split;     // K steps that one split takes
@@ -306,15 +306,17 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   auto source = [&](int step, Source& x, Source& w) {
     const bool live = step < count;
     const int at = first + step;
-    const int range = at >= per_range && a.ranges > 1, local = at - (range ? per_range : 0);
+    const int range = a.ranges > 1 ? at / per_range : 0, local = at - range * per_range;
     const uint32_t kb = (uint32_t)local * kStepBytes + X::chunk(lane);
     const uint32_t k_off = live && kb < (uint32_t)a.kbytes ? kb : kBehind;
-    x = {bx, bx, k_off + (uint32_t)(range ? a.x_range : 0)};
+    const int64_t behind = range * a.x_range;
+    x = {bx, bx, k_off + (uint32_t)behind};
     w = {bw0, bw1, k_off};
-    if (kXT) x.off = 0, x.b0 = by_rows(a.x, a.xpitch, (int64_t)m0 * (int)sizeof(T), local, live);
+    if (kXT)
+      x.off = 0, x.b0 = by_rows(a.x, a.xpitch, (int64_t)m0 * (int)sizeof(T) + behind, local, live);
     if (kWT)
-      w.off = 0, w.b0 = by_rows(range ? a.w1 : a.w0, a.wpitch, (int64_t)n0 * (int)sizeof(T), local,
-                                live);
+      w.off = 0, w.b0 = by_rows(range & 1 ? a.w1 : a.w0, a.wpitch, (int64_t)n0 * (int)sizeof(T),
+                                local, live);
   };
   const uint32_t lds0 =
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
