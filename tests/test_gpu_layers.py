@@ -638,6 +638,51 @@ def test_forward_mode_and_batched_gradients_are_refused(dev):
                                 is_grads_batched=True)
 
 
+# --- registered operators ----------------------------------------------------------------
+
+def test_registered_operators(dev):
+    """opcheck on each operator, and the functions' bits."""
+    op = torch.ops.ppo_amd
+    x, wg, wu, bg, bu, dh = gated_case("fp32", 20, 24, 36, True)
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+    rows, seed = torch.arange(20, device=dev) * 3, torch.tensor([4], device=dev)
+    utils = ("test_schema", "test_autograd_registration", "test_faketensor")
+    torch.library.opcheck(op.dropout, (leaves[0], 0.3, 4, None, rows), test_utils=utils)
+    torch.library.opcheck(op.gated_ffn, (*leaves, "silu", 0.2, 0, seed, rows), test_utils=utils)
+    plain = [v.detach() for v in leaves]
+    torch.library.opcheck(op.quantize_rows, (plain[0],), test_utils=utils)
+    q, s = ppo_amd.quantize_rows(plain[1])
+    torch.library.opcheck(op.int8_linear, (plain[0], q, s, None, None, None), test_utils=utils)
+
+    h, _ = op.gated_ffn(*leaves, "silu", 0.2, 0, seed, rows)
+    z = op.dropout(h, 0.1, 4, None, rows)
+    got = [z.detach(), *torch.autograd.grad(z, leaves, dh.to(dev))]
+    h = ppo_amd.gated_ffn(*leaves, dropout_p=0.2, seed=seed, rows=rows)
+    z = ppo_amd.dropout(h, 0.1, 4, rows)
+    want = [z.detach(), *torch.autograd.grad(z, leaves, dh.to(dev))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_registered_operators_compile(dev):
+    """A compiled layer with its backward is traced whole and equals eager."""
+    op = torch.ops.ppo_amd
+    x, wg, wu, bg, bu, dh = gated_case("fp32", 40, 24, 36, True)
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+
+    def layer(x, wg, wu, bg, bu, seed):
+        h = op.gated_ffn(x, wg, wu, bg, bu, "gelu", 0.2, 0, seed, None)[0]
+        return op.dropout(h, 0.1, 0, seed, None) * 2.0
+
+    compiled = torch.compile(layer, fullgraph=True, backend="aot_eager")
+    for k in (3, 9):
+        seed = torch.tensor([k], device=dev)
+        runs = []
+        for f in (layer, compiled):
+            y = f(*leaves, seed)
+            runs.append([y.detach(), *torch.autograd.grad(y, leaves, dh.to(dev))])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 # --- streams, graphs ---------------------------------------------------------------------------
 
 def test_layers_on_a_side_stream(dev):

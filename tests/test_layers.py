@@ -123,6 +123,43 @@ def test_cpu_tensors_and_types_are_refused():
         ppo_amd.dropout([1.0], 0.1, 1)
 
 
+SCHEMAS = {
+    "dropout": "ppo_amd::dropout(Tensor x, float p, SymInt seed, Tensor? seed_at, Tensor? rows) "
+               "-> Tensor",
+    "gated_ffn": "ppo_amd::gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, "
+                 "Tensor? b_up, str activation, float dropout_p, SymInt seed, Tensor? seed_at, "
+                 "Tensor? rows) -> (Tensor, Tensor)",
+    "quantize_rows": "ppo_amd::quantize_rows(Tensor x) -> (Tensor, Tensor)",
+    "int8_linear": "ppo_amd::int8_linear(Tensor x, Tensor weight, Tensor weight_scale, "
+                   "Tensor? bias, Tensor? x_scale, ScalarType? out_dtype) -> Tensor",
+}
+
+
+@pytest.mark.parametrize("name", sorted(SCHEMAS))
+def test_operator_schema(name):
+    assert str(getattr(torch.ops.ppo_amd, name).default._schema) == SCHEMAS[name]
+
+
+def test_operators_fake_shapes_and_cpu():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    op = torch.ops.ppo_amd
+    with FakeTensorMode():
+        x, w, b = (torch.empty(s, device="cuda", dtype=torch.bfloat16)
+                   for s in ((3, 5, 8), (7, 8), (7,)))
+        assert op.dropout(x, 0.1, 1, None, None).shape == (3, 5, 8)
+        h, saved = op.gated_ffn(x, w, w, b, b, "silu", 0.1, 1, None, None)
+        assert h.shape == (3, 5, 7) and h.dtype == torch.bfloat16
+        assert saved.shape == (2, 15, 8) and saved.dtype == torch.float32
+        grads = op.gated_ffn_backward(h, x, w, w, saved, True, "silu", 0.1, 1, None, None)
+        assert [g.shape for g in grads] == [(3, 5, 8), (7, 8), (7, 8), (7,), (7,)]
+        q, s = op.quantize_rows(w)
+        assert q.shape == (7, 8) and q.dtype == torch.int8 and s.shape == (7,)
+        assert op.int8_linear(x, q, s, None, None, None).shape == (3, 5, 7)
+    with pytest.raises(NotImplementedError):
+        op.dropout(torch.zeros(2, 2), 0.1, 1, None, None)
+
+
 def test_module_arguments():
     with pytest.raises(ValueError):
         ppo_amd.GatedLinear(4, 4, activation="swish")

@@ -137,6 +137,33 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, rows: Optional[torch.Tensor] 
 # ---------------------------------------------------------------------------
 # Gated feed-forward block
 # ---------------------------------------------------------------------------
+def _check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, rows) -> int:
+    """Refuses what the kernels do not take; the activation's number."""
+    _require(x, "x", tuple(DTYPES))
+    device, dtype = x.device, (x.dtype,)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must be [..., D] with D > 0, got {tuple(x.shape)}")
+    D = x.shape[-1]
+    _require(w_gate, "w_gate", dtype, device)
+    _require(w_up, "w_up", dtype, device)
+    if w_gate.dim() != 2 or w_gate.shape[1] != D or w_gate.shape[0] == 0:
+        raise ValueError(f"w_gate must be [F,{D}] with F > 0, got {tuple(w_gate.shape)}")
+    if w_up.shape != w_gate.shape:
+        raise ValueError(f"w_up must be {tuple(w_gate.shape)}, got {tuple(w_up.shape)}")
+    F = w_gate.shape[0]
+    if (b_gate is None) != (b_up is None):
+        raise ValueError("b_gate and b_up go together")
+    for b, name in ((b_gate, "b_gate"), (b_up, "b_up")):
+        if b is not None:
+            _require(b, name, dtype, device)
+            if b.shape != (F,):
+                raise ValueError(f"{name} must be [{F}], got {tuple(b.shape)}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    _check_drop(dropout_p, seed, rows, x.numel() // D, device)
+    return ACTIVATIONS[activation]
+
+
 def _gated_forward(x, wg, wu, bg, bu, act, p, seed, rows, save):
     D, F = x.shape[-1], wg.shape[0]
     M, device, dtype = x.numel() // D, x.device, DTYPES[x.dtype]
@@ -155,6 +182,31 @@ def _gated_forward(x, wg, wu, bg, bu, act, p, seed, rows, save):
     return h, saved
 
 
+def _gated_backward(dh, x, wg, wu, saved, act, p, seed, rows, need):
+    """dx, dwg, dwu, dbg, dbu; None for those that `need` does not ask for."""
+    D, F = x.shape[-1], wg.shape[0]
+    M, device, dtype = x.numel() // D, x.device, DTYPES[x.dtype]
+    new = torch.empty if M else torch.zeros
+    like = dict(dtype=x.dtype, device=device)
+    dx = torch.empty_like(x) if need[0] else None
+    dwg = dwu = dbg = dbu = None
+    if need[1] or need[2]:
+        dwg, dwu = new((F, D), **like), new((F, D), **like)
+    if need[3] or need[4]:
+        dbg, dbu = new(F, **like), new(F, **like)
+    if M:
+        drop = _drop(p, seed, rows)
+        with _on(device):
+            nbytes = _lib.load_layers().ppo_layer_gated_backward_workspace_bytes(dtype, M, D, F)
+            ws = _workspace(nbytes, device)
+            _call("ppo_layer_gated_backward", dh.data_ptr(), x.data_ptr(), wg.data_ptr(),
+                  wu.data_ptr(), saved.data_ptr(), dtype, M, D, F, act, ctypes.byref(drop),
+                  _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu), _ptr(ws), nbytes,
+                  _stream(device))
+    return (dx, dwg if need[1] else None, dwu if need[2] else None, dbg if need[3] else None,
+            dbu if need[4] else None)
+
+
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, bg, bu, act, p, seed, rows):
@@ -170,29 +222,9 @@ class _GatedFFN(torch.autograd.Function):
             raise RuntimeError("gated_ffn can be differentiated once: its backward pass has no "
                                "create_graph")
         x, wg, wu, saved, seed, rows = ctx.saved_tensors
-        D, F = x.shape[-1], wg.shape[0]
-        M, device, dtype = x.numel() // D, x.device, DTYPES[x.dtype]
-        need = ctx.needs_input_grad
-        new = torch.empty if M else torch.zeros
-        like = dict(dtype=x.dtype, device=device)
-        dx = torch.empty_like(x) if need[0] else None
-        dwg = dwu = dbg = dbu = None
-        if need[1] or need[2]:
-            dwg, dwu = new((F, D), **like), new((F, D), **like)
-        if need[3] or need[4]:
-            dbg, dbu = new(F, **like), new(F, **like)
-        if M:
-            dh = dh.contiguous()
-            drop = _drop(ctx.p, ctx.seed if seed is None else seed, rows)
-            with _on(device):
-                nbytes = _lib.load_layers().ppo_layer_gated_backward_workspace_bytes(dtype, M, D, F)
-                ws = _workspace(nbytes, device)
-                _call("ppo_layer_gated_backward", dh.data_ptr(), x.data_ptr(), wg.data_ptr(),
-                      wu.data_ptr(), saved.data_ptr(), dtype, M, D, F, ctx.act,
-                      ctypes.byref(drop), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu),
-                      _ptr(ws), nbytes, _stream(device))
-        return (dx, dwg if need[1] else None, dwu if need[2] else None,
-                dbg if need[3] else None, dbu if need[4] else None, None, None, None, None)
+        grads = _gated_backward(dh.contiguous(), x, wg, wu, saved, ctx.act, ctx.p,
+                                ctx.seed if seed is None else seed, rows, ctx.needs_input_grad)
+        return (*grads, None, None, None, None)
 
 
 def gated_ffn(
@@ -220,29 +252,7 @@ def gated_ffn(
                                     ACTIVATIONS.get(activation), dropout_p, seed, rows)
     if got is not None:
         return got
-    _require(x, "x", tuple(DTYPES))
-    device, dtype = x.device, (x.dtype,)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"x must be [..., D] with D > 0, got {tuple(x.shape)}")
-    D = x.shape[-1]
-    _require(w_gate, "w_gate", dtype, device)
-    _require(w_up, "w_up", dtype, device)
-    if w_gate.dim() != 2 or w_gate.shape[1] != D or w_gate.shape[0] == 0:
-        raise ValueError(f"w_gate must be [F,{D}] with F > 0, got {tuple(w_gate.shape)}")
-    if w_up.shape != w_gate.shape:
-        raise ValueError(f"w_up must be {tuple(w_gate.shape)}, got {tuple(w_up.shape)}")
-    F = w_gate.shape[0]
-    if (b_gate is None) != (b_up is None):
-        raise ValueError("b_gate and b_up go together")
-    for b, name in ((b_gate, "b_gate"), (b_up, "b_up")):
-        if b is not None:
-            _require(b, name, dtype, device)
-            if b.shape != (F,):
-                raise ValueError(f"{name} must be [{F}], got {tuple(b.shape)}")
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    _check_drop(dropout_p, seed, rows, x.numel() // D, device)
-    act = ACTIVATIONS[activation]
+    act = _check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, rows)
     leaves = (x, w_gate, w_up, b_gate, b_up)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
         return _GatedFFN.apply(*leaves, act, dropout_p, seed, rows)

@@ -19,6 +19,16 @@ tensor raises NotImplementedError, as there is no CPU fallback.
       returns, values, old_values?, clip_ratio, vf_clip?, value_coef,
       entropy_coef) -> (scalars[6], dmu, dlog_std, dvalues)
 
+  ppo_amd::dropout(x, p, seed, seed_at?, rows?) -> y
+  ppo_amd::gated_ffn(x, w_gate, w_up, b_gate?, b_up?, activation, dropout_p,
+      seed, seed_at?, rows?) -> (h, saved), saved what the backward pass reads
+  ppo_amd::gated_ffn_backward(dh, x, w_gate, w_up, saved, bias, activation,
+      dropout_p, seed, seed_at?, rows?) -> (dx, dw_gate, dw_up, db_gate, db_up)
+  ppo_amd::quantize_rows(x) -> (q, scale)
+  ppo_amd::int8_linear(x, weight, weight_scale, bias?, x_scale?, out_dtype?) -> y
+      the layers of layers.py; a seed that changes from call to call goes
+      into `seed_at` (int64 [1] on the device), which `seed` stands back for
+
 The loss operators are differentiable in their first output: backward of
 scalars[0] (the total loss; the other scalars are reported values) scales the
 fused kernel's gradients by the incoming gradient, as ops.ppo_loss_discrete
@@ -30,7 +40,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import _lib, ops
+from . import _lib, layers, ops
 
 _NS = "ppo_amd"
 
@@ -144,3 +154,116 @@ def _gaussian_backward(ctx, grad_scalars, grad_dmu, grad_dlog_std, grad_dvalues)
 
 
 ppo_loss_gaussian.register_autograd(_gaussian_backward, setup_context=_gaussian_setup)
+
+
+# ---------------------------------------------------------------------------
+# Feed-forward layers
+# ---------------------------------------------------------------------------
+def _seed(seed: int, seed_at: Optional[Tensor]):
+    return seed if seed_at is None else seed_at
+
+
+@torch.library.custom_op(f"{_NS}::dropout", mutates_args=(), device_types="cuda")
+def dropout(x: Tensor, p: float, seed: int, seed_at: Optional[Tensor],
+            rows: Optional[Tensor]) -> Tensor:
+    y = layers.dropout(x, p, _seed(seed, seed_at), rows)
+    return y.clone() if y is x else y
+
+
+@dropout.register_fake
+def _dropout_fake(x, p, seed, seed_at, rows):
+    return torch.empty_like(x)
+
+
+def _dropout_setup(ctx, inputs, output):
+    _, ctx.p, ctx.seed, seed_at, rows = inputs
+    ctx.save_for_backward(seed_at, rows)
+
+
+def _dropout_backward(ctx, dy):
+    seed_at, rows = ctx.saved_tensors
+    return dropout(dy.contiguous(), ctx.p, ctx.seed, seed_at, rows), None, None, None, None
+
+
+dropout.register_autograd(_dropout_backward, setup_context=_dropout_setup)
+
+
+@torch.library.custom_op(f"{_NS}::gated_ffn", mutates_args=(), device_types="cuda")
+def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tensor],
+              b_up: Optional[Tensor], activation: str, dropout_p: float, seed: int,
+              seed_at: Optional[Tensor], rows: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    s = _seed(seed, seed_at)
+    act = layers._check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, s, rows)
+    return layers._gated_forward(x, w_gate, w_up, b_gate, b_up, act, dropout_p, s, rows, True)
+
+
+@gated_ffn.register_fake
+def _gated_ffn_fake(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, seed_at, rows):
+    F = w_gate.shape[0]
+    M = 1
+    for n in x.shape[:-1]:
+        M = M * n
+    return (x.new_empty((*x.shape[:-1], F)),
+            x.new_empty((2, M, (F + 3) // 4 * 4), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::gated_ffn_backward", mutates_args=(), device_types="cuda")
+def gated_ffn_backward(dh: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, saved: Tensor,
+                       bias: bool, activation: str, dropout_p: float, seed: int,
+                       seed_at: Optional[Tensor], rows: Optional[Tensor]
+                       ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    need = (True, True, True, bias, bias)
+    dx, dwg, dwu, dbg, dbu = layers._gated_backward(
+        dh, x, w_gate, w_up, saved, layers.ACTIVATIONS[activation], dropout_p,
+        _seed(seed, seed_at), rows, need)
+    return (dx, dwg, dwu, x.new_empty(0) if dbg is None else dbg,
+            x.new_empty(0) if dbu is None else dbu)
+
+
+@gated_ffn_backward.register_fake
+def _gated_ffn_backward_fake(dh, x, w_gate, w_up, saved, bias, activation, dropout_p, seed,
+                             seed_at, rows):
+    F = w_gate.shape[0] if bias else 0
+    return (torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up),
+            x.new_empty(F), x.new_empty(F))
+
+
+def _gated_setup(ctx, inputs, output):
+    x, w_gate, w_up, b_gate, _, ctx.activation, ctx.p, ctx.seed, seed_at, rows = inputs
+    ctx.bias = b_gate is not None
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, w_gate, w_up, output[1], seed_at, rows)
+
+
+def _gated_backward(ctx, dh, _):
+    x, w_gate, w_up, saved, seed_at, rows = ctx.saved_tensors
+    dx, dwg, dwu, dbg, dbu = gated_ffn_backward(dh.contiguous(), x, w_gate, w_up, saved, ctx.bias,
+                                                ctx.activation, ctx.p, ctx.seed, seed_at, rows)
+    return (dx, dwg, dwu, dbg if ctx.bias else None, dbu if ctx.bias else None, None, None, None,
+            None, None)
+
+
+gated_ffn.register_autograd(_gated_backward, setup_context=_gated_setup)
+
+
+@torch.library.custom_op(f"{_NS}::quantize_rows", mutates_args=(), device_types="cuda")
+def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
+    return layers.quantize_rows(x)
+
+
+@quantize_rows.register_fake
+def _quantize_rows_fake(x):
+    return (x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::int8_linear", mutates_args=(), device_types="cuda")
+def int8_linear(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
+                x_scale: Optional[Tensor], out_dtype: Optional[torch.dtype]) -> Tensor:
+    return layers.int8_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
+
+
+@int8_linear.register_fake
+def _int8_linear_fake(x, weight, weight_scale, bias, x_scale, out_dtype):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]),
+                       dtype=x.dtype if out_dtype is None else out_dtype)
