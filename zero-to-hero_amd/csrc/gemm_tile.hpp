@@ -667,15 +667,17 @@ constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay belo
 // the least expected time in us.  A workgroup takes `step` a K step and `fixed`
 // for its start and epilogue while it shares its CU (what the CU gets done),
 // and at least `alone` a step and `lone` where it waits for memory; a split
-// adds a second launch, and its partial sums are written and read again.
-// Measured on MI355X (us, bf16 unless said), tile 256 / 128 / 64 without split:
-// gated 4096 x 1024 -> 2048 41.5 / 41.7 / 59.6, 1024 x 2048 -> 2048 49 / 28 / 26,
-// fp32 4096 x 512 -> 1024 134 / 74 / 102; 128 in two splits 79, 33 and 90;
-// fp32 1024 x 1024 -> 512 in 64s and one, two or four splits 40 / 43 / 31.  The
-// rows kernel's time is that of reading W, more for the second to fourth
-// sixteen rows: 16, 32 and 64 rows of 4096 -> 8192 gated 26, 31 and 46, against
-// 25, 26 and 27 for tiles of 64 in two splits; fp32 4096 -> 4096 25, 33 and 52
-// against 44, 44 and 47.
+// adds a launch, and its partial sums are written and read again (in the
+// caches).  The numbers are fitted to 60 products of 64 to 11000 rows, 64 to
+// 16384 columns and 1 to 96 steps, each in up to 12 cuts: the cut chosen takes
+// 1.5% longer than the best on average.  Measured on MI355X (us, bf16 unless
+// said), tile 256 / 128 / 64 without split: gated 4096 x 1024 -> 2048 41 / 42 / 60,
+// 1024 x 2048 -> 2048 49 / 28 / 26, fp32 4096 x 512 -> 1024 134 / 74 / 102; 128 in
+// two splits 79, 33 and 90; fp32 1024 x 1024 -> 512 in 64s and one, two or four
+// splits 40 / 43 / 31.  The rows kernel's time is that of reading W, more for the
+// second to fourth sixteen rows: 16, 32 and 64 rows of 4096 -> 8192 gated 26, 31
+// and 46, against 25, 26 and 27 for tiles of 64 in two splits; fp32 4096 -> 4096
+// 25, 33 and 52 against 44, 44 and 47.
 inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
                           bool by_k_rows = false) {
   GemmPlan p = {-1, 1, 0};
@@ -687,9 +689,9 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
   }
   struct Cost { int tile, per_cu; double step[2], alone[2], fixed, lone; };
   static const Cost kCosts[] = {
-      {256, 1, {1.05, 7.4}, {1.15, 7.4}, 12.0, 12.0},
-      {128, 2, {0.29, 1.9}, {0.65, 1.95}, 5.0, 8.0},
-      {64, 5, {0.10, 0.62}, {0.55, 1.0}, 1.9, 6.0},
+      {256, 1, {0.95, 7.2}, {1.11, 7.2}, 17.6, 10.7},
+      {128, 2, {0.32, 1.8}, {0.52, 2.0}, 4.2, 7.8},
+      {64, 5, {0.19, 0.90}, {0.44, 1.08}, 1.75, 4.6},
   };
   const double steps = (double)div_up(kbytes, kStepBytes);
   for (const Cost& c : kCosts) {
@@ -699,8 +701,7 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
       const double each = ceil(steps / splits);
       const double busy = ceil(groups / kCus) * (each * c.step[fp32] + c.fixed);
       const double waits = ceil(groups / (kCus * c.per_cu)) * (each * c.alone[fp32] + c.lone);
-      // 6 us for the launch, and the sums at 7 TB/s (they stay in the caches)
-      const double join = splits > 1 ? 6.0 + splits * 8.0 * M * wrows / 7e6 : 0.0;
+      const double join = splits > 1 ? 4.0 + splits * 8.0 * M * wrows / 13.6e6 : 0.0;
       const double time = fmax(busy, waits) + join;
       if (p.tile < 0 || time < best) {
         best = time;
