@@ -11,8 +11,11 @@
  * calls on different streams need no ordering as long as their outputs and
  * workspaces differ.
  *
- * Matrices are `dtype` (fp32, bf16 or fp16) with rows of any width; sums,
- * activations and scales are held in fp32 and rounded once, to nearest even.
+ * Matrices are `dtype` (fp32, bf16 or fp16) with rows of any width and any
+ * alignment; sums, activations and scales are held in fp32 and rounded once, to
+ * nearest even.  The products take up to 2^28 - 1 rows, and rows (of x and the
+ * weights, and of 2 F elements in the backward pass) below 4 MiB:
+ * PPO_ERR_TOO_LARGE otherwise.
  */
 #ifndef PPO_LAYERS_H
 #define PPO_LAYERS_H
@@ -102,7 +105,8 @@ int ppo_layer_gated_forward(const void* x, const void* wg, const void* wu, const
  *   dh' = dropout(dh),  du = dh' * act(g),  dg = dh' * u * act'(g)
  *   dx = dg wg + du wu,  dwg = dg^T x,  dwu = du^T x,  dbg, dbu = column sums
  * Outputs that are NULL are not computed (dwg and dwu, and dbg and dbu, go
- * together).  dg and du are rounded to `dtype`, the matrix cores' operand
+ * together).  M > 0 (over no rows the weights' gradients are the caller's
+ * zeros).  dg and du are rounded to `dtype`, the matrix cores' operand
  * type, before the products.  Sums are split and joined in a fixed order:
  * the same inputs give the same bits.
  */

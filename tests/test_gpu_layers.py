@@ -522,6 +522,23 @@ def test_gated_values_that_are_not_finite(dev, M):
     assert torch.equal(h[ok], clean[ok])
 
 
+def test_gated_dropped_values_that_are_not_finite(dev):
+    """Where an infinite g or u is dropped, h is 0 and so are its gradients."""
+    x = torch.ones(64, 8, device=dev)
+    wg, wu = torch.full((12, 8), 0.1, device=dev), torch.full((12, 8), 0.1, device=dev)
+    keep = torch.from_numpy(ref.keep_mask(0.5, 21, np.arange(64), 12)).to(dev)
+    row, col = 5, int((~keep[5]).nonzero()[0])
+    x[row, 0] = 1e30
+    wu[col, 0] = 1e30  # u[row, col] = inf; the column's other elements stay finite
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    h = ppo_amd.gated_ffn(*leaves, activation="tanh", dropout_p=0.5, seed=21)
+    assert h[row, col] == 0
+    pick = torch.zeros_like(h)
+    pick[row, col] = 1.0
+    for g in torch.autograd.grad(h, leaves, pick, retain_graph=True):
+        assert not bool(g.any())
+
+
 def test_gated_refusals(dev):
     x, w, b = torch.randn(4, 8, device=dev), torch.randn(6, 8, device=dev), torch.randn(6, device=dev)
     f = ppo_amd.gated_ffn
@@ -548,6 +565,65 @@ def test_gated_refusals(dev):
     rows += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+# --- offsets past 32 bits ----------------------------------------------------------------
+
+def test_offsets_past_32_bits(dev):
+    """Tensors of more than 2^32 bytes and 2^31 elements: their last rows are
+    what the same rows give alone."""
+    M, C = 70001, 32768  # 2.3e9 elements
+    last = torch.tensor([0, 1, 40000, 65535, 65536, M - 2, M - 1])
+    x = torch.empty(M, C, dtype=torch.bfloat16, device=dev)
+    x[:] = torch.randn(C, device=dev).bfloat16()
+    some = torch.randn(len(last), C, device=dev).bfloat16()
+    x[last.to(dev)] = some
+    y = ppo_amd.dropout(x, 0.5, 3)
+    assert torch.equal(y[last.to(dev)], ppo_amd.dropout(some, 0.5, 3, rows=last.to(dev)))
+    del y
+    q, s = ppo_amd.quantize_rows(x)
+    q1, s1 = ppo_amd.quantize_rows(some)
+    assert torch.equal(q[last.to(dev)], q1) and torch.equal(s[last.to(dev)], s1)
+    w, ws = ppo_amd.quantize_rows(torch.randn(64, C, device=dev))
+    full = ppo_amd.int8_linear(q, w, ws, x_scale=s, out_dtype=torch.bfloat16)  # long rows in
+    assert torch.equal(full[last.to(dev)],
+                       ppo_amd.int8_linear(q1, w, ws, x_scale=s1, out_dtype=torch.bfloat16))
+    del q, full, x
+    torch.cuda.empty_cache()
+    a = torch.randn(M, 64, device=dev).bfloat16()
+    wg, wu = (torch.randn(C, 64, device=dev).bfloat16() / 8 for _ in range(2))
+    wq, ws = ppo_amd.quantize_rows(wg)
+    few = a[last.to(dev)].contiguous()
+    with torch.no_grad():  # large results out
+        h = ppo_amd.gated_ffn(a, wg, wu)
+        torch.testing.assert_close(h[last.to(dev)].float(), ppo_amd.gated_ffn(few, wg, wu).float(),
+                                   rtol=2 ** -7, atol=1e-5)
+        del h
+        z = ppo_amd.int8_linear(a, wq, ws)
+        assert torch.equal(z[last.to(dev)], ppo_amd.int8_linear(few, wq, ws))
+
+
+def test_gradients_past_32_bits(dev):
+    """A backward pass whose dg and du take 9 GB: its sums over 70001 rows
+    against 64-bit products of the same in slices."""
+    M, D, F = 70001, 24, 16384
+    g = torch.Generator(device=dev).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=g)  # noqa: E731
+    x = rnd(M, D).bfloat16().requires_grad_()
+    wg, wu = ((rnd(F, D) * D ** -0.5).bfloat16().requires_grad_() for _ in range(2))
+    dh = rnd(M, F).bfloat16() * 0.1
+    grads = torch.autograd.grad(ppo_amd.gated_ffn(x, wg, wu), [x, wg, wu], dh)
+    d = [t.detach().double() for t in (x, wg, wu)]
+    want = [torch.zeros_like(t) for t in d]
+    for i in range(0, M, 4096):
+        xs = d[0][i:i + 4096]
+        _, gg, uu = ref.gated_ffn(xs, d[1], d[2], None, None, "silu")
+        got = ref.gated_ffn_grads(xs, d[1], d[2], gg, uu, "silu", dh[i:i + 4096].double())
+        want[0][i:i + 4096] = got[0]
+        want[1] += got[1]
+        want[2] += got[2]
+    for got, w, name in zip(grads, want, ("dx", "dwg", "dwu")):
+        check_grad(got, w.cpu(), torch.bfloat16, name)
 
 
 # --- the native host path ----------------------------------------------------------------
@@ -636,51 +712,6 @@ def test_forward_mode_and_batched_gradients_are_refused(dev):
         with pytest.raises(RuntimeError):
             torch.autograd.grad(out, [y], torch.ones(2, *out.shape, device=dev),
                                 is_grads_batched=True)
-
-
-# --- registered operators ----------------------------------------------------------------
-
-def test_registered_operators(dev):
-    """opcheck on each operator, and the functions' bits."""
-    op = torch.ops.ppo_amd
-    x, wg, wu, bg, bu, dh = gated_case("fp32", 20, 24, 36, True)
-    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
-    rows, seed = torch.arange(20, device=dev) * 3, torch.tensor([4], device=dev)
-    utils = ("test_schema", "test_autograd_registration", "test_faketensor")
-    torch.library.opcheck(op.dropout, (leaves[0], 0.3, 4, None, rows), test_utils=utils)
-    torch.library.opcheck(op.gated_ffn, (*leaves, "silu", 0.2, 0, seed, rows), test_utils=utils)
-    plain = [v.detach() for v in leaves]
-    torch.library.opcheck(op.quantize_rows, (plain[0],), test_utils=utils)
-    q, s = ppo_amd.quantize_rows(plain[1])
-    torch.library.opcheck(op.int8_linear, (plain[0], q, s, None, None, None), test_utils=utils)
-
-    h, _ = op.gated_ffn(*leaves, "silu", 0.2, 0, seed, rows)
-    z = op.dropout(h, 0.1, 4, None, rows)
-    got = [z.detach(), *torch.autograd.grad(z, leaves, dh.to(dev))]
-    h = ppo_amd.gated_ffn(*leaves, dropout_p=0.2, seed=seed, rows=rows)
-    z = ppo_amd.dropout(h, 0.1, 4, rows)
-    want = [z.detach(), *torch.autograd.grad(z, leaves, dh.to(dev))]
-    assert all(torch.equal(a, b) for a, b in zip(got, want))
-
-
-def test_registered_operators_compile(dev):
-    """A compiled layer with its backward is traced whole and equals eager."""
-    op = torch.ops.ppo_amd
-    x, wg, wu, bg, bu, dh = gated_case("fp32", 40, 24, 36, True)
-    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
-
-    def layer(x, wg, wu, bg, bu, seed):
-        h = op.gated_ffn(x, wg, wu, bg, bu, "gelu", 0.2, 0, seed, None)[0]
-        return op.dropout(h, 0.1, 0, seed, None) * 2.0
-
-    compiled = torch.compile(layer, fullgraph=True, backend="aot_eager")
-    for k in (3, 9):
-        seed = torch.tensor([k], device=dev)
-        runs = []
-        for f in (layer, compiled):
-            y = f(*leaves, seed)
-            runs.append([y.detach(), *torch.autograd.grad(y, leaves, dh.to(dev))])
-        assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
 # --- streams, graphs ---------------------------------------------------------------------------
@@ -824,6 +855,7 @@ def test_int8_copy_of_the_reference_networks(dev):
     mlp = ppo_amd.MLP(4, 128, 2).to(dev)
     eight = ppo_amd.int8_copy(mlp)
     assert isinstance(eight.net[0], ppo_amd.Int8Linear) and isinstance(mlp.net[0], torch.nn.Linear)
+    assert isinstance(ppo_amd.int8_copy(mlp.net[0]), ppo_amd.Int8Linear)
     obs = torch.randn(50, 4, device=dev)
     # by hand, through the oracle
     x = obs.cpu()

@@ -206,12 +206,14 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
     float v[4], dg[4], du[4], a[4], da[4];
     const float gs[4] = {g[i][0], g[i][1], g[i][2], g[i][3]};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = to_f32(d[i].x[k]);
-    if (drop.mode) drop4(drop, seed, (uint64_t)id[i], (uint32_t)n >> 2, v);
+    for (int k = 0; k < 4; ++k) v[k] = to_f32(d[i].x[k]) * drop.scale;
+    // (a dropped element has no gradient, also where g or u is not finite)
+    bool keep[4];
+    keep4(drop, seed, (uint64_t)id[i], (uint32_t)n >> 2, keep);
     activate_grad<T>(act, gs, a, da);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const bool live = m < M && n + k < F;  // (what is behind F is not the saved values')
+      const bool live = keep[k] && m < M && n + k < F;  // (behind F lies nothing that was saved)
       du[k] = live ? v[k] * a[k] : 0.0f;
       dg[k] = live ? v[k] * u[i][k] * da[k] : 0.0f;
       su[k] += du[k];

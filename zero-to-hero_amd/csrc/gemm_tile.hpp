@@ -6,9 +6,10 @@
 //
 // Everything is laid out in 16-byte chunks of a row: 4 fp32, 8 16-bit or 16
 // int8 elements.  A lane of the matrix instructions below holds one chunk of
-// row lane % 16 (16x16x32 on 16-bit types and 16x16x64 on int8 take the whole
-// chunk; fp32 takes four 16x16x4 steps, one element each: the order of k
-// inside a step is free as long as both operands share it).  So one kernel
+// row lane % 32 or lane % 16 (32x32x16 and 16x16x32 on 16-bit types, 32x32x32
+// and 16x16x64 on int8 take the whole chunk; fp32 takes four instructions, one
+// element each: the order of k inside a step is free as long as both operands
+// share it).  So one kernel
 // serves all types.  W is the instruction's first operand, so a lane ends up
 // with four consecutive columns n of one row m: a vector store, and one call
 // of the dropout generator.

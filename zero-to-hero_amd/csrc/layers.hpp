@@ -234,17 +234,26 @@ __device__ __forceinline__ uint64_t dropout_seed(const Dropout& d) {
   return d.seed_at ? *d.seed_at : d.seed;
 }
 
-// Multipliers of four columns from 4 * group on: dropped elements are
-// selected away, not multiplied by zero, so an infinity or a NaN there goes.
+// Which of the four columns from 4 * group on are kept.
+__device__ __forceinline__ void keep4(const Dropout& d, uint64_t seed, uint64_t row, uint32_t group,
+                                      bool (&keep)[4]) {
+  uint4 w = make_uint4(0, 0, 0, 0);
+  if (d.mode == 1) w = philox(seed, group, row);
+  keep[0] = d.mode == 0 || w.x < d.keep;  // (mode 2: below 0)
+  keep[1] = d.mode == 0 || w.y < d.keep;
+  keep[2] = d.mode == 0 || w.z < d.keep;
+  keep[3] = d.mode == 0 || w.w < d.keep;
+}
+
+// Dropout of those columns: dropped elements are selected away, not multiplied
+// by zero, so an infinity or a NaN there goes.
 __device__ __forceinline__ void drop4(const Dropout& d, uint64_t seed, uint64_t row,
                                       uint32_t group, float (&v)[4]) {
   if (d.mode == 0) return;
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (d.mode == 1) w = philox(seed, group, row);
-  v[0] = w.x < d.keep ? v[0] * d.scale : 0.0f;
-  v[1] = w.y < d.keep ? v[1] * d.scale : 0.0f;
-  v[2] = w.z < d.keep ? v[2] * d.scale : 0.0f;
-  v[3] = w.w < d.keep ? v[3] * d.scale : 0.0f;
+  bool keep[4];
+  keep4(d, seed, row, group, keep);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = keep[i] ? v[i] * d.scale : 0.0f;
 }
 
 }  // namespace ppo

@@ -447,13 +447,10 @@ class _Int8Gated(nn.Module):
 
 def int8_copy(module: nn.Module) -> nn.Module:
     """A copy of `module` for acting, with every nn.Linear and GatedLinear in
-    it (agent.MLP's and GatedMLP's among them) replaced by its 8-bit copy.
-    The copy does not follow later updates: take a new one per rollout."""
-    if isinstance(module, nn.Linear):
-        return Int8Linear(module)
-    if isinstance(module, GatedLinear):
-        return _Int8Gated(module)
-    found = [m for m in module.modules() if isinstance(m, (nn.Linear, GatedLinear))]
+    it (agent.MLP's and GatedMLP's among them; subclasses stay as they are)
+    replaced by its 8-bit copy.  The copy does not follow later updates: take a
+    new one per rollout."""
+    eight = {nn.Linear: Int8Linear, GatedLinear: _Int8Gated}
     # (deepcopy takes what the memo already holds in place of a copy)
-    memo = {id(m): Int8Linear(m) if isinstance(m, nn.Linear) else _Int8Gated(m) for m in found}
+    memo = {id(m): eight[type(m)](m) for m in module.modules() if type(m) in eight}
     return copy.deepcopy(module, memo)
