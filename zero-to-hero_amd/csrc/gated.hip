@@ -63,8 +63,8 @@ struct GatedEpi {
         const v4f vg = {g[4 * b], g[4 * b + 1], g[4 * b + 2], g[4 * b + 3]};
         const v4f vu = {u[4 * b], u[4 * b + 1], u[4 * b + 2], u[4 * b + 3]};
         if (live[b]) {
-          *reinterpret_cast<v4f*>(s) = vg;
-          *reinterpret_cast<v4f*>(s + half) = vu;
+          __builtin_nontemporal_store(vg, reinterpret_cast<v4f*>(s));
+          __builtin_nontemporal_store(vu, reinterpret_cast<v4f*>(s + half));
         }
       }
     }
@@ -75,7 +75,7 @@ struct GatedEpi {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = a[4 * b + i] * u[4 * b + i];
       if (drop.mode) drop4(drop, dropout_seed(drop), (uint64_t)id[b], (uint32_t)n >> 2, v);
-      if (live[b]) store4(h + (int64_t)m[b] * F + n, v, F - n, (F & 3) == 0);
+      if (live[b]) store4<true>(h + (int64_t)m[b] * F + n, v, F - n, (F & 3) == 0);
     }
   }
 };
@@ -105,7 +105,7 @@ struct StoreEpi {
       const int at = other ? m[b] - second : m[b];
       const float v[4] = {c[b][0], c[b][1], c[b][2], c[b][3]};
       if (live[b] && at < rows)
-        store4((other ? out1 : out0) + (int64_t)at * N + n, v, N - n, (N & 3) == 0);
+        store4<true>((other ? out1 : out0) + (int64_t)at * N + n, v, N - n, (N & 3) == 0);
     }
   }
 };

@@ -58,13 +58,20 @@ int with_dtype(int dtype, F&& f) {
 
 // Four consecutive elements, stored together where p allows it (`vec`: the
 // row's start and pitch are multiples of four elements), else those in range.
-template <class T>
+// kStream: results that this kernel and the next do not read again leave the
+// L2 to the operands (int8 8192 x 8192 x 4096 267 -> 252 us, gated
+// 8192 x 4096 -> 8192 with g and u saved 971 -> 904).
+template <bool kStream = false, class T>
 __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count, bool vec) {
   struct __attribute__((aligned(4 * sizeof(T)))) Four { T x[4]; } q;
+  typedef int Words __attribute__((ext_vector_type(sizeof(T))));
 #pragma unroll
   for (int i = 0; i < 4; ++i) q.x[i] = from_f32<T>(v[i]);
   if (vec && count >= 4) {
-    *reinterpret_cast<Four*>(p) = q;
+    if (kStream)
+      __builtin_nontemporal_store(__builtin_bit_cast(Words, q), reinterpret_cast<Words*>(p));
+    else
+      *reinterpret_cast<Four*>(p) = q;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
