@@ -714,6 +714,41 @@ def test_forward_mode_and_batched_gradients_are_refused(dev):
                                 is_grads_batched=True)
 
 
+def test_tangents_without_requires_grad_are_refused(dev):
+    import torch.autograd.forward_ad as fwad
+
+    x, w = torch.randn(4, 8, device=dev), torch.randn(6, 8, device=dev)
+    wq, ws = ppo_amd.quantize_rows(w)
+    q, s = ppo_amd.quantize_rows(x)
+    bias = torch.zeros(6, device=dev)
+
+    def dual(t):
+        return fwad.make_dual(t, torch.ones_like(t))
+
+    for f in (lambda: ppo_amd.dropout(dual(x), 0.5, 1), lambda: ppo_amd.gated_ffn(dual(x), w, w),
+              lambda: ppo_amd.gated_ffn(x, w, dual(w)), lambda: ppo_amd.int8_linear(dual(x), wq, ws),
+              lambda: ppo_amd.int8_linear(x, wq, dual(ws)),
+              lambda: ppo_amd.int8_linear(x, wq, ws, dual(bias)),
+              lambda: ppo_amd.int8_linear(q, wq, ws, x_scale=dual(s), out_dtype=torch.float32)):
+        for mode in (torch.enable_grad, torch.no_grad):
+            with fwad.dual_level(), mode(), pytest.raises((RuntimeError, NotImplementedError)):
+                f()
+
+
+def test_int8_linear_refuses_scales_that_learn(dev):
+    x = torch.randn(4, 8, device=dev)
+    wq, ws = ppo_amd.quantize_rows(torch.randn(6, 8, device=dev))
+    q, s = ppo_amd.quantize_rows(x)
+    learnt = [t.clone().requires_grad_() for t in (ws, s)]
+    calls = (lambda: ppo_amd.int8_linear(x, wq, learnt[0]),
+             lambda: ppo_amd.int8_linear(q, wq, ws, x_scale=learnt[1], out_dtype=torch.float32))
+    for f in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            f()
+        with torch.no_grad():
+            assert f().shape == (4, 6)
+
+
 # --- streams, graphs ---------------------------------------------------------------------------
 
 def test_layers_on_a_side_stream(dev):

@@ -8,9 +8,10 @@ namespace ppo {
 namespace {
 
 // A thread takes 16 bytes of a row (four columns in 32 bits, eight in 16), so
-// that a wave's store is one run of whole lines; stored past the L2, which y
-// rarely fits (bf16 16384 x 8192 106 -> 90 us, fp32 8192 x 8192 94 -> 83).  A workgroup is kX threads along
-// the columns by 256 / kX rows, so narrow rows fill it too.
+// that a wave's store is one run of whole lines; it goes past the L2, which y
+// rarely fits (bf16 16384 x 8192 106 -> 90 us, fp32 8192 x 8192 94 -> 83, small
+// ones as before).  A workgroup is kX threads along the columns by 256 / kX
+// rows, so narrow rows fill it too.
 template <class T, bool kVec>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, int64_t rows, int64_t cols,
                                                       const Dropout d, int tx_bits) {

@@ -323,9 +323,9 @@ PyObject* int8_linear(PyObject* const* a) {  // x, weight, weight_scale, bias, x
     xs = plain(a[4], at::kFloat, dev);
     need(xs.sizes() == x.sizes().slice(0, x.dim() - 1));
   }
-  need(!needs_grad({&x, &bias}));
-  need_no_tangent(x);
-  need_no_tangent(bias);
+  need(!needs_grad({&x, &ws, &bias, &xs}));
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &ws, &bias, &xs})
+    need_no_tangent(*t);
   void* stream = current_stream(dev);
   at::AutoDispatchBelowADInplaceOrView below;
   Tensor out;

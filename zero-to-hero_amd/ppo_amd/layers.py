@@ -26,6 +26,7 @@ import math
 from typing import Optional, Union
 
 import torch
+import torch.autograd.forward_ad as fwd_ad
 from torch import nn
 
 from . import _lib
@@ -55,6 +56,13 @@ def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
 
 def _call(name: str, *args) -> None:
     _lib.check(name, getattr(_lib.load_layers(), name)(*args))
+
+
+def _wants_gradient(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a derivative would have to pass, in either direction."""
+    given = [t for t in tensors if t is not None]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in given)
+            or any(fwd_ad.unpack_dual(t).tangent is not None for t in given))
 
 
 def _check_drop(p: float, seed: Seed, rows: Optional[torch.Tensor], M: int, device) -> None:
@@ -254,7 +262,7 @@ def gated_ffn(
         return got
     act = _check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, rows)
     leaves = (x, w_gate, w_up, b_gate, b_up)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+    if _wants_gradient(*leaves):  # (a tangent is refused there)
         return _GatedFFN.apply(*leaves, act, dropout_p, seed, rows)
     return _gated_forward(*leaves, act, dropout_p, seed, rows, False)[0]
 
@@ -301,7 +309,8 @@ def int8_linear(
     of one x).  Sums are exact in int32 (K <= 131072), scales and bias applied
     in fp32, the result rounded once to out_dtype (default: x's type; needed
     for an int8 x).  bias [N] has the result's type.  For acting: not
-    differentiable, and refused for an x that requires a gradient."""
+    differentiable, and refused where x, a scale or the bias requires a
+    gradient."""
     got = _native().layer_int8_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
     if got is not None:
         return got
@@ -309,7 +318,7 @@ def int8_linear(
     device = x.device
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., K] with K > 0, got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if _wants_gradient(x, weight_scale, bias, x_scale):
         raise RuntimeError("int8_linear has no gradient: call it under torch.no_grad()")
     K = x.shape[-1]
     _require(weight, "weight", (torch.int8,), device)
