@@ -13,9 +13,9 @@
  *
  * Matrices are `dtype` (fp32, bf16 or fp16) with rows of any width and any
  * alignment; sums, activations and scales are held in fp32 and rounded once, to
- * nearest even.  The products take up to 2^28 - 1 rows, and rows (of x and the
- * weights, and of 2 F elements in the backward pass) below 4 MiB:
- * PPO_ERR_TOO_LARGE otherwise.
+ * nearest even.  The products take up to 2^26 rows of x and of each weight,
+ * rows (of x and the weights, and of 2 F elements in the backward pass) below
+ * 4 MiB, and up to 2^34 elements in a result: PPO_ERR_TOO_LARGE otherwise.
  */
 #ifndef PPO_LAYERS_H
 #define PPO_LAYERS_H
@@ -91,8 +91,8 @@ int ppo_layer_int8_linear(const void* x, const int8_t* xq, const float* xs, cons
  *   g = x wg^T + bg,  u = x wu^T + bu,  h = dropout(act(g) * u)
  * for x [M,D], wg and wu [F,D] (nn.Linear's layout), bg and bu [F] (both or
  * neither NULL), h [M,F].  drop may be NULL.  `saved`, when not NULL, is
- * fp32 [2][M][F4] with F4 = F rounded up to 4 and receives g and u for
- * ppo_layer_gated_backward.
+ * fp32 [2][M][F4] with F4 = F rounded up to 4, 16-byte aligned, and receives
+ * g and u for ppo_layer_gated_backward.
  */
 size_t ppo_layer_gated_workspace_bytes(int dtype, int64_t M, int64_t D, int64_t F);
 int ppo_layer_gated_forward(const void* x, const void* wg, const void* wu, const void* bg,

@@ -186,6 +186,16 @@ def test_quantize_rows_is_exact(dev, shape, dtype):
     assert np.array_equal(q.cpu().numpy(), wq)
 
 
+def test_quantize_rows_of_many_rows(dev):
+    """More rows than one launch's threads can be counted for."""
+    M = (1 << 26) + 5
+    x = torch.arange(M * 3, device=dev, dtype=torch.int32).view(M, 3).remainder_(251).half()
+    q, s = ppo_amd.quantize_rows(x)
+    at = torch.tensor([0, 1, (1 << 21) - 1, 1 << 21, (1 << 25) + 7, M - 2, M - 1], device=dev)
+    q1, s1 = ref.quantize_rows(x[at].float().cpu().numpy())
+    assert np.array_equal(q[at].cpu().numpy(), q1) and np.array_equal(s[at].cpu().numpy(), s1)
+
+
 def test_quantize_rows_ties(dev):
     """Quotients at ties and a few units in the last place to either side."""
     k = torch.arange(-126, 127).float() + 0.5

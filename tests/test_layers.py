@@ -112,6 +112,30 @@ def test_gated_arguments():
     assert bwd(work=ctypes.c_void_p(4097)) == 2
 
 
+def test_sizes_that_no_launch_holds():
+    lib = _lib.load_layers()
+    bytes_of = lib.ppo_layer_gated_workspace_bytes
+    back = lib.ppo_layer_gated_backward_workspace_bytes
+    eight = lib.ppo_layer_int8_linear_workspace_bytes
+    # the largest that are documented have a plan, twice as large ones none
+    assert bytes_of(0, 1 << 26, 8, 33) > 0 and back(0, 1 << 26, 8, 256) > 0
+    assert bytes_of(0, 65, 3, 1 << 26) > 0 and eight(1 << 26, 256, 8, 1) > 0
+    assert eight(65, 1 << 26, 7, 1) > 0
+    for M, D, F in ((1 << 28, 8, 33), (64, 8, 1 << 28), (1 << 26, 8, 1 << 10), (1 << 27, 8, 513)):
+        assert bytes_of(0, M, D, F) == 0 and back(0, M, D, F) == 0
+    assert eight(1 << 28, 8, 8, 1) == 0 and eight(8, 1 << 28, 8, 1) == 0
+    assert eight(1 << 26, 1 << 10, 8, 1) == 0
+
+
+def test_saved_alignment():
+    lib = _lib.load_layers()
+    odd = ctypes.c_void_p(4104)
+    assert lib.ppo_layer_gated_forward(P, P, P, None, None, 0, 4, 8, 8, 0, None, P, odd, P, 1 << 40,
+                                       None) == 1
+    assert lib.ppo_layer_gated_backward(P, P, P, P, odd, 0, 4, 8, 8, 0, None, P, P, P, None, None,
+                                        P, 1 << 40, None) == 1
+
+
 def test_cpu_tensors_and_types_are_refused():
     x, w = torch.zeros(4, 8), torch.zeros(6, 8)
     for call in (lambda: ppo_amd.dropout(x, 0.1, 1), lambda: ppo_amd.gated_ffn(x, w, w),

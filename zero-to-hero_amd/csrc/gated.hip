@@ -350,13 +350,13 @@ BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool alig
 bool sizes_ok(int64_t M, int64_t D, int64_t F) { return M >= 0 && D > 0 && F > 0; }
 // The products' operands within what the kernels index.
 bool forward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
-  const int64_t lim = (int64_t)1 << 28;
-  return M < lim && D < lim && F < lim && gemm_fits(M, 2 * F, round_up(D * dtype_size(dtype), 16));
+  return M <= kMaxRows && D <= kMaxRows && F <= kMaxRows &&
+         gemm_fits(M, 2 * F, round_up(D * dtype_size(dtype), 16));
 }
 bool backward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
   const int64_t size = dtype_size(dtype), pitch = 2 * round_up(F, 16) * size;
   return forward_fits(dtype, M, D, F) && gemm_fits(M, D, pitch) && gemm_fits(2 * F, D, pitch) &&
-         div_up(M, kTileM) * div_up(F + 8, kTileF) < ((int64_t)1 << 31);
+         div_up(M, kTileM) * div_up(F + 8, kTileF) < ((int64_t)1 << 24);  // 2^32 threads
 }
 
 // Padded copies of x [M,D] and of the weights [F,D] (those that are not NULL).
@@ -397,7 +397,7 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
       activation > PPO_LAYER_GELU || !bg != !bu)
     return PPO_ERR_INVALID_ARG;
   if (M == 0) return PPO_OK;
-  if (!x || !wg || !wu || !h) return PPO_ERR_INVALID_ARG;
+  if (!x || !wg || !wu || !h || !aligned16(saved)) return PPO_ERR_INVALID_ARG;
   if (!forward_fits(dtype, M, D, F)) return PPO_ERR_TOO_LARGE;
   const bool aligned = aligned16(x) && aligned16(wg) && aligned16(wu);
   const ForwardPlan f = plan_forward(dtype, M, D, F, aligned, (char*)workspace);
@@ -445,7 +445,8 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
       activation > PPO_LAYER_GELU || !dwg != !dwu || !dbg != !dbu)
     return PPO_ERR_INVALID_ARG;
   if (M == 0) return PPO_ERR_INVALID_ARG;  // (the sums over no rows are the caller's zeros)
-  if (!dh || !saved || (dwg && !x) || (dx && (!wg || !wu))) return PPO_ERR_INVALID_ARG;
+  if (!dh || !saved || !aligned16(saved) || (dwg && !x) || (dx && (!wg || !wu)))
+    return PPO_ERR_INVALID_ARG;
   if (!backward_fits(dtype, M, D, F)) return PPO_ERR_TOO_LARGE;
   const bool aligned = aligned16(x) && aligned16(wg) && aligned16(wu);
   const BackwardPlan b = plan_backward(dtype, M, D, F, aligned, (char*)workspace);

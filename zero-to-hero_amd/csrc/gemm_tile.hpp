@@ -661,6 +661,7 @@ struct GemmPlan {
 
 constexpr int kCus = 256;
 constexpr int kRowsMax = 64;       // rows that the rows kernel takes
+constexpr int64_t kMaxRows = (int64_t)1 << 27;   // of either operand
 constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay below 2^31 bytes
 
 // How a product of M rows and `wrows` rows of W (both matrices of a gated one
@@ -715,10 +716,11 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
   return p;
 }
 
-// Checks what the kernels assume of sizes.
+// Checks what the kernels assume of sizes (a grid's threads are counted in 32
+// bits: 128 for each of the smallest tiles, 16 for a column of the rows kernel).
 inline bool gemm_fits(int64_t M, int64_t N, int64_t pitch_bytes) {
-  return M < ((int64_t)1 << 30) && N < ((int64_t)1 << 30) && pitch_bytes < kMaxPitch &&
-         div_up(M, 64) * div_up(N, 32) < ((int64_t)1 << 30);
+  return M <= kMaxRows && N <= kMaxRows && pitch_bytes < kMaxPitch &&
+         div_up(M, 64) * div_up(N, 32) < ((int64_t)1 << 25);
 }
 
 template <class T, bool kXT = false, bool kWT = false, class Epi>

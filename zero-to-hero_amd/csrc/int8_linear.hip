@@ -70,7 +70,7 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
 
 // x / scale to the nearest integer.  The product with 1 / scale is off by at
 // most 1.5e-5 (two roundings of a value up to 127), so it settles all but the
-// quotients within 4e-5 of a tie, one in 12000, which are divided.  
+// quotients within 4e-5 of a tie, one in 12000, which are divided.
 struct Quantizer {
   float scale, inverse;
   bool live, direct;  // direct: 1 / scale is no number to multiply by
@@ -190,9 +190,21 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* x, int64_t
   if (threadIdx.x == 0) scale[r] = s;
 }
 
+// Rows of one launch: a grid's threads (at most 1024 a row) are counted in 32 bits.
+constexpr int64_t kLaunchRows = (int64_t)1 << 21;
+
 template <class T>
 int launch_quantize(const void* x, int64_t rows, int64_t cols, int8_t* q, int64_t pitch,
                     float* scale, hipStream_t stream) {
+  if (rows > kLaunchRows) {
+    for (int64_t r = 0; r < rows; r += kLaunchRows) {
+      const int64_t n = rows - r < kLaunchRows ? rows - r : kLaunchRows;
+      const int st = launch_quantize<T>((const T*)x + r * cols, n, cols, q + r * pitch, pitch,
+                                        scale + r, stream);
+      if (st) return st;
+    }
+    return PPO_OK;
+  }
   const int64_t chunks = div_up(pitch, kPer16<T>);
   auto go = [&](auto threads, auto each) {
     constexpr int kT = decltype(threads)::value, kC = decltype(each)::value;
