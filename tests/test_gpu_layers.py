@@ -234,7 +234,9 @@ def test_quantize_rows_edges(dev):
 
 INT8_SHAPES = [(1, 1, 1), (1, 4, 16), (2, 3, 33), (16, 65, 128), (17, 48, 1000), (33, 17, 130),
                (64, 130, 515), (65, 64, 64), (100, 127, 96), (129, 200, 2049), (300, 513, 64),
-               (70, 64, 8192), (1, 4096, 512), (1, 50, 16384), (4, 100, 4096), (5, 33, 3001), (15, 70, 1092), (16, 48, 1024), (3, 20, 16), (2048, 2048, 160), (3300, 4200, 48), (257, 31, 77)]
+               (70, 64, 8192), (1, 4096, 512), (1, 50, 16384), (4, 100, 4096), (5, 33, 3001),
+               (15, 70, 1092), (16, 48, 1024), (3, 20, 16), (2048, 2048, 160), (3300, 4200, 48),
+               (257, 31, 77), (2, 40, 65536), (33, 70, 20000), (20, 33, 40001)]
 
 
 def _int8_case(dtype, M, N, K, bias):
@@ -373,7 +375,7 @@ ACTS = ["silu", "gelu", "tanh", "relu"]
 GATED_SHAPES = [(1, 1, 1), (1, 8, 4), (3, 5, 7), (2, 64, 33), (16, 31, 17), (17, 128, 96),
                 (33, 72, 50), (64, 200, 65), (65, 64, 64), (128, 128, 256), (100, 333, 127),
                 (257, 129, 31), (300, 96, 520), (70, 2100, 24), (1000, 40, 1030),
-                (2200, 136, 1600)]
+                (2200, 136, 1600), (1, 8200, 40), (33, 16384, 20), (7, 9001, 24)]
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))

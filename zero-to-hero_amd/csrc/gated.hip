@@ -286,6 +286,7 @@ struct Scratch {
 struct ForwardPlan {
   int64_t pitch;  // bytes of a padded row
   bool pad;
+  GemmPlan gemm;
   char *x, *wg, *wu, *partial;
   size_t bytes;
 };
@@ -294,8 +295,9 @@ ForwardPlan plan_forward(int dtype, int64_t M, int64_t D, int64_t F, bool aligne
   const int64_t size = dtype_size(dtype);
   ForwardPlan f = {};
   f.pitch = round_up(D * size, 16);
-  const GemmPlan g = plan_gemm(M, 2 * F, f.pitch, size == 4);
-  f.pad = g.tile != 0 && (!aligned || f.pitch != D * size);
+  const bool odd = f.pitch != D * size;
+  const GemmPlan& g = f.gemm = plan_gemm(M, 2 * F, D * size, size == 4, kTwoMatrices);
+  f.pad = g.tile != 0 && (!aligned || odd);
   Scratch s{ws};
   if (f.pad) {
     f.x = s.take(M * f.pitch);
@@ -319,6 +321,7 @@ struct BackwardPlan {
   bool rest;      // dg and du in two parts each
   int64_t pitch;  // bytes of a row of x and the weights
   bool pad;
+  GemmPlan gx, gw;  // of the products to dx and to the weights' gradients
   char *dgu, *x, *wg, *wu, *sums, *partial;
   size_t bytes;
 };
@@ -339,10 +342,10 @@ BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool alig
     b.wu = s.take(F * b.pitch);
   }
   b.sums = s.take(div_up(M, kTileM) * 2 * F * 4);
-  const GemmPlan gx = plan_gemm(M, D, parts * b.fp * size, size == 4, true),
-                 gw = plan_gemm(2 * b.fp, D, parts / 2 * M * size, size == 4, true);
-  b.partial = s.take((int64_t)(gx.partial_bytes > gw.partial_bytes ? gx.partial_bytes
-                                                                   : gw.partial_bytes));
+  b.gx = plan_gemm(M, D, parts * b.fp * size, size == 4, kByKRows);
+  b.gw = plan_gemm(2 * b.fp, D, parts / 2 * M * size, size == 4, kByKRows);
+  b.partial = s.take((int64_t)(b.gx.partial_bytes > b.gw.partial_bytes ? b.gx.partial_bytes
+                                                                       : b.gw.partial_bytes));
   b.bytes = s.used;
   return b;
 }
@@ -425,7 +428,7 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
     const int F4 = (int)round_up(F, 4);
     const GatedEpi<T> epi = {(const T*)bg, (const T*)bu, (T*)h, saved, M * F4, (int)F, F4,
                              activation, drop_of(drop)};
-    return launch_gemm<T>(a, epi, f.partial, stream);
+    return launch_gemm<T>(a, epi, f.gemm, f.partial, stream);
   });
 }
 
@@ -490,7 +493,7 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
       a.k = F;
       a.ranges = b.rest ? 4 : 2;
       const StoreEpi<T> epi = {(T*)dx, nullptr, (int)M, (int)M, (int)D};
-      if ((st = launch_gemm<T, false, true>(a, epi, b.partial, stream))) return st;
+      if ((st = launch_gemm<T, false, true>(a, epi, b.gx, b.partial, stream))) return st;
     }
     if (dwg) {  // [dg | du]^T x: both operands by their rows m
       a.w0 = a.w1 = b.pad ? b.x : (const char*)x;
@@ -499,7 +502,7 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
       a.ranges = b.rest ? 2 : 1;
       a.x_range = 2 * b.fp * size;
       const StoreEpi<T> epi = {(T*)dwg, (T*)dwu, (int)F, (int)b.fp, (int)D};
-      if ((st = launch_gemm<T, true, true>(a, epi, b.partial, stream))) return st;
+      if ((st = launch_gemm<T, true, true>(a, epi, b.gw, b.partial, stream))) return st;
     }
     return (int)PPO_OK;
   });

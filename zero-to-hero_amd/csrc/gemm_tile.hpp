@@ -676,18 +676,29 @@ constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay belo
 // said), tile 256 / 128 / 64 without split: gated 4096 x 1024 -> 2048 41 / 42 / 60,
 // 1024 x 2048 -> 2048 49 / 28 / 26, fp32 4096 x 512 -> 1024 134 / 74 / 102; 128 in
 // two splits 79, 33 and 90; fp32 1024 x 1024 -> 512 in 64s and one, two or four
-// splits 40 / 43 / 31.  The rows kernel's time is that of reading W, more for the
-// second to fourth sixteen rows: 16, 32 and 64 rows of 4096 -> 8192 gated 26, 31
-// and 46, against 25, 26 and 27 for tiles of 64 in two splits; fp32 4096 -> 4096
-// 25, 33 and 52 against 44, 44 and 47.
-inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t kbytes, bool fp32,
-                          bool by_k_rows = false) {
+// splits 40 / 43 / 31.  The rows kernel's time is that of reading W, or of one
+// workgroup's K where the columns are few, more where a single matrix does not
+// share the reads of x, and three or four times that for rows that start off 4
+// bytes (1 x 8191 -> 2048 gated bf16 58 us, 8192 20).  The tiles, which want a padded copy of
+// rows off 16 bytes, have to be 15% better by this estimate, which is for weights
+// that the caches hold (from HBM the rows kernel loses least).  1, 16, 32 and 64 rows
+// of 4096 -> 8192 gated 24, 25, 32 and 47, against 25, 26, 26 and 27 for tiles of 64 in
+// two or four splits; with weights from HBM 28, 31, 36 and 51 against 31, 32, 33 and
+// 38; of 16384 -> 512 gated 34, 44, 58 and 87 against 18, 20, 20 and 20 in sixteen.
+enum GemmKind { kOneMatrix, kTwoMatrices, kByKRows };
+inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32, GemmKind kind) {
+  const int64_t kbytes = round_up(row_bytes, 16);
   GemmPlan p = {-1, 1, 0};
   double best = 0.0;
-  if (M <= kRowsMax && !by_k_rows) {
+  if (M <= kRowsMax && kind != kByKRows) {
     p.tile = 0;
-    const int sets = M <= 16 ? 1 : M <= 32 ? 2 : 4;  // the kernel's MT
-    best = 2.0 + (double)wrows * kbytes / 5.5e6 * (0.8 + 0.2 * sets);
+    const int set = M <= 16 ? 0 : M <= 32 ? 1 : 2;
+    const double reads[2][3] = {{1.25, 2.0, 3.3}, {1.03, 1.25, 1.8}};
+    const double row[2][3] = {{0.75, 1.3, 2.1}, {1.15, 1.75, 2.6}};
+    const double all = 1.0 + (double)wrows * kbytes / 5.6e6 * reads[kind][set];
+    const double one = 2.4 + (double)kbytes / 1024.0 * row[kind][set];
+    best = fmax(all, one) * (row_bytes % 4 ? set ? 4.0 : 3.0 : 1.0) / 1.15;
+    if (row_bytes != kbytes) best -= 4.0 + 2.0 * (double)wrows * kbytes / 5.3e6;
   }
   struct Cost { int tile, per_cu; double step[2], alone[2], fixed, lone; };
   static const Cost kCosts[] = {
@@ -723,22 +734,32 @@ inline bool gemm_fits(int64_t M, int64_t N, int64_t pitch_bytes) {
          div_up(M, 64) * div_up(N, 32) < ((int64_t)1 << 25);
 }
 
+// p: plan_gemm's for these sizes.
 template <class T, bool kXT = false, bool kWT = false, class Epi>
-int launch_gemm(GemmArgs a, const Epi& epi, char* partial, hipStream_t stream) {
-  const int64_t wrows = (int64_t)a.N * (Epi::kGated ? 2 : 1);
+int launch_gemm(GemmArgs a, const Epi& epi, const GemmPlan& p, char* partial, hipStream_t stream) {
   if (a.ranges == 0) a.ranges = 1;
-  const int64_t kbytes = a.ranges * (kXT ? a.k * (int64_t)sizeof(T) : a.kbytes);
-  const GemmPlan p = plan_gemm(a.M, wrows, kbytes, sizeof(T) == 4, kXT || kWT);
   a.partial = p.splits > 1 ? partial : nullptr;
   if constexpr (!kXT && !kWT) {
     if (p.tile == 0) {
       const dim3 grid((unsigned)div_up(a.N, 16));
-      if (a.M <= 16)
-        hipLaunchKernelGGL((gemm_rows_kernel<T, 1, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
-      else if (a.M <= 32)
-        hipLaunchKernelGGL((gemm_rows_kernel<T, 2, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
-      else
-        hipLaunchKernelGGL((gemm_rows_kernel<T, 4, 4, Epi>), grid, dim3(256), 0, stream, a, epi);
+      // Eight waves where a CU has one workgroup and each wave four runs of K or
+      // more (with weights from HBM, 1 x 8192 -> 2048 gated 26.0 -> 20.6 us, fp32
+      // 52.6 -> 37.6; 1 x 1024 -> 4096 6.5 -> 7.0, 16 x 4096 -> 8192 31 -> 34), except
+      // for many rows of fp32, which the matrix cores bind (64 x 8192 -> 2048 107 -> 114).
+      const bool eight = div_up(a.N, 16) <= kCus && a.kbytes >= 32 * kRunBytes &&
+                         !(sizeof(T) == 4 && a.M > 32);
+      auto go = [&](auto sets, auto waves) {
+        constexpr int MT = decltype(sets)::value, kWaves = decltype(waves)::value;
+        hipLaunchKernelGGL((gemm_rows_kernel<T, MT, kWaves, Epi>), grid, dim3(kWaves * 64), 0,
+                           stream, a, epi);
+      };
+      auto with_waves = [&](auto sets) {
+        if (eight) go(sets, std::integral_constant<int, 8>{});
+        else go(sets, std::integral_constant<int, 4>{});
+      };
+      if (a.M <= 16) with_waves(std::integral_constant<int, 1>{});
+      else if (a.M <= 32) with_waves(std::integral_constant<int, 2>{});
+      else with_waves(std::integral_constant<int, 4>{});
       return last_launch_status();
     }
   }

@@ -341,6 +341,7 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const T* x, const int8_t*
 struct Int8Plan {
   int64_t pitch;
   bool pad_x, pad_w;
+  GemmPlan gemm;
   char *xq, *xs, *wq, *partial;
   size_t bytes;
 };
@@ -348,8 +349,8 @@ struct Int8Plan {
 Int8Plan plan_int8(int64_t M, int64_t N, int64_t K, bool quantize, bool ax, bool aw, char* ws) {
   Int8Plan p = {};
   p.pitch = round_up(K, 16);
-  const GemmPlan g = plan_gemm(M, N, p.pitch, false);
   const bool odd = p.pitch != K;
+  const GemmPlan& g = p.gemm = plan_gemm(M, N, K, false, kOneMatrix);
   p.pad_x = !quantize && g.tile != 0 && (odd || !ax);
   p.pad_w = g.tile != 0 && (odd || !aw);
   size_t used = 0;
@@ -439,8 +440,8 @@ extern "C" int ppo_layer_int8_linear(const void* x, const int8_t* xq, const floa
       if ((st = last_launch_status())) return st;
     }
     // the tile kernel's rows end on 16 bytes (zeros behind K), the rows kernel's on K
-    if (plan_gemm(M, N, p.pitch, false).tile) a.kbytes = p.pitch;
+    if (p.gemm.tile) a.kbytes = p.pitch;
     const Int8Epi<T> epi = {x ? (const float*)p.xs : xs, ws, (const T*)bias, (T*)out, (int)N};
-    return launch_gemm<int8_t>(a, epi, p.partial, stream);
+    return launch_gemm<int8_t>(a, epi, p.gemm, p.partial, stream);
   });
 }
