@@ -108,7 +108,8 @@ int ppo_layer_gated_forward(const void* x, const void* wg, const void* wu, const
  * together).  M > 0 (over no rows the weights' gradients are the caller's
  * zeros).  dg and du are rounded to `dtype`, the matrix cores' operand
  * type, before the products.  Sums are split and joined in a fixed order:
- * the same inputs give the same bits.
+ * the same call gives the same bits (one that asks for other outputs may cut
+ * the sums elsewhere).
  */
 size_t ppo_layer_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t D, int64_t F);
 int ppo_layer_gated_backward(const void* dh, const void* x, const void* wg, const void* wu,

@@ -507,6 +507,24 @@ def test_gated_subsets_and_empties(dev):
     assert torch.equal(dx.view(40, 24), want[0])
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,D,F", [(5, 3, 9), (64, 200, 65), (70, 2100, 24), (300, 96, 520),
+                                   (1000, 40, 1030), (2200, 136, 1600)])
+def test_gated_gradients_of_one_side(dev, dtype, M, D, F):
+    """x's gradient without the weights', and theirs without x's: each product
+    in a launch of its own."""
+    t = TYPES[dtype]
+    x, wg, wu, _, _, dh = gated_case(dtype, M, D, F, False, seed=6)
+    _, g, u = ref.gated_ffn(*d64(x, wg, wu), None, None, "silu")
+    want = ref.gated_ffn_grads(*d64(x, wg, wu), g, u, "silu", dh.double())
+    args = [v.to(dev) for v in (x, wg, wu)]
+    for pick in ([0], [1, 2], [2]):
+        some = [v.clone().requires_grad_(k in pick) for k, v in enumerate(args)]
+        got = torch.autograd.grad(ppo_amd.gated_ffn(*some), [some[k] for k in pick], dh.to(dev))
+        for k, v in zip(pick, got):
+            check_grad(v, want[k], t, ("dx", "dwg", "dwu")[k])
+
+
 def test_gated_same_bits_again(dev):
     """Split sums are joined in a fixed order."""
     for M, D, F in ((96, 2048, 64), (300, 200, 72)):

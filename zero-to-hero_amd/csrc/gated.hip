@@ -322,7 +322,9 @@ struct BackwardPlan {
   int64_t pitch;  // bytes of a row of x and the weights
   bool pad;
   GemmPlan gx, gw;  // of the products to dx and to the weights' gradients
+  PairPlan pair;    // and of both together
   char *dgu, *x, *wg, *wu, *sums, *partial;
+  size_t partial_w;  // where the second of both has its partial sums
   size_t bytes;
 };
 
@@ -342,10 +344,15 @@ BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool alig
     b.wu = s.take(F * b.pitch);
   }
   b.sums = s.take(div_up(M, kTileM) * 2 * F * 4);
-  b.gx = plan_gemm(M, D, parts * b.fp * size, size == 4, kByKRows);
-  b.gw = plan_gemm(2 * b.fp, D, parts / 2 * M * size, size == 4, kByKRows);
-  b.partial = s.take((int64_t)(b.gx.partial_bytes > b.gw.partial_bytes ? b.gx.partial_bytes
-                                                                       : b.gw.partial_bytes));
+  const int64_t kx = parts * b.fp * size, kw = parts / 2 * M * size;
+  b.gx = plan_gemm(M, D, kx, size == 4, kByKRows);
+  b.gw = plan_gemm(2 * b.fp, D, kw, size == 4, kByKRows);
+  b.pair = plan_pair(M, D, kx, 2 * b.fp, D, kw, size == 4, b.gx.us + b.gw.us);
+  const size_t apart = b.gx.partial_bytes > b.gw.partial_bytes ? b.gx.partial_bytes
+                                                               : b.gw.partial_bytes;
+  b.partial_w = (size_t)round_up((int64_t)b.pair.partial_x, 256);
+  const size_t both = b.partial_w + b.pair.partial_w;
+  b.partial = s.take((int64_t)(apart > both ? apart : both));
   b.bytes = s.used;
   return b;
 }
@@ -474,36 +481,39 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
                          div_up(M, kTileM), (int)F, (T*)dbg, (T*)dbu);
       if ((st = last_launch_status())) return st;
     }
-    GemmArgs a = {};
-    a.N = (int)D;
-    a.wpitch = D * size;
     if (b.pad) {
       st = pad_rows<T>(dwg ? x : nullptr, dx ? wg : nullptr, dx ? wu : nullptr, b.x, b.wg, b.wu, M,
                        D, F, b.pitch, stream);
       if (st) return st;
-      a.wpitch = b.pitch;
     }
-    a.x = b.dgu;
-    a.xpitch = (b.rest ? 4 : 2) * b.fp * size;
-    if (dx) {  // [dg | du] [wg; wu], the weights as they lie: k-rows of D columns
-      a.w0 = b.pad ? b.wg : (const char*)wg;
-      a.w1 = b.pad ? b.wu : (const char*)wu;
-      a.M = (int)M;
-      a.kbytes = a.x_range = b.fp * size;
-      a.k = F;
-      a.ranges = b.rest ? 4 : 2;
-      const StoreEpi<T> epi = {(T*)dx, nullptr, (int)M, (int)M, (int)D};
-      if ((st = launch_gemm<T, false, true>(a, epi, b.gx, b.partial, stream))) return st;
+    GemmArgs ax = {};
+    ax.N = (int)D;
+    ax.wpitch = b.pad ? b.pitch : D * size;
+    ax.x = b.dgu;
+    ax.xpitch = (b.rest ? 4 : 2) * b.fp * size;
+    GemmArgs aw = ax;
+    // dx = [dg | du] [wg; wu], the weights as they lie: k-rows of D columns
+    ax.w0 = b.pad ? b.wg : (const char*)wg;
+    ax.w1 = b.pad ? b.wu : (const char*)wu;
+    ax.M = (int)M;
+    ax.kbytes = ax.x_range = b.fp * size;
+    ax.k = F;
+    ax.ranges = b.rest ? 4 : 2;
+    const StoreEpi<T> ex = {(T*)dx, nullptr, (int)M, (int)M, (int)D};
+    // [dwg; dwu] = [dg | du]^T x: both operands by their rows m
+    aw.w0 = aw.w1 = b.pad ? b.x : (const char*)x;
+    aw.M = (int)(2 * b.fp);
+    aw.k = M;
+    aw.ranges = b.rest ? 2 : 1;
+    aw.x_range = 2 * b.fp * size;
+    const StoreEpi<T> ew = {(T*)dwg, (T*)dwu, (int)F, (int)b.fp, (int)D};
+    if (dx && dwg && b.pair.tile) {
+      ax.partial = b.pair.splits_x > 1 ? b.partial : nullptr;
+      aw.partial = b.pair.splits_w > 1 ? b.partial + b.partial_w : nullptr;
+      return launch_pair<T>(ax, aw, ex, ew, b.pair, stream);
     }
-    if (dwg) {  // [dg | du]^T x: both operands by their rows m
-      a.w0 = a.w1 = b.pad ? b.x : (const char*)x;
-      a.M = (int)(2 * b.fp);
-      a.k = M;
-      a.ranges = b.rest ? 2 : 1;
-      a.x_range = 2 * b.fp * size;
-      const StoreEpi<T> epi = {(T*)dwg, (T*)dwu, (int)F, (int)b.fp, (int)D};
-      if ((st = launch_gemm<T, true, true>(a, epi, b.gw, b.partial, stream))) return st;
-    }
+    if (dx && (st = launch_gemm<T, false, true>(ax, ex, b.gx, b.partial, stream))) return st;
+    if (dwg && (st = launch_gemm<T, true, true>(aw, ew, b.gw, b.partial, stream))) return st;
     return (int)PPO_OK;
   });
 }

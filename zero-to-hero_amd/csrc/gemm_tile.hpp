@@ -250,9 +250,13 @@ __device__ __forceinline__ void store_partial(const GemmArgs& a, int split, int 
 // of the step after next go into the freed buffer during the last phase and
 // the first of the next step (issued at once they hold up the instructions
 // behind them; later they arrive late).
+//
+// `block` of `blocks` workgroups that share the tiles of split `split`; lds: two
+// buffers of (BM + BN) * kStepBytes.
 template <class T, int BM, int BN, int kWavesM, int kWavesN, bool kXT, bool kWT, class Epi>
-__global__ void __launch_bounds__(kWavesM* kWavesN * 64)
-    gemm_tile_kernel(const GemmArgs a, const Epi epi) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& a, const Epi& epi,
+                                          char (*lds)[(BM + BN) * kStepBytes], int block,
+                                          int blocks, int split) {
   constexpr int kWaves = kWavesM * kWavesN;
   constexpr int kEdge = 32;  // of a matrix instruction's block
   constexpr int TM = BM / kWavesM / kEdge, TN = BN / kWavesN / kEdge;
@@ -267,15 +271,13 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   constexpr int kBuffer = (BM + BN) * kStepBytes;
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "");
   static_assert(!kGated || (TN % 2 == 0 && !kWT), "");
-  __shared__ __align__(1024) char lds[2][kBuffer];
-
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / kWavesN, wn = wave % kWavesN;
   constexpr int kStepK = kStepBytes / (int)sizeof(T);
   const int per_range = (int)(kXT ? div_up(a.k, kStepK) : div_up(a.kbytes, kStepBytes));
   const int steps = per_range * a.ranges;
-  const int first = blockIdx.y * a.steps_per_split;
+  const int first = split * a.steps_per_split;
   const int count = max(0, min(steps - first, a.steps_per_split));
 
   // --- loads ------------------------------------------------------------------------
@@ -418,8 +420,8 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
 #pragma unroll
           for (int b = 0; b < kBatch; ++b)
             if (live[b]) {
-              store_partial(a, blockIdx.y, 0, kGated ? 2 : 1, m[b], n, c[b]);
-              if constexpr (kGated) store_partial(a, blockIdx.y, 1, 2, m[b], n, c2[b]);
+              store_partial(a, split, 0, kGated ? 2 : 1, m[b], n, c[b]);
+              if constexpr (kGated) store_partial(a, split, 1, 2, m[b], n, c2[b]);
             }
         } else if constexpr (kGated) {
           epi.apply(n, cols, m, live, rows, c, c2);
@@ -440,11 +442,11 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
   constexpr bool kLoop = BM * BN >= 256 * 256;
   const int tiles = a.tiles_m * a.tiles_n;
   Source x, w;
-  locate(blockIdx.x);
+  locate(block);
   source(0, x, w);
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load(i, 1, x, w);
-  for (int id = blockIdx.x;; id += gridDim.x) {
+  for (int id = block;; id += blocks) {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     source(1, x, w);
 #pragma unroll
     for (int i = 0; i < kEarly; ++i) load(i, 0, x, w);
-    if (id == (int)blockIdx.x) stage_barrier<kEarly>();
+    if (id == block) stage_barrier<kEarly>();
 #pragma unroll
     for (int g = 0; g < kFrags; ++g) read(f[0], g, lds[1], 0);
     for (int step = 0; step < count; ++step) {
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     // and the next tile's loads are under way: waiting for it later would wait
     // for those
     const int em0 = m0, en0 = n0;
-    const bool more = kLoop && id + (int)gridDim.x < tiles;
+    const bool more = kLoop && id + blocks < tiles;
     typename Epi::Cols cols = epi.columns(min(en0 + wn * kOut + lane % kLanes * 4, a.N - 1));
     typename Epi::Row states[kRowSets];
     if constexpr (Epi::kRows) {
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     }
     cols.arrived();
     if (more) {
-      locate(id + gridDim.x);
+      locate(id + blocks);
       source(0, x, w);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) load(i, 1, x, w);
@@ -503,6 +505,39 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
     if (!more) break;
     lds_barrier();
   }
+}
+
+template <class T, int BM, int BN, int kWavesM, int kWavesN, bool kXT, bool kWT, class Epi>
+__global__ void __launch_bounds__(kWavesM* kWavesN * 64)
+    gemm_tile_kernel(const GemmArgs a, const Epi epi) {
+  __shared__ __align__(1024) char lds[2][(BM + BN) * kStepBytes];
+  gemm_tile<T, BM, BN, kWavesM, kWavesN, kXT, kWT>(a, epi, lds, blockIdx.x, gridDim.x, blockIdx.y);
+}
+
+// The two products of a backward pass, dY W and dY^T X, in one launch: apart,
+// neither fills the chip for as long as it runs, unless it is cut into splits
+// whose sums are joined (a training step of 256 x 128 -> 256 in fp32 35 -> 26 us, of
+// 4096 x 1024 -> 2048 in bf16 183 -> 151).  The first `span` workgroups are those
+// of the product whose workgroups have more steps.
+struct GemmPair {
+  GemmArgs x, w;
+  int splits_x, splits_w, span;
+  bool w_first;
+};
+template <class T, int BM, int BN, int kWavesM, int kWavesN, class Epi>
+__global__ void __launch_bounds__(kWavesM* kWavesN * 64)
+    gemm_pair_kernel(const GemmPair p, const Epi ex, const Epi ew) {
+  __shared__ __align__(1024) char lds[2][(BM + BN) * kStepBytes];
+  const bool behind = (int)blockIdx.x >= p.span, second = behind != p.w_first;
+  const int at = blockIdx.x - (behind ? p.span : 0);
+  const int tiles = second ? p.w.tiles_m * p.w.tiles_n : p.x.tiles_m * p.x.tiles_n;
+  const int wide = (tiles + 7) / 8 * 8;  // (a split's tiles start on the first XCD)
+  const int split = at / wide, id = at % wide;
+  if (id >= tiles) return;
+  if (second)
+    gemm_tile<T, BM, BN, kWavesM, kWavesN, true, true>(p.w, ew, lds, id, tiles, split);
+  else
+    gemm_tile<T, BM, BN, kWavesM, kWavesN, false, true>(p.x, ex, lds, id, tiles, split);
 }
 
 // The epilogue of one row's four columns.
@@ -525,8 +560,7 @@ __device__ __forceinline__ void apply_one(const Epi& epi, int m, int n,
 
 // Joins the splits of K in their order and applies the epilogue.
 template <class T, class Epi>
-__global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a, const Epi epi,
-                                                        int splits) {
+__device__ __forceinline__ void gemm_join(const GemmArgs& a, const Epi& epi, int splits) {
   constexpr int kHalves = Epi::kGated ? 2 : 1;
   const int64_t groups = div_up(a.N, 4), n4 = groups * 4;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -541,6 +575,22 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a, const 
       sum[h] = s ? sum[h] + v : v;
     }
   apply_one<T>(epi, m, n, epi.columns(n), true, sum);
+}
+
+template <class T, class Epi>
+__global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a, const Epi epi,
+                                                        int splits) {
+  gemm_join<T>(a, epi, splits);
+}
+
+template <class T, class Epi>
+__global__ void __launch_bounds__(256) gemm_join_pair_kernel(const GemmPair p, const Epi ex,
+                                                             const Epi ew) {
+  const bool second = p.splits_x == 1 || blockIdx.y == 1;  // (the only one, or both)
+  if (second)
+    gemm_join<T>(p.w, ew, p.splits_w);
+  else
+    gemm_join<T>(p.x, ex, p.splits_x);
 }
 
 constexpr int kRunBytes = 128;  // of K that a wave of the rows kernel takes at a time
@@ -657,12 +707,27 @@ struct GemmPlan {
   int tile;     // 0: rows kernel, else the tile's edge
   int splits;
   size_t partial_bytes;
+  double us;    // expected
 };
 
 constexpr int kCus = 256;
 constexpr int kRowsMax = 64;       // rows that the rows kernel takes
 constexpr int64_t kMaxRows = (int64_t)1 << 27;   // of either operand
 constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay below 2^31 bytes
+
+// What a workgroup of a tile takes, in us (plan_gemm).
+struct TileCost { int tile, per_cu; double step[2], alone[2], fixed, lone; };
+constexpr TileCost kTileCosts[] = {
+    {256, 1, {0.95, 7.2}, {1.11, 7.2}, 17.6, 10.7},
+    {128, 2, {0.32, 1.8}, {0.52, 2.0}, 4.2, 7.8},
+    {64, 5, {0.19, 0.90}, {0.44, 1.08}, 1.75, 4.6},
+};
+inline double join_cost(int splits, int64_t M, int64_t wrows) {
+  return splits > 1 ? splits * 8.0 * (double)M * wrows / 13.6e6 : 0.0;
+}
+inline size_t partial_size(int splits, int64_t M, int64_t wrows) {
+  return splits > 1 ? (size_t)splits * M * round_up(wrows, 8) * 4 : 0;
+}
 
 // How a product of M rows and `wrows` rows of W (both matrices of a gated one
 // together) over `kbytes` is cut: the tile and the number of splits of K with
@@ -688,7 +753,7 @@ constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay belo
 enum GemmKind { kOneMatrix, kTwoMatrices, kByKRows };
 inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32, GemmKind kind) {
   const int64_t kbytes = round_up(row_bytes, 16);
-  GemmPlan p = {-1, 1, 0};
+  GemmPlan p = {-1, 1, 0, 0.0};
   double best = 0.0;
   if (M <= kRowsMax && kind != kByKRows) {
     p.tile = 0;
@@ -700,21 +765,15 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32
     best = fmax(all, one) * (row_bytes % 4 ? set ? 4.0 : 3.0 : 1.0) / 1.15;
     if (row_bytes != kbytes) best -= 4.0 + 2.0 * (double)wrows * kbytes / 5.3e6;
   }
-  struct Cost { int tile, per_cu; double step[2], alone[2], fixed, lone; };
-  static const Cost kCosts[] = {
-      {256, 1, {0.95, 7.2}, {1.11, 7.2}, 17.6, 10.7},
-      {128, 2, {0.32, 1.8}, {0.52, 2.0}, 4.2, 7.8},
-      {64, 5, {0.19, 0.90}, {0.44, 1.08}, 1.75, 4.6},
-  };
   const double steps = (double)div_up(kbytes, kStepBytes);
-  for (const Cost& c : kCosts) {
+  for (const TileCost& c : kTileCosts) {
     for (int splits = 1; splits <= 16; splits *= 2) {
       if (splits > 1 && steps < 4.0 * splits) break;
       const double groups = (double)(div_up(M, c.tile) * div_up(wrows, c.tile)) * splits;
       const double each = ceil(steps / splits);
       const double busy = ceil(groups / kCus) * (each * c.step[fp32] + c.fixed);
       const double waits = ceil(groups / (kCus * c.per_cu)) * (each * c.alone[fp32] + c.lone);
-      const double join = splits > 1 ? 4.0 + splits * 8.0 * M * wrows / 13.6e6 : 0.0;
+      const double join = (splits > 1 ? 4.0 : 0.0) + join_cost(splits, M, wrows);
       const double time = fmax(busy, waits) + join;
       if (p.tile < 0 || time < best) {
         best = time;
@@ -723,7 +782,42 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32
       }
     }
   }
-  if (p.splits > 1) p.partial_bytes = (size_t)p.splits * M * round_up(wrows, 8) * 4;
+  p.partial_bytes = partial_size(p.splits, M, wrows);
+  p.us = best;
+  return p;
+}
+
+// The same for the two products of a backward pass in one launch (tile 0: they
+// run apart).  Both share the tile; a round of workgroups takes the mean of
+// theirs.
+struct PairPlan {
+  int tile, splits_x, splits_w;
+  size_t partial_x, partial_w;  // bytes
+};
+inline PairPlan plan_pair(int64_t Mx, int64_t Nx, int64_t bytes_x, int64_t Mw, int64_t Nw,
+                          int64_t bytes_w, bool fp32, double apart) {
+  PairPlan p = {0, 1, 1, 0, 0};
+  double best = apart;
+  const double kx = (double)div_up(bytes_x, kStepBytes), kw = (double)div_up(bytes_w, kStepBytes);
+  for (const TileCost& c : kTileCosts) {
+    if (c.tile == 256) continue;
+    const double gx = (double)(div_up(Mx, c.tile) * div_up(Nx, c.tile)),
+                 gw = (double)(div_up(Mw, c.tile) * div_up(Nw, c.tile));
+    for (int sx = 1; sx <= 16 && (sx == 1 || kx >= 4.0 * sx); sx *= 2)
+      for (int sw = 1; sw <= 16 && (sw == 1 || kw >= 4.0 * sw); sw *= 2) {
+        const double groups = gx * sx + gw * sw, ex = ceil(kx / sx), ew = ceil(kw / sw);
+        const double each = (gx * sx * ex + gw * sw * ew) / groups;
+        const double busy = ceil(groups / kCus) * (each * c.step[fp32] + c.fixed);
+        const double waits = fmax(ceil(groups / (kCus * c.per_cu)) * (each * c.alone[fp32] + c.lone),
+                                  fmax(ex, ew) * c.alone[fp32] + c.lone);
+        const double join = sx * sw > 1 ? 4.0 + join_cost(sx, Mx, Nx) + join_cost(sw, Mw, Nw) : 0.0;
+        const double time = fmax(busy, waits) + join;
+        if (time < best) {
+          best = time;
+          p = {c.tile, sx, sw, partial_size(sx, Mx, Nx), partial_size(sw, Mw, Nw)};
+        }
+      }
+  }
   return p;
 }
 
@@ -732,6 +826,15 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32
 inline bool gemm_fits(int64_t M, int64_t N, int64_t pitch_bytes) {
   return M <= kMaxRows && N <= kMaxRows && pitch_bytes < kMaxPitch &&
          div_up(M, 64) * div_up(N, 32) < ((int64_t)1 << 25);
+}
+
+template <class T, bool kXT>
+void cut_gemm(GemmArgs& a, bool gated, int tile, int splits) {
+  const int64_t range_steps = kXT ? div_up(a.k, kStepBytes / (int)sizeof(T))
+                                  : div_up(a.kbytes, kStepBytes);
+  a.steps_per_split = (int)div_up(range_steps * a.ranges, splits);
+  a.tiles_m = (int)div_up(a.M, tile);
+  a.tiles_n = (int)div_up(a.N, gated ? tile / 2 : tile);
 }
 
 // p: plan_gemm's for these sizes.
@@ -763,12 +866,7 @@ int launch_gemm(GemmArgs a, const Epi& epi, const GemmPlan& p, char* partial, hi
       return last_launch_status();
     }
   }
-  const int64_t range_steps = kXT ? div_up(a.k, kStepBytes / (int)sizeof(T))
-                                  : div_up(a.kbytes, kStepBytes);
-  a.steps_per_split = (int)div_up(range_steps * a.ranges, p.splits);
-  const int cols = Epi::kGated ? p.tile / 2 : p.tile;
-  a.tiles_m = (int)div_up(a.M, p.tile);
-  a.tiles_n = (int)div_up(a.N, cols);
+  cut_gemm<T, kXT>(a, Epi::kGated, p.tile, p.splits);
   // (256: a workgroup of the largest tile has a CU to itself and takes tile after tile)
   const int tiles = a.tiles_m * a.tiles_n;
   const dim3 grid((unsigned)(p.tile == 256 && tiles > kCus ? kCus : tiles), (unsigned)p.splits);
@@ -785,6 +883,33 @@ int launch_gemm(GemmArgs a, const Epi& epi, const GemmPlan& p, char* partial, hi
     const int64_t n = (int64_t)a.M * div_up(a.N, 4);
     hipLaunchKernelGGL((gemm_join_kernel<T, Epi>), dim3((unsigned)div_up(n, 256)), dim3(256), 0,
                        stream, a, epi, p.splits);
+  }
+  return last_launch_status();
+}
+
+// x and w: the products of a backward pass, their partial sums where the plan splits.
+template <class T, class Epi>
+int launch_pair(GemmArgs x, GemmArgs w, const Epi& ex, const Epi& ew, const PairPlan& plan,
+                hipStream_t stream) {
+  cut_gemm<T, false>(x, false, plan.tile, plan.splits_x);
+  cut_gemm<T, true>(w, false, plan.tile, plan.splits_w);
+  GemmPair p = {x, w, plan.splits_x, plan.splits_w, 0, w.steps_per_split > x.steps_per_split};
+  const int64_t span_x = round_up(x.tiles_m * x.tiles_n, 8) * plan.splits_x,
+                span_w = round_up(w.tiles_m * w.tiles_n, 8) * plan.splits_w;
+  p.span = (int)(p.w_first ? span_w : span_x);
+  const dim3 grid((unsigned)(span_x + span_w));
+  if (plan.tile == 128)
+    hipLaunchKernelGGL((gemm_pair_kernel<T, 128, 128, 2, 2, Epi>), grid, dim3(256), 0, stream, p,
+                       ex, ew);
+  else
+    hipLaunchKernelGGL((gemm_pair_kernel<T, 64, 64, 2, 1, Epi>), grid, dim3(128), 0, stream, p, ex,
+                       ew);
+  if (plan.splits_x > 1 || plan.splits_w > 1) {
+    const int64_t nx = plan.splits_x > 1 ? (int64_t)x.M * div_up(x.N, 4) : 0,
+                  nw = plan.splits_w > 1 ? (int64_t)w.M * div_up(w.N, 4) : 0;
+    hipLaunchKernelGGL((gemm_join_pair_kernel<T, Epi>),
+                       dim3((unsigned)div_up(nx > nw ? nx : nw, 256), nx && nw ? 2 : 1), dim3(256),
+                       0, stream, p, ex, ew);
   }
   return last_launch_status();
 }
