@@ -162,7 +162,7 @@ constexpr int kTileF = 256;
 // (each of fp: F rounded up to 16 bytes, zeros behind F), the operand of both
 // products; with `rest`, what their rounding to T left follows in the row.
 // With `sums`, a tile's column sums for the biases ([row tiles][2 F], joined in
-// order by bias_join_kernel).
+// order by BiasJoin).
 template <class T>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const float* saved, int64_t M,
                                                          int F, int F4, int act, Dropout drop,
@@ -252,22 +252,41 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
   }
 }
 
-// Column sums over the row tiles, in order.
+// Column sums over the row tiles: kJoinRows sums of every kJoinRows-th tile, and
+// then those, each in order.  64 columns a workgroup.
 constexpr int kJoinRows = 16;
 template <class T>
-__global__ void __launch_bounds__(64 * kJoinRows) bias_join_kernel(const float* sums, int64_t parts,
-                                                                   int F, T* dbg, T* dbu) {
-  __shared__ double part[kJoinRows][64];
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + tx;
-  double s = 0.0;
-  if (c < 2 * F)
-    for (int64_t k = ty; k < parts; k += kJoinRows) s += sums[k * 2 * F + c];
-  part[ty][tx] = s;
-  __syncthreads();
-  if (ty || c >= 2 * F) return;
-  for (int r = 1; r < kJoinRows; ++r) s += part[r][tx];
-  (c < F ? dbg[c] : dbu[c - F]) = from_f32<T>((float)s);
+struct BiasJoin {
+  const float* sums;
+  int64_t parts;
+  T* dbg;
+  T* dbu;
+  int F, blocks;
+  template <int kThreads>
+  __device__ __forceinline__ void run(int block, char* lds) const {
+    constexpr int kLanes = kThreads / 64, kEach = kJoinRows / kLanes;
+    double (*part)[64] = reinterpret_cast<double (*)[64]>(lds);
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int c = block * 64 + tx;
+    double s[kEach] = {};
+    if (c < 2 * F)
+      for (int64_t k = ty; k < parts; k += kJoinRows)
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+          if (k + j * kLanes < parts) s[j] += sums[(k + j * kLanes) * 2 * F + c];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) part[ty + j * kLanes][tx] = s[j];
+    __syncthreads();
+    if (ty || c >= 2 * F) return;
+    double all = s[0];
+    for (int r = 1; r < kJoinRows; ++r) all += part[r][tx];
+    (c < F ? dbg[c] : dbu[c - F]) = from_f32<T>((float)all);
+  }
+};
+template <class T>
+__global__ void __launch_bounds__(64 * kJoinRows) bias_join_kernel(const BiasJoin<T> join) {
+  __shared__ __align__(16) char lds[kJoinRows * 64 * 8];
+  join.template run<64 * kJoinRows>(blockIdx.x, lds);
 }
 
 // A bump allocator over the caller's workspace (or, with a null base, its size).
@@ -475,11 +494,18 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
                        drop_of(drop), (T*)b.dgu, b.fp, (b.rest ? 4 : 2) * b.fp, b.rest,
                        dbg ? (float*)b.sums : nullptr);
     if ((st = last_launch_status())) return st;
-    if (dbg) {
-      hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)div_up(2 * F, 64)),
-                         dim3(64 * kJoinRows), 0, stream, (const float*)b.sums,
-                         div_up(M, kTileM), (int)F, (T*)dbg, (T*)dbu);
+    const bool pair = dx && dwg && b.pair.tile;
+    // The join of few row tiles rides along with the pair (a step of 256 x 128 -> 256
+    // 25.9 -> 24.5 us, 1000 x 1023 -> 1365 70 -> 67, 2048 x 4096 -> 256 71 -> 65); of many, it
+    // would be the last to end (4096 x 1024 -> 2048 156 -> 166).
+    const bool along = pair && div_up(M, kTileM) <= 128;
+    BiasJoin<T> join = {(const float*)b.sums, div_up(M, kTileM), (T*)dbg, (T*)dbu, (int)F,
+                              dbg ? (int)div_up(2 * F, 64) : 0};
+    if (dbg && !along) {
+      hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)join.blocks), dim3(64 * kJoinRows),
+                         0, stream, join);
       if ((st = last_launch_status())) return st;
+      join.blocks = 0;
     }
     if (b.pad) {
       st = pad_rows<T>(dwg ? x : nullptr, dx ? wg : nullptr, dx ? wu : nullptr, b.x, b.wg, b.wu, M,
@@ -507,10 +533,10 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
     aw.ranges = b.rest ? 2 : 1;
     aw.x_range = 2 * b.fp * size;
     const StoreEpi<T> ew = {(T*)dwg, (T*)dwu, (int)F, (int)b.fp, (int)D};
-    if (dx && dwg && b.pair.tile) {
+    if (pair) {
       ax.partial = b.pair.splits_x > 1 ? b.partial : nullptr;
       aw.partial = b.pair.splits_w > 1 ? b.partial + b.partial_w : nullptr;
-      return launch_pair<T>(ax, aw, ex, ew, b.pair, stream);
+      return launch_pair<T>(ax, aw, ex, ew, b.pair, join, stream);
     }
     if (dx && (st = launch_gemm<T, false, true>(ax, ex, b.gx, b.partial, stream))) return st;
     if (dwg && (st = launch_gemm<T, true, true>(aw, ew, b.gw, b.partial, stream))) return st;

@@ -518,18 +518,25 @@ __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
 // neither fills the chip for as long as it runs, unless it is cut into splits
 // whose sums are joined (a training step of 256 x 128 -> 256 in fp32 35 -> 26 us, of
 // 4096 x 1024 -> 2048 in bf16 183 -> 151).  The first `span` workgroups are those
-// of the product whose workgroups have more steps.
+// of the product whose workgroups have more steps.  `extra`, a small task of
+// `blocks` workgroups that needs neither, goes before them.
 struct GemmPair {
   GemmArgs x, w;
   int splits_x, splits_w, span;
   bool w_first;
 };
-template <class T, int BM, int BN, int kWavesM, int kWavesN, class Epi>
+template <class T, int BM, int BN, int kWavesM, int kWavesN, class Epi, class Extra>
 __global__ void __launch_bounds__(kWavesM* kWavesN * 64)
-    gemm_pair_kernel(const GemmPair p, const Epi ex, const Epi ew) {
+    gemm_pair_kernel(const GemmPair p, const Epi ex, const Epi ew, const Extra extra) {
   __shared__ __align__(1024) char lds[2][(BM + BN) * kStepBytes];
-  const bool behind = (int)blockIdx.x >= p.span, second = behind != p.w_first;
-  const int at = blockIdx.x - (behind ? p.span : 0);
+  const int block = (int)blockIdx.x - (extra.blocks + 7) / 8 * 8;
+  if (block < 0) {
+    if ((int)blockIdx.x < extra.blocks)
+      extra.template run<kWavesM * kWavesN * 64>(blockIdx.x, &lds[0][0]);
+    return;
+  }
+  const bool behind = block >= p.span, second = behind != p.w_first;
+  const int at = block - (behind ? p.span : 0);
   const int tiles = second ? p.w.tiles_m * p.w.tiles_n : p.x.tiles_m * p.x.tiles_n;
   const int wide = (tiles + 7) / 8 * 8;  // (a split's tiles start on the first XCD)
   const int split = at / wide, id = at % wide;
@@ -888,22 +895,22 @@ int launch_gemm(GemmArgs a, const Epi& epi, const GemmPlan& p, char* partial, hi
 }
 
 // x and w: the products of a backward pass, their partial sums where the plan splits.
-template <class T, class Epi>
+template <class T, class Epi, class Extra>
 int launch_pair(GemmArgs x, GemmArgs w, const Epi& ex, const Epi& ew, const PairPlan& plan,
-                hipStream_t stream) {
+                const Extra& extra, hipStream_t stream) {
   cut_gemm<T, false>(x, false, plan.tile, plan.splits_x);
   cut_gemm<T, true>(w, false, plan.tile, plan.splits_w);
   GemmPair p = {x, w, plan.splits_x, plan.splits_w, 0, w.steps_per_split > x.steps_per_split};
   const int64_t span_x = round_up(x.tiles_m * x.tiles_n, 8) * plan.splits_x,
                 span_w = round_up(w.tiles_m * w.tiles_n, 8) * plan.splits_w;
   p.span = (int)(p.w_first ? span_w : span_x);
-  const dim3 grid((unsigned)(span_x + span_w));
+  const dim3 grid((unsigned)(round_up(extra.blocks, 8) + span_x + span_w));
   if (plan.tile == 128)
-    hipLaunchKernelGGL((gemm_pair_kernel<T, 128, 128, 2, 2, Epi>), grid, dim3(256), 0, stream, p,
-                       ex, ew);
+    hipLaunchKernelGGL((gemm_pair_kernel<T, 128, 128, 2, 2, Epi, Extra>), grid, dim3(256), 0,
+                       stream, p, ex, ew, extra);
   else
-    hipLaunchKernelGGL((gemm_pair_kernel<T, 64, 64, 2, 1, Epi>), grid, dim3(128), 0, stream, p, ex,
-                       ew);
+    hipLaunchKernelGGL((gemm_pair_kernel<T, 64, 64, 2, 1, Epi, Extra>), grid, dim3(128), 0, stream,
+                       p, ex, ew, extra);
   if (plan.splits_x > 1 || plan.splits_w > 1) {
     const int64_t nx = plan.splits_x > 1 ? (int64_t)x.M * div_up(x.N, 4) : 0,
                   nw = plan.splits_w > 1 ? (int64_t)w.M * div_up(w.N, 4) : 0;
