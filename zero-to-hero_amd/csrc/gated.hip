@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const PadArgs<T> a, int c
       struct __attribute__((aligned(16))) { T e[kN]; } x;
       v4i v = {0, 0, 0, 0};
       if (c + kN <= cols) {
-        v = *reinterpret_cast<const v4i_any*>(in + r * cols + c);
+        v = sizeof(T) == 4 ? *reinterpret_cast<const v4i_any*>(in + r * cols + c)
+                           : load16_shifted((const char*)(in + r * cols + c));
       } else {
 #pragma unroll
         for (int i = 0; i < kN; ++i)

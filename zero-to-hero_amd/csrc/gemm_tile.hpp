@@ -617,8 +617,9 @@ __device__ __forceinline__ v4i load16_upto(const char* p, int left) {
 // that of reading W.  A workgroup takes 16 columns and its waves share K in
 // runs of 128 bytes; W goes straight to registers (no reuse for LDS to serve)
 // from rows of any alignment, and the waves' sums meet in LDS.  Rows of X
-// beyond M repeat the last one and are not stored.
-template <class T, int MT, int kWaves, class Epi>
+// beyond M repeat the last one and are not stored.  kOdd: rows that start off 4
+// bytes.
+template <class T, int MT, int kWaves, bool kOdd, class Epi>
 __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a, const Epi epi) {
   constexpr int kHalves = Epi::kGated ? 2 : 1;
   __shared__ Acc<T> red[kWaves][MT * kHalves][64];
@@ -643,6 +644,10 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
   const int full = kbytes / kRunBytes;  // whole runs
   // kRuns runs' loads are under way before the first is used
   constexpr int kRuns = MT == 1 ? 4 : MT == 2 ? 3 : 2;
+  auto load = [](const char* p) -> v4i {
+    if constexpr (kOdd) return load16_shifted(p);
+    return *reinterpret_cast<const v4i_any*>(p);
+  };
   auto take = [&](int s, auto runs) {
     constexpr int R = decltype(runs)::value;
     v4i wf[R][kHalves][2], xf[R][MT][2];
@@ -653,10 +658,10 @@ __global__ void __launch_bounds__(kWaves * 64) gemm_rows_kernel(const GemmArgs a
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
-          wf[r][h][ks] = *reinterpret_cast<const v4i_any*>(w[h] + k + ks * 64);
+          wf[r][h][ks] = load(w[h] + k + ks * 64);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
-          xf[r][i][ks] = *reinterpret_cast<const v4i_any*>(x[i] + k + ks * 64);
+          xf[r][i][ks] = load(x[i] + k + ks * 64);
       }
     }
 #pragma unroll
@@ -858,10 +863,17 @@ int launch_gemm(GemmArgs a, const Epi& epi, const GemmPlan& p, char* partial, hi
       // for many rows of fp32, which the matrix cores bind (64 x 8192 -> 2048 107 -> 114).
       const bool eight = div_up(a.N, 16) <= kCus && a.kbytes >= 32 * kRunBytes &&
                          !(sizeof(T) == 4 && a.M > 32);
+      const bool odd = sizeof(T) < 4 && (((uintptr_t)a.x | (uintptr_t)a.w0 | (uintptr_t)a.w1 |
+                                          (uintptr_t)a.xpitch | (uintptr_t)a.wpitch) & 3);
       auto go = [&](auto sets, auto waves) {
         constexpr int MT = decltype(sets)::value, kWaves = decltype(waves)::value;
-        hipLaunchKernelGGL((gemm_rows_kernel<T, MT, kWaves, Epi>), grid, dim3(kWaves * 64), 0,
-                           stream, a, epi);
+        constexpr bool kOdd = sizeof(T) < 4;
+        if (odd)
+          hipLaunchKernelGGL((gemm_rows_kernel<T, MT, kWaves, kOdd, Epi>), grid, dim3(kWaves * 64),
+                             0, stream, a, epi);
+        else
+          hipLaunchKernelGGL((gemm_rows_kernel<T, MT, kWaves, false, Epi>), grid, dim3(kWaves * 64),
+                             0, stream, a, epi);
       };
       auto with_waves = [&](auto sets) {
         if (eight) go(sets, std::integral_constant<int, 8>{});

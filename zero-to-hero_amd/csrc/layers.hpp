@@ -56,6 +56,22 @@ int with_dtype(int dtype, F&& f) {
   return f(fp16{});
 }
 
+// Sixteen bytes from any address, as the five aligned words that hold them
+// (none of which lies outside), shifted together: loads that start off 4 bytes
+// take three to four times as long.
+__device__ __forceinline__ v4i load16_shifted(const char* p) {
+  const int off = (int)((uintptr_t)p & 3);
+  typedef int v4i_words __attribute__((ext_vector_type(4), aligned(4)));
+  const char* words = p - off;
+  const v4i lo = *reinterpret_cast<const v4i_words*>(words);
+  const int hi = *reinterpret_cast<const int*>(words + (off ? 16 : 12));
+  v4i r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = (int)__builtin_amdgcn_alignbit(i < 3 ? lo[i + 1] : hi, lo[i], off * 8);
+  return r;
+}
+
 // Four consecutive elements, stored together where p allows it (`vec`: the
 // row's start and pitch are multiples of four elements), else those in range.
 // kStream: results that this kernel and the next do not read again leave the
