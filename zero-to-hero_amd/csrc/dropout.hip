@@ -11,7 +11,9 @@ namespace {
 // that a wave's store is one run of whole lines; it goes past the L2, which y
 // rarely fits (bf16 16384 x 8192 106 -> 90 us, fp32 8192 x 8192 94 -> 83, small
 // ones as before).  A workgroup is kX threads along the columns by 256 / kX
-// rows, so narrow rows fill it too.
+// rows, so narrow rows fill it too.  Rows that start off 16 bytes keep their
+// chunks: shifted words in, an unaligned store out (16384 x 8191 115 us; 290
+// element by element).
 template <class T, bool kVec>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, int64_t rows, int64_t cols,
                                                       const Dropout d, int tx_bits) {
@@ -29,6 +31,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, int64_t 
     struct __attribute__((aligned(16))) Chunk { T v[kN]; } in;
     if (kVec) {
       in = *reinterpret_cast<const Chunk*>(xr);
+    } else if (count == kN) {
+      in = __builtin_bit_cast(Chunk, load16_shifted(reinterpret_cast<const char*>(xr)));
     } else {
 #pragma unroll
       for (int i = 0; i < kN; ++i) in.v[i] = i < count ? xr[i] : from_f32<T>(0.0f);
@@ -42,6 +46,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, int64_t 
     for (int i = 0; i < kN; ++i) in.v[i] = from_f32<T>(v[i / 4][i % 4]);
     if (kVec) {
       __builtin_nontemporal_store(__builtin_bit_cast(v4f, in), reinterpret_cast<v4f*>(yr));
+    } else if (count == kN) {
+      *reinterpret_cast<v4i_any*>(yr) = __builtin_bit_cast(v4i, in);
     } else {
 #pragma unroll
       for (int i = 0; i < kN; ++i)

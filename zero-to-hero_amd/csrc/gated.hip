@@ -110,42 +110,6 @@ struct StoreEpi {
   }
 };
 
-// Up to three matrices of `cols` columns to rows at a pitch, zeros behind each
-// row, in one launch (blockIdx.y).
-template <class T>
-struct PadArgs {
-  const T* in[3];
-  T* out[3];
-  int64_t rows[3];
-};
-template <class T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const PadArgs<T> a, int cols, int pitch) {
-  const T* in = a.in[blockIdx.y];
-  T* out = a.out[blockIdx.y];
-  constexpr int kN = kPer16<T>;
-  // a workgroup takes as many rows at once as 256 threads of 16 bytes cover
-  const int chunks = pitch / kN;
-  int per_row = 256;
-  while (per_row / 2 >= chunks && per_row > 1) per_row >>= 1;
-  const int at = threadIdx.x & (per_row - 1), lanes = 256 / per_row;
-  for (int64_t r = (int64_t)blockIdx.x * lanes + threadIdx.x / per_row; r < a.rows[blockIdx.y];
-       r += (int64_t)gridDim.x * lanes)
-    for (int c = at * kN; c < pitch; c += per_row * kN) {
-      struct __attribute__((aligned(16))) { T e[kN]; } x;
-      v4i v = {0, 0, 0, 0};
-      if (c + kN <= cols) {
-        v = sizeof(T) == 4 ? *reinterpret_cast<const v4i_any*>(in + r * cols + c)
-                           : load16_shifted((const char*)(in + r * cols + c));
-      } else {
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-          x.e[i] = c + i < cols ? in[r * cols + c + i] : from_f32<T>(0.0f);
-        v = __builtin_bit_cast(v4i, x);
-      }
-      *reinterpret_cast<v4i*>(out + r * pitch + c) = v;
-    }
-}
-
 // What rounding x to T leaves (nothing where the rounded value is not finite).
 template <class T>
 __device__ __forceinline__ float rounding_rest(float x) {
@@ -195,6 +159,10 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
     const T* dp = dh + m * F;
     if (vec) {
       d[i] = *reinterpret_cast<const Four*>(dp + c);
+    } else if (sizeof(T) == 2 && n + 8 <= F) {  // (four of eight elements)
+      const v4i eight = load16_shifted(reinterpret_cast<const char*>(dp + n));
+      const int two[2] = {eight[0], eight[1]};
+      __builtin_memcpy(&d[i], two, sizeof(two));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) d[i].x[k] = dp[min(n + k, F - 1)];
@@ -390,16 +358,12 @@ bool backward_fits(int dtype, int64_t M, int64_t D, int64_t F) {
 }
 
 // Padded copies of x [M,D] and of the weights [F,D] (those that are not NULL).
-template <class T>
-int pad_rows(const void* x, const void* wg, const void* wu, char* xp, char* wgp, char* wup,
-             int64_t M, int64_t D, int64_t F, int64_t pitch, hipStream_t stream) {
-  const PadArgs<T> a = {{(const T*)x, (const T*)wg, (const T*)wu},
-                        {(T*)xp, (T*)wgp, (T*)wup},
-                        {x ? M : 0, wg ? F : 0, wu ? F : 0}};
-  const int64_t rows = M > F ? M : F;
-  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(rows < 4096 ? rows : 4096), 3),
-                     dim3(256), 0, stream, a, (int)D, (int)(pitch / sizeof(T)));
-  return last_launch_status();
+int pad_operands(const void* x, const void* wg, const void* wu, char* xp, char* wgp, char* wup,
+                 int64_t M, int64_t F, int64_t bytes, int64_t pitch, hipStream_t stream) {
+  const PadArgs a = {{(const char*)x, (const char*)wg, (const char*)wu},
+                     {xp, wgp, wup},
+                     {x ? M : 0, wg ? F : 0, wu ? F : 0}};
+  return pad_rows(a, bytes, pitch, stream);
 }
 
 bool drop_ok(const ppo_dropout* d) { return !d || (d->p >= 0.0 && d->p <= 1.0); }
@@ -445,7 +409,8 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
     a.M = (int)M;
     a.N = (int)F;
     if (f.pad) {
-      const int st = pad_rows<T>(x, wg, wu, f.x, f.wg, f.wu, M, D, F, f.pitch, stream);
+      const int st = pad_operands(x, wg, wu, f.x, f.wg, f.wu, M, F, D * (int64_t)sizeof(T), f.pitch,
+                                  stream);
       if (st) return st;
       a.x = f.x;
       a.w0 = f.wg;
@@ -509,8 +474,8 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
       join.blocks = 0;
     }
     if (b.pad) {
-      st = pad_rows<T>(dwg ? x : nullptr, dx ? wg : nullptr, dx ? wu : nullptr, b.x, b.wg, b.wu, M,
-                       D, F, b.pitch, stream);
+      st = pad_operands(dwg ? x : nullptr, dx ? wg : nullptr, dx ? wu : nullptr, b.x, b.wg, b.wu, M,
+                        F, D * size, b.pitch, stream);
       if (st) return st;
     }
     GemmArgs ax = {};

@@ -613,6 +613,64 @@ __device__ __forceinline__ v4i load16_upto(const char* p, int left) {
   return r.v;
 }
 
+// The same by few loads: the row, of `bytes` bytes, has its last sixteen shifted
+// where fewer are left.
+__device__ __forceinline__ v4i load16_of_row(const char* p, int left, int bytes, bool odd) {
+  if (left <= 0) return v4i{0, 0, 0, 0};
+  if (bytes < 16) return load16_upto(p, left);
+  const int gone = left < 16 ? 16 - left : 0;
+  const char* at = p - gone;
+  const v4i v = odd || gone ? load16_shifted(at) : *reinterpret_cast<const v4i_any*>(at);
+  uint64_t part[2];
+  __builtin_memcpy(part, &v, 16);
+  if (gone >= 8) {
+    part[0] = part[1] >> (gone - 8) * 8;
+    part[1] = 0;
+  } else if (gone) {
+    part[0] = part[0] >> gone * 8 | part[1] << (8 - gone) * 8;
+    part[1] >>= gone * 8;
+  }
+  v4i r;
+  __builtin_memcpy(&r, part, 16);
+  return r;
+}
+
+// Up to three matrices of rows of `bytes` bytes to rows at a pitch, zeros behind
+// each row, in one launch (blockIdx.y).  odd: some row starts off 4 bytes.
+struct PadArgs {
+  const char* in[3];
+  char* out[3];
+  int64_t rows[3];
+};
+inline __global__ void __launch_bounds__(256) pad_rows_kernel(const PadArgs a, int bytes, int pitch,
+                                                              bool odd) {
+  const char* in = a.in[blockIdx.y];
+  char* out = a.out[blockIdx.y];
+  // a workgroup takes as many rows at once as 256 threads of 16 bytes cover
+  const int chunks = pitch / 16;
+  int per_row = 256;
+  while (per_row / 2 >= chunks && per_row > 1) per_row >>= 1;
+  const int at = threadIdx.x & (per_row - 1), lanes = 256 / per_row;
+  for (int64_t r = (int64_t)blockIdx.x * lanes + threadIdx.x / per_row; r < a.rows[blockIdx.y];
+       r += (int64_t)gridDim.x * lanes)
+    for (int c = at * 16; c < pitch; c += per_row * 16) {
+      *reinterpret_cast<v4i*>(out + r * pitch + c) =
+          load16_of_row(in + r * bytes + c, bytes - c, bytes, odd);
+    }
+}
+
+inline int pad_rows(const PadArgs& a, int64_t bytes, int64_t pitch, hipStream_t stream) {
+  int64_t rows = 0;
+  uintptr_t starts = (uintptr_t)bytes;
+  for (int i = 0; i < 3; ++i) {
+    rows = a.rows[i] > rows ? a.rows[i] : rows;
+    starts |= (uintptr_t)a.in[i];
+  }
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)(rows < 4096 ? rows : 4096), 3), dim3(256), 0,
+                     stream, a, (int)bytes, (int)pitch, (starts & 3) != 0);
+  return last_launch_status();
+}
+
 // Few rows of X (at most 16 * MT): every weight is read once, so the time is
 // that of reading W.  A workgroup takes 16 columns and its waves share K in
 // runs of 128 bytes; W goes straight to registers (no reuse for LDS to serve)
@@ -755,8 +813,8 @@ inline size_t partial_size(int splits, int64_t M, int64_t wrows) {
 // two splits 79, 33 and 90; fp32 1024 x 1024 -> 512 in 64s and one, two or four
 // splits 40 / 43 / 31.  The rows kernel's time is that of reading W, or of one
 // workgroup's K where the columns are few, more where a single matrix does not
-// share the reads of x, and three or four times that for rows that start off 4
-// bytes (1 x 8191 -> 2048 gated bf16 58 us, 8192 20).  The tiles, which want a padded copy of
+// share the reads of x, and two to three times that for rows that start off 4
+// bytes (16 and 64 x 1023 -> 1365 gated bf16 9 and 25 us, 1024 -> 1365 5 and 8).  The tiles, which want a padded copy of
 // rows off 16 bytes, have to be 15% better by this estimate, which is for weights
 // that the caches hold (from HBM the rows kernel loses least).  1, 16, 32 and 64 rows
 // of 4096 -> 8192 gated 24, 25, 32 and 47, against 25, 26, 26 and 27 for tiles of 64 in
@@ -772,9 +830,10 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32
     const int set = M <= 16 ? 0 : M <= 32 ? 1 : 2;
     const double reads[2][3] = {{1.25, 2.0, 3.3}, {1.03, 1.25, 1.8}};
     const double row[2][3] = {{0.75, 1.3, 2.1}, {1.15, 1.75, 2.6}};
+    const double odd[] = {1.8, 2.2, 3.0};
     const double all = 1.0 + (double)wrows * kbytes / 5.6e6 * reads[kind][set];
     const double one = 2.4 + (double)kbytes / 1024.0 * row[kind][set];
-    best = fmax(all, one) * (row_bytes % 4 ? set ? 4.0 : 3.0 : 1.0) / 1.15;
+    best = fmax(all, one) * (row_bytes % 4 ? odd[set] : 1.0) / 1.15;
     if (row_bytes != kbytes) best -= 4.0 + 2.0 * (double)wrows * kbytes / 5.3e6;
   }
   const double steps = (double)div_up(kbytes, kStepBytes);

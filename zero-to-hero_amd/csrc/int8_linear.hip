@@ -52,14 +52,6 @@ struct Int8Epi {
   }
 };
 
-// Rows of int8 at a pitch, zeros behind each row.
-__global__ void __launch_bounds__(256) pad_int8_kernel(const int8_t* in, int64_t rows, int64_t cols,
-                                                       int8_t* out, int64_t pitch) {
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int64_t c = threadIdx.x; c < pitch; c += 256)
-      out[r * pitch + c] = c < cols ? in[r * cols + c] : 0;
-}
-
 // max |x| as its bits: ordered as integers, an infinity above every finite
 // value and a NaN above that, so a row that is not finite shows.
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -422,22 +414,21 @@ extern "C" int ppo_layer_int8_linear(const void* x, const int8_t* xq, const floa
     int st = PPO_OK;
     if (x) {
       st = launch_quantize<T>(x, M, K, (int8_t*)p.xq, p.pitch, (float*)p.xs, stream);
-      a.x = p.xq;
-      a.xpitch = p.pitch;
-    } else if (p.pad_x) {
-      hipLaunchKernelGGL(pad_int8_kernel, dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0,
-                         stream, xq, M, K, (int8_t*)p.xq, p.pitch);
-      a.x = p.xq;
-      a.xpitch = p.pitch;
-      st = last_launch_status();
+      if (st) return st;
     }
-    if (st) return st;
+    if (x || p.pad_x) {
+      a.x = p.xq;
+      a.xpitch = p.pitch;
+    }
     if (p.pad_w) {
-      hipLaunchKernelGGL(pad_int8_kernel, dim3((unsigned)(N < 65536 ? N : 65536)), dim3(256), 0,
-                         stream, wq, N, K, (int8_t*)p.wq, p.pitch);
       a.w0 = p.wq;
       a.wpitch = p.pitch;
-      if ((st = last_launch_status())) return st;
+    }
+    if (p.pad_x || p.pad_w) {
+      const PadArgs pad = {{(const char*)xq, (const char*)wq, nullptr},
+                           {p.xq, p.wq, nullptr},
+                           {p.pad_x ? M : 0, p.pad_w ? N : 0, 0}};
+      if ((st = pad_rows(pad, K, p.pitch, stream))) return st;
     }
     // the tile kernel's rows end on 16 bytes (zeros behind K), the rows kernel's on K
     if (p.gemm.tile) a.kbytes = p.pitch;

@@ -88,6 +88,9 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count, boo
       __builtin_nontemporal_store(__builtin_bit_cast(Words, q), reinterpret_cast<Words*>(p));
     else
       *reinterpret_cast<Four*>(p) = q;
+  } else if (count >= 4) {  // (a start off its size takes the same instruction)
+    typedef Words __attribute__((aligned(1))) WordsAny;
+    *reinterpret_cast<WordsAny*>(p) = __builtin_bit_cast(Words, q);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)

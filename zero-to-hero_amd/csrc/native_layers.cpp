@@ -5,9 +5,9 @@
 // checks.
 //
 // Measured on MI355X, us a call among others, through Python and here: dropout
-// of 128 x 128 with its gradient 112 and 46 (of which torch.autograd.grad itself
-// takes 34), the gated block of 256 x 128 -> 256 with its gradients 183 and 89,
-// int8_linear of one row 16 and 8.
+// of 128 x 128 with its gradient 48 and 28 (of which torch's engine takes 18), the
+// gated block of 256 x 128 -> 256 with its gradients 86 and 54, int8_linear of one
+// row 14 and 7 (another host takes up to twice that in every figure).
 #include "native.hpp"
 
 #include <c10/core/DeviceGuard.h>
