@@ -236,7 +236,8 @@ INT8_SHAPES = [(1, 1, 1), (1, 4, 16), (2, 3, 33), (16, 65, 128), (17, 48, 1000),
                (64, 130, 515), (65, 64, 64), (100, 127, 96), (129, 200, 2049), (300, 513, 64),
                (70, 64, 8192), (1, 4096, 512), (1, 50, 16384), (4, 100, 4096), (5, 33, 3001),
                (15, 70, 1092), (16, 48, 1024), (3, 20, 16), (2048, 2048, 160), (3300, 4200, 48),
-               (257, 31, 77), (2, 40, 65536), (33, 70, 20000), (20, 33, 40001)]
+               (257, 31, 77), (2, 40, 65536), (33, 70, 20000), (20, 33, 40001), (2, 40, 4001),
+               (1, 37, 8190), (16, 48, 512), (13, 33, 601)]
 
 
 def _int8_case(dtype, M, N, K, bias):

@@ -221,17 +221,20 @@ int launch_quantize(const void* x, int64_t rows, int64_t cols, int8_t* q, int64_
 
 // The product of a few rows of floating x, in one launch: every workgroup
 // quantises the rows for itself (into LDS, by 256 / rows threads each), which
-// for up to kFewElements costs it less than a launch of its own would the call
-// (one row of 4096 -> 4096 in bf16: 8.4 us in two kernels), then takes 16
-// columns as the rows kernel does.
+// for up to kFewBytes costs it less than a launch of its own would the call (in
+// two kernels and here, us in a replayed graph: one row of bf16 1024 -> 1024 5.7 and
+// 4.3, 4096 -> 4096 8.1 and 6.9, 8192 -> 4096 11.6 and 11.2; 8 rows of 1024 -> 1024 6.3 and
+// 6.9, of fp32 6.2 and 8.2; 4 of bf16 4096 -> 4096 8.8 and 12.9; the second launch costs
+// the host 3 more), then takes 16 columns as the rows kernel does.  kOdd: rows of w
+// that start off 4 bytes.
 constexpr int kFewRows = 16;
-constexpr int64_t kFewElements = 16384;
+constexpr int64_t kFewBytes = 16384;  // of x
 
-template <class T>
+template <class T, bool kOdd>
 __global__ void __launch_bounds__(256) int8_few_kernel(const T* x, const int8_t* w, int M, int N,
                                                        int K, const float* ws, const T* bias,
                                                        T* out) {
-  __shared__ __align__(16) int8_t xq[kFewElements + kFewRows * 32];
+  __shared__ __align__(16) int8_t xq[kFewBytes / sizeof(T) + kFewRows * 32];
   __shared__ uint32_t tops[kFewRows];
   __shared__ float scales[kFewRows];
   __shared__ v4i red[4][64];
@@ -252,7 +255,10 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const T* x, const int8_t*
     for (int r = 0; r < (int)(sizeof(wf) / sizeof(wf[0])); ++r)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
-        wf[r][ks] = *reinterpret_cast<const v4i_any*>(wr + (s + r * 4) * kRunBytes + ks * 64);
+        if constexpr (kOdd)
+          wf[r][ks] = load16_shifted(wr + (s + r * 4) * kRunBytes + ks * 64);
+        else
+          wf[r][ks] = *reinterpret_cast<const v4i_any*>(wr + (s + r * 4) * kRunBytes + ks * 64);
   };
   if (ahead) fetch(wave, early);
   if (tid < kFewRows) tops[tid] = 0;
@@ -400,9 +406,14 @@ extern "C" int ppo_layer_int8_linear(const void* x, const int8_t* xq, const floa
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   return with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
-    if (x && M <= kFewRows && M * K <= kFewElements) {
-      hipLaunchKernelGGL((int8_few_kernel<T>), dim3((unsigned)div_up(N, 16)), dim3(256), 0, stream,
-                         (const T*)x, wq, (int)M, (int)N, (int)K, ws, (const T*)bias, (T*)out);
+    if (x && M <= kFewRows && M * K <= kFewBytes / (int64_t)sizeof(T)) {
+      auto go = [&](auto odd) {
+        hipLaunchKernelGGL((int8_few_kernel<T, decltype(odd)::value>), dim3((unsigned)div_up(N, 16)),
+                           dim3(256), 0, stream, (const T*)x, wq, (int)M, (int)N, (int)K, ws,
+                           (const T*)bias, (T*)out);
+      };
+      if (((uintptr_t)wq | (uintptr_t)K) & 3) go(std::true_type{});
+      else go(std::false_type{});
       return last_launch_status();
     }
     GemmArgs a = {};
