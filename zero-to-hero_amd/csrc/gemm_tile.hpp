@@ -785,13 +785,14 @@ constexpr int kRowsMax = 64;       // rows that the rows kernel takes
 constexpr int64_t kMaxRows = (int64_t)1 << 27;   // of either operand
 constexpr int64_t kMaxPitch = (int64_t)1 << 22;  // 256 rows of a tile stay below 2^31 bytes
 
-// What a workgroup of a tile takes, in us (plan_gemm).
-struct TileCost { int tile, per_cu; double step[2], alone[2], fixed, lone; };
-constexpr TileCost kTileCosts[] = {
-    {256, 1, {0.95, 7.2}, {1.11, 7.2}, 17.6, 10.7},
-    {128, 2, {0.32, 1.8}, {0.52, 2.0}, 4.2, 7.8},
-    {64, 5, {0.19, 0.90}, {0.44, 1.08}, 1.75, 4.6},
-};
+// What a workgroup of a tile takes, in us (plan_gemm): 8- and 16-bit types and
+// fp32, of rows along k and of k-rows (fitted to 440 cuts of 18 backward passes).
+struct TileCost { int tile, per_cu; double step, alone, fixed, lone; };
+constexpr TileCost kTileCosts[2][2][3] = {
+    {{{256, 1, 0.95, 1.11, 17.6, 10.7}, {128, 2, 0.32, 0.52, 4.2, 7.8}, {64, 5, 0.19, 0.44, 1.75, 4.6}},
+     {{256, 1, 7.2, 7.2, 17.6, 10.7}, {128, 2, 1.8, 2.0, 4.2, 7.8}, {64, 5, 0.90, 1.08, 1.75, 4.6}}},
+    {{{256, 1, 1.32, 1.28, 17.6, 11.6}, {128, 2, 0.49, 0.79, 4.7, 7.8}, {64, 5, 0.20, 0.68, 1.33, 6.8}},
+     {{256, 1, 4.65, 7.4, 21.0, 8.3}, {128, 2, 2.05, 2.16, 2.3, 4.1}, {64, 5, 0.60, 1.43, 1.2, 2.0}}}};
 inline double join_cost(int splits, int64_t M, int64_t wrows) {
   return splits > 1 ? splits * 8.0 * (double)M * wrows / 13.6e6 : 0.0;
 }
@@ -837,13 +838,13 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32
     if (row_bytes != kbytes) best -= 4.0 + 2.0 * (double)wrows * kbytes / 5.3e6;
   }
   const double steps = (double)div_up(kbytes, kStepBytes);
-  for (const TileCost& c : kTileCosts) {
+  for (const TileCost& c : kTileCosts[kind == kByKRows][fp32]) {
     for (int splits = 1; splits <= 16; splits *= 2) {
       if (splits > 1 && steps < 4.0 * splits) break;
       const double groups = (double)(div_up(M, c.tile) * div_up(wrows, c.tile)) * splits;
       const double each = ceil(steps / splits);
-      const double busy = ceil(groups / kCus) * (each * c.step[fp32] + c.fixed);
-      const double waits = ceil(groups / (kCus * c.per_cu)) * (each * c.alone[fp32] + c.lone);
+      const double busy = ceil(groups / kCus) * (each * c.step + c.fixed);
+      const double waits = ceil(groups / (kCus * c.per_cu)) * (each * c.alone + c.lone);
       const double join = (splits > 1 ? 4.0 : 0.0) + join_cost(splits, M, wrows);
       const double time = fmax(busy, waits) + join;
       if (p.tile < 0 || time < best) {
@@ -860,7 +861,8 @@ inline GemmPlan plan_gemm(int64_t M, int64_t wrows, int64_t row_bytes, bool fp32
 
 // The same for the two products of a backward pass in one launch (tile 0: they
 // run apart).  Both share the tile; a round of workgroups takes the mean of
-// theirs.
+// theirs.  Over 18 backward passes in up to 48 cuts the one chosen takes 2.3%
+// longer than the best.
 struct PairPlan {
   int tile, splits_x, splits_w;
   size_t partial_x, partial_w;  // bytes
@@ -870,18 +872,18 @@ inline PairPlan plan_pair(int64_t Mx, int64_t Nx, int64_t bytes_x, int64_t Mw, i
   PairPlan p = {0, 1, 1, 0, 0};
   double best = apart;
   const double kx = (double)div_up(bytes_x, kStepBytes), kw = (double)div_up(bytes_w, kStepBytes);
-  for (const TileCost& c : kTileCosts) {
-    if (c.tile == 256) continue;
+  for (const TileCost& c : kTileCosts[1][fp32]) {
     const double gx = (double)(div_up(Mx, c.tile) * div_up(Nx, c.tile)),
                  gw = (double)(div_up(Mw, c.tile) * div_up(Nw, c.tile));
     for (int sx = 1; sx <= 16 && (sx == 1 || kx >= 4.0 * sx); sx *= 2)
       for (int sw = 1; sw <= 16 && (sw == 1 || kw >= 4.0 * sw); sw *= 2) {
         const double groups = gx * sx + gw * sw, ex = ceil(kx / sx), ew = ceil(kw / sw);
         const double each = (gx * sx * ex + gw * sw * ew) / groups;
-        const double busy = ceil(groups / kCus) * (each * c.step[fp32] + c.fixed);
-        const double waits = fmax(ceil(groups / (kCus * c.per_cu)) * (each * c.alone[fp32] + c.lone),
-                                  fmax(ex, ew) * c.alone[fp32] + c.lone);
-        const double join = sx * sw > 1 ? 4.0 + join_cost(sx, Mx, Nx) + join_cost(sw, Mw, Nw) : 0.0;
+        const double busy = ceil(groups / kCus) * (each * c.step + c.fixed);
+        const double waits = fmax(ceil(groups / (kCus * c.per_cu)) * (each * c.alone + c.lone),
+                                  fmax(ex, ew) * c.alone + c.lone);
+        const double join =
+            sx * sw > 1 ? 4.0 + 2.0 * (join_cost(sx, Mx, Nx) + join_cost(sw, Mw, Nw)) : 0.0;
         const double time = fmax(busy, waits) + join;
         if (time < best) {
           best = time;
@@ -976,7 +978,10 @@ int launch_pair(GemmArgs x, GemmArgs w, const Epi& ex, const Epi& ew, const Pair
                 span_w = round_up(w.tiles_m * w.tiles_n, 8) * plan.splits_w;
   p.span = (int)(p.w_first ? span_w : span_x);
   const dim3 grid((unsigned)(round_up(extra.blocks, 8) + span_x + span_w));
-  if (plan.tile == 128)
+  if (plan.tile == 256)
+    hipLaunchKernelGGL((gemm_pair_kernel<T, 256, 256, 2, 2, Epi, Extra>), grid, dim3(256), 0,
+                       stream, p, ex, ew, extra);
+  else if (plan.tile == 128)
     hipLaunchKernelGGL((gemm_pair_kernel<T, 128, 128, 2, 2, Epi, Extra>), grid, dim3(256), 0,
                        stream, p, ex, ew, extra);
   else
