@@ -22,6 +22,7 @@ Tolerances.  u(t) = finfo(t).eps / 2 bounds one rounding to type t, relative.
                  (an element is a sum of many independently rounded terms).
 """
 
+import ctypes
 import itertools
 import math
 
@@ -117,6 +118,21 @@ def test_dropout_shapes_share_the_mask(dev):
     rows = torch.tensor([7, 7, 2, 7, 29], device=dev)  # the same row again
     z = ppo_amd.dropout(x.view(30, 24)[rows], 0.4, 5, rows=rows)
     assert torch.equal(z, y.view(30, 24)[rows])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(64, 128), (37, 1001), (300, 5), (2, 70001)])
+def test_dropout_in_place(dev, shape, dtype):
+    """The C entry's y may be x itself, also where rows start off a word."""
+    x = rn(torch.Generator().manual_seed(2), TYPES[dtype], *shape).to(dev)
+    for offset in (0, 1):
+        v = at_offset(x, dev, offset)
+        want = ppo_amd.dropout(x, 0.4, 21)
+        drop = _lib.Dropout(0.4, 21, None, None)
+        code = _lib.load_layers().ppo_layer_dropout(
+            v.data_ptr(), v.data_ptr(), {"fp32": 0, "bf16": 1, "fp16": 2}[dtype], *shape,
+            ctypes.byref(drop), torch.cuda.current_stream(dev).cuda_stream)
+        assert code == 0 and torch.equal(v, want)
 
 
 def test_dropout_seeds(dev):
