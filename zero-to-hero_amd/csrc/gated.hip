@@ -159,10 +159,6 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
     const T* dp = dh + m * F;
     if (vec) {
       d[i] = *reinterpret_cast<const Four*>(dp + c);
-    } else if (sizeof(T) == 2 && n + 8 <= F) {  // (four of eight elements)
-      const v4i eight = load16_shifted(reinterpret_cast<const char*>(dp + n));
-      const int two[2] = {eight[0], eight[1]};
-      __builtin_memcpy(&d[i], two, sizeof(two));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) d[i].x[k] = dp[min(n + k, F - 1)];
