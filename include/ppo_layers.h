@@ -107,7 +107,9 @@ int ppo_layer_gated_forward(const void* x, const void* wg, const void* wu, const
  * Outputs that are NULL are not computed (dwg and dwu, and dbg and dbu, go
  * together).  M > 0 (over no rows the weights' gradients are the caller's
  * zeros).  dg and du are rounded to `dtype`, the matrix cores' operand
- * type, before the products.  Sums are split and joined in a fixed order:
+ * type, before the products: a 16-bit gradient is then off by about 1.4 times
+ * what its own rounding makes (in short passes the products take what that
+ * rounding left as well), and an fp16 dg or du past 65504 is infinite.  Sums are split and joined in a fixed order:
  * the same call gives the same bits (one that asks for other outputs may cut
  * the sums elsewhere).
  */

@@ -488,6 +488,41 @@ def test_gated_gradients_of_few_rows(dev, dtype, M, D, F):
         assert diff <= (u_of(t) + u_of(t) ** 2 + 64 * U32) * norm + tiny, name
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,D,F", [(64, 48, 512), (256, 128, 256), (1, 100, 4096), (300, 33, 999)])
+def test_gated_gradients_of_short_passes(dev, dtype, M, D, F):
+    """The products take what the rounding of dg and du left, so the gradients
+    are off by their own rounding and little more.  A gradient y' before it is
+    off y by the 32-bit terms (64 u32) and by dg and du rounded twice (u^2 each,
+    independent, taken 4 times over) in the 2-norm, and RN(y') is at most
+    2 |y' - y| further from y than RN(y) is."""
+    t = TYPES[dtype]
+    x, wg, wu, bg, bu, dh = gated_case(dtype, M, D, F, True, seed=8)
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu, bg, bu)]
+    grads = torch.autograd.grad(ppo_amd.gated_ffn(*leaves), leaves, dh.to(dev))
+    _, g, u = ref.gated_ffn(*d64(x, wg, wu, bg, bu), "silu")
+    want = ref.gated_ffn_grads(*d64(x, wg, wu), g, u, "silu", dh.double())
+    for name, got, w in zip(("dx", "dwg", "dwu", "dbg", "dbu"), grads, want):
+        diff, own = (got.double().cpu() - w).norm(), (w.to(t).double() - w).norm()
+        assert diff <= own + 2 * (4 * u_of(t) ** 2 + 64 * U32) * w.norm(), \
+            f"{name}: {float(diff / own):.4f} of its own rounding"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,D,F", [(1, 64, 4097), (1, 64, 8192), (1024, 64, 1024), (1025, 64, 1024),
+                                   (256, 128, 2052)])
+def test_gated_gradients_on_both_sides_of_short(dev, dtype, M, D, F):
+    """Where a pass stops being short: within both roundings on either side."""
+    t = TYPES[dtype]
+    x, wg, wu, _, _, dh = gated_case(dtype, M, D, F, False, seed=8)
+    leaves = [v.to(dev).requires_grad_() for v in (x, wg, wu)]
+    grads = torch.autograd.grad(ppo_amd.gated_ffn(*leaves), leaves, dh.to(dev))
+    _, g, u = ref.gated_ffn(*d64(x, wg, wu), None, None, "silu")
+    want = ref.gated_ffn_grads(*d64(x, wg, wu), g, u, "silu", dh.double())
+    for name, got, w in zip(("dx", "dwg", "dwu"), grads, want):
+        check_grad(got, w, t, name)
+
+
 def test_gated_dropout_is_dropouts(dev):
     x, wg, wu, bg, bu, _ = gated_case("fp32", 70, 24, 37, True)
     args = [v.to(dev) for v in (x, wg, wu, bg, bu)]

@@ -293,12 +293,23 @@ ForwardPlan plan_forward(int dtype, int64_t M, int64_t D, int64_t F, bool aligne
   return f;
 }
 
-// A 16-bit dg or du is off by up to half a step, which averages out in the sums
-// of both products, except where there are few of them: with 2 x 128 of them,
-// bf16 weight gradients were off by 2.6e-3 in the 2-norm where their own rounding
-// makes 1.7e-3.  Up to this many elements the products take what the rounding
-// left as well, as further ranges of K (their time is that of a launch).
-constexpr int64_t kRestElements = 4096;
+// The products take dg and du in `dtype`, the matrix cores' operand type.  Their
+// roundings are independent, so in a sum they grow as the sum itself does: at any
+// size a 16-bit gradient is off by 2.35e-3 (bf16, 2-norm) where its own rounding
+// makes 1.66e-3, and by less than 1% more than that when the products take what
+// the rounding left as well, as two more ranges of K.  That is done where the
+// backward pass takes little longer than its launches (M, D, F: us without and
+// with, bf16 in a replayed graph: 64 x 512 -> 512 12.4 and 14.1, 256 x 64 -> 128 9.7
+// and 12.6, 32 x 512 -> 2048 16.7 and 19.7); elsewhere it would cost up to two thirds
+// of the products (1024 x 512 -> 512 19.3 and 25.4, 1024 x 4096 -> 512 29 and 48,
+// and of long sums to dx 1 x 512 -> 8192 22.5 and 31.9).  D past 2^14 counts as that:
+// few rows' passes are then bound by reading the weights.
+constexpr int64_t kRestWork = (int64_t)1 << 26;
+constexpr int64_t kRestColumns = 4096;
+bool takes_rest(int64_t size, int64_t M, int64_t D, int64_t F) {
+  constexpr int64_t kLongest = (int64_t)1 << 14;
+  return size == 2 && F <= kRestColumns && M * F <= kRestWork / (D < kLongest ? D : kLongest);
+}
 
 struct BackwardPlan {
   int64_t fp;     // F rounded up to 16 bytes of elements
@@ -319,7 +330,7 @@ BackwardPlan plan_backward(int dtype, int64_t M, int64_t D, int64_t F, bool alig
   b.pitch = round_up(D * size, 16);
   b.pad = !aligned || b.pitch != D * size;
   Scratch s{ws};
-  b.rest = size == 2 && M * F <= kRestElements;
+  b.rest = takes_rest(size, M, D, F);
   const int64_t parts = b.rest ? 4 : 2;
   b.dgu = s.take(M * parts * b.fp * size);
   if (b.pad) {

@@ -254,7 +254,10 @@ def gated_ffn(
     arguments are those of dropout(), whose mask over [M, F] it applies.
     Differentiable once in x, the weights and the biases (create_graph raises):
     g and u are kept for the backward pass in 32 bits (8 M F bytes), the mask
-    is formed again.
+    is formed again.  The gradients of g and u are rounded to x's type for the
+    products behind them: 16-bit gradients are off by up to 1.4 times what
+    their own rounding makes, and in fp16 those past 65504 become infinite
+    (scale the loss accordingly).
     """
     got = _native().layer_gated_ffn(x, w_gate, w_up, b_gate, b_up,
                                     ACTIVATIONS.get(activation), dropout_p, seed, rows)
