@@ -41,6 +41,32 @@ def test_registered_operators(dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_registered_backward_refuses(dev):
+    """The registered backward pass checks its arguments as the functions do."""
+    leaves, dh = _case(dev, 20)
+    x, wg, wu = (t.detach() for t in leaves[:3])
+    saved = torch.randn(2, 20, 36, device=dev)
+    f = torch.ops.ppo_amd.gated_ffn_backward
+
+    def call(dh=dh, x=x, wg=wg, wu=wu, saved=saved, seed_at=None, rows=None):
+        return f(dh, x, wg, wu, saved, True, "silu", 0.1, 1, seed_at, rows)
+
+    assert [tuple(t.shape) for t in call()] == [(20, 24), (36, 24), (36, 24), (36,), (36,)]
+    for kw in (dict(dh=dh[:19].contiguous()), dict(saved=saved[:, :19].contiguous()),
+               dict(dh=dh.t().contiguous().t()), dict(wu=wu[:35].contiguous()),
+               dict(rows=torch.arange(19, device=dev)), dict(seed_at=torch.arange(2, device=dev))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    for kw in (dict(dh=dh.half()), dict(saved=saved.half()),
+               dict(rows=torch.arange(20, device=dev, dtype=torch.int32))):
+        with pytest.raises(TypeError):
+            call(**kw)
+    for kw in (dict(saved=saved.cpu()), dict(rows=torch.arange(20)),
+               dict(seed_at=torch.tensor([1]))):
+        with pytest.raises(RuntimeError, match="no CPU fallback|expected"):
+            call(**kw)
+
+
 def test_registered_operators_compile(dev):
     """A compiled layer with its backward is traced whole and equals eager."""
     op = torch.ops.ppo_amd

@@ -184,6 +184,55 @@ def test_operators_fake_shapes_and_cpu():
         op.dropout(torch.zeros(2, 2), 0.1, 1, None, None)
 
 
+def _backward_faults(torch_device="cuda"):
+    """(arguments of a gated backward, the error) with one of them wrong, as
+    fake tensors: nothing may be launched on them."""
+    bf = torch.bfloat16
+
+    def e(*shape, dtype=bf, device=torch_device):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+    def args(**kw):
+        a = dict(dh=e(3, 5, 7), x=e(3, 5, 8), wg=e(7, 8), wu=e(7, 8),
+                 saved=e(2, 15, 8, dtype=torch.float32), seed_at=None, rows=None)
+        a.update(kw)
+        return a
+
+    i64 = dict(dtype=torch.int64)
+    return [(args(dh=e(2, 5, 7)), ValueError), (args(dh=e(15, 6)), ValueError),
+            (args(dh=e(3, 7, 5).transpose(1, 2)), ValueError),
+            (args(dh=e(3, 5, 7, dtype=torch.float16)), TypeError),
+            (args(dh=e(3, 5, 7, device="cpu")), RuntimeError),
+            (args(saved=e(2, 15, 7, dtype=torch.float32)), ValueError),
+            (args(saved=e(2, 14, 8, dtype=torch.float32)), ValueError),
+            (args(saved=e(2, 15, 8)), TypeError),
+            (args(saved=e(2, 15, 8, dtype=torch.float32, device="cpu")), RuntimeError),
+            (args(wu=e(6, 8)), ValueError), (args(wg=e(7, 9), wu=e(7, 9)), ValueError),
+            (args(wg=e(7, 8, dtype=torch.float32)), TypeError), (args(x=e(3, 4, 8)), ValueError),
+            (args(rows=e(14, **i64)), ValueError), (args(rows=e(15, dtype=torch.int32)), TypeError),
+            (args(rows=e(15, device="cpu", **i64)), RuntimeError),
+            (args(seed_at=e(2, **i64)), ValueError),
+            (args(seed_at=e(1, device="cpu", **i64)), RuntimeError)]
+
+
+def test_backward_operator_refuses():
+    """ppo_amd::gated_ffn_backward checks what it hands to the kernels."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from ppo_amd import torch_ops
+
+    f = torch_ops.gated_ffn_backward._init_fn
+    with FakeTensorMode():
+        for a, error in _backward_faults():
+            with pytest.raises(error, match="must|dtype|expected|no CPU fallback"):
+                f(a["dh"], a["x"], a["wg"], a["wu"], a["saved"], False, "silu", 0.1, 1,
+                  a["seed_at"], a["rows"])
+        with pytest.raises(ValueError, match="activation"):
+            f(a["dh"], a["x"], a["wg"], a["wu"], a["saved"], False, "swish", 0.1, 1, None, None)
+        with pytest.raises(ValueError, match="probability"):
+            f(a["dh"], a["x"], a["wg"], a["wu"], a["saved"], False, "silu", 1.5, 1, None, None)
+
+
 def test_module_arguments():
     with pytest.raises(ValueError):
         ppo_amd.GatedLinear(4, 4, activation="swish")

@@ -145,8 +145,7 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, rows: Optional[torch.Tensor] 
 # ---------------------------------------------------------------------------
 # Gated feed-forward block
 # ---------------------------------------------------------------------------
-def _check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, rows) -> int:
-    """Refuses what the kernels do not take; the activation's number."""
+def _check_gated_operands(x, w_gate, w_up, b_gate=None, b_up=None) -> None:
     _require(x, "x", tuple(DTYPES))
     device, dtype = x.device, (x.dtype,)
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -166,10 +165,33 @@ def _check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, row
             _require(b, name, dtype, device)
             if b.shape != (F,):
                 raise ValueError(f"{name} must be [{F}], got {tuple(b.shape)}")
+
+
+def _check_activation(activation) -> int:
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    _check_drop(dropout_p, seed, rows, x.numel() // D, device)
     return ACTIVATIONS[activation]
+
+
+def _check_gated(x, w_gate, w_up, b_gate, b_up, activation, dropout_p, seed, rows) -> int:
+    """Refuses what the kernels do not take; the activation's number."""
+    _check_gated_operands(x, w_gate, w_up, b_gate, b_up)
+    act = _check_activation(activation)
+    _check_drop(dropout_p, seed, rows, x.numel() // x.shape[-1], x.device)
+    return act
+
+
+def _check_gated_backward(dh, x, w_gate, w_up, saved, dropout_p, seed, rows) -> None:
+    """Refuses what the backward kernels do not take."""
+    _check_gated_operands(x, w_gate, w_up)
+    M, F = x.numel() // x.shape[-1], w_gate.shape[0]
+    _check_drop(dropout_p, seed, rows, M, x.device)
+    _require(dh, "dh", (x.dtype,), x.device)
+    if dh.shape != (*x.shape[:-1], F):
+        raise ValueError(f"dh must be {(*x.shape[:-1], F)}, got {tuple(dh.shape)}")
+    _require(saved, "saved", (torch.float32,), x.device)
+    if saved.shape != (2, M, (F + 3) // 4 * 4):
+        raise ValueError(f"saved must be {(2, M, (F + 3) // 4 * 4)}, got {tuple(saved.shape)}")
 
 
 def _gated_forward(x, wg, wu, bg, bu, act, p, seed, rows, save):

@@ -212,10 +212,11 @@ def gated_ffn_backward(dh: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, save
                        bias: bool, activation: str, dropout_p: float, seed: int,
                        seed_at: Optional[Tensor], rows: Optional[Tensor]
                        ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    act, s = layers._check_activation(activation), _seed(seed, seed_at)
+    layers._check_gated_backward(dh, x, w_gate, w_up, saved, dropout_p, s, rows)
     need = (True, True, True, bias, bias)
-    dx, dwg, dwu, dbg, dbu = layers._gated_backward(
-        dh, x, w_gate, w_up, saved, layers.ACTIVATIONS[activation], dropout_p,
-        _seed(seed, seed_at), rows, need)
+    dx, dwg, dwu, dbg, dbu = layers._gated_backward(dh, x, w_gate, w_up, saved, act, dropout_p, s,
+                                                    rows, need)
     return (dx, dwg, dwu, x.new_empty(0) if dbg is None else dbg,
             x.new_empty(0) if dbu is None else dbu)
 
