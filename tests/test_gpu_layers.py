@@ -781,6 +781,34 @@ def test_saved_tensor_hooks_and_checkpoints(dev):
         assert all(torch.equal(a, b) for a, b in zip(want, grads(wrap)))
 
 
+@pytest.mark.parametrize("which", ["rows", "seed", "rows_type"])
+@pytest.mark.parametrize("native", [True, False])
+def test_hooks_that_hand_back_other_tensors_are_refused(dev, monkeypatch, native, which):
+    """Row ids and seeds of another size or type stop before the kernels."""
+    if not native:
+        monkeypatch.setattr(ppo_amd.layers, "_native", _Declines)
+    rows, seed = torch.arange(30, device=dev), torch.tensor([3], device=dev)
+
+    def unpack(t):
+        if t.dtype != torch.int64:
+            return t
+        if which == "rows_type":
+            return t.int()
+        if which == "rows":
+            return t[:5].clone() if t.numel() == 30 else t
+        return t if t.numel() == 30 else torch.cat([t, t])
+
+    x, w = torch.randn(30, 8, device=dev), torch.randn(12, 8, device=dev)
+    for f in (lambda t: ppo_amd.dropout(t, 0.4, seed, rows=rows),
+              lambda t: ppo_amd.gated_ffn(t, w, w, dropout_p=0.4, seed=seed, rows=rows)):
+        t = x.clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, unpack):
+            y = f(t)
+        with pytest.raises((RuntimeError, ValueError, TypeError),
+                           match="changed|must|dtype|needs Long"):
+            y.sum().backward()
+
+
 def test_forward_mode_and_batched_gradients_are_refused(dev):
     """No silent zeros for what the operators do not offer."""
     import torch.autograd.forward_ad as fwad

@@ -233,6 +233,29 @@ def test_backward_operator_refuses():
             f(a["dh"], a["x"], a["wg"], a["wu"], a["saved"], False, "silu", 1.5, 1, None, None)
 
 
+def test_backward_nodes_refuse_what_hooks_hand_back():
+    """The Python autograd functions check their saved tensors before a launch."""
+    from types import SimpleNamespace
+
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def ctx(*saved):
+        return SimpleNamespace(p=0.1, act=2, seed=None if saved[-2] is not None else 1,
+                               saved_tensors=saved, needs_input_grad=(True,) * 5)
+
+    with FakeTensorMode(), torch.no_grad():
+        for a, error in _backward_faults():
+            with pytest.raises(error, match="must|dtype|expected|no CPU fallback"):
+                dh = a["dh"].contiguous()  # (the node makes it so)
+                if not a["dh"].is_contiguous():
+                    raise ValueError("must be contiguous")
+                layers._GatedFFN.backward(ctx(a["x"], a["wg"], a["wu"], a["saved"], a["seed_at"],
+                                              a["rows"]), dh)
+            if a["seed_at"] is not None or a["rows"] is not None:
+                with pytest.raises(error, match="must|dtype|expected|no CPU fallback"):
+                    layers._Dropout.backward(ctx(a["seed_at"], a["rows"]), a["dh"])
+
+
 def test_module_arguments():
     with pytest.raises(ValueError):
         ppo_amd.GatedLinear(4, 4, activation="swish")

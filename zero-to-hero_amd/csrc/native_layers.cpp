@@ -98,6 +98,21 @@ Tensor like_forward(const Tensor& t, at::ScalarType type, const at::Device& devi
   return t.contiguous();
 }
 
+// dropout's arguments as a node saved them, for M rows.
+Drop saved_drop(AutogradContext* ctx, const Tensor& seed_at, const Tensor& rows,
+                const at::Device& device, int64_t M) {
+  Drop d;
+  d.p = ctx->saved_data["p"].toDouble();
+  d.seed = (uint64_t)ctx->saved_data["seed"].toInt();
+  if (seed_at.defined()) d.seed_at = like_forward(seed_at, at::kLong, device);
+  if (rows.defined()) d.rows = like_forward(rows, at::kLong, device);
+  TORCH_CHECK(!seed_at.defined() || d.seed_at.numel() == 1,
+              "dropout's saved seed has changed its shape");
+  TORCH_CHECK(!rows.defined() || (d.rows.dim() == 1 && d.rows.numel() == M),
+              "dropout's saved rows have changed their shape");
+  return d;
+}
+
 // --- dropout ---------------------------------------------------------------------------
 
 int dropout_into(const Tensor& x, const Tensor& y, const Drop& d) {
@@ -122,13 +137,9 @@ struct DropoutNode : public torch::autograd::Function<DropoutNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list saved = ctx->get_saved_variables();
     if (!g[0].defined()) return {Tensor(), Tensor()};
-    Drop d;
-    d.p = ctx->saved_data["p"].toDouble();
-    d.seed = (uint64_t)ctx->saved_data["seed"].toInt();
-    d.seed_at = saved[0];
-    d.rows = saved[1];
     TORCH_CHECK(dtype_code(g[0].scalar_type()) >= 0, "dropout's gradient is ", g[0].scalar_type());
     const Tensor dy = like_forward(g[0], g[0].scalar_type(), g[0].device());
+    const Drop d = saved_drop(ctx, saved[0], saved[1], dy.device(), dy.numel() / dy.size(-1));
     // linear in x: its derivative is the same mask (create_graph comes again)
     return {apply(dy, &d), Tensor()};
   }
@@ -207,15 +218,13 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
     const Tensor dh = like_forward(g[0], type, dev), x = like_forward(saved[0], type, dev),
                  wg = like_forward(saved[1], type, dev), wu = like_forward(saved[2], type, dev),
                  gu = like_forward(saved[3], at::kFloat, dev);
-    Drop d;
-    d.p = ctx->saved_data["p"].toDouble();
-    d.seed = (uint64_t)ctx->saved_data["seed"].toInt();
-    if (saved[4].defined()) d.seed_at = like_forward(saved[4], at::kLong, dev);
-    if (saved[5].defined()) d.rows = like_forward(saved[5], at::kLong, dev);
-    const int64_t D = x.size(-1), F = wg.size(0), M = x.numel() / D;
-    TORCH_CHECK(wu.sizes() == wg.sizes() && wg.size(-1) == D && dh.numel() == M * F &&
-                    gu.numel() == 2 * M * ((F + 3) / 4 * 4),
+    TORCH_CHECK(x.dim() >= 1 && x.numel() > 0 && wg.dim() == 2 && wg.size(0) > 0 &&
+                    wg.size(1) == x.size(-1) && wu.sizes() == wg.sizes(),
                 "gated_ffn's saved tensors have changed their shapes");
+    const int64_t D = x.size(-1), F = wg.size(0), M = x.numel() / D;
+    TORCH_CHECK(dh.numel() == M * F && gu.numel() == 2 * M * ((F + 3) / 4 * 4),
+                "gated_ffn's saved tensors have changed their shapes");
+    const Drop d = saved_drop(ctx, saved[4], saved[5], dev, M);
     const c10::DeviceGuard guard(dev);
     if (ctx->needs_input_grad(0)) out[0] = at::empty_like(x);
     if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {

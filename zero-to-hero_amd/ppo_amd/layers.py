@@ -108,6 +108,10 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         seed, rows = ctx.saved_tensors
+        # (a saved-tensor hook hands back whatever it likes)
+        _check_drop(ctx.p, ctx.seed if seed is None else seed, rows,
+                    dy.numel() // dy.shape[-1] if dy.numel() else math.prod(dy.shape[:-1]),
+                    dy.device)
         # linear in x: its derivative is the same mask (create_graph comes again)
         return (_Dropout.apply(dy.contiguous(), ctx.p, ctx.seed if seed is None else seed, rows),
                 None, None, None)
@@ -252,8 +256,12 @@ class _GatedFFN(torch.autograd.Function):
             raise RuntimeError("gated_ffn can be differentiated once: its backward pass has no "
                                "create_graph")
         x, wg, wu, saved, seed, rows = ctx.saved_tensors
-        grads = _gated_backward(dh.contiguous(), x, wg, wu, saved, ctx.act, ctx.p,
-                                ctx.seed if seed is None else seed, rows, ctx.needs_input_grad)
+        seed = ctx.seed if seed is None else seed
+        dh = dh.contiguous()
+        # (a saved-tensor hook hands back whatever it likes)
+        _check_gated_backward(dh, x, wg, wu, saved, ctx.p, seed, rows)
+        grads = _gated_backward(dh, x, wg, wu, saved, ctx.act, ctx.p, seed, rows,
+                                ctx.needs_input_grad)
         return (*grads, None, None, None, None)
 
 
