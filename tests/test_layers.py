@@ -5,6 +5,8 @@ and the oracle they are tested against."""
 import ctypes
 import os
 import re
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -32,6 +34,35 @@ def test_exports_match_the_header():
         assert hasattr(lib, name)
     syms = os.popen(f"nm -D --defined-only {_lib.LAYERS_PATH}").read()
     assert set(re.findall(r"\bT (\S+)$", syms, flags=re.M)) == set(names)
+
+
+def test_loads_to_lds_wait_for_their_descriptor(tmp_path):
+    """Five wait states lie between a vector instruction that writes a scalar
+    register and a buffer load that reads it.  The loads to LDS are inline
+    assembly, which the compiler's own hazard handling does not look into, so each
+    block has to wait by itself, whatever stands before it."""
+    objdump = "/opt/rocm/llvm/bin/llvm-objdump"
+    if not os.path.exists(objdump):
+        pytest.skip("no llvm-objdump")
+    lib = shutil.copy(_lib.LAYERS_PATH, tmp_path)
+    subprocess.run([objdump, "--offloading", lib], cwd=tmp_path, check=True, capture_output=True)
+    loads = 0
+    for name in os.listdir(tmp_path):
+        if not name.endswith("gfx950") or os.path.getsize(tmp_path / name) == 0:
+            continue
+        text = subprocess.run([objdump, "-d", "--no-show-raw-insn", "--no-leading-addr",
+                               str(tmp_path / name)], check=True, capture_output=True, text=True)
+        code = [line.split("//")[0].split() for line in text.stdout.splitlines()]
+        for i, words in enumerate(code):
+            if not words or not words[0].startswith("buffer_load") or words[-1] != "lds":
+                continue
+            loads += 1
+            states, j = 0, i - 1
+            while code[j] and (code[j][0] == "s_nop" or code[j][:2] == ["s_mov_b32", "m0,"]):
+                states += int(code[j][1]) + 1 if code[j][0] == "s_nop" else 1
+                j -= 1
+            assert states >= 5, f"{name}: {' '.join(words)} after {states} wait states"
+    assert loads > 0
 
 
 def drop(p, seed=1):

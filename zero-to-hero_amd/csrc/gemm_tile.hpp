@@ -127,12 +127,17 @@ __device__ __forceinline__ v4i buffer_of(const char* p, uint32_t bytes) {
 
 // 64 lanes, 16 bytes each from buffer + offset, to LDS at lds + 16 * lane
 // (`lds` is the same in all lanes).  Nothing in registers is written; the
-// data has arrived after a barrier below that waits for it.
+// data has arrived after a barrier below that waits for it.  A load may read the
+// descriptor five wait states after the vector instruction that wrote it
+// (v_readfirstlane, or v_readlane of a spilled one) at the earliest, and the
+// compiler does not look into the block: the block waits them itself (8192 x 4096 ->
+// 8192 gated forward 899 -> 912 us, backward 1898 -> 1911, int8 242 -> 244).
 __device__ __forceinline__ void load_to_lds(uint32_t lds, v4i buffer, uint32_t offset) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer));
+      "s_nop 3\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer)
+      : "m0");
 }
 
 // Waits until at most kLeft of this wave's loads are under way, and for its
