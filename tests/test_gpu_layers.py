@@ -427,6 +427,36 @@ def test_gated_matches_oracle(dev, shape, dtype):
         check_grad(got, w, t, name)
 
 
+def at_values(dev, t, act, g):
+    """act and act' at the fp64 values g as the operator has them: x = 1 and
+    u = 1, so h = act(g), dwu = act(g) and dwg = act'(g)."""
+    x, one = torch.ones(1, 1, device=dev, dtype=t), torch.ones(len(g), 1, device=dev, dtype=t)
+    wg, wu = g.to(dev, t)[:, None].clone().requires_grad_(), one.clone().requires_grad_()
+    h = ppo_amd.gated_ffn(x, wg, wu, activation=act)
+    dwg, dwu = torch.autograd.grad(h, [wg, wu], torch.ones_like(h))
+    return h.detach()[0], dwu[:, 0], dwg[:, 0]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("act", ACTS)
+def test_gated_activations_far_from_zero(dev, act, dtype):
+    """Values up to the type's largest: act and act' are then g, 1 or 0 to
+    rounding.  Below the smallest normal numbers results may be 0: 1e-36, twice
+    16-bit rounding, and the activation's own few roundings otherwise."""
+    t = TYPES[dtype]
+    far = [20.0, 50.0, 86.0, 88.0, 90.0, 104.0, 1e3, 6e4]
+    if dtype != "fp16":
+        far += [1e6, 1e15, 1e19, 1e20, 1e30, 1e35, 1e37, 1e38, 3e38]
+    g = torch.tensor([s * v for v in far for s in (1.0, -1.0)]).to(t).double()
+    a, da = ref.activation(g, act)
+    tiny = 1e-36 + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    for got, want in zip(at_values(dev, t, act, g), (a, a, da)):
+        assert_within(got, want, want.abs() * (2 * u_of(t) + 8 * U32) + tiny, act)
+    # and past the largest
+    inf = torch.tensor([float("inf")], dtype=torch.float64)
+    assert at_values(dev, t, act, inf)[0][0] == (1.0 if act == "tanh" else float("inf"))
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M,D,F", [(8, 16, 12), (90, 48, 40)])
 def test_gated_gradients_against_differences(dev, act, M, D, F):

@@ -105,22 +105,23 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count, boo
 // tanhf and erff took 14 of the 64 us of 4096 x 1024 -> 2048).
 // ---------------------------------------------------------------------------
 
-// e^x as 2^(x log2 e).  The product's rounding error, up to |x| 2^-24 in the
-// result, is carried along for fp32 (kFine) and below a 16-bit type's own
-// rounding by far otherwise.  Within 127 of zero: e^+-127 is as good as
-// infinity or nothing for the functions below.
+// e^x as 2^(x log2 e), 0 below the smallest normal number.  The product's
+// rounding error, up to |x| 2^-24 in the result, is carried along for fp32
+// (kFine; within the bounds there: e^-150 is 0, as gelu's density needs, which is
+// multiplied by g, and 1 / (1 + e^88) comes out as 0) and below a 16-bit type's own
+// rounding by far otherwise.
 template <bool kFine>
 __device__ __forceinline__ float exponential(float x) {
-  x = fminf(fmaxf(x, -87.0f), 88.0f);
+  if (!kFine) return __builtin_amdgcn_exp2f(x * 1.44269504f);
+  x = fminf(fmaxf(x, -150.0f), 88.0f);
   const float t = x * 1.44269504f;
   const float e = __builtin_amdgcn_exp2f(t);
-  if (!kFine) return e;
   // x log2 e - t, with log2 e = 1.44269504 + 1.9259630e-8
   const float rest = fmaf(x, 1.44269504f, -t) + x * 1.9259630e-8f;
   return fmaf(e, rest * 0.69314718f, e);
 }
 
-// Reciprocal within one unit in the last place.
+// Reciprocal within one unit in the last place; 0 where it is subnormal.
 __device__ __forceinline__ float reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // The normal CDF and its density: with z = |g| / sqrt(2), erfc z =
