@@ -457,6 +457,28 @@ def test_gated_activations_far_from_zero(dev, act, dtype):
     assert at_values(dev, t, act, inf)[0][0] == (1.0 if act == "tanh" else float("inf"))
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gelu_keeps_its_tail(dev, dtype):
+    """gelu and its derivative relative to themselves, also where the CDF is
+    1e-30: t = 1 / (1 + p z) is off by up to 4 u32, which counts up to three
+    times (d ln erfc / d ln t), the polynomial, the exponential and the products
+    by up to 8 together, so 20 u32 of the terms.  16-bit results add their
+    rounding, and their exponential the roundings of g^2 / 2 and of its product with
+    log2 e: g^2 u32."""
+    t = TYPES[dtype]
+    g = torch.cat([-torch.linspace(0.01, 12, 1500), torch.linspace(0.01, 6, 300),
+                   -torch.tensor([2.0, 3, 4, 5, 6])]).to(t).double()
+    a, da = ref.activation(g, "gelu")
+    cdf = 0.5 * torch.erfc(-g * math.sqrt(0.5))
+    terms = cdf + g.abs() * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    rel = 20 * U32 + (0.0 if dtype == "fp32" else g * g * U32)
+    own = 0.0 if dtype == "fp32" else 1.01 * u_of(t)
+    tiny = 1e-37 + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    h, dwu, dwg = at_values(dev, t, "gelu", g)
+    for got, want, scale in ((h, a, a.abs()), (dwu, a, a.abs()), (dwg, da, terms)):
+        assert_within(got, want, rel * scale + own * want.abs() + tiny, "gelu")
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M,D,F", [(8, 16, 12), (90, 48, 40)])
 def test_gated_gradients_against_differences(dev, act, M, D, F):
