@@ -701,6 +701,25 @@ def test_gated_refusals(dev):
         h.sum().backward()
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_gated_library_errors(dev, monkeypatch, native):
+    """Sizes past the limits raise PPOLibraryError, in training as in acting and
+    in the backward pass as in the forward."""
+    if not native:
+        monkeypatch.setattr(ppo_amd.layers, "_native", _Declines)
+    x, w = torch.ones(1, 1 << 20, device=dev), torch.ones(2, 1 << 20, device=dev)
+    for leaf in (x, x.clone().requires_grad_()):  # rows of 4 MiB
+        with pytest.raises(_lib.PPOLibraryError) as e:
+            ppo_amd.gated_ffn(leaf, w, w)
+        assert e.value.code == 3
+    x = torch.ones(1, 1, device=dev, requires_grad=True)
+    w = torch.ones(1 << 19, 1, device=dev)  # rows of 2 F elements: 4 MiB
+    h = ppo_amd.gated_ffn(x, w, w)
+    with pytest.raises(_lib.PPOLibraryError) as e:
+        h.sum().backward()
+    assert e.value.code == 3
+
+
 # --- offsets past 32 bits ----------------------------------------------------------------
 
 def test_offsets_past_32_bits(dev):

@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Device.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Generator.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/graph_task.h>
@@ -126,6 +127,20 @@ inline void check(const char* name, int code, const at::Device& device, void* st
                                              reinterpret_cast<uintptr_t>(stream));
 }
 
+// The same inside an autograd node, where the GIL may be held by nobody.
+inline void check_in_node(const char* name, int code, const at::Device& device, void* stream) {
+  if (code == PPO_OK) return;
+  py::gil_scoped_acquire gil;
+  try {
+    check(name, code, device, stream);
+  } catch (py::error_already_set& e) {
+    e.restore();
+    python_error error;
+    error.persist();
+    throw std::move(error);
+  }
+}
+
 inline PyObject* wrap(const Tensor& t) {
   PyObject* o = THPVariable_Wrap(t);
   if (!o) throw py::error_already_set();
@@ -153,6 +168,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PyErr_Clear();
     Py_RETURN_NONE;
   } catch (py::error_already_set& e) {
+    e.restore();
+    return nullptr;
+  } catch (python_error& e) {
     e.restore();
     return nullptr;
   } catch (const std::exception&) {

@@ -129,8 +129,8 @@ struct DropoutNode : public torch::autograd::Function<DropoutNode> {
     ctx->saved_data["p"] = d->p;
     ctx->saved_data["seed"] = (int64_t)d->seed;
     const Tensor y = at::empty_like(x);
-    const int code = dropout_into(x, y, *d);
-    TORCH_CHECK(code == PPO_OK, "ppo_layer_dropout failed with code ", code);
+    check_in_node("ppo_layer_dropout", dropout_into(x, y, *d), x.device(),
+                  current_stream(x.device()));
     return y;
   }
 
@@ -194,8 +194,8 @@ int gated_forward(const Gated& l, Tensor& h, Tensor* saved) {
 struct GatedNode : public torch::autograd::Function<GatedNode> {
   static Tensor forward(AutogradContext* ctx, at::TensorList, const Gated* l) {
     Tensor h, saved;
-    const int code = gated_forward(*l, h, &saved);
-    TORCH_CHECK(code == PPO_OK, "ppo_layer_gated_forward failed with code ", code);
+    check_in_node("ppo_layer_gated_forward", gated_forward(*l, h, &saved), l->device(),
+                  current_stream(l->device()));
     ctx->save_for_backward({l->x, l->wg, l->wu, saved, l->drop.seed_at, l->drop.rows});
     ctx->saved_data["act"] = (int64_t)l->act;
     ctx->saved_data["p"] = l->drop.p;
@@ -244,7 +244,7 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
         gu.const_data_ptr<float>(), dtype, M, D, F, (int)ctx->saved_data["act"].toInt(), &c,
         ptr(out[0]), ptr(out[1]), ptr(out[2]), bias ? ptr(out[3]) : nullptr,
         bias ? ptr(out[4]) : nullptr, ptr(ws), nbytes, current_stream(dev));
-    TORCH_CHECK(code == PPO_OK, "ppo_layer_gated_backward failed with code ", code);
+    check_in_node("ppo_layer_gated_backward", code, dev, current_stream(dev));
     for (int k = 0; k < n; ++k)
       if (!ctx->needs_input_grad(k)) out[k] = Tensor();
     return out;
