@@ -720,6 +720,56 @@ def test_gated_library_errors(dev, monkeypatch, native):
     assert e.value.code == 3
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,D,F", [(5, 24, 40), (70, 64, 128), (300, 96, 520), (20, 33, 41)])
+def test_operands_at_any_address(dev, dtype, M, D, F):
+    """The C entries with every matrix one element off alignment: the bits of the
+    aligned call, results and gradients among them, and nothing around them."""
+    t, code = TYPES[dtype], {"fp32": 0, "bf16": 1, "fp16": 2}[dtype]
+    lib = _lib.load_layers()
+    x, wg, wu, bg, bu, dh = gated_case(dtype, M, D, F, True)
+    xq, xs = ref.quantize_rows(x.float().numpy())
+    wq, ws = ref.quantize_rows(wg.float().numpy())
+    eight = [torch.from_numpy(a) for a in (xq, xs, wq, ws)]
+    saved = torch.empty(2, M, (F + 3) // 4 * 4, device=dev)
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    drop = ctypes.byref(_lib.Dropout(0.2, 5, None, None))
+
+    def results(offset):
+        def out(*shape):
+            buf = torch.full((math.prod(shape) + 2 * offset,), 7.0, dtype=t, device=dev)
+            outs.append((buf, offset))
+            return buf.data_ptr() + offset * t.itemsize
+
+        outs = []
+        ins = [at_offset(v, dev, offset) for v in (x, wg, wu, bg, bu, dh)]
+        q = [at_offset(v, dev, offset if v.dtype == torch.int8 else 0) for v in eight]
+        p = [v.data_ptr() for v in ins]
+        n = lib.ppo_layer_gated_workspace_bytes(code, M, D, F)
+        work = torch.empty(n, dtype=torch.uint8, device=dev)
+        assert lib.ppo_layer_gated_forward(*p[:5], code, M, D, F, 2, drop, out(M, F),
+                                           saved.data_ptr(), work.data_ptr(), n, stream) == 0
+        n = lib.ppo_layer_gated_backward_workspace_bytes(code, M, D, F)
+        back = torch.empty(n, dtype=torch.uint8, device=dev)
+        grads = [out(M, D), out(F, D), out(F, D), out(F), out(F)]
+        assert lib.ppo_layer_gated_backward(p[5], *p[:3], saved.data_ptr(), code, M, D, F, 2, drop,
+                                            *grads, back.data_ptr(), n, stream) == 0
+        n = lib.ppo_layer_int8_linear_workspace_bytes(M, F, D, 1)
+        more = [torch.empty(n, dtype=torch.uint8, device=dev) for _ in range(2)]
+        assert lib.ppo_layer_int8_linear(p[0], None, None, q[2].data_ptr(), q[3].data_ptr(), p[3],
+                                         code, M, F, D, out(M, F), more[0].data_ptr(), n,
+                                         stream) == 0
+        n = lib.ppo_layer_int8_linear_workspace_bytes(M, F, D, 0)
+        assert lib.ppo_layer_int8_linear(None, q[0].data_ptr(), q[1].data_ptr(), q[2].data_ptr(),
+                                         q[3].data_ptr(), p[3], code, M, F, D, out(M, F),
+                                         more[1].data_ptr(), n, stream) == 0
+        torch.cuda.synchronize()
+        assert all(bool((b[:o] == 7).all() and (b[b.numel() - o:] == 7).all()) for b, o in outs)
+        return [b[o:b.numel() - o] for b, o in outs]
+
+    assert all(torch.equal(a, b) for a, b in zip(results(0), results(1)))
+
+
 # --- offsets past 32 bits ----------------------------------------------------------------
 
 def test_offsets_past_32_bits(dev):

@@ -75,7 +75,7 @@ struct GatedEpi {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = a[4 * b + i] * u[4 * b + i];
       if (drop.mode) drop4(drop, dropout_seed(drop), (uint64_t)id[b], (uint32_t)n >> 2, v);
-      if (live[b]) store4<true>(h + (int64_t)m[b] * F + n, v, F - n, (F & 3) == 0);
+      if (live[b]) store4<true>(h + (int64_t)m[b] * F + n, v, F - n, rows_of_fours(h, F));
     }
   }
 };
@@ -104,8 +104,9 @@ struct StoreEpi {
       const bool other = m[b] >= second;
       const int at = other ? m[b] - second : m[b];
       const float v[4] = {c[b][0], c[b][1], c[b][2], c[b][3]};
+      T* out = other ? out1 : out0;
       if (live[b] && at < rows)
-        store4<true>((other ? out1 : out0) + (int64_t)at * N + n, v, N - n, (N & 3) == 0);
+        store4<true>(out + (int64_t)at * N + n, v, N - n, rows_of_fours(out, N));
     }
   }
 };
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const T* dh, const floa
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;  // four columns, rows ty + 4 i
   const int n = c0 + tx * 4;
   const uint64_t seed = drop.mode ? dropout_seed(drop) : 0;
-  const bool vec = (F & 3) == 0 && ((uintptr_t)dh & (4 * sizeof(T) - 1)) == 0;
+  const bool vec = rows_of_fours(dh, F);
   constexpr int kRows = kTileM / 4;
   struct __attribute__((aligned(4 * sizeof(T)))) Four { T x[4]; };
   v4f g[kRows], u[kRows];

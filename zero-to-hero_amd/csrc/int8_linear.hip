@@ -47,7 +47,7 @@ struct Int8Epi {
         v[i] = (float)c[b][i] * s[b] * cols.scale[i];
         if (bias) v[i] += cols.bias[i];  // (without one, a zero keeps its sign)
       }
-      if (live[b]) store4<true>(out + (int64_t)m[b] * N + n, v, N - n, (N & 3) == 0);
+      if (live[b]) store4<true>(out + (int64_t)m[b] * N + n, v, N - n, rows_of_fours(out, N));
     }
   }
 };

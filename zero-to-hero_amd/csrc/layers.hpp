@@ -72,8 +72,14 @@ __device__ __forceinline__ v4i load16_shifted(const char* p) {
   return r;
 }
 
-// Four consecutive elements, stored together where p allows it (`vec`: the
-// row's start and pitch are multiples of four elements), else those in range.
+// Whether rows of `width` elements from p on start at multiples of four elements.
+template <class T>
+__host__ __device__ __forceinline__ bool rows_of_fours(const T* p, int width) {
+  return (width & 3) == 0 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
+}
+
+// Four consecutive elements, stored together where p allows it (`vec`:
+// rows_of_fours), else those in range.
 // kStream: results that this kernel and the next do not read again leave the
 // L2 to the operands (int8 8192 x 8192 x 4096 267 -> 252 us, gated
 // 8192 x 4096 -> 8192 with g and u saved 971 -> 904).
