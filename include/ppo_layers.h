@@ -37,6 +37,17 @@ extern "C" {
 #define PPO_DTYPE_BF16 1
 #define PPO_DTYPE_F16 2
 
+/*
+ * Workspaces hold copies of operands whose rows do not start at multiples of 16
+ * bytes.  Added to `dtype` (to `quantize` of the 8-bit product's
+ * *_workspace_bytes), this says that x, xq and the weights themselves do, so
+ * that no room for copies is needed unless the rows' length asks for it (x of
+ * ppo_layer_int8_linear may start anywhere).  A call that adds it to operands
+ * that start elsewhere gets PPO_ERR_INVALID_ARG.  Size function and call go
+ * together: without it the workspace is that of operands at any address.
+ */
+#define PPO_LAYER_ALIGNED 0x100
+
 /* The networks' activations (PPO_ACT_RELU, PPO_ACT_TANH) and two more. */
 #define PPO_LAYER_RELU 0
 #define PPO_LAYER_TANH 1

@@ -770,6 +770,41 @@ def test_operands_at_any_address(dev, dtype, M, D, F):
     assert all(torch.equal(a, b) for a, b in zip(results(0), results(1)))
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_scratch_of_aligned_operands(dev, monkeypatch, native):
+    """Calls whose operands need no copies take no memory for them."""
+    if not native:
+        monkeypatch.setattr(ppo_amd.layers, "_native", _Declines)
+    M, D, F = 1024, 2048, 2048  # 16-bit x: 4 MiB, the weights 8 MiB each
+    x, w = (torch.randn(n, D, device=dev).bfloat16() for n in (M, F))
+    leaves = [t.clone().requires_grad_() for t in (x, w, w)]
+    q, s = ppo_amd.quantize_rows(w)
+    xq, xs = ppo_amd.quantize_rows(x)
+    h = ppo_amd.gated_ffn(*leaves)
+    dh = torch.randn_like(h)
+
+    def extra(f, results):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats(dev)
+        before = torch.cuda.memory_allocated(dev)
+        out = f()  # noqa: F841
+        return torch.cuda.max_memory_allocated(dev) - before - results
+
+    with torch.no_grad():
+        assert extra(lambda: ppo_amd.gated_ffn(x, w, w), 2 * M * F) < 1 << 20
+        assert extra(lambda: ppo_amd.int8_linear(xq, q, s, None, xs, torch.bfloat16),
+                     2 * M * F) < 1 << 20
+        assert extra(lambda: ppo_amd.int8_linear(x, q, s), 2 * M * F) < M * D + (1 << 20)
+    # dg and du, no biases: their rows' sums are reserved all the same; and what the
+    # products' splits join
+    lib, on = _lib.load_layers(), _lib.PPO_LAYER_ALIGNED
+    need = lib.ppo_layer_gated_backward_workspace_bytes(1 | on, M, D, F)
+    copies = 2 * (M * D + 2 * F * D)
+    assert lib.ppo_layer_gated_backward_workspace_bytes(1, M, D, F) - need == copies
+    assert extra(lambda: torch.autograd.grad(h, leaves, dh),
+                 2 * (M * D + 2 * F * D)) < need + (1 << 20)
+
+
 # --- offsets past 32 bits ----------------------------------------------------------------
 
 def test_offsets_past_32_bits(dev):

@@ -167,6 +167,47 @@ def test_saved_alignment():
                                         P, 1 << 40, None) == 1
 
 
+def test_workspaces_of_aligned_operands():
+    """No room for copies of operands that need none."""
+    lib, on = _lib.load_layers(), _lib.PPO_LAYER_ALIGNED
+    fwd, bwd = lib.ppo_layer_gated_workspace_bytes, lib.ppo_layer_gated_backward_workspace_bytes
+    eight = lib.ppo_layer_int8_linear_workspace_bytes
+    M, D, F = 8192, 4096, 8192
+    copies = 2 * (M * D + 2 * F * D)
+    assert fwd(1, M, D, F) >= copies and fwd(1 | on, M, D, F) == 0
+    dgu = 2 * 2 * M * F
+    assert bwd(1, M, D, F) >= dgu + copies
+    # (and the biases' sums and joins: 4 bytes of 2 F for every 16 rows)
+    assert dgu <= bwd(1 | on, M, D, F) <= dgu + M // 16 * 2 * F * 4
+    assert eight(M, F, D, 0) >= M * D + F * D and eight(M, F, D, on) == 0
+    assert eight(M, F, D, 1) >= M * D + F * D
+    assert M * D <= eight(M, F, D, 1 | on) <= M * D + 4 * M + 512
+    # rows that are no multiple of 16 bytes need their copies at any address
+    for d in (4095, 4097):
+        assert fwd(1 | on, M, d, F) == fwd(1, M, d, F) > 0
+        assert bwd(1 | on, M, d, F) == bwd(1, M, d, F)
+        assert eight(M, F, d, on) == eight(M, F, d, 0) > 0
+    # a promise that does not hold, and less than was asked for
+    odd = ctypes.c_void_p(4104)
+
+    def gated(x=P, wg=P, wu=P, dtype=on, M=200, D=32, F=64, work=P, nbytes=1 << 40):
+        return (lib.ppo_layer_gated_forward(x, wg, wu, None, None, dtype, M, D + 1, F, 0, None, P,
+                                            None, work, nbytes, None),
+                lib.ppo_layer_gated_backward(P, x, wg, wu, P, dtype, M, D, F, 0, None, P, P, P,
+                                             None, None, work, nbytes, None))
+
+    for kw in (dict(x=odd), dict(wg=odd), dict(wu=odd), dict(dtype=3 | on), dict(dtype=-1)):
+        assert gated(**kw) == (1, 1)
+    assert gated(nbytes=min(fwd(on, 200, 33, 64), bwd(on, 200, 32, 64)) - 1) == (2, 2)
+    f = lib.ppo_layer_int8_linear
+    assert f(None, odd, P, P, P, None, on, 200, 64, 64, P, P, 1 << 40, None) == 1
+    assert f(P, None, None, odd, P, None, on, 200, 64, 64, P, P, 1 << 40, None) == 1
+    need = eight(200, 64, 64, 1 | on)
+    assert f(P, None, None, P, P, None, on, 200, 64, 64, P, P, need - 1, None) == 2
+    # at any address as before
+    assert f(P, None, None, P, P, None, 0, 200, 64, 64, P, P, eight(200, 64, 64, 1) - 1, None) == 2
+
+
 def test_cpu_tensors_and_types_are_refused():
     x, w = torch.zeros(4, 8), torch.zeros(6, 8)
     for call in (lambda: ppo_amd.dropout(x, 0.1, 1), lambda: ppo_amd.gated_ffn(x, w, w),

@@ -268,6 +268,8 @@ struct Scratch {
 
 // Scratch of the forward pass: operands whose rows do not start at multiples
 // of 16 bytes get a padded copy, except for the rows kernel, which takes any.
+// Room for it is asked for where the length of a row or the operands' addresses
+// need it (8192 x 4096 -> 8192 in bf16: 201 MB, and none for aligned operands).
 struct ForwardPlan {
   int64_t pitch;  // bytes of a padded row
   bool pad;
@@ -385,8 +387,9 @@ Dropout drop_of(const ppo_dropout* d) {
 using namespace ppo;
 
 extern "C" size_t ppo_layer_gated_workspace_bytes(int dtype, int64_t M, int64_t D, int64_t F) {
+  const bool aligned = take_aligned(dtype);
   if (!dtype_ok(dtype) || !sizes_ok(M, D, F) || !forward_fits(dtype, M, D, F) || M == 0) return 0;
-  return plan_forward(dtype, M, D, F, false, nullptr).bytes;
+  return plan_forward(dtype, M, D, F, aligned, nullptr).bytes;
 }
 
 extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void* wu,
@@ -395,6 +398,7 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
                                        const ppo_dropout* drop, void* h, float* saved,
                                        void* workspace, size_t workspace_bytes,
                                        void* stream_ptr) {
+  const bool promised = take_aligned(dtype);
   if (!dtype_ok(dtype) || !sizes_ok(M, D, F) || !drop_ok(drop) || activation < 0 ||
       activation > PPO_LAYER_GELU || !bg != !bu)
     return PPO_ERR_INVALID_ARG;
@@ -402,8 +406,9 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
   if (!x || !wg || !wu || !h || !aligned16(saved)) return PPO_ERR_INVALID_ARG;
   if (!forward_fits(dtype, M, D, F)) return PPO_ERR_TOO_LARGE;
   const bool aligned = aligned16(x) && aligned16(wg) && aligned16(wu);
+  if (promised && !aligned) return PPO_ERR_INVALID_ARG;
   const ForwardPlan f = plan_forward(dtype, M, D, F, aligned, (char*)workspace);
-  const size_t need = ppo_layer_gated_workspace_bytes(dtype, M, D, F);
+  const size_t need = plan_forward(dtype, M, D, F, promised, nullptr).bytes;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return PPO_ERR_WORKSPACE;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
@@ -434,8 +439,9 @@ extern "C" int ppo_layer_gated_forward(const void* x, const void* wg, const void
 
 extern "C" size_t ppo_layer_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t D,
                                                            int64_t F) {
+  const bool aligned = take_aligned(dtype);
   if (!dtype_ok(dtype) || !sizes_ok(M, D, F) || !backward_fits(dtype, M, D, F)) return 0;
-  return plan_backward(dtype, M, D, F, false, nullptr).bytes;
+  return plan_backward(dtype, M, D, F, aligned, nullptr).bytes;
 }
 
 extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const void* wg,
@@ -444,6 +450,7 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
                                         const ppo_dropout* drop, void* dx, void* dwg, void* dwu,
                                         void* dbg, void* dbu, void* workspace,
                                         size_t workspace_bytes, void* stream_ptr) {
+  const bool promised = take_aligned(dtype);
   if (!dtype_ok(dtype) || !sizes_ok(M, D, F) || !drop_ok(drop) || activation < 0 ||
       activation > PPO_LAYER_GELU || !dwg != !dwu || !dbg != !dbu)
     return PPO_ERR_INVALID_ARG;
@@ -452,8 +459,9 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
     return PPO_ERR_INVALID_ARG;
   if (!backward_fits(dtype, M, D, F)) return PPO_ERR_TOO_LARGE;
   const bool aligned = aligned16(x) && aligned16(wg) && aligned16(wu);
+  if (promised && !aligned) return PPO_ERR_INVALID_ARG;
   const BackwardPlan b = plan_backward(dtype, M, D, F, aligned, (char*)workspace);
-  if (!workspace || workspace_bytes < ppo_layer_gated_backward_workspace_bytes(dtype, M, D, F) ||
+  if (!workspace || workspace_bytes < plan_backward(dtype, M, D, F, promised, nullptr).bytes ||
       !aligned16(workspace))
     return PPO_ERR_WORKSPACE;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);

@@ -386,21 +386,24 @@ extern "C" int ppo_layer_quantize_rows(const void* x, int dtype, int64_t rows, i
 
 extern "C" size_t ppo_layer_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K,
                                                         int quantize) {
+  const bool aligned = take_aligned(quantize);
   if (M <= 0 || N <= 0 || K <= 0 || K > kMaxInt8K || !gemm_fits(M, N, round_up(K, 16))) return 0;
-  return plan_int8(M, N, K, quantize != 0, false, false, nullptr).bytes;
+  return plan_int8(M, N, K, quantize != 0, aligned, aligned, nullptr).bytes;
 }
 
 extern "C" int ppo_layer_int8_linear(const void* x, const int8_t* xq, const float* xs,
                                      const int8_t* wq, const float* ws, const void* bias,
                                      int dtype, int64_t M, int64_t N, int64_t K, void* out,
                                      void* workspace, size_t workspace_bytes, void* stream_ptr) {
+  const bool promised = take_aligned(dtype);
   if (!dtype_ok(dtype) || M < 0 || N <= 0 || K <= 0) return PPO_ERR_INVALID_ARG;
   if (M == 0) return PPO_OK;
   if (!wq || !ws || !out || (!x && (!xq || !xs))) return PPO_ERR_INVALID_ARG;
   if (K > kMaxInt8K || !gemm_fits(M, N, round_up(K, 16))) return PPO_ERR_TOO_LARGE;
-  const Int8Plan p =
-      plan_int8(M, N, K, x != nullptr, aligned16(xq), aligned16(wq), (char*)workspace);
-  const size_t need = ppo_layer_int8_linear_workspace_bytes(M, N, K, x != nullptr);
+  const bool ax = x || aligned16(xq), aw = aligned16(wq);
+  if (promised && !(ax && aw)) return PPO_ERR_INVALID_ARG;
+  const Int8Plan p = plan_int8(M, N, K, x != nullptr, ax, aw, (char*)workspace);
+  const size_t need = plan_int8(M, N, K, x != nullptr, promised, promised, nullptr).bytes;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return PPO_ERR_WORKSPACE;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);

@@ -31,6 +31,14 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 inline int dtype_size(int dtype) { return dtype == PPO_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype >= PPO_DTYPE_F32 && dtype <= PPO_DTYPE_F16; }
 
+// Takes PPO_LAYER_ALIGNED off an argument; whether it was there.
+template <class I>
+bool take_aligned(I& arg) {
+  const bool there = arg >= 0 && (arg & PPO_LAYER_ALIGNED);
+  if (there) arg &= ~PPO_LAYER_ALIGNED;
+  return there;
+}
+
 // Elements that 16 bytes hold.
 template <class T>
 constexpr int kPer16 = 16 / (int)sizeof(T);

@@ -46,6 +46,14 @@ Tensor scratch(size_t nbytes, const at::Device& device) {
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// PPO_LAYER_ALIGNED where the operands start at multiples of 16 bytes: no room
+// for aligned copies of them is needed then.
+int aligned_flag(std::initializer_list<const Tensor*> operands) {
+  for (const Tensor* t : operands)
+    if ((uintptr_t)t->const_data_ptr() & 15) return 0;
+  return PPO_LAYER_ALIGNED;
+}
+
 std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
   std::vector<int64_t> s = x.sizes().vec();
   s.back() = last;
@@ -178,7 +186,7 @@ struct Gated {
 
 int gated_forward(const Gated& l, Tensor& h, Tensor* saved) {
   const c10::DeviceGuard guard(l.device());
-  const int dtype = dtype_code(l.x.scalar_type());
+  const int dtype = dtype_code(l.x.scalar_type()) | aligned_flag({&l.x, &l.wg, &l.wu});
   h = at::empty(with_last(l.x, l.F), l.x.options());
   if (saved) *saved = at::empty({2, l.M, (l.F + 3) / 4 * 4}, l.x.options().dtype(at::kFloat));
   const size_t nbytes = ppo_layer_gated_workspace_bytes(dtype, l.M, l.D, l.F);
@@ -235,7 +243,7 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
       out[3] = at::empty({F}, x.options());
       out[4] = at::empty({F}, x.options());
     }
-    const int dtype = dtype_code(type);
+    const int dtype = dtype_code(type) | aligned_flag({&x, &wg, &wu});
     const size_t nbytes = ppo_layer_gated_backward_workspace_bytes(dtype, M, D, F);
     const Tensor ws = scratch(nbytes, dev);
     const ppo_dropout c = d.c();
@@ -341,12 +349,13 @@ PyObject* int8_linear(PyObject* const* a) {  // x, weight, weight_scale, bias, x
   const int code = unlocked([&] {
     const c10::DeviceGuard guard(dev);
     out = at::empty(with_last(x, N), x.options().dtype(type));
-    const size_t nbytes = ppo_layer_int8_linear_workspace_bytes(M, N, K, !eight);
+    const int flag = eight ? aligned_flag({&x, &w}) : aligned_flag({&w});
+    const size_t nbytes = ppo_layer_int8_linear_workspace_bytes(M, N, K, (eight ? 0 : 1) | flag);
     const Tensor work = scratch(nbytes, dev);
     return ppo_layer_int8_linear(eight ? nullptr : x.const_data_ptr(),
                                  eight ? x.const_data_ptr<int8_t>() : nullptr,
                                  static_cast<const float*>(ptr(xs)), w.const_data_ptr<int8_t>(),
-                                 in(ws), ptr(bias), dtype_code(type), M, N, K, out.data_ptr(),
+                                 in(ws), ptr(bias), dtype_code(type) | flag, M, N, K, out.data_ptr(),
                                  ptr(work), nbytes, stream);
   });
   check("ppo_layer_int8_linear", code, dev, stream);

@@ -159,6 +159,7 @@ SIGNATURES = {
 # ---------------------------------------------------------------------------
 # libppo_layers.so (include/ppo_layers.h)
 # ---------------------------------------------------------------------------
+PPO_LAYER_ALIGNED = 0x100
 LAYERS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libppo_layers.so")
 
 

@@ -54,6 +54,12 @@ def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _aligned(*operands: torch.Tensor) -> int:
+    """PPO_LAYER_ALIGNED where the operands start at multiples of 16 bytes: no
+    room for aligned copies of them is needed then."""
+    return 0 if any(t.data_ptr() % 16 for t in operands) else _lib.PPO_LAYER_ALIGNED
+
+
 def _call(name: str, *args) -> None:
     _lib.check(name, getattr(_lib.load_layers(), name)(*args))
 
@@ -207,6 +213,7 @@ def _gated_forward(x, wg, wu, bg, bu, act, p, seed, rows, save):
         saved = torch.empty((2, M, (F + 3) // 4 * 4), dtype=torch.float32, device=device)
     if M:
         drop = _drop(p, seed, rows)
+        dtype |= _aligned(x, wg, wu)
         with _on(device):
             nbytes = _lib.load_layers().ppo_layer_gated_workspace_bytes(dtype, M, D, F)
             ws = _workspace(nbytes, device)
@@ -230,6 +237,7 @@ def _gated_backward(dh, x, wg, wu, saved, act, p, seed, rows, need):
         dbg, dbu = new(F, **like), new(F, **like)
     if M:
         drop = _drop(p, seed, rows)
+        dtype |= _aligned(x, wg, wu)
         with _on(device):
             nbytes = _lib.load_layers().ppo_layer_gated_backward_workspace_bytes(dtype, M, D, F)
             ws = _workspace(nbytes, device)
@@ -380,14 +388,15 @@ def int8_linear(
             raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
     out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=device)
     if M:
+        flag = _aligned(x, weight) if eight else _aligned(weight)
         with _on(device):
-            nbytes = _lib.load_layers().ppo_layer_int8_linear_workspace_bytes(M, N, K,
-                                                                              int(not eight))
+            nbytes = _lib.load_layers().ppo_layer_int8_linear_workspace_bytes(
+                M, N, K, int(not eight) | flag)
             ws = _workspace(nbytes, device)
             _call("ppo_layer_int8_linear", None if eight else x.data_ptr(),
                   x.data_ptr() if eight else None, _ptr(x_scale), weight.data_ptr(),
-                  weight_scale.data_ptr(), _ptr(bias), DTYPES[out_dtype], M, N, K, out.data_ptr(),
-                  _ptr(ws), nbytes, _stream(device))
+                  weight_scale.data_ptr(), _ptr(bias), DTYPES[out_dtype] | flag, M, N, K,
+                  out.data_ptr(), _ptr(ws), nbytes, _stream(device))
     return out
 
 
