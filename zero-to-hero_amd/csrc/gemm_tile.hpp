@@ -130,8 +130,10 @@ __device__ __forceinline__ v4i buffer_of(const char* p, uint32_t bytes) {
 // data has arrived after a barrier below that waits for it.  A load may read the
 // descriptor five wait states after the vector instruction that wrote it
 // (v_readfirstlane, or v_readlane of a spilled one) at the earliest, and the
-// compiler does not look into the block: the block waits them itself (8192 x 4096 ->
-// 8192 gated forward 899 -> 912 us, backward 1898 -> 1911, int8 242 -> 244).
+// compiler does not look into the block: the block waits them itself (8192 x 4096
+// -> 8192 gated forward 899 -> 912 us, backward 1898 -> 1911, int8 242 -> 244).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved, and written all the same)
 __device__ __forceinline__ void load_to_lds(uint32_t lds, v4i buffer, uint32_t offset) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
@@ -139,6 +141,7 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, v4i buffer, uint32_t o
       "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer)
       : "m0");
 }
+#pragma clang diagnostic pop
 
 // Waits until at most kLeft of this wave's loads are under way, and for its
 // LDS reads, then for the whole workgroup.
