@@ -1169,3 +1169,37 @@ def test_int8_copy_of_the_reference_networks(dev):
             x = x.clamp(min=0)
     # (a last-bit difference may move a hidden value to the next 8-bit step: 1/127 of its row)
     torch.testing.assert_close(eight(obs).cpu(), x, rtol=0, atol=5e-3)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,bias", [(3, True), (100, False)])
+def test_int8_copy_of_a_gated_layer(dev, M, bias, act, dtype):
+    """One rounding to the layer's type: g and u are off by 4 u32 of their terms,
+    the activation as in check_forward."""
+    t = TYPES[dtype]
+    torch.manual_seed(4)
+    layer = ppo_amd.GatedLinear(40, 72, bias=bias, activation=act).to(dev, t)
+    eight = ppo_amd.int8_copy(layer)
+    x = torch.randn(M, 40, device=dev).to(t)
+    got = eight(x)
+    assert got.dtype == t and got.shape == (M, 72)
+    xq, xs = ref.quantize_rows(x.float().cpu().numpy())
+    sums = []
+    for w, b in ((layer.weight_gate, layer.bias_gate), (layer.weight_up, layer.bias_up)):
+        wq, ws = ref.quantize_rows(w.detach().float().cpu().numpy())
+        b = None if b is None else b.detach().double().cpu()
+        y = torch.from_numpy(ref.int8_linear(xq, xs, wq, ws, None if b is None else b.numpy()))
+        sums.append((y, 4 * U32 * (y.abs() if b is None else (y - b).abs() + b.abs() + y.abs())))
+    (g, eg), (u, eu) = sums
+    a, _ = ref.activation(g, act)
+    want = a * u
+    ea = 1.13 * eg + 8 * U32 * g.abs() + 8 * U32
+    bound = ea * (u.abs() + eu) + a.abs() * eu + 4 * U32 * want.abs()
+    tiny = 2.0 ** -25 if dtype == "fp16" else 0.0
+    assert_within(got, want, bound + u_of(t) * (want.abs() + bound) + tiny, act)
+    # the copy keeps its own parameters
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.add_(1.0)
+    assert torch.equal(eight(x), got)

@@ -474,8 +474,8 @@ class Int8Linear(nn.Module):
 
 
 class _Int8Gated(nn.Module):
-    """The 8-bit copy of a GatedLinear: x is quantised once for both products;
-    no dropout."""
+    """The 8-bit copy of a GatedLinear: x is quantised once for both products,
+    whose results stay in 32 bits up to the block's own; no dropout."""
 
     def __init__(self, layer: GatedLinear) -> None:
         super().__init__()
@@ -486,14 +486,15 @@ class _Int8Gated(nn.Module):
             q, scale = quantize_rows(w.detach())
             self.register_buffer(f"weight_{name}", q)
             self.register_buffer(f"scale_{name}", scale)
-            self.register_buffer(f"bias_{name}", None if b is None else b.detach().clone())
+            self.register_buffer(f"bias_{name}", None if b is None
+                                 else b.detach().to(torch.float32, copy=True))
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         q, s = quantize_rows(x)
-        g = int8_linear(q, self.weight_gate, self.scale_gate, self.bias_gate, s, x.dtype)
-        u = int8_linear(q, self.weight_up, self.scale_up, self.bias_up, s, x.dtype)
-        return self.act(g) * u
+        g = int8_linear(q, self.weight_gate, self.scale_gate, self.bias_gate, s, torch.float32)
+        u = int8_linear(q, self.weight_up, self.scale_up, self.bias_up, s, torch.float32)
+        return torch.mul(self.act(g), u, out=torch.empty_like(g, dtype=x.dtype))
 
 
 def int8_copy(module: nn.Module) -> nn.Module:
