@@ -342,6 +342,18 @@ def test_module_arguments():
     assert layers.ACTIVATIONS.keys() == {"relu", "tanh", "silu", "gelu"}
 
 
+def test_module_seeds_of_any_size():
+    """A module's seed is the low 64 bits of an int, as the functions' is."""
+    m = ppo_amd.GatedMLP(6, 16, 3, dropout=0.1, seed=2**62)
+    assert [int(l.seed) for l in m.hidden] == [-2**63, -2**63 + 1]
+    m.reseed(2**64 - 1)
+    assert [int(l.seed) for l in m.hidden] == [-2, -1]
+    layer = ppo_amd.GatedLinear(4, 4, seed=2**64 - 1)
+    assert int(layer.seed) == -1
+    layer.reseed(-2**63 - 1)
+    assert int(layer.seed) == 2**63 - 1
+
+
 # --- the oracle -------------------------------------------------------------------------
 
 def test_philox_known_answers():

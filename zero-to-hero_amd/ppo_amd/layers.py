@@ -403,11 +403,17 @@ def int8_linear(
 # ---------------------------------------------------------------------------
 # Modules
 # ---------------------------------------------------------------------------
+def _int64(seed: int) -> int:
+    """The low 64 bits of an int as an int64 tensor holds them."""
+    return (seed + 2**63) % 2**64 - 2**63
+
+
 class GatedLinear(nn.Module):
     """gated_ffn with its parameters: weights and biases initialised as two
     nn.Linear's (gate first).  Dropout acts in training mode; `seed` is a
-    buffer (int64 [1], reseed() fills it), so captured graphs read its current
-    value."""
+    buffer (int64 [1], reseed() fills it with the low 64 bits of an int), so
+    captured graphs read its current value.  Nothing else changes it: until the
+    next reseed() a row id (or position) meets the same mask in every call."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True,
                  activation: str = "silu", dropout: float = 0.0, seed: int = 0) -> None:
@@ -421,10 +427,10 @@ class GatedLinear(nn.Module):
         gate, up = (nn.Linear(in_features, out_features, bias) for _ in range(2))
         self.weight_gate, self.bias_gate = gate.weight, gate.bias
         self.weight_up, self.bias_up = up.weight, up.bias
-        self.register_buffer("seed", torch.tensor([seed], dtype=torch.int64))
+        self.register_buffer("seed", torch.tensor([_int64(seed)], dtype=torch.int64))
 
     def reseed(self, seed: int) -> None:
-        self.seed.fill_(seed)
+        self.seed.fill_(_int64(seed))
 
     def forward(self, x: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         p = self.dropout if self.training else 0.0
