@@ -927,9 +927,12 @@ int launch_gemm(GemmArgs a, const Epi& epi, const GemmPlan& p, char* partial, hi
     if (p.tile == 0) {
       const dim3 grid((unsigned)div_up(a.N, 16));
       // Eight waves where a CU has one workgroup and each wave four runs of K or
-      // more (with weights from HBM, 1 x 8192 -> 2048 gated 26.0 -> 20.6 us, fp32
-      // 52.6 -> 37.6; 1 x 1024 -> 4096 6.5 -> 7.0, 16 x 4096 -> 8192 31 -> 34), except
-      // for many rows of fp32, which the matrix cores bind (64 x 8192 -> 2048 107 -> 114).
+      // more (four and eight, with weights from HBM, gated: 1 x 4096 -> 2048 bf16 15.3
+      // and 12.9 us, fp32 29.3 and 23.1; 32 x 4096 -> 4096 bf16 25.5 and 22.4; for 16
+      // rows alike, 2048 -> 4096 11.6 and 12.0; below 32 runs 1 x 1024 -> 4096 6.5 and
+      // 7.0, with more workgroups 16 x 4096 -> 8192 31 and 34), except for many rows of
+      // fp32, which the matrix cores bind (64 x 2050 -> 1000 42 and 44, 6116 -> 3376 94
+      // and 107).
       const bool eight = div_up(a.N, 16) <= kCus && a.kbytes >= 32 * kRunBytes &&
                          !(sizeof(T) == 4 && a.M > 32);
       const bool odd = sizeof(T) < 4 && (((uintptr_t)a.x | (uintptr_t)a.w0 | (uintptr_t)a.w1 |
