@@ -86,8 +86,9 @@ int ppo_layer_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols
 
 /*
  * out[m,n] = (sum_k xq[m,k] * wq[n,k]) * xs[m] * ws[n] + bias[n], the sum
- * exact in int32 (K <= 2^17, else PPO_ERR_TOO_LARGE), scales and bias in
- * fp32.  With x != NULL the rows of x (dtype) are quantised first, as
+ * exact in int32 (K <= 2^17, else PPO_ERR_TOO_LARGE; at K = 2^17 a sum of
+ * nothing but (-128)^2, which ppo_layer_quantize_rows never makes, would wrap),
+ * scales and bias in fp32.  With x != NULL the rows of x (dtype) are quantised first, as
  * ppo_layer_quantize_rows does, and xq and xs are not read; out and bias are
  * of `dtype`.  bias may be NULL.
  */

@@ -166,8 +166,7 @@ def _seed(seed: int, seed_at: Optional[Tensor]):
 @torch.library.custom_op(f"{_NS}::dropout", mutates_args=(), device_types="cuda")
 def dropout(x: Tensor, p: float, seed: int, seed_at: Optional[Tensor],
             rows: Optional[Tensor]) -> Tensor:
-    y = layers.dropout(x, p, _seed(seed, seed_at), rows)
-    return y.clone() if y is x else y
+    return layers.dropout(x, p, _seed(seed, seed_at), rows)
 
 
 @dropout.register_fake
