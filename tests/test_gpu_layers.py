@@ -629,6 +629,22 @@ def test_gated_gradients_of_one_side(dev, dtype, M, D, F):
             check_grad(v, want[k], t, ("dx", "dwg", "dwu")[k])
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,D,F,offset", [(6, 436, 122, 1), (70, 33, 41, 0), (300, 40, 56, 0)])
+def test_gated_gradients_of_the_biases_alone(dev, dtype, M, D, F, offset):
+    """Frozen weights of any alignment: nothing is copied or multiplied."""
+    t = TYPES[dtype]
+    x, wg, wu, bg, bu, dh = gated_case(dtype, M, D, F, True, seed=6)
+    _, g, u = ref.gated_ffn(*d64(x, wg, wu, bg, bu), "silu")
+    want = ref.gated_ffn_grads(*d64(x, wg, wu), g, u, "silu", dh.double())[3:]
+    args = [at_offset(v, dev, offset) for v in (x, wg, wu, bg, bu)]
+    for pick in ([3, 4], [3], [4]):
+        some = [v if k not in pick else v.clone().requires_grad_() for k, v in enumerate(args)]
+        got = torch.autograd.grad(ppo_amd.gated_ffn(*some), [some[k] for k in pick], dh.to(dev))
+        for k, v in zip(pick, got):
+            check_grad(v, want[k - 3], t, ("dbg", "dbu")[k - 3])
+
+
 def test_gated_same_bits_again(dev):
     """Split sums are joined in a fixed order."""
     for M, D, F in ((96, 2048, 64), (300, 200, 72)):

@@ -489,6 +489,7 @@ extern "C" int ppo_layer_gated_backward(const void* dh, const void* x, const voi
       if ((st = last_launch_status())) return st;
       join.blocks = 0;
     }
+    if (!dx && !dwg) return (int)PPO_OK;  // (the biases' gradients alone: nothing to multiply)
     if (b.pad) {
       st = pad_operands(dwg ? x : nullptr, dx ? wg : nullptr, dx ? wu : nullptr, b.x, b.wg, b.wu, M,
                         F, D * size, b.pitch, stream);
