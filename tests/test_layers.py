@@ -352,6 +352,8 @@ def test_module_seeds_of_any_size():
     assert int(layer.seed) == -1
     layer.reseed(-2**63 - 1)
     assert int(layer.seed) == 2**63 - 1
+    layer.reseed(np.int64(7))
+    assert int(layer.seed) == 7 and int(ppo_amd.GatedLinear(4, 4, seed=np.int32(-2)).seed) == -2
 
 
 # --- the oracle -------------------------------------------------------------------------

@@ -405,7 +405,7 @@ def int8_linear(
 # ---------------------------------------------------------------------------
 def _int64(seed: int) -> int:
     """The low 64 bits of an int as an int64 tensor holds them."""
-    return (seed + 2**63) % 2**64 - 2**63
+    return (int(seed) + 2**63) % 2**64 - 2**63
 
 
 class GatedLinear(nn.Module):
