@@ -88,9 +88,9 @@ int ppo_layer_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols
  * out[m,n] = (sum_k xq[m,k] * wq[n,k]) * xs[m] * ws[n] + bias[n], the sum
  * exact in int32 (K <= 2^17, else PPO_ERR_TOO_LARGE; at K = 2^17 a sum of
  * nothing but (-128)^2, which ppo_layer_quantize_rows never makes, would wrap),
- * scales and bias in fp32.  With x != NULL the rows of x (dtype) are quantised first, as
- * ppo_layer_quantize_rows does, and xq and xs are not read; out and bias are
- * of `dtype`.  bias may be NULL.
+ * scales and bias in fp32.  With x != NULL the rows of x (dtype) are quantised
+ * first, as ppo_layer_quantize_rows does, and xq and xs are not read; out and
+ * bias are of `dtype`.  bias may be NULL.
  */
 size_t ppo_layer_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int quantize);
 int ppo_layer_int8_linear(const void* x, const int8_t* xq, const float* xs, const int8_t* wq,
@@ -121,9 +121,9 @@ int ppo_layer_gated_forward(const void* x, const void* wg, const void* wu, const
  * zeros).  dg and du are rounded to `dtype`, the matrix cores' operand
  * type, before the products: a 16-bit gradient is then off by about 1.4 times
  * what its own rounding makes (in short passes the products take what that
- * rounding left as well), and an fp16 dg or du past 65504 is infinite.  Sums are split and joined in a fixed order:
- * the same call gives the same bits (one that asks for other outputs may cut
- * the sums elsewhere).
+ * rounding left as well), and an fp16 dg or du past 65504 is infinite.  Sums
+ * are split and joined in a fixed order: the same call gives the same bits (one
+ * that asks for other outputs may cut the sums elsewhere).
  */
 size_t ppo_layer_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t D, int64_t F);
 int ppo_layer_gated_backward(const void* dh, const void* x, const void* wg, const void* wu,

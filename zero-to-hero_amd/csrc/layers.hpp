@@ -123,8 +123,7 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int count, boo
 // rounding error, up to |x| 2^-24 in the result, is carried along for fp32
 // (kFine; within the bounds there: e^-150 is 0, as gelu's density needs, which is
 // multiplied by g, and 1 / (1 + e^88) comes out as 0) and below a 16-bit type's own
-// rounding by far otherwise.
-// `below`: what x lost in a rounding of its own.
+// rounding by far otherwise.  `below` is what x lost in a rounding of its own.
 template <bool kFine>
 __device__ __forceinline__ float exponential(float x, float below = 0.0f) {
   if (!kFine) return __builtin_amdgcn_exp2f(x * 1.44269504f);
