@@ -19,6 +19,7 @@
 namespace ppo_native {
 Python P;
 extern PyMethodDef kLayerMethods[];  // native_layers.cpp
+extern PyMethodDef kTokenMethods[];  // native_tokens.cpp
 }  // namespace ppo_native
 
 namespace {
@@ -592,6 +593,7 @@ void init(py::object pool, py::object stats, py::object fail, const std::vector<
 PYBIND11_MODULE(_native, m) {
   m.def("init", &init);
   m.def("scale_grads", &scale_grads);
-  if (PyModule_AddFunctions(m.ptr(), kMethods) || PyModule_AddFunctions(m.ptr(), kLayerMethods))
+  if (PyModule_AddFunctions(m.ptr(), kMethods) || PyModule_AddFunctions(m.ptr(), kLayerMethods) ||
+      PyModule_AddFunctions(m.ptr(), kTokenMethods))
     throw py::error_already_set();
 }

@@ -1,0 +1,266 @@
+// The clipped policy loss with a KL term over wide rows of logits, forward and
+// gradient in one pass: a row stays in the registers of its group of lanes from
+// the read to the write.
+#include "tokens_rows.hpp"
+
+namespace ppo {
+namespace {
+
+struct Policy {
+  const float *old, *adv, *ref;
+  Weights weights;
+  float lo, hi, kl_coef, entropy_coef, grad_scale;
+  int per_sequence;
+  Saved* saved;
+  float* coef;   // [2][n]
+  double* sums;
+};
+
+// What a row adds to the sums.
+struct RowLoss {
+  float w, policy, kl, H, approx_kl, clipped;
+  __device__ __forceinline__ void add_to(double (&sums)[kSums]) const {
+    sums[0] += (double)w * policy;
+    sums[1] += (double)w * kl;
+    sums[2] += (double)w * H;
+    sums[3] += (double)w * approx_kl;
+    sums[4] += (double)w * clipped;
+  }
+};
+
+// e^d - d - 1: its series where the difference would cancel (to |d| = 1, where the
+// next term is below 2^-28 of the sum).
+__device__ __forceinline__ float kl_estimate(float d) {
+  if (!(fabsf(d) <= 1.0f)) return expf(d) - d - 1.0f;
+  float q = 1.0f / 479001600.0f;
+  constexpr float kInv[] = {1.0f / 39916800, 1.0f / 3628800, 1.0f / 362880, 1.0f / 40320,
+                            1.0f / 5040,     1.0f / 720,     1.0f / 120,    1.0f / 24,
+                            1.0f / 6,        0.5f};
+#pragma unroll
+  for (float k : kInv) q = fmaf(d, q, k);
+  return d * d * q;
+}
+
+// The row's loss, its gradient's terms G and E for an incoming gradient of 1.
+__device__ __forceinline__ RowLoss policy_row(const Policy& p, const Rows& rows, int64_t r, float w,
+                                              const RowTerms& t, float& G, float& E) {
+  const float old = p.old[r], adv = p.adv[p.per_sequence ? r / rows.T : r];
+  const float ratio = expf((float)(t.lp - (double)old));
+  const float clipped = ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio;
+  const float u = ratio * adv, v = clipped * adv;
+  RowLoss o = {w, -(u > v ? v : u), 0.0f, t.H, (float)((double)old - t.lp),
+               ratio < p.lo || ratio > p.hi ? 1.0f : 0.0f};
+  G = u > v ? 0.0f : -u;
+  if (p.ref) {
+    const float d = (float)((double)p.ref[r] - t.lp);
+    o.kl = kl_estimate(d);
+    if (p.kl_coef != 0.0f) G -= p.kl_coef * (o.kl + d);  // (e^d - 1)
+  }
+  G *= w;
+  E = -p.entropy_coef * w;
+  return o;
+}
+
+__device__ __forceinline__ void leave_row(const Policy& p, const Rows& rows, int64_t r,
+                                          const RowTerms& t, float G, float E) {
+  if (p.saved) p.saved[r] = saved_of(t, 0.0f);
+  if (p.coef) {
+    p.coef[r] = G;
+    p.coef[rows.n + r] = E;
+  }
+}
+// (a masked row's terms are never read again but for its zero coefficients)
+__device__ __forceinline__ void leave_masked(const Policy& p, const Rows& rows, int64_t r) {
+  if (p.coef) p.coef[r] = p.coef[rows.n + r] = 0.0f;
+}
+
+template <class T, int G, int V, bool kC>
+__global__ void __launch_bounds__(G < 256 ? 256 : G) policy_kernel(Rows rows, Policy p, T* dlogits) {
+  constexpr int kBlock = G < 256 ? 256 : G, kGroups = kBlock / G;
+  __shared__ Stat s_part[kBlock / kWave];
+  __shared__ Grad s_grad;
+  __shared__ double s_sums[kSums];
+  const int t = threadIdx.x % G;
+  double sums[kSums] = {};
+  const float inverse = inverse_count(p.weights);
+  if (G > kWave && threadIdx.x < kSums) s_sums[threadIdx.x] = 0.0;
+  for (int64_t r = (int64_t)blockIdx.x * kGroups + group_of<G>(); r < rows.n;
+       r += (int64_t)gridDim.x * kGroups) {
+    T* out = dlogits + r * rows.A;
+    if (!rows.live(r)) {
+      if (dlogits) write_zeros<T, G>(out, rows.A, t);
+      if (t == 0) leave_masked(p, rows, r);
+      continue;
+    }
+    const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
+    const int a = rows.action(r);
+    const float la = action_logit(row, a);
+    RowRegs<T, G, V> x(row, rows.A, t);
+    x.take_out(a, t);
+    Stat st = x.template stat<true>(rows.c);
+    Grad g;
+    auto finish = [&](double(&to)[kSums]) {
+      const RowTerms terms = row_terms<true>(st, la, rows.c);
+      float gl, ge;
+      const float w = row_weight(p.weights, inverse, r / rows.T);
+      const RowLoss loss = policy_row(p, rows, r, w, terms, gl, ge);
+      if (t == 0) {
+        loss.add_to(to);
+        leave_row(p, rows, r, terms, gl, ge);
+      }
+      g = row_grad(saved_of(terms, 0.0f), gl * p.grad_scale, ge * p.grad_scale, rows.inv_tau, a);
+    };
+    if (G > kWave) {
+      st = block_join<true>(st, rows.c, s_part);
+      if (threadIdx.x < kWave) {
+        finish(s_sums);
+        if (t == 0) s_grad = g;
+      }
+      lds_barrier();
+      g = s_grad;
+    } else {
+      st = lanes_join<G <= kWave ? G : kWave, true>(st, rows.c);
+      finish(sums);
+    }
+    if (dlogits) x.template write<kC>(g, rows.c, out, t);
+  }
+  if (G <= kWave) {
+    leave_sums(sums, p.sums);
+    return;
+  }
+  lds_barrier();
+  if (threadIdx.x < kSums)
+    p.sums[(int64_t)threadIdx.x * kMaxPartials + blockIdx.x] = s_sums[threadIdx.x];
+}
+
+// The same from rows' parts (join_kernel), where a row has several workgroups.
+struct PolicyJoin {
+  static constexpr bool kWholeWave = false;
+  Policy p;
+  double sums[kSums];
+  int64_t n;
+
+  __device__ __forceinline__ void masked(int64_t r) const {
+    if (p.coef) p.coef[r] = p.coef[n + r] = 0.0f;
+  }
+  template <bool kEntropy>
+  __device__ __forceinline__ void row(const Rows& rows, int64_t r, Stat x, float la, bool first) {
+    const RowTerms t = row_terms<kEntropy>(x, la, rows.c);
+    float G, E;
+    const float w = row_weight(p.weights, inverse_count(p.weights), r / rows.T);
+    const RowLoss loss = policy_row(p, rows, r, w, t, G, E);
+    if (!first) return;
+    loss.add_to(sums);
+    leave_row(p, rows, r, t, G, E);
+  }
+  __device__ __forceinline__ void end() { leave_sums(sums, p.sums); }
+};
+
+struct PolicyGrad {
+  const Saved* saved;
+  const float* coef;
+  float grad_scale;
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, float, int a) const {
+    return row_grad(saved[r], grad_scale * coef[r], grad_scale * coef[rows.n + r], rows.inv_tau, a);
+  }
+};
+
+// The scalars from the workgroups' sums, in their order.
+__global__ void __launch_bounds__(1024) policy_scalars_kernel(const double* sums, int n,
+                                                              double kl_coef, double entropy_coef,
+                                                              float* scalars) {
+  __shared__ double part[16][kSums];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) {
+    double v = 0.0;
+    for (int i = threadIdx.x; i < n; i += 1024) v += sums[(int64_t)k * kMaxPartials + i];
+    v = lanes_sum<kWave>(v);
+    if (lane == 0) part[wave][k] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  double all[kSums] = {};
+  for (int w = 0; w < 16; ++w)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) all[k] += part[w][k];
+  // (a term of coefficient 0 has no part in the loss, whatever it comes to)
+  double loss = all[0];
+  if (kl_coef != 0.0) loss += kl_coef * all[1];
+  if (entropy_coef != 0.0) loss -= entropy_coef * all[2];
+  scalars[PPO_TOKEN_SCALAR_LOSS] = (float)loss;
+  scalars[PPO_TOKEN_SCALAR_POLICY] = (float)all[0];
+  scalars[PPO_TOKEN_SCALAR_KL] = (float)all[1];
+  scalars[PPO_TOKEN_SCALAR_ENTROPY] = (float)all[2];
+  scalars[PPO_TOKEN_SCALAR_APPROX_KL] = (float)all[3];
+  scalars[PPO_TOKEN_SCALAR_CLIPFRAC] = (float)all[4];
+}
+
+template <class T>
+int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& partials,
+               hipStream_t stream) {
+  const int dtype = sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16;
+  const int64_t chunks = chunks_of(rows.A, dtype);
+  const bool grad_entropy = p.entropy_coef != 0.0f;
+  auto go = [&](auto lanes, auto held) {
+    constexpr int G = decltype(lanes)::value, V = decltype(held)::value;
+    constexpr int kBlock = G < 256 ? 256 : G;
+    partials = launch_blocks(div_up(rows.n, kBlock / G), kMaxPartials);
+    if (grad_entropy)
+      hipLaunchKernelGGL((policy_kernel<T, G, V, true>), dim3(partials), dim3(kBlock), 0, stream,
+                         rows, p, dlogits);
+    else
+      hipLaunchKernelGGL((policy_kernel<T, G, V, false>), dim3(partials), dim3(kBlock), 0, stream,
+                         rows, p, dlogits);
+    return last_launch_status();
+  };
+  return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
+    PolicyJoin join = {p, {}, rows.n};
+    partials = launch_blocks(rows.n, kMaxPartials);
+    if (const int code = launch_statistics<T, true, false>(rows, s, join, stream)) return code;
+    if (!dlogits) return (int)PPO_OK;
+    const PolicyGrad grad = {p.saved, p.coef, p.grad_scale};
+    return grad_entropy
+               ? launch_gradient<T, true>(rows, grad, nullptr, 0.0f, dlogits, stream)
+               : launch_gradient<T, false>(rows, grad, nullptr, 0.0f, dlogits, stream);
+  });
+}
+
+}  // namespace
+}  // namespace ppo
+
+extern "C" int ppo_token_policy_loss(const ppo_token_rows* r, const float* old_log_probs,
+                                     const float* advantages, const float* ref_log_probs,
+                                     const ppo_token_loss* loss, float* scalars, float* saved,
+                                     float* coef, void* dlogits, void* workspace,
+                                     size_t workspace_bytes, void* stream_ptr) {
+  using namespace ppo;
+  Rows rows;
+  if (const int code = take_rows(r, true, rows)) return code;
+  if (!loss || !scalars || !(loss->clip_low >= 0.0) || !(loss->clip_high >= 0.0) ||
+      !isfinite(loss->kl_coef) || !isfinite(loss->entropy_coef))
+    return PPO_ERR_INVALID_ARG;
+  if (loss->kl_coef != 0.0 && !ref_log_probs && rows.n) return PPO_ERR_INVALID_ARG;
+  if (rows.n && (!old_log_probs || !advantages)) return PPO_ERR_INVALID_ARG;
+  if ((saved == nullptr) != (coef == nullptr) || (dlogits && !saved && rows.n) ||
+      (saved && !aligned16(saved)) || (uintptr_t)dlogits % dtype_size(r->dtype))
+    return PPO_ERR_INVALID_ARG;
+  const Scratch s = scratch_of(workspace, rows.S, rows.T, rows.A, r->dtype);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < s.bytes) return PPO_ERR_WORKSPACE;
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  Weights weights;
+  if (const int code = take_weights(rows, loss, s, stream, weights)) return code;
+  Policy p = {old_log_probs, advantages, ref_log_probs, weights, (float)(1.0 - loss->clip_low),
+              (float)(1.0 + loss->clip_high), (float)loss->kl_coef, (float)loss->entropy_coef,
+              (float)loss->grad_scale, loss->advantages_per_sequence,
+              reinterpret_cast<Saved*>(saved), coef, s.sums};
+  int partials = 0;
+  if (rows.n)
+    if (const int code = with_dtype(r->dtype, [&](auto zero) {
+          return run_policy<decltype(zero)>(rows, p, s, (decltype(zero)*)dlogits, partials, stream);
+        }))
+      return code;
+  hipLaunchKernelGGL(policy_scalars_kernel, dim3(1), dim3(1024), 0, stream, s.sums, partials,
+                     loss->kl_coef, loss->entropy_coef, scalars);
+  return last_launch_status();
+}

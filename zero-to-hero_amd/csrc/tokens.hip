@@ -1,0 +1,311 @@
+// Token policies: log-probabilities and entropies of the taken actions, their
+// gradient, the preference loss over them, and what all of these operators
+// share on the host: checks, weights, scratch.
+#include "tokens_rows.hpp"
+
+namespace ppo {
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+// A row's statistics by several workgroups: down to 512 chunks (8 KB) each, as
+// many as fill the chip four times over.
+int row_splits(int64_t rows, int64_t A, int dtype) {
+  if (rows <= 0) return 1;
+  int64_t s = div_up(1024, rows);
+  const int64_t most = chunks_of(A, dtype) / 512;
+  if (s > most) s = most;
+  if (s > kMaxSplits) s = kMaxSplits;
+  return s < 1 ? 1 : (int)s;
+}
+
+Scratch scratch_of(void* workspace, int64_t S, int64_t T, int64_t A, int dtype) {
+  char* p = static_cast<char*>(workspace);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* here = p ? p + at : nullptr;
+    at += (size_t)round_up((int64_t)bytes, 256);
+    return here;
+  };
+  Scratch s;
+  s.counts = reinterpret_cast<int*>(take(kCountBlocks * sizeof(int)));
+  s.lengths = reinterpret_cast<int*>(take((size_t)S * sizeof(int)));
+  s.sums = reinterpret_cast<double*>(take(sizeof(double) * kSums * kMaxPartials));
+  s.parts = reinterpret_cast<Stat*>(take((size_t)(S * T) * row_splits(S * T, A, dtype) *
+                                         sizeof(Stat)));
+  s.bytes = at;
+  return s;
+}
+
+static bool sizes_ok(int64_t S, int64_t T, int64_t A) {
+  return A <= ((int64_t)1 << 30) && (T == 0 || S < ((int64_t)1 << 31) / T) && S < ((int64_t)1 << 31) &&
+         T < ((int64_t)1 << 31) && S * T <= ((int64_t)1 << 46) / A;
+}
+
+int take_rows(const ppo_token_rows* r, bool actions, Rows& out) {
+  if (!r || !dtype_ok(r->dtype) || r->sequences < 0 || r->tokens < 0 || r->A <= 0 ||
+      !(r->temperature > 0.0))
+    return PPO_ERR_INVALID_ARG;
+  const float c = (float)(1.44269504088896340736 / r->temperature);
+  const float inv_tau = (float)(1.0 / r->temperature);
+  if (!(c > 0.0f) || !(c < INFINITY)) return PPO_ERR_INVALID_ARG;
+  if (!sizes_ok(r->sequences, r->tokens, r->A)) return PPO_ERR_TOO_LARGE;
+  out = {r->logits, r->actions, r->mask, r->sequences * r->tokens, r->tokens, r->sequences,
+         (int)r->A, r->actions_are_int64, c, inv_tau};
+  if (out.n == 0) return PPO_OK;
+  const uintptr_t size = dtype_size(r->dtype);
+  if (!r->logits || (uintptr_t)r->logits % size || (actions && !r->actions))
+    return PPO_ERR_INVALID_ARG;
+  return PPO_OK;
+}
+
+namespace {
+
+// Rows that count, by workgroup.
+__global__ void __launch_bounds__(256) count_rows_kernel(const uint8_t* mask, int64_t n, int* counts) {
+  __shared__ int part[4];
+  int k = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    k += mask[i] != 0;
+  const int lane = threadIdx.x & (kWave - 1);
+  k = (int)lanes_sum<kWave>((float)k);  // (a lane's few hundred: exact)
+  if (lane == 0) part[threadIdx.x / kWave] = k;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+
+// Rows that count in each sequence, a wave to a sequence, and by workgroup the
+// sequences that have any.
+__global__ void __launch_bounds__(256) count_sequences_kernel(const uint8_t* mask, int64_t S,
+                                                              int64_t T, int* lengths, int* counts) {
+  __shared__ int part[4];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  int some = 0;
+  for (int64_t s = (int64_t)blockIdx.x * 4 + wave; s < S; s += (int64_t)gridDim.x * 4) {
+    int k = 0;
+    for (int64_t i = lane; i < T; i += kWave) k += mask[s * T + i] != 0;
+    const double all = lanes_sum<kWave>((double)k);
+    if (lane == 0) lengths[s] = (int)all;
+    some += all > 0.0;
+  }
+  if (lane == 0) part[wave] = some;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+
+}  // namespace
+
+int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, hipStream_t stream,
+                 Weights& w) {
+  const bool sequences = loss->reduction == PPO_SEQUENCE_MEAN;
+  if ((loss->reduction != PPO_TOKEN_MEAN && !sequences) || !(loss->denominator >= 0.0) ||
+      !(loss->grad_scale > 0.0) || !(loss->grad_scale < INFINITY))
+    return PPO_ERR_INVALID_ARG;
+  w = {nullptr, nullptr, 0, 0.0f};
+  if (loss->denominator > 0.0) w.inverse = (float)(1.0 / loss->denominator);
+  if (!rows.mask) {
+    // every sequence is as long as the others
+    if (loss->denominator > 0.0)
+      w.inverse = (float)(1.0 / (sequences ? loss->denominator * (double)rows.T : loss->denominator));
+    else
+      w.inverse = rows.n ? (float)(1.0 / (double)rows.n) : 0.0f;
+    return PPO_OK;
+  }
+  if (rows.n == 0) return PPO_OK;
+  if (sequences) {
+    w.partials = launch_blocks(div_up(rows.S, 4), kCountBlocks);
+    w.counts = s.counts;
+    w.lengths = s.lengths;
+    hipLaunchKernelGGL(count_sequences_kernel, dim3(w.partials), dim3(256), 0, stream, rows.mask,
+                       rows.S, rows.T, s.lengths, s.counts);
+  } else if (!(w.inverse > 0.0f)) {
+    w.partials = launch_blocks(div_up(rows.n, 1024), kCountBlocks);
+    w.counts = s.counts;
+    hipLaunchKernelGGL(count_rows_kernel, dim3(w.partials), dim3(256), 0, stream, rows.mask, rows.n,
+                       s.counts);
+  }
+  return last_launch_status();
+}
+
+namespace {
+
+// What ppo_token_log_probs leaves of a row.
+struct LogProbs {
+  static constexpr bool kWholeWave = false;
+  const float* minus;
+  float *log_probs, *entropy;
+  Saved* saved;
+
+  __device__ __forceinline__ void masked(int64_t r) const {
+    log_probs[r] = 0.0f;
+    if (entropy) entropy[r] = 0.0f;
+  }
+  template <bool kEntropy>
+  __device__ __forceinline__ void row(const Rows& rows, int64_t r, Stat x, float la, bool first) {
+    const RowTerms t = row_terms<kEntropy>(x, la, rows.c);
+    if (!first) return;
+    log_probs[r] = (float)(minus ? t.lp - (double)minus[r] : t.lp);
+    if (entropy) entropy[r] = t.H;
+    if (saved) saved[r] = saved_of(t, 0.0f);
+  }
+  __device__ __forceinline__ void end() const {}
+};
+
+// The gradient of a row's log-probability and entropy.
+struct LogProbsGrad {
+  const Saved* saved;
+  const float *dlp, *dent;
+
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, float up, int a) const {
+    return row_grad(saved[r], dlp ? up * dlp[r] : 0.0f, dent ? up * dent[r] : 0.0f, rows.inv_tau, a);
+  }
+};
+
+// A workgroup to a pair: the two sequences' sums in 64 bits, the loss, and the
+// coefficient of each of their rows.  The sums are over differences to the
+// reference's log-probabilities, so they are small where the policies are alike.
+__global__ void __launch_bounds__(256) preference_kernel(
+    const float* rel, const uint8_t* mask, int64_t pairs, int64_t T, double beta, double margin,
+    double smoothing, int average, double* losses, float* rewards, float* coef) {
+  __shared__ double part[4][4];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  for (int64_t i = blockIdx.x; i < pairs; i += gridDim.x) {
+    double sum[2], n[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t at = (i + k * pairs) * T;
+      double x = 0.0, m = 0.0;
+      for (int64_t t = threadIdx.x; t < T; t += 256)
+        if (!mask || mask[at + t]) {
+          x += (double)rel[at + t];
+          m += 1.0;
+        }
+      x = lanes_sum<kWave>(x);
+      m = lanes_sum<kWave>(m);
+      if (lane == 0) {
+        part[wave][k] = x;
+        part[wave][2 + k] = m;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      sum[k] = (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
+      n[k] = (part[0][2 + k] + part[1][2 + k]) + (part[2][2 + k] + part[3][2 + k]);
+    }
+    __syncthreads();
+    const double w0 = average && n[0] > 0.0 ? 1.0 / n[0] : 1.0;
+    const double w1 = average && n[1] > 0.0 ? 1.0 / n[1] : 1.0;
+    const double r0 = beta * sum[0] * w0, r1 = beta * sum[1] * w1;
+    const double m = r0 - r1 - margin;
+    // -log sigmoid(m) = max(-m, 0) + log(1 + e^-|m|), and sigmoid(m) from the same e
+    const double e = exp(-fabs(m)), soft = log1p(e);
+    const double up = soft + fmax(-m, 0.0), down = soft + fmax(m, 0.0);
+    const double sig = m >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
+    const double not_sig = m >= 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);
+    // sigmoid(m) - (1 - smoothing) without the cancellation at m large
+    const double dm = (smoothing == 0.0 ? -not_sig : sig - (1.0 - smoothing)) / (double)pairs;
+    if (threadIdx.x == 0) {
+      // (0 times an infinite part is no part)
+      losses[i] = (smoothing < 1.0 ? (1.0 - smoothing) * up : 0.0) +
+                  (smoothing > 0.0 ? smoothing * down : 0.0) + (m == m ? 0.0 : m);
+      rewards[i] = (float)r0;
+      rewards[i + pairs] = (float)r1;
+    }
+    for (int64_t t = threadIdx.x; t < 2 * T; t += 256) {
+      const bool second = t >= T;
+      const int64_t at = second ? (i + pairs) * T + (t - T) : i * T + t;
+      const double w = second ? -w1 : w0;
+      coef[at] = !mask || mask[at] ? (float)(dm * beta * w) : 0.0f;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) mean_kernel(const double* x, int64_t n, float* out) {
+  __shared__ double part[4];
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 256) v += x[i];
+  v = lanes_sum<kWave>(v);
+  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) *out = (float)(((part[0] + part[1]) + (part[2] + part[3])) / (double)n);
+}
+
+}  // namespace
+}  // namespace ppo
+
+extern "C" size_t ppo_token_workspace_bytes(int64_t sequences, int64_t tokens, int64_t A,
+                                            int dtype) {
+  using namespace ppo;
+  if (sequences <= 0 || tokens <= 0 || A <= 0 || !dtype_ok(dtype) ||
+      !sizes_ok(sequences, tokens, A))
+    return 0;
+  return scratch_of(nullptr, sequences, tokens, A, dtype).bytes;
+}
+
+extern "C" int ppo_token_log_probs(const ppo_token_rows* r, const float* minus, float* log_probs,
+                                   float* entropy, float* saved, void* workspace,
+                                   size_t workspace_bytes, void* stream_ptr) {
+  using namespace ppo;
+  Rows rows;
+  if (const int code = take_rows(r, true, rows)) return code;
+  if (rows.n == 0) return PPO_OK;
+  if (!log_probs || (saved && !aligned16(saved))) return PPO_ERR_INVALID_ARG;
+  const Scratch s = scratch_of(workspace, rows.S, rows.T, rows.A, r->dtype);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < s.bytes) return PPO_ERR_WORKSPACE;
+  const LogProbs emit = {minus, log_probs, entropy, reinterpret_cast<Saved*>(saved)};
+  return with_dtype(r->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    return entropy ? launch_statistics<T, true, true>(rows, s, emit, (hipStream_t)stream_ptr)
+                   : launch_statistics<T, false, true>(rows, s, emit, (hipStream_t)stream_ptr);
+  });
+}
+
+extern "C" int ppo_token_log_probs_backward(const ppo_token_rows* r, const float* saved,
+                                            const float* d_log_probs, const float* d_entropy,
+                                            const float* scale, double held, void* dlogits,
+                                            void* stream_ptr) {
+  using namespace ppo;
+  Rows rows;
+  if (const int code = take_rows(r, true, rows)) return code;
+  if (rows.n == 0) return PPO_OK;
+  if (!saved || !aligned16(saved) || (!d_log_probs && !d_entropy) || !dlogits || (held != 0.0 && !scale) ||
+      (uintptr_t)dlogits % dtype_size(r->dtype))
+    return PPO_ERR_INVALID_ARG;
+  const LogProbsGrad grad = {reinterpret_cast<const Saved*>(saved), d_log_probs, d_entropy};
+  return with_dtype(r->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    hipStream_t stream = (hipStream_t)stream_ptr;
+    return d_entropy
+               ? launch_gradient<T, true>(rows, grad, scale, (float)held, (T*)dlogits, stream)
+               : launch_gradient<T, false>(rows, grad, scale, (float)held, (T*)dlogits, stream);
+  });
+}
+
+extern "C" size_t ppo_token_preference_workspace_bytes(int64_t sequences) {
+  return sequences > 0 ? (size_t)sequences / 2 * sizeof(double) : 0;
+}
+
+extern "C" int ppo_token_preference(const float* relative, const uint8_t* mask, int64_t sequences,
+                                    int64_t tokens, double beta, double margin, double smoothing,
+                                    int average, float* loss, float* rewards, float* coef,
+                                    void* workspace, size_t workspace_bytes, void* stream_ptr) {
+  using namespace ppo;
+  if (sequences <= 0 || sequences % 2 || tokens < 0 || !isfinite(beta) || !isfinite(margin) ||
+      !(smoothing >= 0.0 && smoothing <= 1.0) || !loss || !rewards ||
+      (tokens > 0 && (!relative || !coef)))
+    return PPO_ERR_INVALID_ARG;
+  if (!sizes_ok(sequences, tokens, 1)) return PPO_ERR_TOO_LARGE;
+  if (!workspace || !aligned16(workspace) ||
+      workspace_bytes < ppo_token_preference_workspace_bytes(sequences))
+    return PPO_ERR_WORKSPACE;
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  const int64_t pairs = sequences / 2;
+  double* losses = static_cast<double*>(workspace);
+  hipLaunchKernelGGL(preference_kernel, dim3(launch_blocks(pairs, kMaxPartials)), dim3(256), 0,
+                     stream, relative, mask, pairs, tokens, beta, margin, smoothing, average,
+                     losses, rewards, coef);
+  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(256), 0, stream, losses, pairs, loss);
+  return last_launch_status();
+}

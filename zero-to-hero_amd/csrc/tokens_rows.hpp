@@ -1,0 +1,253 @@
+// Passes over rows of logits by any number of workgroups to a row: the statistics
+// (read once, nothing kept) and a gradient from them (read once, written once).
+#pragma once
+
+#include <type_traits>
+
+#include "tokens.hpp"
+
+namespace ppo {
+
+// Statistics of chunks [part / splits) of a row, by G lanes, four chunks of each
+// lane in flight; the sums follow the running maximum.
+template <class T, int G, bool kEntropy>
+__device__ __forceinline__ Stat stream_stat(const T* row, int A, int a, float c, int t, int part,
+                                            int splits) {
+  constexpr int kN = kPer16<T>, kU = 4;
+  const Cut<T> cut(row, A);
+  const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
+  const int per = (cut.nvec + splits - 1) / splits;
+  const int end = min(cut.nvec, (part + 1) * per);
+  const int b = a - cut.head, va = a >= 0 && b >= 0 ? b / kN : -1;  // the action's chunk
+  Stat x = {kNegInf, 0.0f, 0.0f};
+  if (part == 0 && t < cut.ends) {
+    const int col = cut.end_column(t);
+    const float l = col == a ? kNegInf : to_f32(row[col]);
+    x.m = l;
+    const float d = l == kNegInf ? l : (l - l) * c;  // (NaN and +inf give NaN)
+    x.s = exp2_fast(d);
+  }
+  for (int i = part * per + t; i < end; i += G * kU) {
+    v4i w[kU];
+#pragma unroll
+    for (int k = 0; k < kU; ++k)
+      w[k] = i + k * G < end ? __builtin_nontemporal_load(body + i + k * G) : no_chunk<T>();
+    float m = x.m;
+#pragma unroll
+    for (int k = 0; k < kU; ++k) {
+      if (i + k * G == va) knock_out<T>(w[k], b - va * kN);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) m = fmaxf(m, unpack<T>(w[k], j));
+    }
+    rebase<kEntropy>(x, m, c);
+    if (m == kNegInf) m = 0.0f;
+    float s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kU; ++k)
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        const float d = (unpack<T>(w[k], j) - m) * c, e = exp2_fast(d);
+        (j & 1 ? s2 : x.s) += e;
+        if (kEntropy) x.u = fmaf(e, fmaxf(d, -1e30f), x.u);
+      }
+    x.s += s2;
+  }
+  return x;
+}
+
+template <class T>
+__device__ __forceinline__ float action_logit(const T* row, int a) {
+  return a >= 0 ? to_f32(row[a]) : PPO_NAN;
+}
+
+// One group to a row and the row finished by it (kDirect), or `splits` workgroups to
+// a row that leave their parts.  What bounds it: HBM reads.
+template <class T, int G, bool kEntropy, bool kDirect, class Emit>
+__global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, Stat* parts,
+                                                         int splits) {
+  __shared__ Stat s_part[4];
+  const int t = threadIdx.x % G;
+  const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const int64_t r = kDirect ? group : group / splits;
+  if (r >= rows.n) return;  // (with G = 256 the whole workgroup)
+  const int part = kDirect ? 0 : (int)(group - r * splits);
+  if (!rows.live(r)) {
+    if (kDirect && t == 0) emit.masked(r);
+    return;
+  }
+  const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
+  const int a = rows.actions ? rows.action(r) : -1;
+  const float la = kDirect ? action_logit(row, a) : 0.0f;
+  Stat x = stream_stat<T, G, kEntropy>(row, rows.A, a, rows.c, t, part, splits);
+  if (G > kWave) {
+    x = block_join<kEntropy>(x, rows.c, s_part);
+    if (threadIdx.x >= kWave) return;
+  } else {
+    x = lanes_join<G <= kWave ? G : kWave, kEntropy>(x, rows.c);
+  }
+  if constexpr (kDirect)
+    emit.template row<kEntropy>(rows, r, x, la, t == 0);
+  else if (t == 0)
+    parts[group] = x;
+}
+
+// A wave to a row: its parts joined in the order of their lanes, and the row
+// finished by its lane 0, or by the wave (kWholeWave).
+template <class T, bool kEntropy, class Emit>
+__global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit, const Stat* parts,
+                                                  int splits) {
+  const int lane = threadIdx.x;
+  for (int64_t r = blockIdx.x; r < rows.n; r += gridDim.x) {
+    if (!rows.live(r)) {
+      if (lane == 0) emit.masked(r);
+      continue;
+    }
+    const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
+    const int a = rows.actions ? rows.action(r) : -1;
+    const float la = action_logit(row, a);
+    Stat x = lane < splits ? parts[r * splits + lane] : Stat{kNegInf, 0.0f, 0.0f};
+    x = lanes_join<kWave, kEntropy>(x, rows.c);
+    if constexpr (Emit::kWholeWave)
+      emit.row(rows, r, row, x, lane);
+    else
+      emit.template row<kEntropy>(rows, r, x, la, lane == 0);
+  }
+  emit.end();
+}
+
+template <class T, bool kEntropy, bool kMayDirect, class Emit>
+int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, hipStream_t stream) {
+  const int dtype = sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16;  // (sizes alike)
+  const int splits = row_splits(rows.n, rows.A, dtype);
+  if constexpr (kMayDirect)
+    if (splits == 1) {
+      const int64_t chunks = chunks_of(rows.A, dtype);
+      auto go = [&](auto lanes) {
+        constexpr int G = decltype(lanes)::value;
+        hipLaunchKernelGGL((statistics_kernel<T, G, kEntropy, true, Emit>),
+                           dim3((unsigned)div_up(rows.n, 256 / G)), dim3(256), 0, stream, rows, emit,
+                           nullptr, 1);
+        return last_launch_status();
+      };
+      if (chunks <= 64) return go(std::integral_constant<int, 16>{});
+      if (chunks <= 512) return go(std::integral_constant<int, 64>{});
+      return go(std::integral_constant<int, 256>{});
+    }
+  if (rows.n > ((int64_t)1 << 31) / splits - 1) return PPO_ERR_TOO_LARGE;
+  hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
+                     dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
+                     splits);
+  hipLaunchKernelGGL((join_kernel<T, kEntropy, Emit>), dim3(launch_blocks(rows.n, kMaxPartials)),
+                     dim3(64), 0, stream, rows, emit, s.parts, splits);
+  return last_launch_status();
+}
+
+// dlogits from the logits and the rows' terms: G lanes to a piece of a row, four
+// chunks to a lane.  What bounds it: HBM, one read and one write of the rows.
+constexpr int kGradU = 4;
+template <class T, int G, bool kC, class Terms>
+__global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, const float* scale,
+                                                       float held, T* dlogits, int64_t pieces) {
+  constexpr int kN = kPer16<T>;
+  const float up = scale ? *scale : 1.0f;
+  if (held != 0.0f && up == held) return;
+  const int t = threadIdx.x % G;
+  const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const int64_t r = group / pieces;
+  if (r >= rows.n) return;
+  const int piece = (int)(group - r * pieces);
+  const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
+  T* out = dlogits + r * rows.A;
+  const bool live = rows.live(r);
+  const Cut<T> cut(live ? row : out, rows.A);
+  const int first = piece * (G * kGradU) + t;
+  T* to = out + cut.head;
+  const int64_t per = (int64_t)G * kN;
+  const bool ends = piece == 0 && t < cut.ends;
+  const int end_col = ends ? cut.end_column(t) : 0;
+  if (!live) {
+    const v4i none = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < kGradU; ++k)
+      if (first + k * G < cut.nvec) store16(to + (int64_t)first * kN + k * per, none, true);
+    if (ends) out[end_col] = from_f32<T>(0.0f);
+    return;
+  }
+  const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
+  v4i w[kGradU];
+#pragma unroll
+  for (int k = 0; k < kGradU; ++k)
+    if (first + k * G < cut.nvec) w[k] = __builtin_nontemporal_load(body + first + k * G);
+  const float end = ends ? to_f32(row[end_col]) : kNegInf;
+  const Grad g = terms.row(rows, r, up, rows.actions ? rows.action(r) : -1);
+  const bool vec = ((uintptr_t)to & 15) == 0;
+  const int b = g.a - cut.head;
+  const int va = g.a >= 0 && b >= 0 ? b / kN : -1;
+#pragma unroll
+  for (int k = 0; k < kGradU; ++k) {
+    const int v = first + k * G;
+    if (v >= cut.nvec) continue;
+    float d[kN];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      d[j] = grad_at<kC>(g, rows.c, unpack<T>(w[k], j));
+      if (v == va && j == b - va * kN) d[j] = g.da;
+    }
+    store16(to + (int64_t)v * kN, pack<T>(d), vec);
+  }
+  if (ends) out[end_col] = from_f32<T>(end_col == g.a ? g.da : grad_at<kC>(g, rows.c, end));
+}
+
+template <class T, bool kC, class Terms>
+int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, float held,
+                    T* dlogits, hipStream_t stream) {
+  const int dtype = sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16;
+  const int64_t chunks = chunks_of(rows.A, dtype);
+  auto go = [&](auto lanes) {
+    constexpr int G = decltype(lanes)::value;
+    const int64_t pieces = div_up(chunks, G * kGradU);
+    if (rows.n > (((int64_t)1 << 31) - 1) / pieces) return (int)PPO_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((gradient_kernel<T, G, kC, Terms>),
+                       dim3((unsigned)div_up(rows.n * pieces, 256 / G)), dim3(256), 0, stream, rows,
+                       terms, scale, held, dlogits, pieces);
+    return last_launch_status();
+  };
+  if (chunks <= 64) return go(std::integral_constant<int, 16>{});
+  if (chunks <= 512) return go(std::integral_constant<int, 64>{});
+  return go(std::integral_constant<int, 256>{});
+}
+
+// How a pass that keeps its rows in registers is laid out: held(lanes, chunks a
+// lane) for the smallest group that holds a row, or split() where a row does not
+// fit, or rows are so few that one workgroup to each would leave most of the chip
+// empty, or the gradients lie otherwise in 16 bytes than the logits (not `alike`).
+// (without gradients: as if they started at a multiple of 16, so that a loss has the
+// same bits with and without them where its caller allocates them so)
+inline bool lies_alike(const void* logits, const void* dlogits) {
+  return ((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0;
+}
+template <int N>
+using Int = std::integral_constant<int, N>;
+template <class Held, class Split>
+int with_row_shape(int64_t rows, int64_t chunks, bool alike, Held&& held, Split&& split) {
+  if (!alike) return split();
+  if (chunks <= 16 * 1) return held(Int<16>{}, Int<1>{});
+  if (chunks <= 16 * 4) return held(Int<16>{}, Int<4>{});
+  if (chunks <= 64 * 4) return held(Int<64>{}, Int<4>{});
+  if (chunks <= 64 * 8) return held(Int<64>{}, Int<8>{});
+  if (rows < 64 && chunks > 2048) return split();
+  if (chunks <= 256 * 4) return held(Int<256>{}, Int<4>{});
+  if (chunks <= 256 * 6) return held(Int<256>{}, Int<6>{});
+  if (chunks <= 256 * 8) return held(Int<256>{}, Int<8>{});
+  if (chunks <= 512 * 6) return held(Int<512>{}, Int<6>{});
+  if (chunks <= 512 * 8) return held(Int<512>{}, Int<8>{});
+  if (chunks <= 1024 * 6) return held(Int<1024>{}, Int<6>{});
+  if (chunks <= 1024 * 8) return held(Int<1024>{}, Int<8>{});
+  if (chunks <= 1024 * 10) return held(Int<1024>{}, Int<10>{});
+  if (chunks <= 1024 * 12) return held(Int<1024>{}, Int<12>{});
+  if (chunks <= 1024 * 14) return held(Int<1024>{}, Int<14>{});
+  if (chunks <= 1024 * 16) return held(Int<1024>{}, Int<16>{});
+  return split();
+}
+
+}  // namespace ppo

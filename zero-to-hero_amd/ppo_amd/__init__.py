@@ -16,6 +16,9 @@ include/ppo_amd.h) behind the reference's own PPO surface:
   layers    gated_ffn, dropout, quantize_rows, int8_linear and the modules
             GatedLinear, GatedMLP, Int8Linear, int8_copy: the feed-forward
             layers of larger policies (libppo_layers.so)
+  tokens    token_log_probs, token_policy_loss, preference_loss,
+            distillation_loss, top_logits: policies over up to a vocabulary of
+            actions, trained on sequences (libppo_tokens.so)
   torch_ops the hot path as registered operators, torch.ops.ppo_amd.*
             (gae, gae_normalize, normalize_advantages, ppo_loss_discrete,
             ppo_loss_gaussian), visible to torch.compile and the dispatcher
@@ -62,6 +65,15 @@ from .ops import (
     sample_categorical,
     sample_gaussian,
 )
+from .tokens import (
+    PreferenceStats,
+    TokenStats,
+    distillation_loss,
+    preference_loss,
+    token_log_probs,
+    token_policy_loss,
+    top_logits,
+)
 from . import torch_ops  # registers torch.ops.ppo_amd.*
 from .env import CartPoleVec
 from .optim import ClippedAdam
@@ -87,14 +99,17 @@ __all__ = [
     "PPOAgent",
     "PPOConfig",
     "PendingStep",
+    "PreferenceStats",
     "RolloutBuffer",
     "RolloutStep",
+    "TokenStats",
     "TrainingConfig",
     "Transition",
     "VecPPO",
     "cartpole_sizes",
     "check_waits",
     "discounted_returns",
+    "distillation_loss",
     "dropout",
     "gae",
     "gae_normalize",
@@ -114,7 +129,11 @@ __all__ = [
     "ppo_loss_gaussian_fused",
     "ppo_mlp_cat_grads",
     "ppo_mlp_cat_step",
+    "preference_loss",
     "quantize_rows",
     "sample_categorical",
     "sample_gaussian",
+    "token_log_probs",
+    "token_policy_loss",
+    "top_logits",
 ]

@@ -220,6 +220,93 @@ def load_layers() -> ctypes.CDLL:
     return _layers
 
 
+# ---------------------------------------------------------------------------
+# libppo_tokens.so (include/ppo_tokens.h)
+# ---------------------------------------------------------------------------
+PPO_TOKEN_SAVED = 8
+PPO_TOKEN_SCALARS = 6
+PPO_TOKEN_MAX_K = 256
+TOKEN_SCALAR_NAMES = ("loss", "policy", "kl", "entropy", "approx_kl", "clipfrac")
+TOKEN_REDUCTIONS = {"token": 0, "sequence": 1}
+TOKENS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libppo_tokens.so")
+
+
+class TokenRows(ctypes.Structure):
+    """struct ppo_token_rows (include/ppo_tokens.h)."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("actions", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("sequences", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("A", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("actions_are_int64", ctypes.c_int),
+        ("temperature", ctypes.c_double),
+    ]
+
+
+class TokenLoss(ctypes.Structure):
+    """struct ppo_token_loss (include/ppo_tokens.h)."""
+
+    _fields_ = [
+        ("clip_low", ctypes.c_double),
+        ("clip_high", ctypes.c_double),
+        ("kl_coef", ctypes.c_double),
+        ("entropy_coef", ctypes.c_double),
+        ("denominator", ctypes.c_double),
+        ("grad_scale", ctypes.c_double),
+        ("reduction", ctypes.c_int),
+        ("advantages_per_sequence", ctypes.c_int),
+    ]
+
+
+_rows = ctypes.POINTER(TokenRows)
+_loss = ctypes.POINTER(TokenLoss)
+
+# name -> (restype, argtypes); one entry per function in include/ppo_tokens.h
+TOKEN_SIGNATURES = {
+    "ppo_token_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "ppo_token_log_probs": (_int, [_rows, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppo_token_log_probs_backward": (_int, [_rows, _vp, _vp, _vp, _vp, _f64, _vp, _vp]),
+    "ppo_token_policy_loss": (
+        _int, [_rows, _vp, _vp, _vp, _loss, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppo_token_preference_workspace_bytes": (_sz, [_i64]),
+    "ppo_token_preference": (
+        _int,
+        [_vp, _vp, _i64, _i64, _f64, _f64, _f64, _int, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "ppo_token_distillation": (
+        _int, [_rows, _vp, _int, _vp, _int, _i64, _loss, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppo_token_distillation_backward": (
+        _int, [_rows, _vp, _int, _vp, _int, _i64, _vp, _vp, _f64, _vp, _vp]),
+    "ppo_token_top_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "ppo_token_top": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
+}
+
+_tokens = None
+
+
+def load_tokens() -> ctypes.CDLL:
+    """Load libppo_tokens.so once and attach the prototypes; raise if absent."""
+    global _tokens
+    if _tokens is None:
+        load()
+        if not os.path.exists(TOKENS_PATH):
+            raise RuntimeError(
+                f"{TOKENS_PATH} is not built. Build it with `python -m ppo_amd.build` "
+                "(or __graft_entry__.build()); ppo_amd has no CPU fallback."
+            )
+        lib = ctypes.CDLL(TOKENS_PATH)
+        for name, (res, args) in TOKEN_SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+        _tokens = lib
+    return _tokens
+
+
 _lib = None
 
 
