@@ -256,8 +256,9 @@ int dense_gradient(const Rows& rows, const Teacher& teacher, const Saved* saved,
   const DistillGrad grad = {saved, grad_scale};
   if (const int code = launch_gradient<T, false>(rows, grad, scale, held, dlogits, stream))
     return code;
-  hipLaunchKernelGGL((entries_kernel<T>), dim3(launch_blocks(rows.n, kMaxPartials)), dim3(64), 0,
-                     stream, rows, teacher, saved, scale, held, grad_scale, dlogits);
+  hipLaunchKernelGGL((entries_kernel<T>),
+                     dim3(launch_blocks(rows.n, held != 0.0f ? kHeldBlocks : kMaxPartials)), dim3(64),
+                     0, stream, rows, teacher, saved, scale, held, grad_scale, dlogits);
   return last_launch_status();
 }
 

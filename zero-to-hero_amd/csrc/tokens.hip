@@ -162,32 +162,41 @@ struct LogProbsGrad {
   }
 };
 
-// A workgroup to a pair: the two sequences' sums in 64 bits, the loss, and the
-// coefficient of each of their rows.  The sums are over differences to the
-// reference's log-probabilities, so they are small where the policies are alike.
-__global__ void __launch_bounds__(256) preference_kernel(
-    const float* rel, const uint8_t* mask, int64_t pairs, int64_t T, double beta, double margin,
-    double smoothing, int average, double* losses, float* rewards, float* coef) {
-  __shared__ double part[4][4];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  for (int64_t i = blockIdx.x; i < pairs; i += gridDim.x) {
-    double sum[2], n[2];
+struct Preferences {
+  const float* rel;
+  const uint8_t* mask;
+  int64_t pairs, T;
+  double beta, margin, smoothing;
+  int average;
+  double* losses;
+  float *rewards, *coef;
+};
+
+// Pair i by G lanes, a wave or a workgroup of four: the two sequences' sums in 64 bits,
+// the loss, and the coefficient of each of their rows.  The sums are over differences
+// to the reference's log-probabilities, so they are small where the policies are
+// alike.  Returns the loss.
+template <int G>
+__device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, double (*part)[4]) {
+  const int t = threadIdx.x % G, wave = threadIdx.x / kWave;
+  double sum[2], n[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int64_t at = (i + k * pairs) * T;
-      double x = 0.0, m = 0.0;
-      for (int64_t t = threadIdx.x; t < T; t += 256)
-        if (!mask || mask[at + t]) {
-          x += (double)rel[at + t];
-          m += 1.0;
-        }
-      x = lanes_sum<kWave>(x);
-      m = lanes_sum<kWave>(m);
-      if (lane == 0) {
-        part[wave][k] = x;
-        part[wave][2 + k] = m;
+  for (int k = 0; k < 2; ++k) {
+    const int64_t at = (i + k * p.pairs) * p.T;
+    double x = 0.0, m = 0.0;
+    for (int64_t j = t; j < p.T; j += G)
+      if (!p.mask || p.mask[at + j]) {
+        x += (double)p.rel[at + j];
+        m += 1.0;
       }
+    sum[k] = lanes_sum<kWave>(x);
+    n[k] = lanes_sum<kWave>(m);
+    if (G > kWave && (t & (kWave - 1)) == 0) {
+      part[wave][k] = sum[k];
+      part[wave][2 + k] = n[k];
     }
+  }
+  if (G > kWave) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -195,30 +204,54 @@ __global__ void __launch_bounds__(256) preference_kernel(
       n[k] = (part[0][2 + k] + part[1][2 + k]) + (part[2][2 + k] + part[3][2 + k]);
     }
     __syncthreads();
-    const double w0 = average && n[0] > 0.0 ? 1.0 / n[0] : 1.0;
-    const double w1 = average && n[1] > 0.0 ? 1.0 / n[1] : 1.0;
-    const double r0 = beta * sum[0] * w0, r1 = beta * sum[1] * w1;
-    const double m = r0 - r1 - margin;
-    // -log sigmoid(m) = max(-m, 0) + log(1 + e^-|m|), and sigmoid(m) from the same e
-    const double e = exp(-fabs(m)), soft = log1p(e);
-    const double up = soft + fmax(-m, 0.0), down = soft + fmax(m, 0.0);
-    const double sig = m >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
-    const double not_sig = m >= 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);
-    // sigmoid(m) - (1 - smoothing) without the cancellation at m large
-    const double dm = (smoothing == 0.0 ? -not_sig : sig - (1.0 - smoothing)) / (double)pairs;
-    if (threadIdx.x == 0) {
-      // (0 times an infinite part is no part)
-      losses[i] = (smoothing < 1.0 ? (1.0 - smoothing) * up : 0.0) +
-                  (smoothing > 0.0 ? smoothing * down : 0.0) + (m == m ? 0.0 : m);
-      rewards[i] = (float)r0;
-      rewards[i + pairs] = (float)r1;
-    }
-    for (int64_t t = threadIdx.x; t < 2 * T; t += 256) {
-      const bool second = t >= T;
-      const int64_t at = second ? (i + pairs) * T + (t - T) : i * T + t;
-      const double w = second ? -w1 : w0;
-      coef[at] = !mask || mask[at] ? (float)(dm * beta * w) : 0.0f;
-    }
+  }
+  const double w0 = p.average && n[0] > 0.0 ? 1.0 / n[0] : 1.0;
+  const double w1 = p.average && n[1] > 0.0 ? 1.0 / n[1] : 1.0;
+  const double r0 = p.beta * sum[0] * w0, r1 = p.beta * sum[1] * w1;
+  const double m = r0 - r1 - p.margin;
+  // -log sigmoid(m) = max(-m, 0) + log(1 + e^-|m|), and sigmoid(m) from the same e
+  const double e = exp(-fabs(m)), soft = log1p(e);
+  const double up = soft + fmax(-m, 0.0), down = soft + fmax(m, 0.0);
+  const double sig = m >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e);
+  const double not_sig = m >= 0.0 ? e / (1.0 + e) : 1.0 / (1.0 + e);
+  // sigmoid(m) - (1 - smoothing), without the cancellation at m large
+  const double dm = p.smoothing * sig - (1.0 - p.smoothing) * not_sig;
+  if (t == 0) {
+    p.rewards[i] = (float)r0;
+    p.rewards[i + p.pairs] = (float)r1;
+  }
+  for (int64_t j = t; j < 2 * p.T; j += G) {
+    const bool second = j >= p.T;
+    const int64_t at = second ? (i + p.pairs) * p.T + (j - p.T) : i * p.T + j;
+    const double g = dm / (double)p.pairs * p.beta * (second ? -w1 : w0);
+    p.coef[at] = !p.mask || p.mask[at] ? (float)g : 0.0f;
+  }
+  // (0 times an infinite part is no part; a NaN margin stays one)
+  return (p.smoothing < 1.0 ? (1.0 - p.smoothing) * up : 0.0) +
+         (p.smoothing > 0.0 ? p.smoothing * down : 0.0) + (m == m ? 0.0 : m);
+}
+
+// Few tokens: one workgroup of sixteen waves takes all pairs and their mean, one launch
+// where two would take 5 us more.
+constexpr int64_t kFewTokens = 32768;
+__global__ void __launch_bounds__(1024) few_preferences_kernel(Preferences p, float* loss) {
+  __shared__ double part[16];
+  const int wave = threadIdx.x / kWave;
+  double v = 0.0;
+  for (int64_t i = wave; i < p.pairs; i += 16) v += pair_loss<kWave>(p, i, nullptr);
+  if ((threadIdx.x & (kWave - 1)) == 0) part[wave] = v;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  double all = 0.0;
+  for (int w = 0; w < 16; ++w) all += part[w];
+  *loss = (float)(all / (double)p.pairs);
+}
+
+__global__ void __launch_bounds__(256) preferences_kernel(Preferences p) {
+  __shared__ double part[4][4];
+  for (int64_t i = blockIdx.x; i < p.pairs; i += gridDim.x) {
+    const double v = pair_loss<256>(p, i, part);
+    if (threadIdx.x == 0) p.losses[i] = v;
   }
 }
 
@@ -301,11 +334,14 @@ extern "C" int ppo_token_preference(const float* relative, const uint8_t* mask, 
       workspace_bytes < ppo_token_preference_workspace_bytes(sequences))
     return PPO_ERR_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_ptr;
-  const int64_t pairs = sequences / 2;
-  double* losses = static_cast<double*>(workspace);
-  hipLaunchKernelGGL(preference_kernel, dim3(launch_blocks(pairs, kMaxPartials)), dim3(256), 0,
-                     stream, relative, mask, pairs, tokens, beta, margin, smoothing, average,
-                     losses, rewards, coef);
-  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(256), 0, stream, losses, pairs, loss);
+  const Preferences p = {relative, mask, sequences / 2, tokens, beta, margin, smoothing, average,
+                         static_cast<double*>(workspace), rewards, coef};
+  if (sequences * tokens <= kFewTokens) {
+    hipLaunchKernelGGL(few_preferences_kernel, dim3(1), dim3(1024), 0, stream, p, loss);
+    return last_launch_status();
+  }
+  hipLaunchKernelGGL(preferences_kernel, dim3(launch_blocks(p.pairs, kMaxPartials)), dim3(256), 0,
+                     stream, p);
+  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(256), 0, stream, p.losses, p.pairs, loss);
   return last_launch_status();
 }

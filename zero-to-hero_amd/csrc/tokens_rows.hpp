@@ -2,11 +2,15 @@
 // (read once, nothing kept) and a gradient from them (read once, written once).
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "tokens.hpp"
 
 namespace ppo {
+
+template <int N>
+using Int = std::integral_constant<int, N>;
 
 // Statistics of chunks [part / splits) of a row, by G lanes, four chunks of each
 // lane in flight; the sums follow the running maximum.
@@ -129,9 +133,9 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, hipS
                            nullptr, 1);
         return last_launch_status();
       };
-      if (chunks <= 64) return go(std::integral_constant<int, 16>{});
-      if (chunks <= 512) return go(std::integral_constant<int, 64>{});
-      return go(std::integral_constant<int, 256>{});
+      if (chunks <= 64) return go(Int<16>{});
+      if (chunks <= 512) return go(Int<64>{});
+      return go(Int<256>{});
     }
   if (rows.n > ((int64_t)1 << 31) / splits - 1) return PPO_ERR_TOO_LARGE;
   hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
@@ -152,52 +156,57 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
   const float up = scale ? *scale : 1.0f;
   if (held != 0.0f && up == held) return;
   const int t = threadIdx.x % G;
-  const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
-  const int64_t r = group / pieces;
-  if (r >= rows.n) return;
-  const int piece = (int)(group - r * pieces);
-  const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
-  T* out = dlogits + r * rows.A;
-  const bool live = rows.live(r);
-  const Cut<T> cut(live ? row : out, rows.A);
-  const int first = piece * (G * kGradU) + t;
-  T* to = out + cut.head;
-  const int64_t per = (int64_t)G * kN;
-  const bool ends = piece == 0 && t < cut.ends;
-  const int end_col = ends ? cut.end_column(t) : 0;
-  if (!live) {
-    const v4i none = {0, 0, 0, 0};
+  const int64_t groups = rows.n * pieces, step = (int64_t)gridDim.x * (256 / G);
+  for (int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; group < groups;
+       group += step) {
+    const int64_t r = group / pieces;
+    const int piece = (int)(group - r * pieces);
+    const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
+    T* out = dlogits + r * rows.A;
+    const bool live = rows.live(r);
+    const Cut<T> cut(live ? row : out, rows.A);
+    const int first = piece * (G * kGradU) + t;
+    T* to = out + cut.head;
+    const int64_t per = (int64_t)G * kN;
+    const bool ends = piece == 0 && t < cut.ends;
+    const int end_col = ends ? cut.end_column(t) : 0;
+    if (!live) {
+      const v4i none = {0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < kGradU; ++k)
+        if (first + k * G < cut.nvec) store16(to + (int64_t)first * kN + k * per, none, true);
+      if (ends) out[end_col] = from_f32<T>(0.0f);
+      continue;
+    }
+    const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
+    v4i w[kGradU];
 #pragma unroll
     for (int k = 0; k < kGradU; ++k)
-      if (first + k * G < cut.nvec) store16(to + (int64_t)first * kN + k * per, none, true);
-    if (ends) out[end_col] = from_f32<T>(0.0f);
-    return;
-  }
-  const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
-  v4i w[kGradU];
+      if (first + k * G < cut.nvec) w[k] = __builtin_nontemporal_load(body + first + k * G);
+    const float end = ends ? to_f32(row[end_col]) : kNegInf;
+    const Grad g = terms.row(rows, r, up, rows.actions ? rows.action(r) : -1);
+    const bool vec = ((uintptr_t)to & 15) == 0;
+    const int b = g.a - cut.head;
+    const int va = g.a >= 0 && b >= 0 ? b / kN : -1;
 #pragma unroll
-  for (int k = 0; k < kGradU; ++k)
-    if (first + k * G < cut.nvec) w[k] = __builtin_nontemporal_load(body + first + k * G);
-  const float end = ends ? to_f32(row[end_col]) : kNegInf;
-  const Grad g = terms.row(rows, r, up, rows.actions ? rows.action(r) : -1);
-  const bool vec = ((uintptr_t)to & 15) == 0;
-  const int b = g.a - cut.head;
-  const int va = g.a >= 0 && b >= 0 ? b / kN : -1;
+    for (int k = 0; k < kGradU; ++k) {
+      const int v = first + k * G;
+      if (v >= cut.nvec) continue;
+      float d[kN];
 #pragma unroll
-  for (int k = 0; k < kGradU; ++k) {
-    const int v = first + k * G;
-    if (v >= cut.nvec) continue;
-    float d[kN];
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      d[j] = grad_at<kC>(g, rows.c, unpack<T>(w[k], j));
-      if (v == va && j == b - va * kN) d[j] = g.da;
+      for (int j = 0; j < kN; ++j) {
+        d[j] = grad_at<kC>(g, rows.c, unpack<T>(w[k], j));
+        if (v == va && j == b - va * kN) d[j] = g.da;
+      }
+      store16(to + (int64_t)v * kN, pack<T>(d), vec);
     }
-    store16(to + (int64_t)v * kN, pack<T>(d), vec);
+    if (ends) out[end_col] = from_f32<T>(end_col == g.a ? g.da : grad_at<kC>(g, rows.c, end));
   }
-  if (ends) out[end_col] = from_f32<T>(end_col == g.a ? g.da : grad_at<kC>(g, rows.c, end));
 }
 
+// A pass that may find nothing to do has workgroups enough to fill the chip, and few
+// enough to end in 2 us (131072 of them took 29); one that has work one to a piece.
+constexpr int64_t kHeldBlocks = 2048;
 template <class T, bool kC, class Terms>
 int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, float held,
                     T* dlogits, hipStream_t stream) {
@@ -206,15 +215,15 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
   auto go = [&](auto lanes) {
     constexpr int G = decltype(lanes)::value;
     const int64_t pieces = div_up(chunks, G * kGradU);
-    if (rows.n > (((int64_t)1 << 31) - 1) / pieces) return (int)PPO_ERR_TOO_LARGE;
+    const int64_t most = held != 0.0f ? kHeldBlocks : ((int64_t)1 << 31) - 1;
     hipLaunchKernelGGL((gradient_kernel<T, G, kC, Terms>),
-                       dim3((unsigned)div_up(rows.n * pieces, 256 / G)), dim3(256), 0, stream, rows,
-                       terms, scale, held, dlogits, pieces);
+                       dim3((unsigned)std::min(div_up(rows.n * pieces, 256 / G), most)), dim3(256),
+                       0, stream, rows, terms, scale, held, dlogits, pieces);
     return last_launch_status();
   };
-  if (chunks <= 64) return go(std::integral_constant<int, 16>{});
-  if (chunks <= 512) return go(std::integral_constant<int, 64>{});
-  return go(std::integral_constant<int, 256>{});
+  if (chunks <= 64) return go(Int<16>{});
+  if (chunks <= 512) return go(Int<64>{});
+  return go(Int<256>{});
 }
 
 // How a pass that keeps its rows in registers is laid out: held(lanes, chunks a
@@ -226,8 +235,6 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
 inline bool lies_alike(const void* logits, const void* dlogits) {
   return ((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0;
 }
-template <int N>
-using Int = std::integral_constant<int, N>;
 template <class Held, class Split>
 int with_row_shape(int64_t rows, int64_t chunks, bool alike, Held&& held, Split&& split) {
   if (!alike) return split();

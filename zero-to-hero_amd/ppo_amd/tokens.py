@@ -372,6 +372,9 @@ def token_log_probs(
     and nothing of the row is read.  A logit of -inf is an action that cannot
     be taken.  Both results are differentiable once in the logits
     (create_graph raises)."""
+    got = _native().token_log_probs(logits, actions, mask, temperature, entropy)
+    if got is not None:
+        return got
     _check_logits(logits, temperature)
     _check_actions(logits, actions, mask)
     if _wants_gradient(logits):
@@ -443,6 +446,12 @@ def token_policy_loss(
     and forms it anew from the logits if not, which costs another pass and
     gives the same: either is rounded once."""
     clip_high = clip_low if clip_high is None else clip_high
+    got = _native().token_policy_loss(
+        logits, actions, old_log_probs, advantages, ref_log_probs, mask, clip_low, clip_high,
+        kl_coef, entropy_coef, temperature, _lib.TOKEN_REDUCTIONS.get(reduction), denominator,
+        grad_scale)
+    if got is not None:
+        return got[0], TokenStats(zip(_lib.TOKEN_SCALAR_NAMES, got[1]))
     per_sequence = _check_policy(logits, actions, old_log_probs, advantages, ref_log_probs, mask,
                                  clip_low, clip_high, kl_coef, entropy_coef, temperature)
     _check_weights(reduction, denominator, grad_scale)
@@ -499,6 +508,10 @@ def preference_loss(
     the rewards beta times the log ratios, reported values.  Sums over tokens
     are formed in 64 bits from differences rounded once, so the policy may lie
     close to its reference."""
+    got = _native().preference_loss(logits, actions, ref_log_probs, mask, beta, label_smoothing,
+                                    margin, average, temperature)
+    if got is not None:
+        return got[0], PreferenceStats(zip(("chosen", "rejected"), got[1]))
     _check_preference(logits, actions, ref_log_probs, mask, beta, label_smoothing, margin,
                       temperature)
     if _wants_gradient(logits):
@@ -546,6 +559,11 @@ def distillation_loss(
     one id add up; an id from A on gives NaN; a row without entries adds 0 to
     the loss and counts.  mask, reduction, denominator and grad_scale are
     token_policy_loss's.  Differentiable once in the student's logits alone."""
+    got = _native().distillation_loss(logits, teacher_logits, teacher_ids, mask, temperature,
+                                      _lib.TOKEN_REDUCTIONS.get(reduction), denominator,
+                                      grad_scale)
+    if got is not None:
+        return got
     _check_distillation(logits, teacher_logits, teacher_ids, mask, temperature)
     _check_weights(reduction, denominator, grad_scale)
     if _wants_gradient(teacher_logits):
@@ -563,6 +581,9 @@ def top_logits(logits: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor
     256.  Equal logits come in the order of their columns (0 and -0 are equal),
     NaN before everything, as torch.sort(descending=True, stable=True) puts
     them.  A up to 2^22.  Not differentiable."""
+    got = _native().top_logits(logits, k)
+    if got is not None:
+        return got
     _check_logits(logits, 1.0)
     A = logits.shape[-1]
     if not isinstance(k, int) or isinstance(k, bool):
