@@ -27,40 +27,29 @@ struct Teacher {
   }
 };
 
-// The K entries of a row over G lanes (16, or a wave).
-template <int G>
-struct Entries {
-  static constexpr int kN = kMaxK / G;
-  int col[kN];
-  float t[kN];     // the teacher's logits
-  float m, s;      // their largest, and the sum of 2^(c (t - m))
-  float q[kN];
-
-  __device__ __forceinline__ Entries(const Teacher& teacher, int64_t r, int A, float c, int lane) {
-    m = kNegInf;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int k = i * G + lane;
-      col[i] = k < teacher.K ? teacher.column(r, k, A) : -1;
-      t[i] = col[i] >= 0 ? teacher.logit(r, k) : col[i] == -1 ? kNegInf : PPO_NAN;
-      m = fmaxf(m, t[i]);
-    }
-    m = lanes_max<G>(m);
-    // (no entries, or none but -inf: all q are 0)
-    const float base = m == kNegInf ? 0.0f : m;
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      q[i] = exp2_fast((t[i] - base) * c);
-      s += q[i];
-    }
-    s = lanes_sum<G>(s);
-    const float inv = s == 0.0f ? 0.0f : 1.0f / s;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) q[i] *= inv;
+// A row's entries in LDS, K of each: column, q, the sum of q over the column's entries,
+// and the student's logit there.
+struct Board {
+  int* col;
+  float *q, *sum, *l;
+  __device__ __forceinline__ Board(int* p, int K, int group) {
+    const int per = (K + 3) & ~3;
+    col = p + group * 4 * per;
+    q = reinterpret_cast<float*>(col) + per;
+    sum = q + per;
+    l = sum + per;
   }
-  // 1, 0 without entries, NaN with one that is not finite.
-  __device__ __forceinline__ float total() const { return s == 0.0f ? 0.0f : s / s; }
+};
+size_t board_bytes(int K, int groups) { return (size_t)groups * 4 * round_up(K, 4) * 4; }
+
+// What the entries come to: sum q (1; 0 without entries; NaN with one that is not finite)
+// and the loss but for the student's m and log s:
+//   sum_k q_k (log q_k - log p_k) = c ln 2 (gap + total (m - top)) + log s - log_s.
+struct Entries {
+  float total, gap, top, log_s;
+  __device__ __forceinline__ float loss(float m, float s_log, float c) const {
+    return total == 0.0f ? 0.0f : fmaf(c * kLn2, gap + (m - top), s_log - log_s);
+  }
 };
 
 // log s, in 64 bits up to its rounding.
@@ -74,44 +63,72 @@ __device__ __forceinline__ float log_of(float s) {
   return (float)fma((double)n, kLn2d, twice_atanh((double)f - 1.0, (double)f + 1.0));
 }
 
-// sum_k q_k (log q_k - log p_k) of the row, in every lane.
+// The entries of row r, by G lanes of one wave (whose LDS accesses are in order), while
+// the row itself is on its way.
 template <class T, int G>
-__device__ __forceinline__ float row_loss(const Entries<G>& e, const T* row, float m, float s,
-                                          float c) {
-  float x = 0.0f;
-#pragma unroll
-  for (int i = 0; i < Entries<G>::kN; ++i)
-    if (e.col[i] != -1 && e.q[i] != 0.0f) {
-      const float l = e.col[i] >= 0 ? to_f32(row[e.col[i]]) : PPO_NAN;
-      x = fmaf(e.q[i], (e.t[i] - e.m) - (l - m), x);
+__device__ __forceinline__ Entries take_entries(const Teacher& teacher, int64_t r, const T* row,
+                                                int A, float c, int lane, const Board& b) {
+  const int K = teacher.K;
+  float m = kNegInf, top = kNegInf;
+  for (int k = lane; k < K; k += G) {
+    const int col = teacher.column(r, k, A);
+    const float t = col >= 0 ? teacher.logit(r, k) : col == -1 ? kNegInf : PPO_NAN;
+    const float l = col >= 0 ? to_f32(row[col]) : kNegInf;
+    b.col[k] = col;
+    b.q[k] = t;
+    b.l[k] = l;
+    m = fmaxf(m, t);
+    top = fmaxf(top, l);
+  }
+  for (int k = K + lane; k < ((K + 3) & ~3); k += G) b.col[k] = -1;
+  m = lanes_max<G>(m);
+  top = lanes_max<G>(top);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  // (no entries, or none but -inf: all q are 0)
+  const float base = m == kNegInf ? 0.0f : m;
+  if (top == kNegInf) top = 0.0f;
+  float s = 0.0f, gap = 0.0f;
+  for (int k = lane; k < K; k += G) {
+    const float t = b.q[k] - base, q = exp2_fast(t * c);
+    s += q;
+    // (an entry that weighs nothing adds nothing, whatever its logits)
+    if (q != 0.0f) gap = fmaf(q, t - (b.l[k] - top), gap);
+    b.q[k] = q;
+  }
+  s = lanes_sum<G>(s);
+  gap = lanes_sum<G>(gap);
+  const float inv = s == 0.0f ? 0.0f : 1.0f / s;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int k = lane; k < K; k += G) b.q[k] *= inv;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  // Entries of one column write its sum, all of them.  Such are rare: they are looked for
+  // four at a time, and summed only where there are any.
+  for (int k = lane; k < K; k += G) {
+    const int col = b.col[k];
+    float q = b.q[k];
+    int same = 0;
+    for (int i = 0; i < K; i += 4) {
+      const v4i four = *reinterpret_cast<const v4i*>(b.col + i);
+      same += (four[0] == col) + (four[1] == col) + (four[2] == col) + (four[3] == col);
     }
-  x = lanes_sum<G>(x);
-  return e.s == 0.0f ? 0.0f : fmaf(c * kLn2, x, log_of(s) - log_of(e.s));
+    if (col >= 0 && same > 1) {
+      q = 0.0f;
+      for (int i = 0; i < K; ++i) q += b.col[i] == col ? b.q[i] : 0.0f;
+    }
+    b.sum[k] = q;
+  }
+  return {s == 0.0f ? 0.0f : s / s, gap * inv, top, s == 0.0f ? 0.0f : log_of(s)};
 }
 
-// Writes the entries' columns: tau w (p - q), q summed over entries of one column
-// (each of them writes the same value).
-template <class T, int G>
-__device__ __forceinline__ void write_entries(const Entries<G>& e, const T* row, T* out, int K,
-                                              float m, float inv_s, float c, float W, int lane,
-                                              float* s_q, int* s_col) {
-#pragma unroll
-  for (int i = 0; i < Entries<G>::kN; ++i) {
-    const int k = i * G + lane;
-    if (k < K) {
-      s_q[k] = e.q[i];
-      s_col[k] = e.col[i];
+// The entries' columns: tau w (p - q).
+template <class T>
+__device__ __forceinline__ void write_entries(const Board& b, int K, float m, float inv_s, float c,
+                                              float W, T* out, int t, int lanes) {
+  for (int k = t; k < K; k += lanes)
+    if (b.col[k] >= 0) {
+      const float p = exp2_fast((b.l[k] - m) * c) * inv_s;
+      out[b.col[k]] = from_f32<T>(W * (p - b.sum[k]));
     }
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (one wave's LDS is in order)
-#pragma unroll
-  for (int i = 0; i < Entries<G>::kN; ++i) {
-    if (i * G >= K || e.col[i] < 0) continue;
-    float q = 0.0f;
-    for (int k = 0; k < K; ++k) q += s_col[k] == e.col[i] ? s_q[k] : 0.0f;
-    const float p = exp2_fast((to_f32(row[e.col[i]]) - m) * c) * inv_s;
-    out[e.col[i]] = from_f32<T>(W * (p - q));
-  }
 }
 
 struct Distill {
@@ -127,15 +144,22 @@ struct Distill {
   }
 };
 
+// A row's scalars, from its first wave to the others.
+struct RowShare {
+  Grad g;
+  float inv_s, W;
+};
+
 template <class T, int G, int V>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) distill_kernel(Rows rows, Distill d, T* dlogits) {
-  constexpr int kBlock = G < 256 ? 256 : G, kGroups = kBlock / G;
-  constexpr int kTeam = G < kWave ? G : kWave;
+__global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
+    distill_kernel(Rows rows, Distill d, T* dlogits) {
+  constexpr int kBlock = kRowBlock<G>, kGroups = kBlock / G;
+  constexpr int kTeam = G < kWave ? G : kWave;  // the lanes that take the entries
+  extern __shared__ int s_board[];
   __shared__ Stat s_part[kBlock / kWave];
-  __shared__ Grad s_grad;
-  __shared__ float s_q[kGroups][kMaxK];
-  __shared__ int s_col[kGroups][kMaxK];
-  const int t = threadIdx.x % G, group = group_of<G>();
+  __shared__ RowShare s_row;
+  const int t = threadIdx.x % G, group = group_of<G>(), K = d.teacher.K;
+  const Board board(s_board, K, group);
   double sums[1] = {};
   const float inverse = inverse_count(d.weights);
   for (int64_t r = (int64_t)blockIdx.x * kGroups + group; r < rows.n;
@@ -147,47 +171,42 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) distill_kernel(Rows rows, D
     }
     const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
     RowRegs<T, G, V> x(row, rows.A, t);
+    Entries e = {};
+    if (G <= kWave || threadIdx.x < kWave)
+      e = take_entries<T, kTeam>(d.teacher, r, row, rows.A, rows.c, t, board);
     x.take_out(-1, t);
     Stat st = x.template stat<false>(rows.c);
-    Grad g;
-    // (the first wave of the row's lanes takes the entries)
-    const float W = d.tau * row_weight(d.weights, inverse, r / rows.T);
-    auto finish = [&](const Entries<kTeam>& e) {
-      const float loss = row_loss<T, kTeam>(e, row, st.m, st.s, rows.c);
-      g = {st.m, W * d.grad_scale * e.total() * (1.0f / st.s), 0.0f, 0.0f, -1};
+    RowShare share;
+    auto finish = [&] {
+      const float W = d.tau * row_weight(d.weights, inverse, r / rows.T), inv_s = 1.0f / st.s;
+      share = {{st.m, W * d.grad_scale * e.total * inv_s, 0.0f, 0.0f, -1}, inv_s, W * d.grad_scale};
       if (t == 0) {
-        sums[0] += (double)W * loss;
-        d.leave(r, st.m, st.s, W, e.total());
+        sums[0] += (double)W * e.loss(st.m, log_of(st.s), rows.c);
+        d.leave(r, st.m, st.s, W, e.total);
       }
     };
-    auto fix = [&](const Entries<kTeam>& e) {
-      write_entries<T, kTeam>(e, row, out, d.teacher.K, st.m, 1.0f / st.s, rows.c, W * d.grad_scale,
-                              t, s_q[group], s_col[group]);
-    };
-    if constexpr (G > kWave) {
+    if (G > kWave) {
       st = block_join<false>(st, rows.c, s_part);
       if (threadIdx.x < kWave) {
-        const Entries<kTeam> e(d.teacher, r, rows.A, rows.c, t);
-        finish(e);
-        if (t == 0) s_grad = g;
+        finish();
+        if (t == 0) s_row = share;
       }
       lds_barrier();
-      g = s_grad;
-      if (dlogits) {
-        x.template write<false>(g, rows.c, out, t);
-        __syncthreads();  // (the whole row is written before the entries' columns)
-        if (threadIdx.x < kWave) fix(Entries<kTeam>(d.teacher, r, rows.A, rows.c, t));
-      }
+      share = s_row;
     } else {
       st = lanes_join<kTeam, false>(st, rows.c);
-      const Entries<kTeam> e(d.teacher, r, rows.A, rows.c, t);
-      finish(e);
-      if (dlogits) {
-        x.template write<false>(g, rows.c, out, t);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        fix(e);
-      }
+      finish();
     }
+    if (!dlogits) continue;
+    x.template write<false>(share.g, rows.c, out, t);
+    // (the row is written before the entries' columns)
+    if (G > kWave)
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    write_entries<T>(board, K, share.g.m, share.inv_s, rows.c, share.W, out, t, G);
+    // (wave 0's next entries wait for the others to have read these)
+    if (G > kWave) lds_barrier();
   }
   leave_sums(sums, d.sums);
 }
@@ -198,14 +217,14 @@ struct DistillJoin {
   double sums[1];
   __device__ __forceinline__ void masked(int64_t) const {}
   template <class T>
-  __device__ __forceinline__ void row(const Rows& rows, int64_t r, const T* row, Stat x,
-                                      int lane) {
-    const Entries<kWave> e(d.teacher, r, rows.A, rows.c, lane);
+  __device__ __forceinline__ void row(const Rows& rows, int64_t r, const T* row, Stat x, int lane) {
+    __shared__ int s_board[4 * kMaxK];
+    const Entries e = take_entries<T, kWave>(d.teacher, r, row, rows.A, rows.c, lane,
+                                             Board(s_board, d.teacher.K, 0));
     const float W = d.tau * row_weight(d.weights, inverse_count(d.weights), r / rows.T);
-    const float loss = row_loss<T, kWave>(e, row, x.m, x.s, rows.c);
     if (lane != 0) return;
-    sums[0] += (double)W * loss;
-    d.leave(r, x.m, x.s, W, e.total());
+    sums[0] += (double)W * e.loss(x.m, log_of(x.s), rows.c);
+    d.leave(r, x.m, x.s, W, e.total);
   }
   __device__ __forceinline__ void end() { leave_sums(sums, d.sums); }
 };
@@ -224,18 +243,20 @@ template <class T>
 __global__ void __launch_bounds__(64) entries_kernel(Rows rows, Teacher teacher, const Saved* saved,
                                                      const float* scale, float held,
                                                      float grad_scale, T* dlogits) {
-  __shared__ float s_q[kMaxK];
-  __shared__ int s_col[kMaxK];
+  __shared__ int s_board[4 * kMaxK];
   const float up = scale ? *scale : 1.0f;
   if (held != 0.0f && up == held) return;
   const int lane = threadIdx.x;
+  const Board board(s_board, teacher.K, 0);
   for (int64_t r = blockIdx.x; r < rows.n; r += gridDim.x) {
     if (!rows.live(r)) continue;
     const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
     const Saved s = saved[r];
-    const Entries<kWave> e(teacher, r, rows.A, rows.c, lane);
-    write_entries<T, kWave>(e, row, dlogits + r * rows.A, teacher.K, s.m, s.inv_s, rows.c,
-                            up * grad_scale * s.weight, lane, s_q, s_col);
+    take_entries<T, kWave>(teacher, r, row, rows.A, rows.c, lane, board);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    write_entries<T>(board, teacher.K, s.m, s.inv_s, rows.c, up * grad_scale * s.weight,
+                     dlogits + r * rows.A, lane, kWave);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -269,10 +290,10 @@ int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits
   const int64_t chunks = chunks_of(rows.A, dtype);
   auto go = [&](auto lanes, auto held) {
     constexpr int G = decltype(lanes)::value, V = decltype(held)::value;
-    constexpr int kBlock = G < 256 ? 256 : G;
+    constexpr int kBlock = kRowBlock<G>;
     partials = launch_blocks(div_up(rows.n, kBlock / G), kMaxPartials);
-    hipLaunchKernelGGL((distill_kernel<T, G, V>), dim3(partials), dim3(kBlock), 0, stream, rows, d,
-                       dlogits);
+    hipLaunchKernelGGL((distill_kernel<T, G, V>), dim3(partials), dim3(kBlock),
+                       board_bytes(d.teacher.K, kBlock / G), stream, rows, d, dlogits);
     return last_launch_status();
   };
   return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {

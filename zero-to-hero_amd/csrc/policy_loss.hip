@@ -75,8 +75,9 @@ __device__ __forceinline__ void leave_masked(const Policy& p, const Rows& rows, 
 }
 
 template <class T, int G, int V, bool kC>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) policy_kernel(Rows rows, Policy p, T* dlogits) {
-  constexpr int kBlock = G < 256 ? 256 : G, kGroups = kBlock / G;
+__global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
+    policy_kernel(Rows rows, Policy p, T* dlogits) {
+  constexpr int kBlock = kRowBlock<G>, kGroups = kBlock / G;
   __shared__ Stat s_part[kBlock / kWave];
   __shared__ Grad s_grad;
   __shared__ double s_sums[kSums];
@@ -216,7 +217,7 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
   const bool grad_entropy = p.entropy_coef != 0.0f;
   auto go = [&](auto lanes, auto held) {
     constexpr int G = decltype(lanes)::value, V = decltype(held)::value;
-    constexpr int kBlock = G < 256 ? 256 : G;
+    constexpr int kBlock = kRowBlock<G>;
     partials = launch_blocks(div_up(rows.n, kBlock / G), kMaxPartials);
     if (grad_entropy)
       hipLaunchKernelGGL((policy_kernel<T, G, V, true>), dim3(partials), dim3(kBlock), 0, stream,

@@ -358,8 +358,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_buffer(const void* p, in
 }
 constexpr int kPastCaches = 2;  // the buffer instructions' nt bit
 
-// A row, V chunks a lane (V G of them hold it), straight through: no branch in any
-// pass over them.
+// A row, V chunks a lane: between V G / 2 and V G of them hold it.  The loads go
+// straight through; a pass over the chunks leaves out the rounds of G that lie behind
+// the last, of which there may be some in the second half (`reaches`).
 template <class T, int G, int V>
 struct RowRegs {
   static constexpr int kN = kPer16<T>;
@@ -381,6 +382,11 @@ struct RowRegs {
         raw[i] = __builtin_nontemporal_load(body + i * G + t);
     end_col = t < cut.ends ? cut.end_column(t) : -1;
     end = end_col >= 0 ? to_f32(row[end_col]) : kNegInf;
+  }
+
+  // (at 128 registers to a lane the branches spill; those layouts come in finer steps)
+  __device__ __forceinline__ bool reaches(int i) const {
+    return G >= 512 || i < V / 2 || i * G < cut.nvec;
   }
 
   // The compiler would unpack 16-bit chunks once and keep them so, in twice the
@@ -410,6 +416,7 @@ struct RowRegs {
     float m = end;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      if (!reaches(i)) continue;
       turn(i, m);
 #pragma unroll
       for (int j = 0; j < kN; ++j) m = fmaxf(m, unpack<T>(raw[i], j));
@@ -426,6 +433,7 @@ struct RowRegs {
     add(end, x.s);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      if (!reaches(i)) continue;
       turn(i, x.s);
 #pragma unroll
       for (int j = 0; j < kN; j += 2) {
@@ -445,6 +453,7 @@ struct RowRegs {
     const auto buf = chunk_buffer(body, kBuffer ? cut.nvec : 0);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      if (!reaches(i)) continue;
       float d[kN];
       turn(i, last);
 #pragma unroll

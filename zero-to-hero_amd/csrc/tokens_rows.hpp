@@ -230,6 +230,14 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
 // lane) for the smallest group that holds a row, or split() where a row does not
 // fit, or rows are so few that one workgroup to each would leave most of the chip
 // empty, or the gradients lie otherwise in 16 bytes than the logits (not `alike`).
+// A pass's workgroup, and the waves a SIMD is to hold at least: two workgroups of 512
+// lanes (65536 bf16 218 -> 214 us, 50304 198 -> 187); smaller ones do better with the
+// registers (32768 191 us, 211 with four waves to a SIMD).
+template <int G>
+constexpr int kRowBlock = G < 256 ? 256 : G;
+template <int G>
+constexpr int kRowWaves = G >= 512 ? 4 : 1;
+
 // (without gradients: as if they started at a multiple of 16, so that a loss has the
 // same bits with and without them where its caller allocates them so)
 inline bool lies_alike(const void* logits, const void* dlogits) {
@@ -242,17 +250,15 @@ int with_row_shape(int64_t rows, int64_t chunks, bool alike, Held&& held, Split&
   if (chunks <= 16 * 4) return held(Int<16>{}, Int<4>{});
   if (chunks <= 64 * 4) return held(Int<64>{}, Int<4>{});
   if (chunks <= 64 * 8) return held(Int<64>{}, Int<8>{});
-  if (rows < 64 && chunks > 2048) return split();
-  if (chunks <= 256 * 4) return held(Int<256>{}, Int<4>{});
-  if (chunks <= 256 * 6) return held(Int<256>{}, Int<6>{});
+  if (chunks <= 64 * 16) return held(Int<64>{}, Int<16>{});
+  if (rows < 64 && chunks > 256 * 8) return split();
   if (chunks <= 256 * 8) return held(Int<256>{}, Int<8>{});
-  if (chunks <= 512 * 6) return held(Int<512>{}, Int<6>{});
-  if (chunks <= 512 * 8) return held(Int<512>{}, Int<8>{});
-  if (chunks <= 1024 * 6) return held(Int<1024>{}, Int<6>{});
-  if (chunks <= 1024 * 8) return held(Int<1024>{}, Int<8>{});
+  if (chunks <= 256 * 16) return held(Int<256>{}, Int<16>{});
+  if (chunks <= 512 * 10) return held(Int<512>{}, Int<10>{});
+  if (chunks <= 512 * 13) return held(Int<512>{}, Int<13>{});
+  if (chunks <= 512 * 16) return held(Int<512>{}, Int<16>{});
   if (chunks <= 1024 * 10) return held(Int<1024>{}, Int<10>{});
-  if (chunks <= 1024 * 12) return held(Int<1024>{}, Int<12>{});
-  if (chunks <= 1024 * 14) return held(Int<1024>{}, Int<14>{});
+  if (chunks <= 1024 * 13) return held(Int<1024>{}, Int<13>{});
   if (chunks <= 1024 * 16) return held(Int<1024>{}, Int<16>{});
   return split();
 }
