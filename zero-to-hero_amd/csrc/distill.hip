@@ -32,15 +32,15 @@ struct Teacher {
 struct Board {
   int* col;
   float *q, *sum, *l;
-  __device__ __forceinline__ Board(int* p, int K, int group) {
+  __device__ __forceinline__ Board(int* p, int K, int place) {
     const int per = (K + 3) & ~3;
-    col = p + group * 4 * per;
+    col = p + place * 4 * per;
     q = reinterpret_cast<float*>(col) + per;
     sum = q + per;
     l = sum + per;
   }
 };
-size_t board_bytes(int K, int groups) { return (size_t)groups * 4 * round_up(K, 4) * 4; }
+size_t board_bytes(int K, int boards) { return (size_t)boards * 4 * round_up(K, 4) * 4; }
 
 // What the entries come to: sum q (1; 0 without entries; NaN with one that is not finite)
 // and the loss but for the student's m and log s:
@@ -150,35 +150,52 @@ struct RowShare {
   float inv_s, W;
 };
 
+// The columns of a row's entries come after the whole row is written.  A workgroup's
+// first wave puts them off until the next row's barrier, before which every wave has
+// waited for its stores (its loads of that row, which follow them, are in by then), so
+// that no wave waits for memory between two rows; there are two boards for that.
 template <class T, int G, int V>
 __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
-    distill_kernel(Rows rows, Distill d, T* dlogits) {
+    distill_kernel(Rows rows, Distill d, Order order, T* dlogits) {
   constexpr int kBlock = kRowBlock<G>, kGroups = kBlock / G;
   constexpr int kTeam = G < kWave ? G : kWave;  // the lanes that take the entries
   extern __shared__ int s_board[];
   __shared__ Stat s_part[kBlock / kWave];
   __shared__ RowShare s_row;
   const int t = threadIdx.x % G, group = group_of<G>(), K = d.teacher.K;
-  const Board board(s_board, K, group);
+  int place = group;
+  const T* before = nullptr;  // the row whose entries are still to be written, and its terms
+  RowShare of_before;
   double sums[1] = {};
   const float inverse = inverse_count(d.weights);
-  for (int64_t r = (int64_t)blockIdx.x * kGroups + group; r < rows.n;
-       r += (int64_t)gridDim.x * kGroups) {
+  const T* logits = static_cast<const T*>(rows.logits);
+  const Walk<G> walk(rows, order, (int64_t)gridDim.x * kGroups);
+  auto dead = [&](int64_t r) {
+    if (dlogits) write_zeros<T, G>(dlogits + r * rows.A, rows.A, t);
+  };
+  int64_t i = walk.from((int64_t)blockIdx.x * kGroups + group, dead);
+  int64_t r = i < rows.n ? walk.row(i) : -1;
+  auto row_at = [&](int64_t k) { return k >= 0 ? logits + k * rows.A : nullptr; };
+  auto flush = [&](const T* row, const RowShare& s, int at) {
+    write_entries<T>(Board(s_board, K, at), K, s.g.m, s.inv_s, rows.c, s.W,
+                     dlogits + (row - logits), t, kTeam);
+  };
+  RowRegs<T, G, V> x(row_at(r), rows.A, t);
+  while (r >= 0) {
     T* out = dlogits + r * rows.A;
-    if (!rows.live(r)) {
-      if (dlogits) write_zeros<T, G>(out, rows.A, t);
-      continue;
-    }
-    const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
-    RowRegs<T, G, V> x(row, rows.A, t);
+    const T* row = logits + r * rows.A;
+    const Board board(s_board, K, place);
     Entries e = {};
     if (G <= kWave || threadIdx.x < kWave)
       e = take_entries<T, kTeam>(d.teacher, r, row, rows.A, rows.c, t, board);
+    const float W = d.tau * row_weight(d.weights, inverse, r / rows.T);
+    i = walk.from(i + walk.step, dead);
+    const int64_t next = i < rows.n ? walk.row(i) : -1;
     x.take_out(-1, t);
     Stat st = x.template stat<false>(rows.c);
     RowShare share;
     auto finish = [&] {
-      const float W = d.tau * row_weight(d.weights, inverse, r / rows.T), inv_s = 1.0f / st.s;
+      const float inv_s = 1.0f / st.s;
       share = {{st.m, W * d.grad_scale * e.total * inv_s, 0.0f, 0.0f, -1}, inv_s, W * d.grad_scale};
       if (t == 0) {
         sums[0] += (double)W * e.loss(st.m, log_of(st.s), rows.c);
@@ -186,10 +203,12 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
       }
     };
     if (G > kWave) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       st = block_join<false>(st, rows.c, s_part);
       if (threadIdx.x < kWave) {
         finish();
         if (t == 0) s_row = share;
+        if (before) flush(before, of_before, 1 - place);
       }
       lds_barrier();
       share = s_row;
@@ -197,16 +216,27 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
       st = lanes_join<kTeam, false>(st, rows.c);
       finish();
     }
-    if (!dlogits) continue;
-    x.template write<false>(share.g, rows.c, out, t);
-    // (the row is written before the entries' columns)
-    if (G > kWave)
-      __syncthreads();
-    else
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    write_entries<T>(board, K, share.g.m, share.inv_s, rows.c, share.W, out, t, G);
-    // (wave 0's next entries wait for the others to have read these)
-    if (G > kWave) lds_barrier();
+    share = {shared_by<G>(share.g), shared_by<G>(share.inv_s), shared_by<G>(share.W)};
+    if (dlogits) {
+      if (kRowAfterRow<G>)
+        x.template write<false>(share.g, rows.c, out, rows.A, t, row_at(next));
+      else
+        x.template write<false>(share.g, rows.c, out, rows.A, t);
+      if (G > kWave) {
+        before = row;
+        of_before = share;
+        place = 1 - place;
+      } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        flush(row, share, place);
+      }
+    }
+    if (!dlogits || !kRowAfterRow<G>) x = RowRegs<T, G, V>(row_at(next), rows.A, t);
+    r = next;
+  }
+  if (G > kWave) {
+    __syncthreads();
+    if (before && threadIdx.x < kWave) flush(before, of_before, 1 - place);
   }
   leave_sums(sums, d.sums);
 }
@@ -291,15 +321,19 @@ int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits
   auto go = [&](auto lanes, auto held) {
     constexpr int G = decltype(lanes)::value, V = decltype(held)::value;
     constexpr int kBlock = kRowBlock<G>;
-    partials = launch_blocks(div_up(rows.n, kBlock / G), kMaxPartials);
+    partials = launch_blocks(div_up(rows.n, kBlock / G), kRowBlocks<G>);
+    Order order = {};
+    if (kRowAfterRow<G> && rows.mask) order = take_order(rows, s, stream);
     hipLaunchKernelGGL((distill_kernel<T, G, V>), dim3(partials), dim3(kBlock),
-                       board_bytes(d.teacher.K, kBlock / G), stream, rows, d, dlogits);
+                       board_bytes(d.teacher.K, std::max(2, kBlock / G)), stream, rows, d, order,
+                       dlogits);
     return last_launch_status();
   };
   return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
     const DistillJoin join = {d, {}};
     partials = launch_blocks(rows.n, kMaxPartials);
-    if (const int code = launch_statistics<T, false, false>(rows, s, join, stream)) return code;
+    if (const int code = launch_statistics<T, false, false>(rows, s, join, true, stream))
+      return code;
     if (!dlogits) return (int)PPO_OK;
     return dense_gradient<T>(rows, d.teacher, d.saved, nullptr, 0.0f, d.grad_scale, dlogits, stream);
   });

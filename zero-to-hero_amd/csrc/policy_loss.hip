@@ -41,23 +41,33 @@ __device__ __forceinline__ float kl_estimate(float d) {
   return d * d * q;
 }
 
+// A row's inputs beside its logits.
+struct RowIn {
+  float old, adv, ref, w;
+};
+__device__ __forceinline__ RowIn row_in(const Policy& p, const Rows& rows, int64_t r,
+                                        float inverse) {
+  const int64_t seq = r / rows.T;
+  return {p.old[r], p.adv[p.per_sequence ? seq : r], p.ref ? p.ref[r] : 0.0f,
+          row_weight(p.weights, inverse, seq)};
+}
+
 // The row's loss, its gradient's terms G and E for an incoming gradient of 1.
-__device__ __forceinline__ RowLoss policy_row(const Policy& p, const Rows& rows, int64_t r, float w,
-                                              const RowTerms& t, float& G, float& E) {
-  const float old = p.old[r], adv = p.adv[p.per_sequence ? r / rows.T : r];
-  const float ratio = expf((float)(t.lp - (double)old));
+__device__ __forceinline__ RowLoss policy_row(const Policy& p, const RowIn& in, const RowTerms& t,
+                                              float& G, float& E) {
+  const float ratio = expf((float)(t.lp - (double)in.old));
   const float clipped = ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio;
-  const float u = ratio * adv, v = clipped * adv;
-  RowLoss o = {w, -(u > v ? v : u), 0.0f, t.H, (float)((double)old - t.lp),
+  const float u = ratio * in.adv, v = clipped * in.adv;
+  RowLoss o = {in.w, -(u > v ? v : u), 0.0f, t.H, (float)((double)in.old - t.lp),
                ratio < p.lo || ratio > p.hi ? 1.0f : 0.0f};
   G = u > v ? 0.0f : -u;
   if (p.ref) {
-    const float d = (float)((double)p.ref[r] - t.lp);
+    const float d = (float)((double)in.ref - t.lp);
     o.kl = kl_estimate(d);
     if (p.kl_coef != 0.0f) G -= p.kl_coef * (o.kl + d);  // (e^d - 1)
   }
-  G *= w;
-  E = -p.entropy_coef * w;
+  G *= in.w;
+  E = -p.entropy_coef * in.w;
   return o;
 }
 
@@ -76,7 +86,7 @@ __device__ __forceinline__ void leave_masked(const Policy& p, const Rows& rows, 
 
 template <class T, int G, int V, bool kC>
 __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
-    policy_kernel(Rows rows, Policy p, T* dlogits) {
+    policy_kernel(Rows rows, Policy p, Order order, T* dlogits) {
   constexpr int kBlock = kRowBlock<G>, kGroups = kBlock / G;
   __shared__ Stat s_part[kBlock / kWave];
   __shared__ Grad s_grad;
@@ -85,26 +95,30 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
   double sums[kSums] = {};
   const float inverse = inverse_count(p.weights);
   if (G > kWave && threadIdx.x < kSums) s_sums[threadIdx.x] = 0.0;
-  for (int64_t r = (int64_t)blockIdx.x * kGroups + group_of<G>(); r < rows.n;
-       r += (int64_t)gridDim.x * kGroups) {
-    T* out = dlogits + r * rows.A;
-    if (!rows.live(r)) {
-      if (dlogits) write_zeros<T, G>(out, rows.A, t);
-      if (t == 0) leave_masked(p, rows, r);
-      continue;
-    }
-    const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
-    const int a = rows.action(r);
-    const float la = action_logit(row, a);
-    RowRegs<T, G, V> x(row, rows.A, t);
+  const T* logits = static_cast<const T*>(rows.logits);
+  const Walk<G> walk(rows, order, (int64_t)gridDim.x * kGroups);
+  auto dead = [&](int64_t r) {
+    if (dlogits) write_zeros<T, G>(dlogits + r * rows.A, rows.A, t);
+    if (t == 0) leave_masked(p, rows, r);
+  };
+  int64_t i = walk.from((int64_t)blockIdx.x * kGroups + group_of<G>(), dead);
+  int64_t r = i < rows.n ? walk.row(i) : -1;
+  auto row_at = [&](int64_t k) { return k >= 0 ? logits + k * rows.A : nullptr; };
+  RowRegs<T, G, V> x(row_at(r), rows.A, t);
+  int a = r >= 0 ? rows.action(r) : -1;
+  while (r >= 0) {
+    const float la = action_logit(logits + r * rows.A, a);
+    const RowIn in = row_in(p, rows, r, inverse);
+    i = walk.from(i + walk.step, dead);
+    const int64_t next = i < rows.n ? walk.row(i) : -1;
+    const int next_a = next >= 0 ? rows.action(next) : -1;
     x.take_out(a, t);
     Stat st = x.template stat<true>(rows.c);
     Grad g;
     auto finish = [&](double(&to)[kSums]) {
       const RowTerms terms = row_terms<true>(st, la, rows.c);
       float gl, ge;
-      const float w = row_weight(p.weights, inverse, r / rows.T);
-      const RowLoss loss = policy_row(p, rows, r, w, terms, gl, ge);
+      const RowLoss loss = policy_row(p, in, terms, gl, ge);
       if (t == 0) {
         loss.add_to(to);
         leave_row(p, rows, r, terms, gl, ge);
@@ -123,7 +137,15 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
       st = lanes_join<G <= kWave ? G : kWave, true>(st, rows.c);
       finish(sums);
     }
-    if (dlogits) x.template write<kC>(g, rows.c, out, t);
+    g = shared_by<G>(g);
+    if (dlogits && kRowAfterRow<G>)
+      x.template write<kC>(g, rows.c, dlogits + r * rows.A, rows.A, t, row_at(next));
+    else {
+      if (dlogits) x.template write<kC>(g, rows.c, dlogits + r * rows.A, rows.A, t);
+      x = RowRegs<T, G, V>(row_at(next), rows.A, t);
+    }
+    r = next;
+    a = next_a;
   }
   if (G <= kWave) {
     leave_sums(sums, p.sums);
@@ -148,8 +170,8 @@ struct PolicyJoin {
   __device__ __forceinline__ void row(const Rows& rows, int64_t r, Stat x, float la, bool first) {
     const RowTerms t = row_terms<kEntropy>(x, la, rows.c);
     float G, E;
-    const float w = row_weight(p.weights, inverse_count(p.weights), r / rows.T);
-    const RowLoss loss = policy_row(p, rows, r, w, t, G, E);
+    const RowLoss loss =
+        policy_row(p, row_in(p, rows, r, inverse_count(p.weights)), t, G, E);
     if (!first) return;
     loss.add_to(sums);
     leave_row(p, rows, r, t, G, E);
@@ -218,19 +240,22 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
   auto go = [&](auto lanes, auto held) {
     constexpr int G = decltype(lanes)::value, V = decltype(held)::value;
     constexpr int kBlock = kRowBlock<G>;
-    partials = launch_blocks(div_up(rows.n, kBlock / G), kMaxPartials);
+    partials = launch_blocks(div_up(rows.n, kBlock / G), kRowBlocks<G>);
+    Order order = {};
+    if (kRowAfterRow<G> && rows.mask) order = take_order(rows, s, stream);
     if (grad_entropy)
       hipLaunchKernelGGL((policy_kernel<T, G, V, true>), dim3(partials), dim3(kBlock), 0, stream,
-                         rows, p, dlogits);
+                         rows, p, order, dlogits);
     else
       hipLaunchKernelGGL((policy_kernel<T, G, V, false>), dim3(partials), dim3(kBlock), 0, stream,
-                         rows, p, dlogits);
+                         rows, p, order, dlogits);
     return last_launch_status();
   };
   return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
     PolicyJoin join = {p, {}, rows.n};
     partials = launch_blocks(rows.n, kMaxPartials);
-    if (const int code = launch_statistics<T, true, false>(rows, s, join, stream)) return code;
+    if (const int code = launch_statistics<T, true, false>(rows, s, join, true, stream))
+      return code;
     if (!dlogits) return (int)PPO_OK;
     const PolicyGrad grad = {p.saved, p.coef, p.grad_scale};
     return grad_entropy

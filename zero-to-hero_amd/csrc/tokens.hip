@@ -29,7 +29,8 @@ Scratch scratch_of(void* workspace, int64_t S, int64_t T, int64_t A, int dtype) 
     return here;
   };
   Scratch s;
-  s.counts = reinterpret_cast<int*>(take(kCountBlocks * sizeof(int)));
+  s.counts = reinterpret_cast<int*>(take((kCountBlocks + 1) * sizeof(int)));
+  s.order = reinterpret_cast<int*>(take((size_t)(S * T) * sizeof(int)));
   s.lengths = reinterpret_cast<int*>(take((size_t)S * sizeof(int)));
   s.sums = reinterpret_cast<double*>(take(sizeof(double) * kSums * kMaxPartials));
   s.parts = reinterpret_cast<Stat*>(take((size_t)(S * T) * row_splits(S * T, A, dtype) *
@@ -94,7 +95,40 @@ __global__ void __launch_bounds__(256) count_sequences_kernel(const uint8_t* mas
   if (threadIdx.x == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
+// Rows that count, ascending, then the others, by one workgroup: 1024 rows a round, a
+// wave's by ballot, the waves' by their sums.  (A second walk, from the end, places the
+// others, so that neither needs the other's number.)
+__global__ void __launch_bounds__(1024) order_kernel(const uint8_t* mask, int n, int* order,
+                                                     int* live) {
+  __shared__ int part[2][16];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  int done = 0;  // rows that count before this round
+  for (int base = 0, k = 0; base < n; base += 1024, k ^= 1) {
+    const int r = base + threadIdx.x;
+    const bool in = r < n && mask[r] != 0;
+    const unsigned long long votes = __ballot(in);
+    if (lane == 0) part[k][wave] = __builtin_popcountll(votes);
+    __syncthreads();  // (two sets of sums: one barrier a round)
+    int before = 0, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += part[k][w];
+      all += part[k][w];
+    }
+    const int mine = done + before + __builtin_popcountll(votes & ((1ull << lane) - 1));
+    if (r < n) order[in ? mine : n - 1 - (r - mine)] = r;
+    done += all;
+  }
+  if (threadIdx.x == 0) *live = done;
+}
+
 }  // namespace
+
+Order take_order(const Rows& rows, const Scratch& s, hipStream_t stream) {
+  int* live = s.counts + kCountBlocks;
+  hipLaunchKernelGGL(order_kernel, dim3(1), dim3(1024), 0, stream, rows.mask, (int)rows.n, s.order,
+                     live);
+  return {s.order, live};
+}
 
 int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, hipStream_t stream,
                  Weights& w) {
@@ -290,8 +324,10 @@ extern "C" int ppo_token_log_probs(const ppo_token_rows* r, const float* minus, 
   const LogProbs emit = {minus, log_probs, entropy, reinterpret_cast<Saved*>(saved)};
   return with_dtype(r->dtype, [&](auto zero) {
     using T = decltype(zero);
-    return entropy ? launch_statistics<T, true, true>(rows, s, emit, (hipStream_t)stream_ptr)
-                   : launch_statistics<T, false, true>(rows, s, emit, (hipStream_t)stream_ptr);
+    hipStream_t stream = (hipStream_t)stream_ptr;
+    const bool again = saved && rows.n * rows.A * (int64_t)sizeof(T) <= kReadAgain;
+    return entropy ? launch_statistics<T, true, true>(rows, s, emit, again, stream)
+                   : launch_statistics<T, false, true>(rows, s, emit, again, stream);
   });
 }
 

@@ -172,7 +172,8 @@ __device__ __forceinline__ void store16(void* p, v4i w, bool aligned) {
 // How a row is cut into chunks and ends.
 template <class T>
 struct Cut {
-  int head, nvec, ends;
+  int head = 0, nvec = 0, ends = 0;
+  Cut() = default;
   __device__ __forceinline__ Cut(const T* row, int A) {
     const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
     head = min(off ? kPer16<T> - off : 0, A);
@@ -340,6 +341,23 @@ __device__ __forceinline__ float grad_at(const Grad& g, float c, float l) {
 // ---------------------------------------------------------------------------
 // A row in registers
 // ---------------------------------------------------------------------------
+// A value that all lanes of a row's group share: in a scalar register where the group is
+// whole waves.
+template <int G>
+__device__ __forceinline__ float shared_by(float x) {
+  if (G < kWave) return x;
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+template <int G>
+__device__ __forceinline__ int shared_by(int x) {
+  return G < kWave ? x : __builtin_amdgcn_readfirstlane(x);
+}
+template <int G>
+__device__ __forceinline__ Grad shared_by(const Grad& g) {
+  return {shared_by<G>(g.m), shared_by<G>(g.B), shared_by<G>(g.C), shared_by<G>(g.da),
+          shared_by<G>(g.a)};
+}
+
 // The workgroup's group that this lane is in; of a wave's or a workgroup's the
 // compiler is told that it is one.
 template <int G>
@@ -353,8 +371,12 @@ __device__ __forceinline__ int group_of() {
 // them: loads behind the last give 0, stores there write nothing, and one offset
 // a lane serves all of them.  (Rows of 16 lanes, four to a wave, have addresses of
 // their own.)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_buffer(const void* p, int chunks) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, chunks * 16, 0x00027000);
+// The descriptor starts at the round's own first chunk: the lane's offset is then the same
+// in every round, and no register holds one for each.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_buffer(const v4i* chunks, int count,
+                                                               int round) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<v4i*>(chunks) + round, 0,
+                                           max(count - round, 0) * 16, 0x00027000);
 }
 constexpr int kPastCaches = 2;  // the buffer instructions' nt bit
 
@@ -370,18 +392,25 @@ struct RowRegs {
   Cut<T> cut;
   int end_col; // its column, -1: none
 
-  __device__ __forceinline__ RowRegs(const T* row, int A, int t) : cut(row, A) {
+  // No row: nothing is read.
+  static __device__ __forceinline__ Cut<T> cut_of(const T* row, int A) {
+    return row ? Cut<T>(row, A) : Cut<T>();
+  }
+  __device__ __forceinline__ void load_end(const T* row, int t) {
+    end_col = t < cut.ends ? cut.end_column(t) : -1;
+    end = end_col >= 0 ? to_f32(row[end_col]) : kNegInf;
+  }
+  __device__ __forceinline__ RowRegs(const T* row, int A, int t) : cut(cut_of(row, A)) {
     const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
-    const auto buf = chunk_buffer(body, kBuffer ? cut.nvec : 0);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if constexpr (kBuffer)
         raw[i] = __builtin_bit_cast(
-            v4i, __builtin_amdgcn_raw_buffer_load_b128(buf, (i * G + t) * 16, 0, kPastCaches));
+            v4i, __builtin_amdgcn_raw_buffer_load_b128(chunk_buffer(body, cut.nvec, i * G), t * 16, 0,
+                                                       kPastCaches));
       else if (i * G + t < cut.nvec)
         raw[i] = __builtin_nontemporal_load(body + i * G + t);
-    end_col = t < cut.ends ? cut.end_column(t) : -1;
-    end = end_col >= 0 ? to_f32(row[end_col]) : kNegInf;
+    load_end(row, t);
   }
 
   // (at 128 registers to a lane the branches spill; those layouts come in finer steps)
@@ -445,32 +474,46 @@ struct RowRegs {
     return x;
   }
 
-  // `out` lies in 16 bytes as the logits' row does.
+  // `out` lies in 16 bytes as the logits' row does.  With a `next` row (null: none) each
+  // chunk's registers take that row's as soon as its own gradient is on its way, so that
+  // reads and writes overlap however few rows a CU holds.
   template <bool kC>
-  __device__ __forceinline__ void write(const Grad& g, float c, T* out, int t) {
-    T* body = out + cut.head;
+  __device__ __forceinline__ void write(const Grad& g, float c, T* out, int A, int t,
+                                        const T* next = nullptr) {
+    v4i* body = reinterpret_cast<v4i*>(out + cut.head);
+    const Cut<T> now = cut;
+    const int now_col = end_col;
+    const float now_end = end;
+    cut = cut_of(next, A);
+    const v4i* from = reinterpret_cast<const v4i*>(next + cut.head);
     float last = 0.0f;
-    const auto buf = chunk_buffer(body, kBuffer ? cut.nvec : 0);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (!reaches(i)) continue;
-      float d[kN];
-      turn(i, last);
+      if (G >= 512 || i < V / 2 || i * G < now.nvec) {
+        float d[kN];
+        turn(i, last);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) d[j] = grad_at<kC>(g, c, unpack<T>(raw[i], j));
-      const v4i w = pack<T>(d);
-      last = d[0];
+        for (int j = 0; j < kN; ++j) d[j] = grad_at<kC>(g, c, unpack<T>(raw[i], j));
+        const v4i w = pack<T>(d);
+        last = d[0];
+        if constexpr (kBuffer)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, w),
+                                                 chunk_buffer(body, now.nvec, i * G), t * 16, 0,
+                                                 kPastCaches);
+        else if (i * G + t < now.nvec)
+          __builtin_nontemporal_store(w, body + i * G + t);
+      }
       if constexpr (kBuffer)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, w), buf, (i * G + t) * 16, 0,
-                                               kPastCaches);
-      else if (i * G + t < cut.nvec)
-        __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(body) + i * G + t);
+        raw[i] = __builtin_bit_cast(
+            v4i, __builtin_amdgcn_raw_buffer_load_b128(chunk_buffer(from, cut.nvec, i * G), t * 16, 0,
+                                                       kPastCaches));
     }
-    if (end_col >= 0) out[end_col] = from_f32<T>(grad_at<kC>(g, c, end));
+    load_end(next, t);
+    if (now_col >= 0) out[now_col] = from_f32<T>(grad_at<kC>(g, c, now_end));
     // the action's own element, by the lane that wrote its place
-    const int b = g.a - cut.head;
-    const bool inside = g.a >= 0 && b >= 0 && b < cut.nvec * kN;
-    if (inside ? (b / kN) % G == t : (g.a >= 0 && g.a == end_col)) out[g.a] = from_f32<T>(g.da);
+    const int b = g.a - now.head;
+    const bool inside = g.a >= 0 && b >= 0 && b < now.nvec * kN;
+    if (inside ? (b / kN) % G == t : (g.a >= 0 && g.a == now_col)) out[g.a] = from_f32<T>(g.da);
   }
 };
 
@@ -508,10 +551,20 @@ __device__ __forceinline__ float row_weight(const Weights& w, float inverse, int
   return w.lengths ? inverse / (float)w.lengths[seq] : inverse;
 }
 
-// Scratch: counts, lengths, partial sums, then the split statistics.
+// The rows in the order in which a launch takes them: those that count, then the others,
+// each in their own (null: as they lie, and whether one counts is looked up).  Where a
+// workgroup has a handful of long rows, taking every so many of the first kind gives
+// all of them as many.
+struct Order {
+  const int* rows;
+  const int* live;  // how many count
+};
+
+// Scratch: counts, lengths, the order, partial sums, then the split statistics.
 struct Scratch {
   int* counts;
   int* lengths;
+  int* order;
   double* sums;   // [kSums][kMaxPartials]
   Stat* parts;    // [rows][splits]
   size_t bytes;
@@ -548,6 +601,9 @@ int take_rows(const ppo_token_rows* r, bool actions, Rows& out);
 // Checks a loss's weights; enqueues the counting they need.
 int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, hipStream_t stream,
                  Weights& w);
+
+// Enqueues the ordering of rows (mask given).
+Order take_order(const Rows& rows, const Scratch& s, hipStream_t stream);
 
 inline int launch_blocks(int64_t groups, int64_t most) {
   return (int)(groups < most ? groups : most);

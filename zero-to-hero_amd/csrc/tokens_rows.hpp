@@ -12,12 +12,14 @@ namespace ppo {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// Statistics of chunks [part / splits) of a row, by G lanes, four chunks of each
-// lane in flight; the sums follow the running maximum.
+// Statistics of chunks [part / splits) of a row, by G lanes, two chunks of each lane at
+// a time (four and eight are slower: 50304 bf16 69, 72 and 76 us of 4096 rows; of short
+// rows one); the sums follow the running maximum.  `again`: the rows are read again
+// soon, and stay in the caches.
 template <class T, int G, bool kEntropy>
 __device__ __forceinline__ Stat stream_stat(const T* row, int A, int a, float c, int t, int part,
-                                            int splits) {
-  constexpr int kN = kPer16<T>, kU = 4;
+                                            int splits, bool again) {
+  constexpr int kN = kPer16<T>, kU = G == 16 ? 1 : 2;
   const Cut<T> cut(row, A);
   const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
   const int per = (cut.nvec + splits - 1) / splits;
@@ -35,7 +37,9 @@ __device__ __forceinline__ Stat stream_stat(const T* row, int A, int a, float c,
     v4i w[kU];
 #pragma unroll
     for (int k = 0; k < kU; ++k)
-      w[k] = i + k * G < end ? __builtin_nontemporal_load(body + i + k * G) : no_chunk<T>();
+      w[k] = i + k * G >= end ? no_chunk<T>()
+             : again          ? body[i + k * G]
+                              : __builtin_nontemporal_load(body + i + k * G);
     float m = x.m;
 #pragma unroll
     for (int k = 0; k < kU; ++k) {
@@ -68,7 +72,7 @@ __device__ __forceinline__ float action_logit(const T* row, int a) {
 // a row that leave their parts.  What bounds it: HBM reads.
 template <class T, int G, bool kEntropy, bool kDirect, class Emit>
 __global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, Stat* parts,
-                                                         int splits) {
+                                                         int splits, bool again) {
   __shared__ Stat s_part[4];
   const int t = threadIdx.x % G;
   const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -82,7 +86,8 @@ __global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, S
   const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
   const int a = rows.actions ? rows.action(r) : -1;
   const float la = kDirect ? action_logit(row, a) : 0.0f;
-  Stat x = stream_stat<T, G, kEntropy>(row, rows.A, a, rows.c, t, part, splits);
+  Stat x = stream_stat<T, G, kEntropy>(row, rows.A, a, rows.c, t, part, splits,
+                                                again);
   if (G > kWave) {
     x = block_join<kEntropy>(x, rows.c, s_part);
     if (threadIdx.x >= kWave) return;
@@ -119,8 +124,13 @@ __global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit, const St
   emit.end();
 }
 
+// Logits that the last-level cache holds from the forward to the backward pass (at 412 MB
+// of them 208 -> 200 us for both, at 537 as much as without).
+constexpr int64_t kReadAgain = (int64_t)512 << 20;
+
 template <class T, bool kEntropy, bool kMayDirect, class Emit>
-int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, hipStream_t stream) {
+int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, bool again,
+                      hipStream_t stream) {
   const int dtype = sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16;  // (sizes alike)
   const int splits = row_splits(rows.n, rows.A, dtype);
   if constexpr (kMayDirect)
@@ -130,7 +140,7 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, hipS
         constexpr int G = decltype(lanes)::value;
         hipLaunchKernelGGL((statistics_kernel<T, G, kEntropy, true, Emit>),
                            dim3((unsigned)div_up(rows.n, 256 / G)), dim3(256), 0, stream, rows, emit,
-                           nullptr, 1);
+                           nullptr, 1, again);
         return last_launch_status();
       };
       if (chunks <= 64) return go(Int<16>{});
@@ -140,7 +150,7 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, hipS
   if (rows.n > ((int64_t)1 << 31) / splits - 1) return PPO_ERR_TOO_LARGE;
   hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
                      dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
-                     splits);
+                     splits, again);
   hipLaunchKernelGGL((join_kernel<T, kEntropy, Emit>), dim3(launch_blocks(rows.n, kMaxPartials)),
                      dim3(64), 0, stream, rows, emit, s.parts, splits);
   return last_launch_status();
@@ -237,6 +247,43 @@ template <int G>
 constexpr int kRowBlock = G < 256 ? 256 : G;
 template <int G>
 constexpr int kRowWaves = G >= 512 ? 4 : 1;
+
+// Workgroups of 512 and 1024 lanes, of which a CU holds two or one, take row after row
+// and read the next one while they write (131072 bf16 909 -> 851 us of 8192 rows); so
+// there are as many as run at once, and the rows are ordered for them.  Smaller ones
+// overlap by their number, and come as the rows do (32768 85 us, 93 the other way).
+template <int G>
+constexpr bool kRowAfterRow = G >= 512;
+template <int G>
+constexpr int kRowBlocks = G == 1024 ? 256 : G == 512 ? 512 : kMaxPartials;
+
+// The rows of a group: every step-th from its first on.
+template <int G>
+struct Walk {
+  const Rows& rows;
+  Order order;
+  int64_t step;
+  int live;
+
+  __device__ __forceinline__ Walk(const Rows& rows_, const Order& order_, int64_t step_)
+      : rows(rows_), order(order_), step(step_),
+        live(kRowAfterRow<G> && order.rows ? *order.live : (int)rows.n) {}
+  __device__ __forceinline__ int64_t row(int64_t i) const {
+    return kRowAfterRow<G> && order.rows ? order.rows[i] : i;
+  }
+  // From place i on the next one whose row counts (rows.n: none); dead(row) for those
+  // before it that do not.
+  template <class Dead>
+  __device__ __forceinline__ int64_t from(int64_t i, Dead&& dead) const {
+    if (kRowAfterRow<G>) {
+      if (i < live) return i;
+      for (; i < rows.n; i += step) dead(row(i));
+      return rows.n;
+    }
+    for (; i < rows.n && !rows.live(i); i += step) dead(i);
+    return i;
+  }
+};
 
 // (without gradients: as if they started at a multiple of 16, so that a loss has the
 // same bits with and without them where its caller allocates them so)
