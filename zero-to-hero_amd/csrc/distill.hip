@@ -78,7 +78,7 @@ __device__ __forceinline__ Entries take_entries(const Teacher& teacher, int64_t 
     b.q[k] = t;
     b.l[k] = l;
     m = fmaxf(m, t);
-    top = fmaxf(top, l);
+    if (t != kNegInf) top = fmaxf(top, l);  // (an entry that weighs nothing has no part)
   }
   for (int k = K + lane; k < ((K + 3) & ~3); k += G) b.col[k] = -1;
   m = lanes_max<G>(m);

@@ -218,11 +218,12 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
   for (int k = 0; k < 2; ++k) {
     const int64_t at = (i + k * p.pairs) * p.T;
     double x = 0.0, m = 0.0;
-    for (int64_t j = t; j < p.T; j += G)
-      if (!p.mask || p.mask[at + j]) {
-        x += (double)p.rel[at + j];
-        m += 1.0;
-      }
+    for (int64_t j = t; j < p.T; j += G) {
+      const bool live = !p.mask || p.mask[at + j];
+      const float rel = p.rel[at + j];  // (both loads at once)
+      x += live ? (double)rel : 0.0;
+      m += live ? 1.0 : 0.0;
+    }
     sum[k] = lanes_sum<kWave>(x);
     n[k] = lanes_sum<kWave>(m);
     if (G > kWave && (t & (kWave - 1)) == 0) {

@@ -2,28 +2,30 @@
 // 64-bit whole number (the logit's order above, the column's complement below), by
 // which no two of a row are alike: ties need no care of their own.
 //
-// A workgroup holds a row, or a part of one, in registers.  The K-th largest of its
-// lanes' own maxima bounds the K-th largest element from below, so the few elements
-// from there on (about K of them) are all there is to sort, by counting for each
-// how many precede it.  Rows of many equal logits, where too many reach the bound,
-// are settled by searching for the threshold itself.  What bounds it: HBM reads.
+// A workgroup takes a row, or a part of one.  Its lanes keep the largest of what they
+// read, in four segments each; the K-th largest of the lanes' own maxima bounds the K-th
+// largest element from below, so the few segments that reach it (about K of them) are
+// all that is looked at again, and the few elements there that do are sorted, by
+// counting for each how many precede it.  Rows in which too many reach the bound (many
+// equal logits) are settled by a radix search for the threshold itself.  What bounds
+// it: HBM reads; a row is in the caches when parts of it are read again.
 #include "tokens_rows.hpp"
 
 namespace ppo {
 namespace {
 
 constexpr int kMaxK = PPO_TOKEN_MAX_K;
-// Elements that are sorted at most: about what fewer than kMaxK lanes of one chunk each
-// hold together.
-constexpr int kSorted = 8 * kMaxK;
+constexpr int kSorted = 2048;  // elements that are sorted at most
+constexpr int kSegments = 4;
 
 typedef unsigned long long u64;
 
 // A logit's order as an unsigned number above 0; -0 is 0, NaN is before everything.
+constexpr unsigned kNanOrder = 0xFFFFFFFFu;
 __device__ __forceinline__ unsigned order_of(float l) {
   const unsigned b = __builtin_bit_cast(unsigned, l + 0.0f);
   const unsigned k = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
-  return l != l ? 0xFFFFFFFFu : k;
+  return l != l ? kNanOrder : k;
 }
 __device__ __forceinline__ u64 place(unsigned order, int col) {
   return (u64)order << 32 | (unsigned)~col;
@@ -33,11 +35,21 @@ __device__ __forceinline__ int column_of(u64 x) { return (int)~(unsigned)x; }
 template <int G>
 struct Board {
   u64 list[kSorted];
-  unsigned best[G];
+  union {
+    unsigned best[G];
+    unsigned short again[kSegments * G];  // lane + G segment of segments to look at again
+    int bins[256];
+  };
   unsigned bound;
-  int count, total;
+  int count, items;
   int part[G / kWave];
 };
+
+template <int G>
+__device__ __forceinline__ void append(Board<G>& b, unsigned order, int col) {
+  const int at = atomicAdd(&b.count, 1);
+  if (at < kSorted) b.list[at] = place(order, col);
+}
 
 // The sum of a whole number over the workgroup, for every lane.  Two barriers.
 template <int G>
@@ -52,16 +64,14 @@ __device__ __forceinline__ int block_count(int x, Board<G>& b) {
   return n;
 }
 
-// Leaves in b.list the workgroup's elements among which its K largest are, and in
-// b.count how many (at most kSorted).  each(f) calls f(order, column) for every element
-// of the lane; `best` is the largest order among them, 0 without any.
-template <int G, class Each>
-__device__ __forceinline__ void gather(Board<G>& b, int K, int columns, unsigned best, Each&& each) {
+// The largest 16-bit prefix that K lanes' best reach (1 if fewer lanes have any), for
+// every lane; b.count and b.items are 0 afterwards.
+template <int G>
+__device__ __forceinline__ unsigned bound_of(Board<G>& b, int K, unsigned best) {
   b.best[threadIdx.x] = best;
-  if (threadIdx.x == 0) b.count = 0;
+  if (threadIdx.x == 0) b.count = b.items = 0;
   lds_barrier();
   if (threadIdx.x < kWave) {
-    // the largest 16-bit prefix that K lanes' best reach (0 if fewer have any)
     unsigned v[G / kWave];
 #pragma unroll
     for (int i = 0; i < G / kWave; ++i) v[i] = b.best[i * kWave + threadIdx.x];
@@ -75,40 +85,7 @@ __device__ __forceinline__ void gather(Board<G>& b, int K, int columns, unsigned
     if (threadIdx.x == 0) b.bound = bound > 1 ? bound : 1;  // (order 0 is no element)
   }
   lds_barrier();
-  const unsigned bound = b.bound;
-  auto collect = [&](auto&& takes) {
-    each([&](unsigned order, int col) {
-      if (!takes(order, col)) return;
-      const int at = atomicAdd(&b.count, 1);
-      if (at < kSorted) b.list[at] = place(order, col);
-    });
-  };
-  if (best >= bound) collect([&](unsigned order, int) { return order >= bound; });
-  lds_barrier();
-  if (b.count <= kSorted) return;
-  // Too many equal ones: the K-th largest order exactly, then the column up to which
-  // elements of that order are among the K.
-  lds_barrier();
-  unsigned kth = 0;
-  for (unsigned bit = 1u << 31; bit; bit >>= 1) {
-    int n = 0;
-    each([&](unsigned order, int) { n += order >= (kth | bit); });
-    if (block_count(n, b) >= K) kth |= bit;
-  }
-  int above = 0;
-  each([&](unsigned order, int) { above += order > kth; });
-  const int ties = K - block_count(above, b);
-  int last = 0;  // the smallest column with `ties` elements of order kth up to it
-  for (int step = 1 << 30; step; step >>= 1) {
-    if (last + step > columns) continue;
-    int n = 0;
-    each([&](unsigned order, int col) { n += order == kth && col < last + step; });
-    if (block_count(n, b) < ties) last += step;
-  }
-  if (threadIdx.x == 0) b.count = 0;
-  lds_barrier();
-  collect([&](unsigned order, int col) { return order > kth || (order == kth && col <= last); });
-  lds_barrier();
+  return b.bound;
 }
 
 // Calls out(rank, element) for each of the listed elements among the K largest.
@@ -123,39 +100,182 @@ __device__ __forceinline__ void ranked(const Board<G>& b, int K, Out&& out) {
   }
 }
 
-// Part `p` of `parts` of each row; one part: the row's results, else its largest
+// A row, or a part of one from column `from` on.
+template <class T, int G>
+struct Part {
+  static constexpr int kN = kPer16<T>;
+  const T* row;
+  const v4i* body;
+  int from;
+  Cut<T> cut;
+  int rounds;  // of G chunks a segment
+
+  __device__ __forceinline__ Part(const T* row_, int from_, int width)
+      : row(row_), from(from_), cut(row_ + from_, width) {
+    body = reinterpret_cast<const v4i*>(row + from + cut.head);
+    rounds = (cut.nvec + kSegments * G - 1) / (kSegments * G);
+  }
+  __device__ __forceinline__ int end_column(int e) const { return from + cut.end_column(e); }
+  __device__ __forceinline__ int column(int chunk) const { return from + cut.head + chunk * kN; }
+
+  // f(order, column) for each element of the lane.
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int t = threadIdx.x;
+    if (t < cut.ends) f(order_of(to_f32(row[end_column(t)])), end_column(t));
+    for (int i = t; i < cut.nvec; i += G) {
+      const v4i w = body[i];
+#pragma unroll
+      for (int j = 0; j < kN; ++j) f(order_of(unpack<T>(w, j)), column(i) + j);
+    }
+  }
+};
+
+// Too many elements reach the bound: the K-th largest order, byte by byte, the elements
+// above it, and of those equal to it the first ones by column.
+template <class T, int G>
+__device__ void settle(const Part<T, G>& p, Board<G>& b, int K) {
+  const int t = threadIdx.x;
+  unsigned kth = 0;
+  int left = K;  // elements of the K among those that share kth's leading bytes
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    lds_barrier();
+    for (int i = t; i < 256; i += G) b.bins[i] = 0;
+    lds_barrier();
+    p.each([&](unsigned order, int) {
+      if (shift < 24 && (order ^ kth) >> (shift + 8)) return;
+      const int bin = order >> shift & 255;
+      // (equal logits: one lane counts for the others)
+      const u64 active = __ballot(1), alike = __ballot(bin == __builtin_amdgcn_readfirstlane(bin));
+      if (alike == active) {
+        if ((t & (kWave - 1)) == __builtin_ctzll(active))
+          atomicAdd(&b.bins[bin], __builtin_popcountll(active));
+      } else {
+        atomicAdd(&b.bins[bin], 1);
+      }
+    });
+    lds_barrier();
+    int bin = 255;
+    for (; bin > 0 && b.bins[bin] < left; --bin) left -= b.bins[bin];
+    kth |= (unsigned)bin << shift;
+  }
+  lds_barrier();
+  if (t == 0) b.count = 0;
+  lds_barrier();
+  p.each([&](unsigned order, int col) {
+    if (order > kth) append(b, order, col);
+  });
+  lds_barrier();
+  // `left` of the equal ones: the head's elements, the chunks round by round, the tail's
+  auto ends = [&](int e, int last) {
+    if (t == 0)
+      for (; e < last && left > 0; ++e)
+        if (order_of(to_f32(p.row[p.end_column(e)])) == kth) {
+          append(b, kth, p.end_column(e));
+          --left;
+        }
+    if (t == 0) b.items = left;
+    lds_barrier();
+    left = b.items;
+    lds_barrier();
+  };
+  ends(0, p.cut.head);
+  for (int base = 0; base < p.cut.nvec && left > 0; base += G) {
+    const int i = base + t;
+    unsigned mine = 0;
+    if (i < p.cut.nvec) {
+      const v4i w = p.body[i];
+#pragma unroll
+      for (int j = 0; j < Part<T, G>::kN; ++j)
+        mine |= (unsigned)(order_of(unpack<T>(w, j)) == kth) << j;
+    }
+    // how many lie before this lane's: by its wave's bits, and the waves before
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < Part<T, G>::kN; ++j)
+      n += __builtin_popcountll(__ballot(mine >> j & 1) & ((1ull << (t & (kWave - 1))) - 1));
+    const int all = __builtin_amdgcn_readlane(n + __builtin_popcount(mine), kWave - 1);
+    if ((t & (kWave - 1)) == 0) b.part[t / kWave] = all;
+    lds_barrier();
+    int total = 0;
+    for (int w = 0; w < G / kWave; ++w) {
+      if (w < t / kWave) n += b.part[w];
+      total += b.part[w];
+    }
+    for (int j = 0; j < Part<T, G>::kN; ++j)
+      if (mine >> j & 1) {
+        if (n < left) append(b, kth, p.column(i) + j);
+        ++n;
+      }
+    left = total < left ? left - total : 0;
+    lds_barrier();
+  }
+  ends(p.cut.head, p.cut.ends);
+}
+
+// Part `q` of `parts` of each row; one part: the row's results, else its largest
 // elements to `found` [rows][parts][K], 0 behind the last.
-template <class T, int G, int V>
-__global__ void __launch_bounds__(G) top_kernel(const T* logits, int64_t rows, int A, int K,
-                                                int parts, int per, T* values, int64_t* ids,
-                                                u64* found) {
-  constexpr int kN = kPer16<T>;
+template <class T, int G>
+__global__ void __launch_bounds__(G) top_kernel(const T* logits, int A, int K, int parts, int per,
+                                                T* values, int64_t* ids, u64* found) {
+  constexpr int kN = kPer16<T>, kU = 4;
   __shared__ Board<G> b;
   const int t = threadIdx.x;
   const int64_t r = (int64_t)blockIdx.x / parts;
-  const int p = (int)((int64_t)blockIdx.x - r * parts);
-  const T* row = logits + r * A;
-  const int from = p * per, width = min(per, A - from);
-  RowRegs<T, G, V> x(row + from, width, t);
-  auto each = [&](auto&& f) {
-    if (x.end_col >= 0) f(order_of(x.end), from + x.end_col);
+  const int q = (int)((int64_t)blockIdx.x - r * parts);
+  const int from = q * per, width = min(per, A - from), want = min(K, width);
+  const Part<T, G> p(logits + r * A, from, width);
+
+  // (the largest of a segment as a float, and whether a NaN was among them)
+  unsigned best[kSegments], most = 0;
+  const float end = t < p.cut.ends ? to_f32(p.row[p.end_column(t)]) : kNegInf;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float none = 0.0f;
-      x.turn(i, none);
-      if (i * G + t >= x.cut.nvec) continue;
-      const int col = from + x.cut.head + (i * G + t) * kN;
+  for (int s = 0; s < kSegments; ++s) {
+    float m = kNegInf;
+    bool nan = false;
+    const int first = s * p.rounds * G + t, last = min(p.cut.nvec, (s + 1) * p.rounds * G);
+    for (int i = first; i < last; i += G * kU) {
+      v4i w[kU];
 #pragma unroll
-      for (int j = 0; j < kN; ++j) f(order_of(unpack<T>(x.raw[i], j)), col + j);
+      for (int k = 0; k < kU; ++k)
+        w[k] = i + k * G < last ? p.body[i + k * G] : no_chunk<T>();
+#pragma unroll
+      for (int k = 0; k < kU; ++k)
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+          const float l = unpack<T>(w[k], j);
+          m = fmaxf(m, l);
+          nan |= l != l;
+        }
     }
-  };
-  unsigned best = 0;
-  each([&](unsigned order, int) { best = order > best ? order : best; });
-  gather<G>(b, min(K, width), A, best, each);
+    best[s] = first < last ? (nan ? kNanOrder : order_of(m)) : 0;
+    most = max(most, best[s]);
+  }
+  const unsigned end_order = t < p.cut.ends ? order_of(end) : 0;
+  const unsigned bound = bound_of(b, want, max(most, end_order));
+  if (end_order >= bound) append(b, end_order, p.end_column(t));
+#pragma unroll
+  for (int s = 0; s < kSegments; ++s)
+    if (best[s] >= bound) b.again[atomicAdd(&b.items, 1)] = (unsigned short)(s * G + t);
+  lds_barrier();
+  const int items = b.items * p.rounds;
+  for (int i = t; i < items; i += G) {
+    const int item = i / p.rounds, who = b.again[item], s = who / G;
+    const int chunk = (s * p.rounds + i - item * p.rounds) * G + who % G;
+    if (chunk >= min(p.cut.nvec, (s + 1) * p.rounds * G)) continue;
+    const v4i w = p.body[chunk];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      const unsigned order = order_of(unpack<T>(w, j));
+      if (order >= bound) append(b, order, p.column(chunk) + j);
+    }
+  }
+  lds_barrier();
+  if (b.count > kSorted) settle(p, b, want);
   if (parts == 1) {
     ranked<G>(b, K, [&](int rank, u64 e) {
       const int col = column_of(e);
-      values[r * K + rank] = row[col];
+      values[r * K + rank] = p.row[col];
       ids[r * K + rank] = col;
     });
   } else {
@@ -181,14 +301,29 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
   for (int i = 0; i < kMergeV; ++i) {
     const int k = i * 1024 + threadIdx.x;
     x[i] = k < n ? from[k] : 0;
-    const unsigned order = (unsigned)(x[i] >> 32);
-    best = order > best ? order : best;
+    best = max(best, (unsigned)(x[i] >> 32));
   }
-  gather<1024>(b, K, A, best, [&](auto&& f) {
+  const unsigned bound = bound_of(b, K, best);
+#pragma unroll
+  for (int i = 0; i < kMergeV; ++i)
+    if ((unsigned)(x[i] >> 32) >= bound) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));
+  lds_barrier();
+  if (b.count > kSorted) {  // (no two are alike: the K-th by its bits)
+    lds_barrier();
+    u64 kth = 0;
+    for (u64 bit = 1ull << 63; bit; bit >>= 1) {
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < kMergeV; ++i) above += x[i] >= (kth | bit);
+      if (block_count(above, b) >= K) kth |= bit;
+    }
+    if (threadIdx.x == 0) b.count = 0;
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < kMergeV; ++i)
-      if (x[i]) f((unsigned)(x[i] >> 32), column_of(x[i]));
-  });
+      if (x[i] >= kth) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));
+    lds_barrier();
+  }
   ranked<1024>(b, K, [&](int rank, u64 e) {
     const int col = column_of(e);
     values[r * K + rank] = logits[r * A + col];
@@ -196,19 +331,19 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
   });
 }
 
-// Parts of a row: what a workgroup can hold, and so many that few rows fill the chip.
+// Parts of a row, so many that few rows fill the chip, of 16 KB at least and of 2^16
+// elements at most.
 struct TopPlan {
   int parts, per;
 };
+constexpr int64_t kPartElements = 1 << 16;
 TopPlan plan_of(int64_t rows, int64_t A, int dtype) {
-  const int64_t size = dtype_size(dtype), most = (int64_t)1024 * 16 * (16 / size);
-  int64_t parts = div_up(A, most);
-  if (rows < 128 && A * size > 32768) {
-    const int64_t fill = div_up(256, rows), small = div_up(A * size, 16384);
-    const int64_t more = fill < small ? fill : small;
-    if (more > parts) parts = more;
-  }
-  if (parts > kMaxParts) parts = kMaxParts;  // (2^22 elements: 64 of 2^16)
+  const int64_t size = dtype_size(dtype);
+  int64_t parts = div_up(A, kPartElements);
+  if (rows >= 512) parts = 1;
+  if (rows < 256 && A * size > 32768)
+    parts = std::max(parts, std::min(div_up(512, rows), div_up(A * size, 16384)));
+  if (parts > kMaxParts) parts = kMaxParts;
   // (parts start at multiples of 16 bytes of the row)
   const int64_t per = round_up(div_up(A, parts), 16 / size);
   return {(int)div_up(A, per), (int)per};
@@ -231,12 +366,11 @@ extern "C" int ppo_token_top(const void* logits, int dtype, int64_t rows, int64_
   if (!dtype_ok(dtype) || rows < 0 || A <= 0 || K <= 0 || K > A) return PPO_ERR_INVALID_ARG;
   if (rows == 0) return PPO_OK;
   if (!logits || !values || !ids || (uintptr_t)logits % dtype_size(dtype) ||
-      (uintptr_t)values % dtype_size(dtype))
+      (uintptr_t)values % dtype_size(dtype) || (uintptr_t)ids % 8)
     return PPO_ERR_INVALID_ARG;
   if (K > kMaxK || A > ((int64_t)1 << 22)) return PPO_ERR_TOO_LARGE;
   const TopPlan plan = plan_of(rows, A, dtype);
-  if (rows > (((int64_t)1 << 31) - 1) / plan.parts)
-    return PPO_ERR_TOO_LARGE;
+  if (rows > (((int64_t)1 << 31) - 1) / plan.parts) return PPO_ERR_TOO_LARGE;
   if (plan.parts > 1 && (!workspace || !aligned16(workspace) ||
                          workspace_bytes < ppo_token_top_workspace_bytes(rows, A, K, dtype)))
     return PPO_ERR_WORKSPACE;
@@ -246,20 +380,14 @@ extern "C" int ppo_token_top(const void* logits, int dtype, int64_t rows, int64_
     using T = decltype(zero);
     const T* in = static_cast<const T*>(logits);
     T* out = static_cast<T*>(values);
-    auto go = [&](auto lanes, auto held) {
-      constexpr int G = decltype(lanes)::value, V = decltype(held)::value;
-      hipLaunchKernelGGL((top_kernel<T, G, V>), dim3((unsigned)(rows * plan.parts)), dim3(G), 0,
-                         stream, in, rows, (int)A, (int)K, plan.parts, plan.per, out, ids, found);
+    // (K of G lanes' maxima: with many more lanes than K the bound lies close)
+    auto go = [&](auto lanes) {
+      constexpr int G = decltype(lanes)::value;
+      hipLaunchKernelGGL((top_kernel<T, G>), dim3((unsigned)(rows * plan.parts)), dim3(G), 0, stream,
+                         in, (int)A, (int)K, plan.parts, plan.per, out, ids, found);
       return last_launch_status();
     };
-    const int64_t chunks = chunks_of(plan.per, dtype);
-    const int code = chunks <= 256 * 1    ? go(Int<256>{}, Int<1>{})
-                     : chunks <= 256 * 2  ? go(Int<256>{}, Int<2>{})
-                     : chunks <= 256 * 4  ? go(Int<256>{}, Int<4>{})
-                     : chunks <= 256 * 8  ? go(Int<256>{}, Int<8>{})
-                     : chunks <= 512 * 8  ? go(Int<512>{}, Int<8>{})
-                     : chunks <= 1024 * 8 ? go(Int<1024>{}, Int<8>{})
-                                          : go(Int<1024>{}, Int<16>{});
+    const int code = K <= 96 ? go(Int<256>{}) : K <= 192 ? go(Int<512>{}) : go(Int<1024>{});
     if (code || plan.parts == 1) return code;
     hipLaunchKernelGGL((top_merge_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, stream, in,
                        (int)A, (int)K, plan.parts, out, ids, found);
