@@ -40,7 +40,7 @@ struct Board {
     l = sum + per;
   }
 };
-size_t board_bytes(int K, int boards) { return (size_t)boards * 4 * round_up(K, 4) * 4; }
+int board_ints(int K) { return 4 * (int)round_up(K, 4); }
 
 // What the entries come to: sum q (1; 0 without entries; NaN with one that is not finite)
 // and the loss but for the student's m and log s:
@@ -120,15 +120,20 @@ __device__ __forceinline__ Entries take_entries(const Teacher& teacher, int64_t 
   return {s == 0.0f ? 0.0f : s / s, gap * inv, top, s == 0.0f ? 0.0f : log_of(s)};
 }
 
-// The entries' columns: tau w (p - q).
-template <class T>
+// The entries' columns, those that `in` has: tau w (p - q).
+struct AllColumns {
+  __device__ __forceinline__ bool has(int) const { return true; }
+};
+template <class T, class In = AllColumns>
 __device__ __forceinline__ void write_entries(const Board& b, int K, float m, float inv_s, float c,
-                                              float W, T* out, int t, int lanes) {
-  for (int k = t; k < K; k += lanes)
-    if (b.col[k] >= 0) {
-      const float p = exp2_fast((b.l[k] - m) * c) * inv_s;
-      out[b.col[k]] = from_f32<T>(W * (p - b.sum[k]));
-    }
+                                              float W, T* out, int t, int lanes,
+                                              const In& in = In{}) {
+  for (int k = t; k < K; k += lanes) {
+    const int col = b.col[k];
+    if (col < 0 || !in.has(col)) continue;
+    const float p = exp2_fast((b.l[k] - m) * c) * inv_s;
+    out[col] = from_f32<T>(W * (p - b.sum[k]));
+  }
 }
 
 struct Distill {
@@ -259,36 +264,68 @@ struct DistillJoin {
   __device__ __forceinline__ void end() { leave_sums(sums, d.sums); }
 };
 
-struct DistillGrad {
-  const Saved* saved;
-  float grad_scale;
-  __device__ __forceinline__ Grad row(const Rows&, int64_t r, float up, int) const {
-    const Saved s = saved[r];
-    return {s.m, up * grad_scale * s.weight * s.pa * s.inv_s, 0.0f, 0.0f, -1};
+// Where the pieces of a row are written apart: each takes the row's entries for itself and
+// writes those among its own columns.
+struct DistillTerms : GradientTerms {
+  static constexpr bool kAfter = true;
+  Teacher teacher;
+  float inv_s, W;  // of the row at hand
+
+  template <class T, int G>
+  __device__ __forceinline__ Entries take(const Rows& rows, int64_t r, const T* row, int* board) {
+    constexpr int kTeam = G < kWave ? G : kWave;
+    return take_entries<T, kTeam>(teacher, r, row, rows.A, rows.c, threadIdx.x % kTeam,
+                                  Board(board, teacher.K, 0));
+  }
+  template <class T, int G>
+  __device__ __forceinline__ void after(const Rows& rows, const Grad& g, T* out,
+                                        const PieceColumns& cols, int t, int* board) const {
+    write_entries<T>(Board(board, teacher.K, 0), teacher.K, g.m, inv_s, rows.c, W, out, t,
+                     G < kWave ? G : kWave, cols);
   }
 };
 
-// The entries' columns after a dense pass over the rows, a wave to a row.
-template <class T>
-__global__ void __launch_bounds__(64) entries_kernel(Rows rows, Teacher teacher, const Saved* saved,
-                                                     const float* scale, float held,
-                                                     float grad_scale, T* dlogits) {
-  __shared__ int s_board[4 * kMaxK];
-  const float up = scale ? *scale : 1.0f;
-  if (held != 0.0f && up == held) return;
-  const int lane = threadIdx.x;
-  const Board board(s_board, teacher.K, 0);
-  for (int64_t r = blockIdx.x; r < rows.n; r += gridDim.x) {
-    if (!rows.live(r)) continue;
-    const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
+// From what the forward pass saved.
+struct DistillGrad : DistillTerms {
+  const Saved* saved;
+  float grad_scale;
+  template <class T, int G>
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T* row, float up, int, int,
+                                      bool, int* board) {
+    take<T, G>(rows, r, row, board);
     const Saved s = saved[r];
-    take_entries<T, kWave>(teacher, r, row, rows.A, rows.c, lane, board);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    write_entries<T>(board, teacher.K, s.m, s.inv_s, rows.c, up * grad_scale * s.weight,
-                     dlogits + r * rows.A, lane, kWave);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    inv_s = s.inv_s;
+    W = up * grad_scale * s.weight;
+    return {s.m, W * s.pa * s.inv_s, 0.0f, 0.0f, -1};
   }
-}
+};
+
+// From the parts of the rows' statistics, in the forward pass of few rows.
+struct DistillSplit : DistillTerms {
+  Distill d;
+  const Stat* parts;
+  int splits;
+  float inverse;
+
+  __device__ __forceinline__ void begin() { inverse = inverse_count(d.weights); }
+  __device__ __forceinline__ void masked(const Rows&, int64_t r, bool first) const {
+    if (first) d.sums[r] = 0.0;
+  }
+  template <class T, int G>
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T* row, float, int, int t,
+                                      bool first, int* board) {
+    const Entries e = take<T, G>(rows, r, row, board);
+    const Stat x = join_parts<G, false>(parts, r, splits, rows.c);
+    const float weight = d.tau * row_weight(d.weights, inverse, r / rows.T);
+    inv_s = 1.0f / x.s;
+    W = weight * d.grad_scale;
+    if (first && t == 0) {
+      d.sums[r] = (double)weight * e.loss(x.m, log_of(x.s), rows.c);
+      d.leave(r, x.m, x.s, weight, e.total);
+    }
+    return {x.m, W * e.total * inv_s, 0.0f, 0.0f, -1};
+  }
+};
 
 __global__ void __launch_bounds__(256) distill_scalar_kernel(const double* sums, int n, double tau,
                                                              float* scalar) {
@@ -304,13 +341,8 @@ __global__ void __launch_bounds__(256) distill_scalar_kernel(const double* sums,
 template <class T>
 int dense_gradient(const Rows& rows, const Teacher& teacher, const Saved* saved, const float* scale,
                    float held, float grad_scale, T* dlogits, hipStream_t stream) {
-  const DistillGrad grad = {saved, grad_scale};
-  if (const int code = launch_gradient<T, false>(rows, grad, scale, held, dlogits, stream))
-    return code;
-  hipLaunchKernelGGL((entries_kernel<T>),
-                     dim3(launch_blocks(rows.n, held != 0.0f ? kHeldBlocks : kMaxPartials)), dim3(64),
-                     0, stream, rows, teacher, saved, scale, held, grad_scale, dlogits);
-  return last_launch_status();
+  const DistillGrad grad = {{{}, teacher, 0.0f, 0.0f}, saved, grad_scale};
+  return launch_gradient<T, false>(rows, grad, scale, held, dlogits, board_ints(teacher.K), stream);
 }
 
 template <class T>
@@ -325,12 +357,20 @@ int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits
     Order order = {};
     if (kRowAfterRow<G> && rows.mask) order = take_order(rows, s, stream);
     hipLaunchKernelGGL((distill_kernel<T, G, V>), dim3(partials), dim3(kBlock),
-                       board_bytes(d.teacher.K, std::max(2, kBlock / G)), stream, rows, d, order,
+                       (size_t)board_ints(d.teacher.K) * std::max(2, kBlock / G) * sizeof(int), stream, rows, d, order,
                        dlogits);
     return last_launch_status();
   };
   return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
     const DistillJoin join = {d, {}};
+    if (dlogits && rows.n <= kMaxPartials) {
+      DistillSplit split = {{{}, d.teacher, 0.0f, 0.0f}, d, s.parts, 1, 0.0f};
+      partials = (int)rows.n;
+      if (const int code = launch_parts<T, false>(rows, s, join, true, stream, split.splits))
+        return code;
+      return launch_gradient<T, false>(rows, split, nullptr, 0.0f, dlogits,
+                                       board_ints(d.teacher.K), stream);
+    }
     partials = launch_blocks(rows.n, kMaxPartials);
     if (const int code = launch_statistics<T, false, false>(rows, s, join, true, stream))
       return code;

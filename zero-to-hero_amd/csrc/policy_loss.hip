@@ -179,12 +179,49 @@ struct PolicyJoin {
   __device__ __forceinline__ void end() { leave_sums(sums, p.sums); }
 };
 
-struct PolicyGrad {
+struct PolicyGrad : GradientTerms {
   const Saved* saved;
   const float* coef;
   float grad_scale;
-  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, float, int a) const {
+  template <class T, int G>
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T*, float, int a, int, bool,
+                                      int*) const {
     return row_grad(saved[r], grad_scale * coef[r], grad_scale * coef[rows.n + r], rows.inv_tau, a);
+  }
+};
+
+// Rows' parts joined where the gradient is formed, by each piece of a row for itself: a
+// launch less.  A row's own sums stand in the place of a workgroup's.
+struct PolicySplit : GradientTerms {
+  Policy p;
+  const Stat* parts;
+  int splits;
+  float inverse;
+
+  __device__ __forceinline__ void begin() { inverse = inverse_count(p.weights); }
+  __device__ __forceinline__ void leave(const Rows& rows, int64_t r, const RowLoss& loss) const {
+    double sums[kSums] = {};
+    loss.add_to(sums);
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) p.sums[(int64_t)k * kMaxPartials + r] = sums[k];
+  }
+  __device__ __forceinline__ void masked(const Rows& rows, int64_t r, bool first) const {
+    if (!first) return;
+    leave_masked(p, rows, r);
+    leave(rows, r, RowLoss{});
+  }
+  template <class T, int G>
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T* row, float, int a, int t,
+                                      bool first, int*) const {
+    const RowTerms terms = row_terms<true>(join_parts<G, true>(parts, r, splits, rows.c),
+                                           action_logit(row, a), rows.c);
+    float gl, ge;
+    const RowLoss loss = policy_row(p, row_in(p, rows, r, inverse), terms, gl, ge);
+    if (first && t == 0) {
+      leave(rows, r, loss);
+      leave_row(p, rows, r, terms, gl, ge);
+    }
+    return row_grad(saved_of(terms, 0.0f), gl * p.grad_scale, ge * p.grad_scale, rows.inv_tau, a);
   }
 };
 
@@ -253,14 +290,23 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
   };
   return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
     PolicyJoin join = {p, {}, rows.n};
+    if (dlogits && rows.n <= kMaxPartials) {
+      PolicySplit split = {{}, p, s.parts, 1, 0.0f};
+      partials = (int)rows.n;
+      if (const int code =
+              launch_parts<T, true>(rows, s, join, true, stream, split.splits))
+        return code;
+      return grad_entropy
+                 ? launch_gradient<T, true>(rows, split, nullptr, 0.0f, dlogits, 0, stream)
+                 : launch_gradient<T, false>(rows, split, nullptr, 0.0f, dlogits, 0, stream);
+    }
     partials = launch_blocks(rows.n, kMaxPartials);
     if (const int code = launch_statistics<T, true, false>(rows, s, join, true, stream))
       return code;
     if (!dlogits) return (int)PPO_OK;
-    const PolicyGrad grad = {p.saved, p.coef, p.grad_scale};
-    return grad_entropy
-               ? launch_gradient<T, true>(rows, grad, nullptr, 0.0f, dlogits, stream)
-               : launch_gradient<T, false>(rows, grad, nullptr, 0.0f, dlogits, stream);
+    const PolicyGrad grad = {{}, p.saved, p.coef, p.grad_scale};
+    return grad_entropy ? launch_gradient<T, true>(rows, grad, nullptr, 0.0f, dlogits, 0, stream)
+                        : launch_gradient<T, false>(rows, grad, nullptr, 0.0f, dlogits, 0, stream);
   });
 }
 

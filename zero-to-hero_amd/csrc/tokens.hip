@@ -187,11 +187,13 @@ struct LogProbs {
 };
 
 // The gradient of a row's log-probability and entropy.
-struct LogProbsGrad {
+struct LogProbsGrad : GradientTerms {
   const Saved* saved;
   const float *dlp, *dent;
 
-  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, float up, int a) const {
+  template <class T, int G>
+  __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T*, float up, int a, int,
+                                      bool, int*) const {
     return row_grad(saved[r], dlp ? up * dlp[r] : 0.0f, dent ? up * dent[r] : 0.0f, rows.inv_tau, a);
   }
 };
@@ -218,6 +220,7 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
   for (int k = 0; k < 2; ++k) {
     const int64_t at = (i + k * p.pairs) * p.T;
     double x = 0.0, m = 0.0;
+#pragma unroll 4
     for (int64_t j = t; j < p.T; j += G) {
       const bool live = !p.mask || p.mask[at + j];
       const float rel = p.rel[at + j];  // (both loads at once)
@@ -255,11 +258,13 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
     p.rewards[i] = (float)r0;
     p.rewards[i + p.pairs] = (float)r1;
   }
-  for (int64_t j = t; j < 2 * p.T; j += G) {
-    const bool second = j >= p.T;
-    const int64_t at = second ? (i + p.pairs) * p.T + (j - p.T) : i * p.T + j;
-    const double g = dm / (double)p.pairs * p.beta * (second ? -w1 : w0);
-    p.coef[at] = !p.mask || p.mask[at] ? (float)g : 0.0f;
+  const double each = dm / (double)p.pairs * p.beta;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float g = (float)(each * (k ? -w1 : w0));
+    const int64_t at = (i + k * p.pairs) * p.T;
+#pragma unroll 4
+    for (int64_t j = t; j < p.T; j += G) p.coef[at + j] = !p.mask || p.mask[at + j] ? g : 0.0f;
   }
   // (0 times an infinite part is no part; a NaN margin stays one)
   return (p.smoothing < 1.0 ? (1.0 - p.smoothing) * up : 0.0) +
@@ -343,13 +348,13 @@ extern "C" int ppo_token_log_probs_backward(const ppo_token_rows* r, const float
   if (!saved || !aligned16(saved) || (!d_log_probs && !d_entropy) || !dlogits || (held != 0.0 && !scale) ||
       (uintptr_t)dlogits % dtype_size(r->dtype))
     return PPO_ERR_INVALID_ARG;
-  const LogProbsGrad grad = {reinterpret_cast<const Saved*>(saved), d_log_probs, d_entropy};
+  const LogProbsGrad grad = {{}, reinterpret_cast<const Saved*>(saved), d_log_probs, d_entropy};
   return with_dtype(r->dtype, [&](auto zero) {
     using T = decltype(zero);
     hipStream_t stream = (hipStream_t)stream_ptr;
     return d_entropy
-               ? launch_gradient<T, true>(rows, grad, scale, (float)held, (T*)dlogits, stream)
-               : launch_gradient<T, false>(rows, grad, scale, (float)held, (T*)dlogits, stream);
+               ? launch_gradient<T, true>(rows, grad, scale, (float)held, (T*)dlogits, 0, stream)
+               : launch_gradient<T, false>(rows, grad, scale, (float)held, (T*)dlogits, 0, stream);
   });
 }
 

@@ -114,8 +114,7 @@ __global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit, const St
     const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
     const int a = rows.actions ? rows.action(r) : -1;
     const float la = action_logit(row, a);
-    Stat x = lane < splits ? parts[r * splits + lane] : Stat{kNegInf, 0.0f, 0.0f};
-    x = lanes_join<kWave, kEntropy>(x, rows.c);
+    const Stat x = join_parts<kWave, kEntropy>(parts, r, splits, rows.c);
     if constexpr (Emit::kWholeWave)
       emit.row(rows, r, row, x, lane);
     else
@@ -127,6 +126,28 @@ __global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit, const St
 // Logits that the last-level cache holds from the forward to the backward pass (at 412 MB
 // of them 208 -> 200 us for both, at 537 as much as without).
 constexpr int64_t kReadAgain = (int64_t)512 << 20;
+
+// Enqueues the parts of every row's statistics; their number.
+template <class T, bool kEntropy, class Emit>
+int launch_parts(const Rows& rows, const Scratch& s, const Emit& emit, bool again,
+                 hipStream_t stream, int& splits) {
+  splits = row_splits(rows.n, rows.A, sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16);
+  if (rows.n > (((int64_t)1 << 31) - 1) / splits) return PPO_ERR_TOO_LARGE;
+  hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
+                     dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
+                     splits, again);
+  return last_launch_status();
+}
+
+// The parts of row r as one, by every group of lanes that asks for them (groups smaller
+// than a wave have rows of one part).
+template <int G, bool kEntropy>
+__device__ __forceinline__ Stat join_parts(const Stat* parts, int64_t r, int splits, float c) {
+  if (G < kWave) return parts[r];
+  const int lane = threadIdx.x & (kWave - 1);
+  const Stat x = lane < splits ? parts[r * splits + lane] : Stat{kNegInf, 0.0f, 0.0f};
+  return lanes_join<kWave, kEntropy>(x, c);
+}
 
 template <class T, bool kEntropy, bool kMayDirect, class Emit>
 int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, bool again,
@@ -147,25 +168,46 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, bool
       if (chunks <= 512) return go(Int<64>{});
       return go(Int<256>{});
     }
-  if (rows.n > ((int64_t)1 << 31) / splits - 1) return PPO_ERR_TOO_LARGE;
-  hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
-                     dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
-                     splits, again);
+  int parts;
+  if (const int code = launch_parts<T, kEntropy>(rows, s, emit, again, stream, parts)) return code;
   hipLaunchKernelGGL((join_kernel<T, kEntropy, Emit>), dim3(launch_blocks(rows.n, kMaxPartials)),
                      dim3(64), 0, stream, rows, emit, s.parts, splits);
   return last_launch_status();
 }
+
+// What a gradient pass asks of a row, by the G lanes of one of its pieces: begin() comes
+// before the first, with all lanes of every wave; row() gives its terms (called by whole groups, so lanes may work together; `first`: the row's first
+// piece, t the lane in its group, board the group's or the wave's share of LDS), masked()
+// is called for a row that does not count, after() when the piece is written (kAfter).
+struct GradientTerms {
+  static constexpr bool kAfter = false;
+  __device__ __forceinline__ void begin() {}
+  __device__ __forceinline__ void masked(const Rows&, int64_t, bool) const {}
+};
+
+// Columns of a piece of a row: [from, to) of its body, and its ends where it is the first.
+struct PieceColumns {
+  int from, to, body, body_end;
+  bool first;
+  __device__ __forceinline__ bool has(int col) const {
+    return col >= body && col < body_end ? col >= from && col < to : first;
+  }
+};
 
 // dlogits from the logits and the rows' terms: G lanes to a piece of a row, four
 // chunks to a lane.  What bounds it: HBM, one read and one write of the rows.
 constexpr int kGradU = 4;
 template <class T, int G, bool kC, class Terms>
 __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, const float* scale,
-                                                       float held, T* dlogits, int64_t pieces) {
+                                                       float held, T* dlogits, int64_t pieces,
+                                                       int board_ints) {
   constexpr int kN = kPer16<T>;
+  extern __shared__ int s_boards[];
   const float up = scale ? *scale : 1.0f;
   if (held != 0.0f && up == held) return;
+  terms.begin();
   const int t = threadIdx.x % G;
+  int* board = s_boards + threadIdx.x / (G < kWave ? G : kWave) * board_ints;
   const int64_t groups = rows.n * pieces, step = (int64_t)gridDim.x * (256 / G);
   for (int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; group < groups;
        group += step) {
@@ -186,6 +228,7 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
       for (int k = 0; k < kGradU; ++k)
         if (first + k * G < cut.nvec) store16(to + (int64_t)first * kN + k * per, none, true);
       if (ends) out[end_col] = from_f32<T>(0.0f);
+      terms.masked(rows, r, piece == 0 && t == 0);
       continue;
     }
     const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
@@ -194,7 +237,8 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
     for (int k = 0; k < kGradU; ++k)
       if (first + k * G < cut.nvec) w[k] = __builtin_nontemporal_load(body + first + k * G);
     const float end = ends ? to_f32(row[end_col]) : kNegInf;
-    const Grad g = terms.row(rows, r, up, rows.actions ? rows.action(r) : -1);
+    const Grad g = terms.template row<T, G>(rows, r, row, up, rows.actions ? rows.action(r) : -1, t,
+                                            piece == 0, board);
     const bool vec = ((uintptr_t)to & 15) == 0;
     const int b = g.a - cut.head;
     const int va = g.a >= 0 && b >= 0 ? b / kN : -1;
@@ -211,6 +255,18 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
       store16(to + (int64_t)v * kN, pack<T>(d), vec);
     }
     if (ends) out[end_col] = from_f32<T>(end_col == g.a ? g.da : grad_at<kC>(g, rows.c, end));
+    if constexpr (Terms::kAfter) {
+      if (G > kWave)
+        __syncthreads();  // (the piece is written, by all its waves)
+      else
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int from = cut.head + piece * (G * kGradU) * kN;
+      const PieceColumns cols = {from, from + G * kGradU * kN, cut.head, cut.head + cut.nvec * kN,
+                                 piece == 0};
+      if (G <= kWave || threadIdx.x < kWave)
+        terms.template after<T, G>(rows, g, out, cols, t, board);
+      if (G > kWave) lds_barrier();
+    }
   }
 }
 
@@ -219,7 +275,7 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
 constexpr int64_t kHeldBlocks = 2048;
 template <class T, bool kC, class Terms>
 int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, float held,
-                    T* dlogits, hipStream_t stream) {
+                    T* dlogits, int board_ints, hipStream_t stream) {
   const int dtype = sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16;
   const int64_t chunks = chunks_of(rows.A, dtype);
   auto go = [&](auto lanes) {
@@ -228,7 +284,8 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
     const int64_t most = held != 0.0f ? kHeldBlocks : ((int64_t)1 << 31) - 1;
     hipLaunchKernelGGL((gradient_kernel<T, G, kC, Terms>),
                        dim3((unsigned)std::min(div_up(rows.n * pieces, 256 / G), most)), dim3(256),
-                       0, stream, rows, terms, scale, held, dlogits, pieces);
+                       (size_t)board_ints * (256 / std::min(G, kWave)) * sizeof(int), stream, rows,
+                       terms, scale, held, dlogits, pieces, board_ints);
     return last_launch_status();
   };
   if (chunks <= 64) return go(Int<16>{});
@@ -285,8 +342,9 @@ struct Walk {
   }
 };
 
-// (without gradients: as if they started at a multiple of 16, so that a loss has the
-// same bits with and without them where its caller allocates them so)
+// Whether gradients lie in 16 bytes as the logits do.  (Without gradients: as if they
+// started at a multiple of 16, as a caller's allocation does, so that such a loss takes
+// the same layout and has the same bits with and without them.)
 inline bool lies_alike(const void* logits, const void* dlogits) {
   return ((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0;
 }
