@@ -29,6 +29,26 @@ tensor raises NotImplementedError, as there is no CPU fallback.
       the layers of layers.py; a seed that changes from call to call goes
       into `seed_at` (int64 [1] on the device), which `seed` stands back for
 
+  ppo_amd::token_log_probs(logits, actions, mask?, temperature)
+      -> (log_probs, entropy, saved), saved what the backward pass reads
+  ppo_amd::token_policy_loss(logits, actions, old_log_probs, advantages,
+      ref_log_probs?, mask?, clip_low, clip_high, kl_coef, entropy_coef,
+      temperature, reduction, denominator?) -> (scalars[6], saved, coef)
+  ppo_amd::preference_loss(logits, actions, ref_log_probs?, mask?, beta,
+      label_smoothing, margin, average, temperature)
+      -> (loss, rewards, saved, coef)
+  ppo_amd::token_log_probs_backward(logits, actions, mask?, temperature, saved,
+      d_log_probs, d_entropy?, scale?) -> dlogits
+      the backward pass of these three: a loss's coef is its gradient in the
+      log-probabilities (and entropies), scale its incoming gradient
+  ppo_amd::distillation_loss(logits, teacher_logits, teacher_ids, mask?,
+      temperature, reduction, denominator?) -> (loss, saved), and
+  ppo_amd::distillation_loss_backward(logits, teacher_logits, teacher_ids,
+      mask?, temperature, saved, scale) -> dlogits
+  ppo_amd::top_logits(logits, k) -> (values, ids)
+      the token policies of tokens.py; the losses form their gradient in the
+      backward pass here, from the logits
+
 The loss operators are differentiable in their first output: backward of
 scalars[0] (the total loss; the other scalars are reported values) scales the
 fused kernel's gradients by the incoming gradient, as ops.ppo_loss_discrete
@@ -40,7 +60,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import _lib, layers, ops
+from . import _lib, layers, ops, tokens
 
 _NS = "ppo_amd"
 
@@ -267,3 +287,225 @@ def int8_linear(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
 def _int8_linear_fake(x, weight, weight_scale, bias, x_scale, out_dtype):
     return x.new_empty((*x.shape[:-1], weight.shape[0]),
                        dtype=x.dtype if out_dtype is None else out_dtype)
+
+
+# ---------------------------------------------------------------------------
+# Token policies
+# ---------------------------------------------------------------------------
+def _row_floats(logits: Tensor) -> Tensor:
+    return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+
+
+def _row_count(logits: Tensor):
+    n = 1
+    for k in logits.shape[:-1]:
+        n = n * k
+    return n
+
+
+def _saved_like(logits: Tensor) -> Tensor:
+    return logits.new_empty((_row_count(logits), _lib.PPO_TOKEN_SAVED), dtype=torch.float32)
+
+
+def _check_saved(logits: Tensor, saved: Tensor) -> None:
+    tokens._require(saved, "saved", (torch.float32,), logits.device)
+    if saved.shape != (_row_count(logits), _lib.PPO_TOKEN_SAVED):
+        raise ValueError(f"saved must be {(_row_count(logits), _lib.PPO_TOKEN_SAVED)}, got "
+                         f"{tuple(saved.shape)}")
+
+
+def _check_scalar(logits: Tensor, scale: Optional[Tensor]) -> None:
+    if scale is not None:
+        tokens._require(scale, "scale", (torch.float32,), logits.device)
+        if scale.numel() != 1:
+            raise ValueError(f"scale must hold one value, got {scale.numel()}")
+
+
+@torch.library.custom_op(f"{_NS}::token_log_probs", mutates_args=(), device_types="cuda")
+def token_log_probs(logits: Tensor, actions: Tensor, mask: Optional[Tensor], temperature: float
+                    ) -> tuple[Tensor, Tensor, Tensor]:
+    tokens._check_logits(logits, temperature)
+    tokens._check_actions(logits, actions, mask)
+    return tokens._log_probs(logits, actions, mask, temperature, None, True, True)
+
+
+@token_log_probs.register_fake
+def _token_log_probs_fake(logits, actions, mask, temperature):
+    return _row_floats(logits), _row_floats(logits), _saved_like(logits)
+
+
+@torch.library.custom_op(f"{_NS}::token_log_probs_backward", mutates_args=(), device_types="cuda")
+def token_log_probs_backward(logits: Tensor, actions: Tensor, mask: Optional[Tensor],
+                             temperature: float, saved: Tensor, d_log_probs: Tensor,
+                             d_entropy: Optional[Tensor], scale: Optional[Tensor]) -> Tensor:
+    tokens._check_logits(logits, temperature)
+    tokens._check_actions(logits, actions, mask)
+    _check_saved(logits, saved)
+    _check_scalar(logits, scale)
+    tokens._check_rows(logits, d_log_probs, "d_log_probs", (torch.float32,))
+    if d_entropy is not None:
+        tokens._check_rows(logits, d_entropy, "d_entropy", (torch.float32,))
+    return tokens._log_probs_backward(logits, actions, mask, temperature, saved, d_log_probs,
+                                      d_entropy, scale)
+
+
+@token_log_probs_backward.register_fake
+def _token_log_probs_backward_fake(logits, actions, mask, temperature, saved, d_log_probs,
+                                   d_entropy, scale):
+    return torch.empty_like(logits)
+
+
+def _token_log_probs_setup(ctx, inputs, output):
+    logits, actions, mask, ctx.temperature = inputs
+    ctx.mark_non_differentiable(output[2])
+    ctx.save_for_backward(logits, actions, mask, output[2])
+
+
+def _token_log_probs_grad(ctx, dlp, dH, _):
+    logits, actions, mask, saved = ctx.saved_tensors
+    d = token_log_probs_backward(logits, actions, mask, ctx.temperature, saved, dlp.contiguous(),
+                                 dH.contiguous(), None)
+    return d, None, None, None
+
+
+token_log_probs.register_autograd(_token_log_probs_grad, setup_context=_token_log_probs_setup)
+
+
+@torch.library.custom_op(f"{_NS}::token_policy_loss", mutates_args=(), device_types="cuda")
+def token_policy_loss(logits: Tensor, actions: Tensor, old_log_probs: Tensor, advantages: Tensor,
+                      ref_log_probs: Optional[Tensor], mask: Optional[Tensor], clip_low: float,
+                      clip_high: float, kl_coef: float, entropy_coef: float, temperature: float,
+                      reduction: str, denominator: Optional[float]
+                      ) -> tuple[Tensor, Tensor, Tensor]:
+    per_sequence = tokens._check_policy(logits, actions, old_log_probs, advantages, ref_log_probs,
+                                        mask, clip_low, clip_high, kl_coef, entropy_coef,
+                                        temperature)
+    tokens._check_weights(reduction, denominator, 1.0)
+    loss = tokens._loss(reduction, denominator, 1.0, clip_low, clip_high, kl_coef, entropy_coef,
+                        per_sequence)
+    scalars, saved, coef, _ = tokens._policy(logits, actions, old_log_probs, advantages,
+                                             ref_log_probs, mask, temperature, loss, True, False)
+    return scalars, saved, coef.view(2, *logits.shape[:-1])
+
+
+@token_policy_loss.register_fake
+def _token_policy_loss_fake(logits, actions, old_log_probs, advantages, ref_log_probs, mask,
+                            clip_low, clip_high, kl_coef, entropy_coef, temperature, reduction,
+                            denominator):
+    return (logits.new_empty(_lib.PPO_TOKEN_SCALARS, dtype=torch.float32), _saved_like(logits),
+            logits.new_empty((2, *logits.shape[:-1]), dtype=torch.float32))
+
+
+def _token_policy_setup(ctx, inputs, output):
+    logits, actions, mask, ctx.temperature = inputs[0], inputs[1], inputs[5], inputs[10]
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.save_for_backward(logits, actions, mask, output[1], output[2])
+
+
+def _token_policy_grad(ctx, d_scalars, *_):
+    logits, actions, mask, saved, coef = ctx.saved_tensors
+    d = token_log_probs_backward(logits, actions, mask, ctx.temperature, saved, coef[0], coef[1],
+                                 d_scalars[0].clone())
+    return (d,) + (None,) * 12
+
+
+token_policy_loss.register_autograd(_token_policy_grad, setup_context=_token_policy_setup)
+
+
+@torch.library.custom_op(f"{_NS}::preference_loss", mutates_args=(), device_types="cuda")
+def preference_loss(logits: Tensor, actions: Tensor, ref_log_probs: Optional[Tensor],
+                    mask: Optional[Tensor], beta: float, label_smoothing: float, margin: float,
+                    average: bool, temperature: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    tokens._check_preference(logits, actions, ref_log_probs, mask, beta, label_smoothing, margin,
+                             temperature)
+    relative, _, saved = tokens._log_probs(logits, actions, mask, temperature, ref_log_probs, False,
+                                           True)
+    loss, rewards, coef = tokens._preference(relative, mask, beta, margin, label_smoothing, average)
+    return loss, rewards, saved, coef
+
+
+@preference_loss.register_fake
+def _preference_loss_fake(logits, actions, ref_log_probs, mask, beta, label_smoothing, margin,
+                          average, temperature):
+    return (logits.new_empty((), dtype=torch.float32),
+            logits.new_empty(logits.shape[0], dtype=torch.float32), _saved_like(logits),
+            _row_floats(logits))
+
+
+def _preference_setup(ctx, inputs, output):
+    logits, actions, mask, ctx.temperature = inputs[0], inputs[1], inputs[3], inputs[8]
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.save_for_backward(logits, actions, mask, output[2], output[3])
+
+
+def _preference_grad(ctx, d_loss, *_):
+    logits, actions, mask, saved, coef = ctx.saved_tensors
+    d = token_log_probs_backward(logits, actions, mask, ctx.temperature, saved, coef, None,
+                                 d_loss.contiguous())
+    return (d,) + (None,) * 8
+
+
+preference_loss.register_autograd(_preference_grad, setup_context=_preference_setup)
+
+
+@torch.library.custom_op(f"{_NS}::distillation_loss", mutates_args=(), device_types="cuda")
+def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor,
+                      mask: Optional[Tensor], temperature: float, reduction: str,
+                      denominator: Optional[float]) -> tuple[Tensor, Tensor]:
+    tokens._check_distillation(logits, teacher_logits, teacher_ids, mask, temperature)
+    tokens._check_weights(reduction, denominator, 1.0)
+    loss = tokens._loss(reduction, denominator, 1.0)
+    out, saved, _ = tokens._distill(logits, teacher_logits, teacher_ids, mask, temperature, loss,
+                                    True, False)
+    return out, saved
+
+
+@distillation_loss.register_fake
+def _distillation_loss_fake(logits, teacher_logits, teacher_ids, mask, temperature, reduction,
+                            denominator):
+    return logits.new_empty((), dtype=torch.float32), _saved_like(logits)
+
+
+@torch.library.custom_op(f"{_NS}::distillation_loss_backward", mutates_args=(),
+                         device_types="cuda")
+def distillation_loss_backward(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor,
+                               mask: Optional[Tensor], temperature: float, saved: Tensor,
+                               scale: Tensor) -> Tensor:
+    tokens._check_distillation(logits, teacher_logits, teacher_ids, mask, temperature)
+    _check_saved(logits, saved)
+    _check_scalar(logits, scale)
+    return tokens._distill_backward(logits, teacher_logits, teacher_ids, mask, temperature, saved,
+                                    scale)
+
+
+@distillation_loss_backward.register_fake
+def _distillation_loss_backward_fake(logits, teacher_logits, teacher_ids, mask, temperature, saved,
+                                     scale):
+    return torch.empty_like(logits)
+
+
+def _distillation_setup(ctx, inputs, output):
+    logits, teacher, ids, mask, ctx.temperature = inputs[:5]
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(logits, teacher, ids, mask, output[1])
+
+
+def _distillation_grad(ctx, d_loss, _):
+    logits, teacher, ids, mask, saved = ctx.saved_tensors
+    d = distillation_loss_backward(logits, teacher, ids, mask, ctx.temperature, saved,
+                                   d_loss.contiguous())
+    return (d,) + (None,) * 6
+
+
+distillation_loss.register_autograd(_distillation_grad, setup_context=_distillation_setup)
+
+
+@torch.library.custom_op(f"{_NS}::top_logits", mutates_args=(), device_types="cuda")
+def top_logits(logits: Tensor, k: int) -> tuple[Tensor, Tensor]:
+    return tokens.top_logits(logits, k)
+
+
+@top_logits.register_fake
+def _top_logits_fake(logits, k):
+    shape = (*logits.shape[:-1], k)
+    return logits.new_empty(shape), logits.new_empty(shape, dtype=torch.int64)
