@@ -23,7 +23,10 @@
  * logits, the action and the row's other inputs are not read, its
  * log-probability, entropy and gradients are 0, and it has no part in a loss.
  *
- * Rows times A below 2^46, rows below 2^31, A up to 2^30: PPO_ERR_TOO_LARGE
+ * Logits that another stream writes during a call give undefined results (top's
+ * columns lie in their rows all the same).
+ *
+ * Rows times A up to 2^46, rows below 2^31, A up to 2^30: PPO_ERR_TOO_LARGE
  * otherwise.
  */
 #ifndef PPO_TOKENS_H

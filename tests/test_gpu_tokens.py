@@ -641,6 +641,27 @@ def test_top_logits_ties_and_values_that_are_not_finite(dev, dtype, A):
     assert bool(same.all())
 
 
+def test_top_logits_that_change_meanwhile(dev):
+    """Logits written by another stream during the call: which are found is undefined,
+    but every column lies in its row and every value is NaN or was there."""
+    g = torch.Generator(dev).manual_seed(3)
+    for R, A in ((2, 131072), (700, 4000)):
+        x = torch.randn(R, A, device=dev, generator=g)
+        noise = torch.randn(R, A, device=dev, generator=g)
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            with torch.cuda.stream(side):
+                for _ in range(8):
+                    x.neg_()
+                    x.copy_(noise)
+            v, i = ppo_amd.top_logits(x, 40)
+            torch.cuda.synchronize()
+            assert bool(((i >= 0) & (i < A)).all())
+        v, i = ppo_amd.top_logits(x, 40)
+        assert torch.equal(v, x.gather(1, i)) and torch.equal(v, x.sort(1, descending=True).values[:, :40])
+
+
 # --- whole calls -----------------------------------------------------------------------------------
 
 def losses(dev, t, S=4, T=9, A=2500, K=12, seed=5):

@@ -88,16 +88,27 @@ __device__ __forceinline__ unsigned bound_of(Board<G>& b, int K, unsigned best) 
   return b.bound;
 }
 
-// Calls out(rank, element) for each of the listed elements among the K largest.
+// Calls out(rank, element) for each of the listed elements among the K largest, and for
+// ranks that none has with element 0.  (There are such only where the logits change
+// between the looks at them; no address may then come from what was never found.)
 template <int G, class Out>
 __device__ __forceinline__ void ranked(const Board<G>& b, int K, Out&& out) {
-  const int n = b.count;
+  const int n = min(b.count, kSorted);
   for (int i = threadIdx.x; i < n; i += G) {
     const u64 x = b.list[i];
     int rank = 0;
     for (int k = 0; k < n; ++k) rank += b.list[k] > x;
     if (rank < K) out(rank, x);
   }
+  for (int k = n + threadIdx.x; k < K; k += G) out(k, 0);
+}
+
+// A row's result of one rank.
+template <class T>
+__device__ __forceinline__ void leave(const T* row, u64 x, T* value, int64_t* id) {
+  const int col = x ? column_of(x) : 0;
+  *value = x ? row[col] : from_f32<T>(PPO_NAN);
+  *id = col;
 }
 
 // A row, or a part of one from column `from` on.
@@ -274,14 +285,11 @@ __global__ void __launch_bounds__(G) top_kernel(const T* logits, int A, int K, i
   if (b.count > kSorted) settle(p, b, want);
   if (parts == 1) {
     ranked<G>(b, K, [&](int rank, u64 e) {
-      const int col = column_of(e);
-      values[r * K + rank] = p.row[col];
-      ids[r * K + rank] = col;
+      leave(p.row, e, values + r * K + rank, ids + r * K + rank);
     });
   } else {
     u64* to = found + (int64_t)blockIdx.x * K;
     ranked<G>(b, K, [&](int rank, u64 e) { to[rank] = e; });
-    for (int k = width + t; k < K; k += G) to[k] = 0;
   }
 }
 
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
   const unsigned bound = bound_of(b, K, best);
 #pragma unroll
   for (int i = 0; i < kMergeV; ++i)
-    if ((unsigned)(x[i] >> 32) >= bound) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));
+    if ((unsigned)(x[i] >> 32) >= bound) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));  // (above 0)
   lds_barrier();
   if (b.count > kSorted) {  // (no two are alike: the K-th by its bits)
     lds_barrier();
@@ -321,13 +329,11 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < kMergeV; ++i)
-      if (x[i] >= kth) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));
+      if (x[i] && x[i] >= kth) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));
     lds_barrier();
   }
   ranked<1024>(b, K, [&](int rank, u64 e) {
-    const int col = column_of(e);
-    values[r * K + rank] = logits[r * A + col];
-    ids[r * K + rank] = col;
+    leave(logits + r * A, e, values + r * K + rank, ids + r * K + rank);
   });
 }
 
