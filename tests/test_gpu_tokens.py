@@ -319,7 +319,8 @@ def policy_want(c, S, T, tau, low, high, kc, ec, mask, reduction, denominator, t
     return order, want, bound
 
 
-POLICY_SHAPES = [(1, 1, 1), (2, 3, 5), (16, 16, 18), (3, 5, 300), (4, 9, 1000), (3, 4, 2111),
+POLICY_SHAPES = [(1, 1, 1), (2, 3, 5), (16, 16, 18), (64, 65, 900), (3, 50, 200), (3, 5, 300),
+                 (4, 9, 1000), (3, 4, 2111),
                  (2, 35, 4097), (3, 30, 9001), (2, 40, 17000), (5, 13, 33000), (2, 33, 70001),
                  (3, 2, 131071), (2, 32, 129000), (1, 2, 300001)]
 
@@ -423,7 +424,8 @@ def test_policy_loss_first_update(dev):
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(2, 1, 1), (2, 1, 7), (4, 9, 40), (8, 31, 1000), (6, 300, 257),
-                                   (2, 40, 9000), (4, 17, 40001), (2, 1, 300001)])
+                                   (2, 40, 9000), (4, 17, 40001), (2, 1, 300001), (2, 9000, 7),
+                                   (2, 17001, 5), (40, 900, 3)])
 def test_preference_loss_matches_oracle(dev, shape, dtype):
     S, T, A = shape
     t, k = TYPES[dtype], S + T + A
@@ -503,7 +505,9 @@ def distill_case(seed, t, tt, S, T, A, K):
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1), (2, 3, 5, 3), (16, 16, 18, 18), (3, 5, 300, 20),
                                    (4, 9, 1000, 64), (3, 4, 2111, 65), (2, 35, 4097, 100),
                                    (2, 40, 17000, 256), (5, 13, 33000, 7), (2, 32, 70001, 64),
-                                   (3, 2, 131071, 200), (2, 32, 129000, 64), (1, 2, 300001, 33)])
+                                   (3, 2, 131071, 200), (2, 32, 129000, 64), (1, 2, 300001, 33),
+                                   (2, 70, 40, 200), (3, 7, 300, 256), (5, 9, 500, 130),
+                                   (2, 9, 257, 129)])
 def test_distillation_matches_oracle(dev, shape, dtype):
     S, T, A, K = shape
     t, k = TYPES[dtype], S + T + A + K
@@ -660,6 +664,56 @@ def test_top_logits_that_change_meanwhile(dev):
             assert bool(((i >= 0) & (i < A)).all())
         v, i = ppo_amd.top_logits(x, 40)
         assert torch.equal(v, x.gather(1, i)) and torch.equal(v, x.sort(1, descending=True).values[:, :40])
+
+
+# Every layout with more rows than its workgroups take at once: rows, how often.
+MANY_ROWS = [(18, 512, 300), (200, 512, 300), (400, 512, 300), (900, 4096, 36), (3000, 512, 81),
+             (6000, 512, 81), (9000, 256, 36), (30000, 256, 36), (40000, 128, 9), (50304, 128, 9),
+             (65536, 128, 9), (80000, 128, 6), (100000, 128, 6), (131072, 128, 6)]
+
+
+@pytest.mark.parametrize("A, rows, times", MANY_ROWS)
+@pytest.mark.parametrize("name", ["policy", "distillation"])
+def test_many_rows(dev, name, A, rows, times):
+    """The same rows `times` times, each left out every third time: gradients as of the
+    rows by themselves, bit for bit, zeros for those left out, and sums that are a
+    multiple (of terms of one sign; a sum in 64 bits, rounded once)."""
+    t = torch.bfloat16
+    g = torch.Generator(dev).manual_seed(A)
+    rn = lambda *n: torch.randn(*n, generator=g, device=dev)  # noqa: E731
+    x = (rn(rows, A) * 2).to(t)
+    a = torch.randint(0, A, (rows,), generator=g, device=dev)
+    if name == "policy":
+        lp = ppo_amd.token_log_probs(x, a)
+        rest = (lp + 0.3 * rn(rows), rn(rows).abs() + 0.1, lp + 0.2 * rn(rows))
+        call = lambda x, a, rest, mask: ppo_amd.token_policy_loss(  # noqa: E731
+            x, a, *rest, mask, kl_coef=0.1, entropy_coef=0.01, denominator=1000.0)
+    else:
+        K = min(32, A)
+        rest = (rn(rows, K) * 2, rn(rows, A).topk(K).indices)  # (no id twice: no loss below 0)
+        call = lambda x, a, rest, mask: (ppo_amd.distillation_loss(  # noqa: E731
+            x, *rest, mask, denominator=1000.0), {})
+
+    def run(x, a, rest, mask):
+        x = x.detach().requires_grad_()
+        loss, stats = call(x, a, rest, mask)
+        return loss.detach(), stats, torch.autograd.grad(loss, [x])[0]
+
+    loss, stats, d = run(x, a, rest, None)
+    again = lambda v: v.repeat(times, *[1] * (v.dim() - 1))  # noqa: E731
+    out = (torch.arange(rows, device=dev) + torch.arange(times, device=dev)[:, None]) % 3 == 0
+    mask = ~out.view(-1)
+    many, many_stats, dm = run(again(x), again(a), [again(v) for v in rest], mask)
+    dm = dm.view(times, rows, A)
+    for k in range(times):
+        assert torch.equal(dm[k][~out[k]], d[~out[k]]), k
+        assert not dm[k][out[k]].any(), k
+    n = times * 2 / 3
+    for one, all_ in ((stats[k], many_stats[k]) for k in ("policy", "kl", "entropy", "clipfrac")
+                      if stats):
+        assert abs(float(all_) - n * float(one)) <= 2 * U32 * n * abs(float(one))
+    if not stats:
+        assert abs(float(many) - n * float(loss)) <= 2 * U32 * n * abs(float(loss))
 
 
 # --- whole calls -----------------------------------------------------------------------------------

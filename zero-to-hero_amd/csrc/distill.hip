@@ -28,19 +28,22 @@ struct Teacher {
 };
 
 // A row's entries in LDS, K of each: column, q, the sum of q over the column's entries,
-// and the student's logit there.
+// and the student's logit there; and marks of the columns met, 32 kMarkWords bits by a hash.
+constexpr int kMarkWords = 128;
 struct Board {
   int* col;
   float *q, *sum, *l;
+  unsigned* marks;
   __device__ __forceinline__ Board(int* p, int K, int place) {
     const int per = (K + 3) & ~3;
-    col = p + place * 4 * per;
+    col = p + place * (4 * per + kMarkWords);
     q = reinterpret_cast<float*>(col) + per;
     sum = q + per;
     l = sum + per;
+    marks = reinterpret_cast<unsigned*>(l) + per;
   }
 };
-int board_ints(int K) { return 4 * (int)round_up(K, 4); }
+int board_ints(int K) { return 4 * (int)round_up(K, 4) + kMarkWords; }
 
 // What the entries come to: sum q (1; 0 without entries; NaN with one that is not finite)
 // and the loss but for the student's m and log s:
@@ -81,6 +84,7 @@ __device__ __forceinline__ Entries take_entries(const Teacher& teacher, int64_t 
     if (t != kNegInf) top = fmaxf(top, l);  // (an entry that weighs nothing has no part)
   }
   for (int k = K + lane; k < ((K + 3) & ~3); k += G) b.col[k] = -1;
+  for (int k = lane; k < kMarkWords; k += G) b.marks[k] = 0;
   m = lanes_max<G>(m);
   top = lanes_max<G>(top);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -101,19 +105,28 @@ __device__ __forceinline__ Entries take_entries(const Teacher& teacher, int64_t 
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   for (int k = lane; k < K; k += G) b.q[k] *= inv;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  // Entries of one column write its sum, all of them.  Such are rare: they are looked for
-  // four at a time, and summed only where there are any.
+  // Entries of one column write its sum, all of them.  Such are rare: only where a column's
+  // mark is there already are they looked for, four at a time, and summed.
+  int met = 0;
+  for (int k = lane; k < K; k += G)
+    if (b.col[k] >= 0) {
+      const unsigned h = (unsigned)b.col[k] * 0x9E3779B1u >> 20;  // 12 bits
+      met |= atomicOr(&b.marks[h >> 5], 1u << (h & 31)) >> (h & 31) & 1;
+    }
+  const bool twice = lanes_max<G>((float)met) != 0.0f;
   for (int k = lane; k < K; k += G) {
     const int col = b.col[k];
     float q = b.q[k];
-    int same = 0;
-    for (int i = 0; i < K; i += 4) {
-      const v4i four = *reinterpret_cast<const v4i*>(b.col + i);
-      same += (four[0] == col) + (four[1] == col) + (four[2] == col) + (four[3] == col);
-    }
-    if (col >= 0 && same > 1) {
-      q = 0.0f;
-      for (int i = 0; i < K; ++i) q += b.col[i] == col ? b.q[i] : 0.0f;
+    if (twice && col >= 0) {
+      int same = 0;
+      for (int i = 0; i < K; i += 4) {
+        const v4i four = *reinterpret_cast<const v4i*>(b.col + i);
+        same += (four[0] == col) + (four[1] == col) + (four[2] == col) + (four[3] == col);
+      }
+      if (same > 1) {
+        q = 0.0f;
+        for (int i = 0; i < K; ++i) q += b.col[i] == col ? b.q[i] : 0.0f;
+      }
     }
     b.sum[k] = q;
   }
@@ -164,7 +177,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
     distill_kernel(Rows rows, Distill d, Order order, T* dlogits) {
   constexpr int kBlock = kRowBlock<G>, kGroups = kBlock / G;
   constexpr int kTeam = G < kWave ? G : kWave;  // the lanes that take the entries
-  extern __shared__ int s_board[];
+  extern __shared__ __attribute__((aligned(16))) int s_board[];
   __shared__ Stat s_part[kBlock / kWave];
   __shared__ RowShare s_row;
   const int t = threadIdx.x % G, group = group_of<G>(), K = d.teacher.K;
@@ -253,7 +266,7 @@ struct DistillJoin {
   __device__ __forceinline__ void masked(int64_t) const {}
   template <class T>
   __device__ __forceinline__ void row(const Rows& rows, int64_t r, const T* row, Stat x, int lane) {
-    __shared__ int s_board[4 * kMaxK];
+    __shared__ __attribute__((aligned(16))) int s_board[4 * kMaxK + kMarkWords];
     const Entries e = take_entries<T, kWave>(d.teacher, r, row, rows.A, rows.c, lane,
                                              Board(s_board, d.teacher.K, 0));
     const float W = d.tau * row_weight(d.weights, inverse_count(d.weights), r / rows.T);
@@ -357,11 +370,12 @@ int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits
     Order order = {};
     if (kRowAfterRow<G> && rows.mask) order = take_order(rows, s, stream);
     hipLaunchKernelGGL((distill_kernel<T, G, V>), dim3(partials), dim3(kBlock),
-                       (size_t)board_ints(d.teacher.K) * std::max(2, kBlock / G) * sizeof(int), stream, rows, d, order,
-                       dlogits);
+                       (size_t)board_ints(d.teacher.K) * std::max(2, kBlock / G) * sizeof(int), stream,
+                       rows, d, order, dlogits);
     return last_launch_status();
   };
-  return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
+  const int least = board_ints(d.teacher.K) <= kQuadBoard ? 16 : 64;
+  return with_row_shape<true>(rows.n, chunks, lies_alike(rows.logits, dlogits), least, go, [&] {
     const DistillJoin join = {d, {}};
     if (dlogits && rows.n <= kMaxPartials) {
       DistillSplit split = {{{}, d.teacher, 0.0f, 0.0f}, d, s.parts, 1, 0.0f};

@@ -288,7 +288,7 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
                          rows, p, order, dlogits);
     return last_launch_status();
   };
-  return with_row_shape(rows.n, chunks, lies_alike(rows.logits, dlogits), go, [&] {
+  return with_row_shape<false>(rows.n, chunks, lies_alike(rows.logits, dlogits), 16, go, [&] {
     PolicyJoin join = {p, {}, rows.n};
     if (dlogits && rows.n <= kMaxPartials) {
       PolicySplit split = {{}, p, s.parts, 1, 0.0f};

@@ -208,7 +208,7 @@ struct Preferences {
   float *rewards, *coef;
 };
 
-// Pair i by G lanes, a wave or a workgroup of four: the two sequences' sums in 64 bits,
+// Pair i by G lanes, a wave or a workgroup: the two sequences' sums in 64 bits,
 // the loss, and the coefficient of each of their rows.  The sums are over differences
 // to the reference's log-probabilities, so they are small where the policies are
 // alike.  Returns the loss.
@@ -238,8 +238,11 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      sum[k] = (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
-      n[k] = (part[0][2 + k] + part[1][2 + k]) + (part[2][2 + k] + part[3][2 + k]);
+      sum[k] = n[k] = 0.0;
+      for (int w = 0; w < G / kWave; ++w) {
+        sum[k] += part[w][k];
+        n[k] += part[w][2 + k];
+      }
     }
     __syncthreads();
   }
@@ -271,19 +274,24 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
          (p.smoothing > 0.0 ? p.smoothing * down : 0.0) + (m == m ? 0.0 : m);
 }
 
-// Few tokens: one workgroup of sixteen waves takes all pairs and their mean, one launch
-// where two would take 5 us more.
+// Few tokens: one workgroup takes all pairs and their mean, one launch where two would
+// take 5 us more; a wave to a pair, or all sixteen where there are few pairs.
 constexpr int64_t kFewTokens = 32768;
 __global__ void __launch_bounds__(1024) few_preferences_kernel(Preferences p, float* loss) {
-  __shared__ double part[16];
+  __shared__ double part[16][4];
   const int wave = threadIdx.x / kWave;
   double v = 0.0;
+  if (p.pairs < 8) {
+    for (int64_t i = 0; i < p.pairs; ++i) v += pair_loss<1024>(p, i, part);
+    if (threadIdx.x == 0) *loss = (float)(v / (double)p.pairs);
+    return;
+  }
   for (int64_t i = wave; i < p.pairs; i += 16) v += pair_loss<kWave>(p, i, nullptr);
-  if ((threadIdx.x & (kWave - 1)) == 0) part[wave] = v;
+  if ((threadIdx.x & (kWave - 1)) == 0) part[wave][0] = v;
   __syncthreads();
   if (threadIdx.x != 0) return;
   double all = 0.0;
-  for (int w = 0; w < 16; ++w) all += part[w];
+  for (int w = 0; w < 16; ++w) all += part[w][0];
   *loss = (float)(all / (double)p.pairs);
 }
 

@@ -100,6 +100,16 @@ __global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, S
     parts[group] = x;
 }
 
+// The parts of row r as one, by every group of lanes that asks for them (groups smaller
+// than a wave have rows of one part).
+template <int G, bool kEntropy>
+__device__ __forceinline__ Stat join_parts(const Stat* parts, int64_t r, int splits, float c) {
+  if (G < kWave) return parts[r];
+  const int lane = threadIdx.x & (kWave - 1);
+  const Stat x = lane < splits ? parts[r * splits + lane] : Stat{kNegInf, 0.0f, 0.0f};
+  return lanes_join<kWave, kEntropy>(x, c);
+}
+
 // A wave to a row: its parts joined in the order of their lanes, and the row
 // finished by its lane 0, or by the wave (kWholeWave).
 template <class T, bool kEntropy, class Emit>
@@ -137,16 +147,6 @@ int launch_parts(const Rows& rows, const Scratch& s, const Emit& emit, bool agai
                      dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
                      splits, again);
   return last_launch_status();
-}
-
-// The parts of row r as one, by every group of lanes that asks for them (groups smaller
-// than a wave have rows of one part).
-template <int G, bool kEntropy>
-__device__ __forceinline__ Stat join_parts(const Stat* parts, int64_t r, int splits, float c) {
-  if (G < kWave) return parts[r];
-  const int lane = threadIdx.x & (kWave - 1);
-  const Stat x = lane < splits ? parts[r * splits + lane] : Stat{kNegInf, 0.0f, 0.0f};
-  return lanes_join<kWave, kEntropy>(x, c);
 }
 
 template <class T, bool kEntropy, bool kMayDirect, class Emit>
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
                                                        float held, T* dlogits, int64_t pieces,
                                                        int board_ints) {
   constexpr int kN = kPer16<T>;
-  extern __shared__ int s_boards[];
+  extern __shared__ __attribute__((aligned(16))) int s_boards[];
   const float up = scale ? *scale : 1.0f;
   if (held != 0.0f && up == held) return;
   terms.begin();
@@ -273,6 +273,9 @@ __global__ void __launch_bounds__(256) gradient_kernel(Rows rows, Terms terms, c
 // A pass that may find nothing to do has workgroups enough to fill the chip, and few
 // enough to end in 2 us (131072 of them took 29); one that has work one to a piece.
 constexpr int64_t kHeldBlocks = 2048;
+// Words of LDS that each of a workgroup's sixteen groups of 16 lanes may have; with more,
+// rows go one to a wave.
+constexpr int kQuadBoard = 640;
 template <class T, bool kC, class Terms>
 int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, float held,
                     T* dlogits, int board_ints, hipStream_t stream) {
@@ -288,15 +291,20 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
                        terms, scale, held, dlogits, pieces, board_ints);
     return last_launch_status();
   };
-  if (chunks <= 64) return go(Int<16>{});
+  if (chunks <= 64 && board_ints <= kQuadBoard) return go(Int<16>{});
   if (chunks <= 512) return go(Int<64>{});
   return go(Int<256>{});
 }
 
 // How a pass that keeps its rows in registers is laid out: held(lanes, chunks a
 // lane) for the smallest group that holds a row, or split() where a row does not
-// fit, or rows are so few that one workgroup to each would leave most of the chip
-// empty, or the gradients lie otherwise in 16 bytes than the logits (not `alike`).
+// fit, or the gradients lie otherwise in 16 bytes than the logits (not `alike`), or rows
+// are so few that one workgroup to each takes longer, the more so the larger it is (a row
+// of 131072 bf16 24 us by itself; 32 of them 14 split, 128 27 either way; of 50304 100
+// rows 15 and 16; of 30000 40 rows 13 either way).  Many rows of up to 128 chunks go four
+// to a wave, which then takes their sums' ends together (16384 x 1000 bf16 24 us, 31 one
+// to a wave); none go four to a wave (`least` 64) that need more LDS than that leaves, and
+// of more than 64 chunks none that take entries (`single`).
 // A pass's workgroup, and the waves a SIMD is to hold at least: two workgroups of 512
 // lanes (65536 bf16 218 -> 214 us, 50304 198 -> 187); smaller ones do better with the
 // registers (32768 191 us, 211 with four waves to a SIMD).
@@ -348,16 +356,22 @@ struct Walk {
 inline bool lies_alike(const void* logits, const void* dlogits) {
   return ((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0;
 }
-template <class Held, class Split>
-int with_row_shape(int64_t rows, int64_t chunks, bool alike, Held&& held, Split&& split) {
+template <bool kSingle, class Held, class Split>
+int with_row_shape(int64_t rows, int64_t chunks, bool alike, int least, Held&& held,
+                   Split&& split) {
   if (!alike) return split();
-  if (chunks <= 16 * 1) return held(Int<16>{}, Int<1>{});
-  if (chunks <= 16 * 4) return held(Int<16>{}, Int<4>{});
+  if (least <= 16) {
+    if (chunks <= 16 * 1) return held(Int<16>{}, Int<1>{});
+    if (chunks <= 16 * 2) return held(Int<16>{}, Int<2>{});
+    if (chunks <= 16 * 4) return held(Int<16>{}, Int<4>{});
+  }
+  if constexpr (!kSingle)
+    if (chunks <= 16 * 8 && rows >= 4096) return held(Int<16>{}, Int<8>{});
   if (chunks <= 64 * 4) return held(Int<64>{}, Int<4>{});
   if (chunks <= 64 * 8) return held(Int<64>{}, Int<8>{});
   if (chunks <= 64 * 16) return held(Int<64>{}, Int<16>{});
-  if (rows < 64 && chunks > 256 * 8) return split();
   if (chunks <= 256 * 8) return held(Int<256>{}, Int<8>{});
+  if (rows < (chunks <= 256 * 16 ? 40 : 64)) return split();
   if (chunks <= 256 * 16) return held(Int<256>{}, Int<16>{});
   if (chunks <= 512 * 10) return held(Int<512>{}, Int<10>{});
   if (chunks <= 512 * 13) return held(Int<512>{}, Int<13>{});
