@@ -425,7 +425,8 @@ def test_policy_loss_first_update(dev):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(2, 1, 1), (2, 1, 7), (4, 9, 40), (8, 31, 1000), (6, 300, 257),
                                    (2, 40, 9000), (4, 17, 40001), (2, 1, 300001), (2, 9000, 7),
-                                   (2, 17001, 5), (40, 900, 3)])
+                                   (2, 17001, 5), (40, 900, 3), (4, 3000, 5),
+                                   (10, 65, 9), (130, 3, 6), (2000, 17, 3), (4, 9000, 2)])
 def test_preference_loss_matches_oracle(dev, shape, dtype):
     S, T, A = shape
     t, k = TYPES[dtype], S + T + A
@@ -604,7 +605,9 @@ def test_distillation_edges(dev, A):
 @pytest.mark.parametrize("shape", [(1, 1, 1), (3, 5, 5), (200, 18, 4), (7, 300, 256), (5, 1003, 64),
                                    (300, 2049, 17), (9, 8200, 200), (130, 9000, 1), (3, 16385, 50),
                                    (129, 33001, 64), (130, 66001, 100), (2, 131072, 256),
-                                   (1, 262147, 50), (1, 2000001, 256)])
+                                   (1, 262147, 50), (1, 2000001, 256),
+                                   (600, 4097, 48), (300, 512, 256), (1000, 33, 20), (5, 8200, 33),
+                                   (40, 511, 49)])
 def test_top_logits_match_a_stable_sort(dev, shape, dtype):
     R, A, k = shape
     x, _, g = rows_of(R + A + k, TYPES[dtype], R, A)

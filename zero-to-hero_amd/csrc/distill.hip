@@ -359,7 +359,7 @@ int dense_gradient(const Rows& rows, const Teacher& teacher, const Saved* saved,
 }
 
 template <class T>
-int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits, int& partials,
+int run_distill(const Rows& rows, Distill& d, const Scratch& s, T* dlogits, int& partials,
                 hipStream_t stream) {
   const int dtype = sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16;
   const int64_t chunks = chunks_of(rows.A, dtype);
@@ -368,7 +368,10 @@ int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits
     constexpr int kBlock = kRowBlock<G>;
     partials = launch_blocks(div_up(rows.n, kBlock / G), kRowBlocks<G>);
     Order order = {};
-    if (kRowAfterRow<G> && rows.mask) order = take_order(rows, s, stream);
+    if (kRowAfterRow<G> && rows.mask)
+      order = take_order(rows, d.weights, s, stream);
+    else
+      count_weights(rows, d.weights, s, stream);
     hipLaunchKernelGGL((distill_kernel<T, G, V>), dim3(partials), dim3(kBlock),
                        (size_t)board_ints(d.teacher.K) * std::max(2, kBlock / G) * sizeof(int), stream,
                        rows, d, order, dlogits);
@@ -376,6 +379,7 @@ int run_distill(const Rows& rows, const Distill& d, const Scratch& s, T* dlogits
   };
   const int least = board_ints(d.teacher.K) <= kQuadBoard ? 16 : 64;
   return with_row_shape<true>(rows.n, chunks, lies_alike(rows.logits, dlogits), least, go, [&] {
+    count_weights(rows, d.weights, s, stream);
     const DistillJoin join = {d, {}};
     if (dlogits && rows.n <= kMaxPartials) {
       DistillSplit split = {{{}, d.teacher, 0.0f, 0.0f}, d, s.parts, 1, 0.0f};
@@ -418,10 +422,10 @@ extern "C" int ppo_token_distillation(const ppo_token_rows* r, const void* teach
   if (!workspace || !aligned16(workspace) || workspace_bytes < s.bytes) return PPO_ERR_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_ptr;
   Weights weights;
-  if (const int code = take_weights(rows, loss, s, stream, weights)) return code;
-  const Distill d = {{teacher, ids, teacher_dtype, ids_are_int64, (int)K}, weights,
-                     (float)r->temperature, (float)loss->grad_scale,
-                     reinterpret_cast<Saved*>(saved), s.sums};
+  if (const int code = take_weights(rows, loss, s, weights)) return code;
+  Distill d = {{teacher, ids, teacher_dtype, ids_are_int64, (int)K}, weights,
+               (float)r->temperature, (float)loss->grad_scale, reinterpret_cast<Saved*>(saved),
+               s.sums};
   int partials = 0;
   if (rows.n)
     if (const int code = with_dtype(r->dtype, [&](auto zero) {

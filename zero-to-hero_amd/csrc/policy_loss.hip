@@ -279,7 +279,10 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
     constexpr int kBlock = kRowBlock<G>;
     partials = launch_blocks(div_up(rows.n, kBlock / G), kRowBlocks<G>);
     Order order = {};
-    if (kRowAfterRow<G> && rows.mask) order = take_order(rows, s, stream);
+    if (kRowAfterRow<G> && rows.mask)
+      order = take_order(rows, p.weights, s, stream);
+    else
+      count_weights(rows, p.weights, s, stream);
     if (grad_entropy)
       hipLaunchKernelGGL((policy_kernel<T, G, V, true>), dim3(partials), dim3(kBlock), 0, stream,
                          rows, p, order, dlogits);
@@ -289,6 +292,7 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
     return last_launch_status();
   };
   return with_row_shape<false>(rows.n, chunks, lies_alike(rows.logits, dlogits), 16, go, [&] {
+    count_weights(rows, p.weights, s, stream);
     PolicyJoin join = {p, {}, rows.n};
     if (dlogits && rows.n <= kMaxPartials) {
       PolicySplit split = {{}, p, s.parts, 1, 0.0f};
@@ -333,7 +337,7 @@ extern "C" int ppo_token_policy_loss(const ppo_token_rows* r, const float* old_l
   if (!workspace || !aligned16(workspace) || workspace_bytes < s.bytes) return PPO_ERR_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_ptr;
   Weights weights;
-  if (const int code = take_weights(rows, loss, s, stream, weights)) return code;
+  if (const int code = take_weights(rows, loss, s, weights)) return code;
   Policy p = {old_log_probs, advantages, ref_log_probs, weights, (float)(1.0 - loss->clip_low),
               (float)(1.0 + loss->clip_high), (float)loss->kl_coef, (float)loss->entropy_coef,
               (float)loss->grad_scale, loss->advantages_per_sequence,

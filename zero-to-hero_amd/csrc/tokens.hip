@@ -123,15 +123,29 @@ __global__ void __launch_bounds__(1024) order_kernel(const uint8_t* mask, int n,
 
 }  // namespace
 
-Order take_order(const Rows& rows, const Scratch& s, hipStream_t stream) {
+void count_weights(const Rows& rows, const Weights& w, const Scratch& s, hipStream_t stream) {
+  if (w.lengths)
+    hipLaunchKernelGGL(count_sequences_kernel, dim3(w.partials), dim3(256), 0, stream, rows.mask,
+                       rows.S, rows.T, s.lengths, s.counts);
+  else if (w.counts)
+    hipLaunchKernelGGL(count_rows_kernel, dim3(w.partials), dim3(256), 0, stream, rows.mask, rows.n,
+                       s.counts);
+}
+
+Order take_order(const Rows& rows, Weights& w, const Scratch& s, hipStream_t stream) {
   int* live = s.counts + kCountBlocks;
+  if (w.counts && !w.lengths) {  // (the order counts the rows, 4 us less)
+    w.counts = live;
+    w.partials = 1;
+  } else {
+    count_weights(rows, w, s, stream);
+  }
   hipLaunchKernelGGL(order_kernel, dim3(1), dim3(1024), 0, stream, rows.mask, (int)rows.n, s.order,
                      live);
   return {s.order, live};
 }
 
-int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, hipStream_t stream,
-                 Weights& w) {
+int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, Weights& w) {
   const bool sequences = loss->reduction == PPO_SEQUENCE_MEAN;
   if ((loss->reduction != PPO_TOKEN_MEAN && !sequences) || !(loss->denominator >= 0.0) ||
       !(loss->grad_scale > 0.0) || !(loss->grad_scale < INFINITY))
@@ -151,15 +165,11 @@ int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s,
     w.partials = launch_blocks(div_up(rows.S, 4), kCountBlocks);
     w.counts = s.counts;
     w.lengths = s.lengths;
-    hipLaunchKernelGGL(count_sequences_kernel, dim3(w.partials), dim3(256), 0, stream, rows.mask,
-                       rows.S, rows.T, s.lengths, s.counts);
   } else if (!(w.inverse > 0.0f)) {
     w.partials = launch_blocks(div_up(rows.n, 1024), kCountBlocks);
     w.counts = s.counts;
-    hipLaunchKernelGGL(count_rows_kernel, dim3(w.partials), dim3(256), 0, stream, rows.mask, rows.n,
-                       s.counts);
   }
-  return last_launch_status();
+  return PPO_OK;
 }
 
 namespace {
@@ -208,20 +218,22 @@ struct Preferences {
   float *rewards, *coef;
 };
 
-// Pair i by G lanes, a wave or a workgroup: the two sequences' sums in 64 bits,
-// the loss, and the coefficient of each of their rows.  The sums are over differences
-// to the reference's log-probabilities, so they are small where the policies are
-// alike.  Returns the loss.
-template <int G>
-__device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, double (*part)[4]) {
-  const int t = threadIdx.x % G, wave = threadIdx.x / kWave;
+// Pair i by `lanes` lanes (t: this one), a wave or a team of waves that all come here,
+// with i behind the last pair too: the two sequences' sums in 64 bits, the loss, and the
+// coefficient of each of their rows.  The sums are over differences to the reference's
+// log-probabilities, so they are small where the policies are alike.  Returns the loss.
+template <bool kTeam>
+__device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, int t, int lanes,
+                                            double (*part)[4]) {
+  const int wave = threadIdx.x / kWave;
+  const int64_t T = i < p.pairs ? p.T : 0;
   double sum[2], n[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int64_t at = (i + k * p.pairs) * p.T;
     double x = 0.0, m = 0.0;
 #pragma unroll 4
-    for (int64_t j = t; j < p.T; j += G) {
+    for (int64_t j = t; j < T; j += lanes) {
       const bool live = !p.mask || p.mask[at + j];
       const float rel = p.rel[at + j];  // (both loads at once)
       x += live ? (double)rel : 0.0;
@@ -229,23 +241,25 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
     }
     sum[k] = lanes_sum<kWave>(x);
     n[k] = lanes_sum<kWave>(m);
-    if (G > kWave && (t & (kWave - 1)) == 0) {
+    if (kTeam && (t & (kWave - 1)) == 0) {
       part[wave][k] = sum[k];
       part[wave][2 + k] = n[k];
     }
   }
-  if (G > kWave) {
+  if (kTeam) {
     __syncthreads();
+    const int first = wave - t / kWave;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       sum[k] = n[k] = 0.0;
-      for (int w = 0; w < G / kWave; ++w) {
+      for (int w = first; w < first + lanes / kWave; ++w) {
         sum[k] += part[w][k];
         n[k] += part[w][2 + k];
       }
     }
     __syncthreads();
   }
+  if (i >= p.pairs) return 0.0;
   const double w0 = p.average && n[0] > 0.0 ? 1.0 / n[0] : 1.0;
   const double w1 = p.average && n[1] > 0.0 ? 1.0 / n[1] : 1.0;
   const double r0 = p.beta * sum[0] * w0, r1 = p.beta * sum[1] * w1;
@@ -267,50 +281,65 @@ __device__ __forceinline__ double pair_loss(const Preferences& p, int64_t i, dou
     const float g = (float)(each * (k ? -w1 : w0));
     const int64_t at = (i + k * p.pairs) * p.T;
 #pragma unroll 4
-    for (int64_t j = t; j < p.T; j += G) p.coef[at + j] = !p.mask || p.mask[at + j] ? g : 0.0f;
+    for (int64_t j = t; j < T; j += lanes) p.coef[at + j] = !p.mask || p.mask[at + j] ? g : 0.0f;
   }
   // (0 times an infinite part is no part; a NaN margin stays one)
   return (p.smoothing < 1.0 ? (1.0 - p.smoothing) * up : 0.0) +
          (p.smoothing > 0.0 ? p.smoothing * down : 0.0) + (m == m ? 0.0 : m);
 }
 
-// Few tokens: one workgroup takes all pairs and their mean, one launch where two would
-// take 5 us more; a wave to a pair, or all sixteen where there are few pairs.
-constexpr int64_t kFewTokens = 32768;
+// Pairs whose sequences a wave takes by itself (pairs of 31 tokens 4 us, 7 by more).
+constexpr int64_t kWaveTokens = 512;
+
+// Few pairs: one workgroup takes them all and their mean, one launch where two would
+// take 5 us more; a wave to a pair, or up to eight pairs at once by a share of the sixteen
+// waves each (a pair of 16384 tokens 140 -> 17 us).
+constexpr int64_t kFewTokens = 32768, kFewPairs = 16;
 __global__ void __launch_bounds__(1024) few_preferences_kernel(Preferences p, float* loss) {
-  __shared__ double part[16][4];
-  const int wave = threadIdx.x / kWave;
+  __shared__ double part[16][4], losses[16];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   double v = 0.0;
-  if (p.pairs < 8) {
-    for (int64_t i = 0; i < p.pairs; ++i) v += pair_loss<1024>(p, i, part);
-    if (threadIdx.x == 0) *loss = (float)(v / (double)p.pairs);
-    return;
+  if (p.pairs <= 8 && p.T > kWaveTokens) {
+    const int lanes = p.pairs == 1 ? 1024 : p.pairs == 2 ? 512 : p.pairs <= 4 ? 256 : 128;
+    const int t = threadIdx.x & (lanes - 1);
+    v = pair_loss<true>(p, threadIdx.x / lanes, t, lanes, part);
+    if (t != 0) v = 0.0;  // (a pair's loss once)
+  } else if (wave < p.pairs) {
+    v = pair_loss<false>(p, wave, lane, kWave, nullptr);
   }
-  for (int64_t i = wave; i < p.pairs; i += 16) v += pair_loss<kWave>(p, i, nullptr);
-  if ((threadIdx.x & (kWave - 1)) == 0) part[wave][0] = v;
+  if (lane == 0) losses[wave] = v;
   __syncthreads();
   if (threadIdx.x != 0) return;
   double all = 0.0;
-  for (int w = 0; w < 16; ++w) all += part[w][0];
+  for (int w = 0; w < 16; ++w) all += losses[w];
   *loss = (float)(all / (double)p.pairs);
 }
 
-__global__ void __launch_bounds__(256) preferences_kernel(Preferences p) {
-  __shared__ double part[4][4];
-  for (int64_t i = blockIdx.x; i < p.pairs; i += gridDim.x) {
-    const double v = pair_loss<256>(p, i, part);
-    if (threadIdx.x == 0) p.losses[i] = v;
+// A wave to a pair, or a workgroup.
+template <bool kTeam>
+__global__ void __launch_bounds__(1024) preferences_kernel(Preferences p) {
+  __shared__ double part[16][4];
+  const int lanes = kTeam ? blockDim.x : kWave, teams = blockDim.x / lanes;
+  const int t = threadIdx.x % lanes;
+  for (int64_t i = (int64_t)blockIdx.x * teams + threadIdx.x / lanes; i < p.pairs;
+       i += (int64_t)gridDim.x * teams) {
+    const double v = pair_loss<kTeam>(p, i, t, lanes, part);
+    if (t == 0) p.losses[i] = v;
   }
 }
 
-__global__ void __launch_bounds__(256) mean_kernel(const double* x, int64_t n, float* out) {
-  __shared__ double part[4];
+__global__ void __launch_bounds__(1024) mean_kernel(const double* x, int64_t n, float* out) {
+  __shared__ double part[16];
   double v = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 256) v += x[i];
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) v += x[i];
   v = lanes_sum<kWave>(v);
   if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = v;
   __syncthreads();
-  if (threadIdx.x == 0) *out = (float)(((part[0] + part[1]) + (part[2] + part[3])) / (double)n);
+  if (threadIdx.x != 0) return;
+  double all = 0.0;
+  for (int w = 0; w < 16; ++w) all += part[w];
+  *out = (float)(all / (double)n);
 }
 
 }  // namespace
@@ -386,12 +415,16 @@ extern "C" int ppo_token_preference(const float* relative, const uint8_t* mask, 
   hipStream_t stream = (hipStream_t)stream_ptr;
   const Preferences p = {relative, mask, sequences / 2, tokens, beta, margin, smoothing, average,
                          static_cast<double*>(workspace), rewards, coef};
-  if (sequences * tokens <= kFewTokens) {
+  if (sequences * tokens <= kFewTokens && p.pairs <= kFewPairs) {
     hipLaunchKernelGGL(few_preferences_kernel, dim3(1), dim3(1024), 0, stream, p, loss);
     return last_launch_status();
   }
-  hipLaunchKernelGGL(preferences_kernel, dim3(launch_blocks(p.pairs, kMaxPartials)), dim3(256), 0,
-                     stream, p);
-  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(256), 0, stream, p.losses, p.pairs, loss);
+  if (tokens <= kWaveTokens)
+    hipLaunchKernelGGL(preferences_kernel<false>,
+                       dim3(launch_blocks(div_up(p.pairs, 4), kMaxPartials)), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL(preferences_kernel<true>, dim3(launch_blocks(p.pairs, kMaxPartials)),
+                       dim3(tokens > 2048 ? 1024 : 256), 0, stream, p);
+  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, stream, p.losses, p.pairs, loss);
   return last_launch_status();
 }

@@ -598,12 +598,11 @@ int row_splits(int64_t rows, int64_t A, int dtype);
 Scratch scratch_of(void* workspace, int64_t S, int64_t T, int64_t A, int dtype);
 // Checks rows; fills what kernels take.
 int take_rows(const ppo_token_rows* r, bool actions, Rows& out);
-// Checks a loss's weights; enqueues the counting they need.
-int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, hipStream_t stream,
-                 Weights& w);
-
-// Enqueues the ordering of rows (mask given).
-Order take_order(const Rows& rows, const Scratch& s, hipStream_t stream);
+// Checks a loss's weights; what they need counted.
+int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, Weights& w);
+// Enqueues the counting, or the ordering of rows (mask given) and the counting.
+void count_weights(const Rows& rows, const Weights& w, const Scratch& s, hipStream_t stream);
+Order take_order(const Rows& rows, Weights& w, const Scratch& s, hipStream_t stream);
 
 inline int launch_blocks(int64_t groups, int64_t most) {
   return (int)(groups < most ? groups : most);

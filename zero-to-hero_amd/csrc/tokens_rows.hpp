@@ -371,7 +371,7 @@ int with_row_shape(int64_t rows, int64_t chunks, bool alike, int least, Held&& h
   if (chunks <= 64 * 8) return held(Int<64>{}, Int<8>{});
   if (chunks <= 64 * 16) return held(Int<64>{}, Int<16>{});
   if (chunks <= 256 * 8) return held(Int<256>{}, Int<8>{});
-  if (rows < (chunks <= 256 * 16 ? 40 : 64)) return split();
+  if (rows < (chunks <= 256 * 16 ? 40 : 65)) return split();
   if (chunks <= 256 * 16) return held(Int<256>{}, Int<16>{});
   if (chunks <= 512 * 10) return held(Int<512>{}, Int<10>{});
   if (chunks <= 512 * 13) return held(Int<512>{}, Int<13>{});

@@ -15,7 +15,9 @@ namespace ppo {
 namespace {
 
 constexpr int kMaxK = PPO_TOKEN_MAX_K;
-constexpr int kSorted = 2048;  // elements that are sorted at most
+// Elements that are sorted at most.
+template <int G>
+constexpr int kSorted = G == kWave ? 512 : 2048;
 constexpr int kSegments = 4;
 
 typedef unsigned long long u64;
@@ -34,7 +36,7 @@ __device__ __forceinline__ int column_of(u64 x) { return (int)~(unsigned)x; }
 
 template <int G>
 struct Board {
-  u64 list[kSorted];
+  u64 list[kSorted<G>];
   union {
     unsigned best[G];
     unsigned short again[kSegments * G];  // lane + G segment of segments to look at again
@@ -48,7 +50,7 @@ struct Board {
 template <int G>
 __device__ __forceinline__ void append(Board<G>& b, unsigned order, int col) {
   const int at = atomicAdd(&b.count, 1);
-  if (at < kSorted) b.list[at] = place(order, col);
+  if (at < kSorted<G>) b.list[at] = place(order, col);
 }
 
 // The sum of a whole number over the workgroup, for every lane.  Two barriers.
@@ -93,7 +95,7 @@ __device__ __forceinline__ unsigned bound_of(Board<G>& b, int K, unsigned best) 
 // between the looks at them; no address may then come from what was never found.)
 template <int G, class Out>
 __device__ __forceinline__ void ranked(const Board<G>& b, int K, Out&& out) {
-  const int n = min(b.count, kSorted);
+  const int n = min(b.count, kSorted<G>);
   for (int i = threadIdx.x; i < n; i += G) {
     const u64 x = b.list[i];
     int rank = 0;
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(G) top_kernel(const T* logits, int A, int K, i
     }
   }
   lds_barrier();
-  if (b.count > kSorted) settle(p, b, want);
+  if (b.count > kSorted<G>) settle(p, b, want);
   if (parts == 1) {
     ranked<G>(b, K, [&](int rank, u64 e) {
       leave(p.row, e, values + r * K + rank, ids + r * K + rank);
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
   for (int i = 0; i < kMergeV; ++i)
     if ((unsigned)(x[i] >> 32) >= bound) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));  // (above 0)
   lds_barrier();
-  if (b.count > kSorted) {  // (no two are alike: the K-th by its bits)
+  if (b.count > kSorted<1024>) {  // (no two are alike: the K-th by its bits)
     lds_barrier();
     u64 kth = 0;
     for (u64 bit = 1ull << 63; bit; bit >>= 1) {
@@ -343,6 +345,9 @@ struct TopPlan {
   int parts, per;
 };
 constexpr int64_t kPartElements = 1 << 16;
+// Bytes of a row that a wave takes by itself (16384 x 2000 bf16 49 -> 31 us; 4096 x 4000
+// fp32 20 -> 22).
+constexpr int64_t kWaveRow = 8192;
 TopPlan plan_of(int64_t rows, int64_t A, int dtype) {
   const int64_t size = dtype_size(dtype);
   int64_t parts = div_up(A, kPartElements);
@@ -393,7 +398,11 @@ extern "C" int ppo_token_top(const void* logits, int dtype, int64_t rows, int64_
                          in, (int)A, (int)K, plan.parts, plan.per, out, ids, found);
       return last_launch_status();
     };
-    const int code = K <= 96 ? go(Int<256>{}) : K <= 192 ? go(Int<512>{}) : go(Int<1024>{});
+    const int code = plan.parts == 1 && A * dtype_size(dtype) <= kWaveRow && (K <= 48 || A <= 512)
+                         ? go(Int<kWave>{})
+                     : K <= 96  ? go(Int<256>{})
+                     : K <= 192 ? go(Int<512>{})
+                                : go(Int<1024>{});
     if (code || plan.parts == 1) return code;
     hipLaunchKernelGGL((top_merge_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, stream, in,
                        (int)A, (int)K, plan.parts, out, ids, found);
