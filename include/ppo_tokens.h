@@ -26,8 +26,8 @@
  * Logits that another stream writes during a call give undefined results (top's
  * columns lie in their rows all the same).
  *
- * Rows times A up to 2^46, rows below 2^31, A up to 2^30: PPO_ERR_TOO_LARGE
- * otherwise.
+ * Rows times A up to 2^46, A up to 2^30, rows below 2^24 (2^22 in top; more where a row
+ * takes fewer than 256 lanes): PPO_ERR_TOO_LARGE otherwise.
  */
 #ifndef PPO_TOKENS_H
 #define PPO_TOKENS_H

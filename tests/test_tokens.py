@@ -63,6 +63,21 @@ def test_rows_are_checked_by_every_call(kw, code):
     assert lib.ppo_token_distillation_backward(rows(**kw), P, 0, P, 1, 3, P, P, 0.0, P, None) == code
 
 
+def test_launches_that_do_not_fit():
+    """Calls of 2^32 lanes are refused before anything is enqueued."""
+    lib = _lib.load_tokens()
+    f, top, big = lib.ppo_token_log_probs, lib.ppo_token_top, 1 << 44
+    for S, A, dtype in ((1 << 28, 18, 0), (1 << 26, 600, 1), (1 << 24, 4096, 0), (1 << 24, 16384, 2)):
+        for entropy in (None, P):
+            assert f(rows(S=S, T=1, A=A, dtype=dtype), None, P, entropy, None, P, big, None) == 3
+        assert top(P, dtype, S, A, 3, P, P, None, 0, None) == 3
+    # (gradients that lie otherwise in 16 bytes than the logits take a workgroup a row)
+    assert lib.ppo_token_policy_loss(rows(S=1 << 24, T=1, A=18), P, P, None, loss(), P, P, P,
+                                     ctypes.c_void_p(4100), P, big, None) == 3
+    assert lib.ppo_token_distillation(rows(S=1 << 24, T=1, A=18), P, 0, P, 1, 3, loss(), P, P,
+                                      ctypes.c_void_p(4100), P, big, None) == 3
+
+
 def test_log_probs_arguments():
     lib = _lib.load_tokens()
     f = lib.ppo_token_log_probs

@@ -1,6 +1,9 @@
 // Distillation from a teacher's K top logits over wide rows of the student's,
 // forward and gradient in one pass: dlogits_j = tau w (p_j - q_j), dense in p and
-// with at most K columns of q.
+// with at most K columns of q.  Those are written over the dense row afterwards, from
+// LDS, so that no element of the row asks whether it is one.  What bounds it: HBM, one
+// read and one write of the student's logits (4096 x 65536 bf16 with a mask 194 us, 4.8
+// TB/s); few rows the chain of launches (24 x 262144 21 in a graph).
 #include "tokens_rows.hpp"
 
 namespace ppo {
@@ -379,6 +382,8 @@ int run_distill(const Rows& rows, Distill& d, const Scratch& s, T* dlogits, int&
   };
   const int least = board_ints(d.teacher.K) <= kQuadBoard ? 16 : 64;
   return with_row_shape<true>(rows.n, chunks, lies_alike(rows.logits, dlogits), least, go, [&] {
+    if (!fits_launch(rows.n * row_splits(rows.n, rows.A, dtype), 256))
+      return (int)PPO_ERR_TOO_LARGE;
     count_weights(rows, d.weights, s, stream);
     const DistillJoin join = {d, {}};
     if (dlogits && rows.n <= kMaxPartials) {

@@ -1,6 +1,11 @@
 // The clipped policy loss with a KL term over wide rows of logits, forward and
 // gradient in one pass: a row stays in the registers of its group of lanes from
-// the read to the write.
+// the read to the write.  With G and E the row's dloss/dlog p_a and dloss/dH,
+//   dlogits_j = (G ([j = a] - p_j) - E p_j (log p_j + H)) / temperature,
+// which needs the whole row's sums before its first element: hence registers, or the
+// caches for rows that do not fit.  What bounds it: HBM, one read and one write of the
+// logits (8192 x 131072 bf16 849 us, 5.06 TB/s; 4096 x 32768 with a mask 86, 5.2);
+// few rows the chain of launches (528 x 500 fp32 16 in a graph).
 #include "tokens_rows.hpp"
 
 namespace ppo {
@@ -292,6 +297,8 @@ int run_policy(const Rows& rows, Policy& p, const Scratch& s, T* dlogits, int& p
     return last_launch_status();
   };
   return with_row_shape<false>(rows.n, chunks, lies_alike(rows.logits, dlogits), 16, go, [&] {
+    if (!fits_launch(rows.n * row_splits(rows.n, rows.A, dtype), 256))
+      return (int)PPO_ERR_TOO_LARGE;
     count_weights(rows, p.weights, s, stream);
     PolicyJoin join = {p, {}, rows.n};
     if (dlogits && rows.n <= kMaxPartials) {

@@ -604,6 +604,8 @@ int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s,
 void count_weights(const Rows& rows, const Weights& w, const Scratch& s, hipStream_t stream);
 Order take_order(const Rows& rows, Weights& w, const Scratch& s, hipStream_t stream);
 
+// A launch has fewer than 2^32 lanes.
+inline bool fits_launch(int64_t blocks, int lanes) { return blocks < ((int64_t)1 << 32) / lanes; }
 inline int launch_blocks(int64_t groups, int64_t most) {
   return (int)(groups < most ? groups : most);
 }

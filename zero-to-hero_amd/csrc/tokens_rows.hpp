@@ -142,7 +142,7 @@ template <class T, bool kEntropy, class Emit>
 int launch_parts(const Rows& rows, const Scratch& s, const Emit& emit, bool again,
                  hipStream_t stream, int& splits) {
   splits = row_splits(rows.n, rows.A, sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16);
-  if (rows.n > (((int64_t)1 << 31) - 1) / splits) return PPO_ERR_TOO_LARGE;
+  if (!fits_launch(rows.n * splits, 256)) return PPO_ERR_TOO_LARGE;
   hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
                      dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
                      splits, again);
@@ -159,9 +159,10 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, bool
       const int64_t chunks = chunks_of(rows.A, dtype);
       auto go = [&](auto lanes) {
         constexpr int G = decltype(lanes)::value;
-        hipLaunchKernelGGL((statistics_kernel<T, G, kEntropy, true, Emit>),
-                           dim3((unsigned)div_up(rows.n, 256 / G)), dim3(256), 0, stream, rows, emit,
-                           nullptr, 1, again);
+        const int64_t blocks = div_up(rows.n, 256 / G);
+        if (!fits_launch(blocks, 256)) return (int)PPO_ERR_TOO_LARGE;
+        hipLaunchKernelGGL((statistics_kernel<T, G, kEntropy, true, Emit>), dim3((unsigned)blocks),
+                           dim3(256), 0, stream, rows, emit, nullptr, 1, again);
         return last_launch_status();
       };
       if (chunks <= 64) return go(Int<16>{});
@@ -284,7 +285,7 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
   auto go = [&](auto lanes) {
     constexpr int G = decltype(lanes)::value;
     const int64_t pieces = div_up(chunks, G * kGradU);
-    const int64_t most = held != 0.0f ? kHeldBlocks : ((int64_t)1 << 31) - 1;
+    const int64_t most = held != 0.0f ? kHeldBlocks : ((int64_t)1 << 24) - 1;  // (2^32 lanes)
     hipLaunchKernelGGL((gradient_kernel<T, G, kC, Terms>),
                        dim3((unsigned)std::min(div_up(rows.n * pieces, 256 / G), most)), dim3(256),
                        (size_t)board_ints * (256 / std::min(G, kWave)) * sizeof(int), stream, rows,
@@ -300,8 +301,8 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
 // lane) for the smallest group that holds a row, or split() where a row does not
 // fit, or the gradients lie otherwise in 16 bytes than the logits (not `alike`), or rows
 // are so few that one workgroup to each takes longer, the more so the larger it is (a row
-// of 131072 bf16 24 us by itself; 32 of them 14 split, 128 27 either way; of 50304 100
-// rows 15 and 16; of 30000 40 rows 13 either way).  Many rows of up to 128 chunks go four
+// of 131072 bf16 24 us by itself; 32 of them 14 split, 64 17, 128 27 either way; of 50304
+// 100 rows 15 and 16; of 30000 40 rows 13 either way).  Many rows of up to 128 chunks go four
 // to a wave, which then takes their sums' ends together (16384 x 1000 bf16 24 us, 31 one
 // to a wave); none go four to a wave (`least` 64) that need more LDS than that leaves, and
 // of more than 64 chunks none that take entries (`single`).
