@@ -322,7 +322,8 @@ def policy_want(c, S, T, tau, low, high, kc, ec, mask, reduction, denominator, t
 POLICY_SHAPES = [(1, 1, 1), (2, 3, 5), (16, 16, 18), (64, 65, 900), (3, 50, 200), (3, 5, 300),
                  (4, 9, 1000), (3, 4, 2111),
                  (2, 35, 4097), (3, 30, 9001), (2, 40, 17000), (5, 13, 33000), (2, 33, 70001),
-                 (3, 2, 131071), (2, 32, 129000), (1, 2, 300001)]
+                 (3, 2, 131071), (2, 32, 129000), (1, 2, 300001), (2, 33, 150000),
+                 (2, 33, 196000)]
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -508,7 +509,7 @@ def distill_case(seed, t, tt, S, T, A, K):
                                    (2, 40, 17000, 256), (5, 13, 33000, 7), (2, 32, 70001, 64),
                                    (3, 2, 131071, 200), (2, 32, 129000, 64), (1, 2, 300001, 33),
                                    (2, 70, 40, 200), (3, 7, 300, 256), (5, 9, 500, 130),
-                                   (2, 9, 257, 129)])
+                                   (2, 9, 257, 129), (2, 33, 150000, 64), (2, 33, 196000, 20)])
 def test_distillation_matches_oracle(dev, shape, dtype):
     S, T, A, K = shape
     t, k = TYPES[dtype], S + T + A + K
@@ -672,7 +673,7 @@ def test_top_logits_that_change_meanwhile(dev):
 # Every layout with more rows than its workgroups take at once: rows, how often.
 MANY_ROWS = [(18, 512, 300), (200, 512, 300), (400, 512, 300), (900, 4096, 36), (3000, 512, 81),
              (6000, 512, 81), (9000, 256, 36), (30000, 256, 36), (40000, 128, 9), (50304, 128, 9),
-             (65536, 128, 9), (80000, 128, 6), (100000, 128, 6), (131072, 128, 6)]
+             (65536, 128, 9), (80000, 128, 6), (100000, 128, 6), (131072, 128, 6), (160001, 128, 6), (196600, 128, 6)]
 
 
 @pytest.mark.parametrize("A, rows, times", MANY_ROWS)

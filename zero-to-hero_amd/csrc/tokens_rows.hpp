@@ -298,8 +298,9 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
 }
 
 // How a pass that keeps its rows in registers is laid out: held(lanes, chunks a
-// lane) for the smallest group that holds a row, or split() where a row does not
-// fit, or the gradients lie otherwise in 16 bytes than the logits (not `alike`), or rows
+// lane) for the smallest group that holds a row (the last two spill a tenth of it, and
+// are faster all the same: 1024 x 163840 bf16 196 us read twice, 171; 196608 228, 209),
+// or split() where a row does not fit, or the gradients lie otherwise in 16 bytes than the logits (not `alike`), or rows
 // are so few that one workgroup to each takes longer, the more so the larger it is (a row
 // of 131072 bf16 24 us by itself; 32 of them 14 split, 64 17, 128 27 either way; of 50304
 // 100 rows 15 and 16; of 30000 40 rows 13 either way).  Many rows of up to 128 chunks go four
@@ -380,6 +381,8 @@ int with_row_shape(int64_t rows, int64_t chunks, bool alike, int least, Held&& h
   if (chunks <= 1024 * 10) return held(Int<1024>{}, Int<10>{});
   if (chunks <= 1024 * 13) return held(Int<1024>{}, Int<13>{});
   if (chunks <= 1024 * 16) return held(Int<1024>{}, Int<16>{});
+  if (chunks <= 1024 * 20) return held(Int<1024>{}, Int<20>{});
+  if (chunks <= 1024 * 24) return held(Int<1024>{}, Int<24>{});
   return split();
 }
 
