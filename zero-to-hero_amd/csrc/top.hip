@@ -315,7 +315,20 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
     x[i] = k < n ? from[k] : 0;
     best = max(best, (unsigned)(x[i] >> 32));
   }
-  const unsigned bound = bound_of(b, K, best);
+  // A bound of the K-th largest: where each part gives its share of the K, the least of the
+  // last ones (it lets about three times K by of random rows, and is there 2 us before
+  // the closer one); of many candidates the closer one.
+  unsigned bound;
+  if (n <= kSorted<1024>) {
+    if (threadIdx.x == 0) b.count = 0;
+    const int lane = threadIdx.x & (kWave - 1), share = (K + parts - 1) / parts;
+    bound = lane < parts ? (unsigned)(from[lane * K + share - 1] >> 32) : ~0u;
+    for (int d = 1; d < kWave; d <<= 1) bound = min(bound, (unsigned)__shfl_xor((int)bound, d));
+    bound = max(bound, 1u);
+    lds_barrier();
+  } else {
+    bound = bound_of(b, K, best);
+  }
 #pragma unroll
   for (int i = 0; i < kMergeV; ++i)
     if ((unsigned)(x[i] >> 32) >= bound) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));  // (above 0)
