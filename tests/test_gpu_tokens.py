@@ -16,6 +16,7 @@ import torch
 import ppo_amd
 from oracle import tokens_oracle as ref
 from ppo_amd import _lib, tokens
+from ppo_amd.ops import _native
 
 pytestmark = pytest.mark.gpu
 
@@ -758,6 +759,62 @@ def test_gradients_against_differences(dev, name):
         want = (dx.double() * v.double()).sum()
         scale = float(dx.double().norm()) + 1e-3
         assert abs(float(slope - want)) <= 1e-2 * scale
+
+
+class Declines:
+    """A host path that leaves every call to the interpreted one."""
+
+    def __init__(self, native):
+        self.native = native
+
+    def __getattr__(self, name):
+        return self.native.capture_id if name == "capture_id" else lambda *args: None
+
+
+@pytest.mark.parametrize("A, K", [(60, 12), (2500, 200), (40000, 7)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_interpreted_path_gives_the_same_bits(dev, monkeypatch, dtype, A, K):
+    t = TYPES[dtype]
+    f, x = losses(dev, t, A=A, K=K)
+
+    def run():
+        out = []
+        for loss in f.values():
+            xg = x.clone().requires_grad_()
+            y = loss(xg)
+            with torch.no_grad():
+                out.append(loss(x))
+            for up in (1.0, 0.25, 1.0):  # formed with the loss, anew, and anew again
+                out += [y.detach(), *torch.autograd.grad(y * up, [xg], retain_graph=True)]
+            with torch.autograd.graph.saved_tensors_hooks(lambda s: s.cpu(), lambda s: s.to(dev)):
+                xg = x.clone().requires_grad_()
+                out += torch.autograd.grad(loss(xg) * 0.25, [xg])
+        a = torch.zeros(x.shape[:-1], dtype=torch.int32, device=dev)
+        z = torch.linspace(-3, 0, a.numel(), device=dev).view(a.shape)
+        _, stats = ppo_amd.token_policy_loss(x, a, z, z[:, 0].contiguous(), z, reduction="sequence",
+                                             kl_coef=0.1, denominator=7.0)
+        out += stats.values()
+        _, stats = ppo_amd.preference_loss(x, a, None, None, 0.2, 0.1, 0.3, True, 0.9)
+        out += [*stats.values(), *ppo_amd.top_logits(x, min(A, 50))]
+        return out
+
+    here = run()
+    parameter = torch.nn.Parameter(x)
+    y = f["policy"](parameter)
+    assert torch.equal(y, f["policy"](x))
+    native = _native()
+    monkeypatch.setattr(tokens, "_native", lambda: Declines(native))
+    there = run()
+    assert len(here) == len(there) > 40
+    for n, (p, q) in enumerate(zip(here, there)):
+        assert p.dtype == q.dtype and p.shape == q.shape and torch.equal(p, q), n
+    for wrong in (lambda s: s.double(), lambda s: s[:1], lambda s: s.cpu()):
+        for loss in f.values():
+            with torch.autograd.graph.saved_tensors_hooks(lambda s: s, wrong):
+                xg = x.clone().requires_grad_()
+                y = loss(xg)
+                with pytest.raises(RuntimeError):
+                    torch.autograd.grad(y, [xg])
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))

@@ -121,12 +121,18 @@ def _saved(logits) -> torch.Tensor:
     return torch.empty((S * T, _lib.PPO_TOKEN_SAVED), dtype=torch.float32, device=logits.device)
 
 
-def _like_forward(t, dtype, shape, what) -> torch.Tensor:
+def _like_forward(t, dtype, shape, device, what) -> torch.Tensor:
     """What a saved-tensor hook hands back, as the forward pass had it."""
-    if t.dtype != dtype or t.shape != shape or t.device.type != "cuda":
+    if t.dtype != dtype or t.shape != shape or t.device != device:
         raise RuntimeError(f"{what}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on "
-                           f"{t.device}, expected {dtype} {tuple(shape)}")
+                           f"{t.device}, expected {dtype} {tuple(shape)} on {device}")
     return t.contiguous()
+
+
+def _like(logits, actions, mask):
+    """What the tensors of every row are, for _saved_rows."""
+    return (logits.shape, logits.device, logits.dtype, *(None if t is None else t.dtype
+                                                         for t in (actions, mask)))
 
 
 def _once(what: str) -> None:
@@ -255,7 +261,7 @@ class _LogProbs(torch.autograd.Function):
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, actions, mask, saved)
-        ctx.like = logits.shape, logits.dtype, actions.dtype
+        ctx.like = _like(logits, actions, mask)
         return lp, H
 
     @staticmethod
@@ -271,13 +277,14 @@ class _LogProbs(torch.autograd.Function):
 
 def _saved_rows(ctx, what):
     """logits, actions, mask, saved and what else a node saved, checked."""
-    shape, dtype, actions_dtype = ctx.like
+    shape, device, dtype, actions_dtype, mask_dtype = ctx.like
     logits, actions, mask, saved, *more = ctx.saved_tensors
     rows = shape[:-1]
-    return (_like_forward(logits, dtype, shape, what),
-            None if actions is None else _like_forward(actions, actions_dtype, rows, what),
-            None if mask is None else _like_forward(mask, mask.dtype, rows, what),
-            _like_forward(saved, torch.float32, (math.prod(rows), _lib.PPO_TOKEN_SAVED), what),
+    return (_like_forward(logits, dtype, shape, device, what),
+            None if actions is None else _like_forward(actions, actions_dtype, rows, device, what),
+            None if mask is None else _like_forward(mask, mask_dtype, rows, device, what),
+            _like_forward(saved, torch.float32, (math.prod(rows), _lib.PPO_TOKEN_SAVED), device,
+                          what),
             *more)
 
 
@@ -290,7 +297,7 @@ class _PolicyLoss(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(scalars)
         ctx.save_for_backward(logits, actions, mask, saved, coef)
-        ctx.like = logits.shape, logits.dtype, actions.dtype
+        ctx.like = _like(logits, actions, mask)
         total = torch.empty(0, dtype=torch.float32, device=logits.device)
         total.set_(scalars.untyped_storage(), scalars.storage_offset(), ())
         return total, scalars
@@ -301,7 +308,8 @@ class _PolicyLoss(torch.autograd.Function):
         if grad_loss is None:
             return (None,) * 8
         logits, actions, mask, saved, coef = _saved_rows(ctx, "token_policy_loss")
-        coef = _like_forward(coef, torch.float32, (2, saved.shape[0]), "token_policy_loss")
+        coef = _like_forward(coef, torch.float32, (2, saved.shape[0]), saved.device,
+                             "token_policy_loss")
         d = _log_probs_backward(logits, actions, mask, ctx.temperature, saved, coef[0], coef[1],
                                 _scale(grad_loss), ctx.held.take(), ctx.held.value)
         return (d,) + (None,) * 7
@@ -316,7 +324,7 @@ class _PreferenceLoss(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(rewards)
         ctx.save_for_backward(logits, actions, mask, saved, coef)
-        ctx.like = logits.shape, logits.dtype, actions.dtype
+        ctx.like = _like(logits, actions, mask)
         return loss, rewards
 
     @staticmethod
@@ -325,7 +333,8 @@ class _PreferenceLoss(torch.autograd.Function):
         if grad_loss is None:
             return (None,) * 9
         logits, actions, mask, saved, coef = _saved_rows(ctx, "preference_loss")
-        coef = _like_forward(coef, torch.float32, logits.shape[:-1], "preference_loss")
+        coef = _like_forward(coef, torch.float32, logits.shape[:-1], logits.device,
+                             "preference_loss")
         d = _log_probs_backward(logits, actions, mask, ctx.temperature, saved, coef, None,
                                 _scale(grad_loss))
         return (d,) + (None,) * 8
@@ -337,7 +346,7 @@ class _DistillationLoss(torch.autograd.Function):
         out, saved, d = _distill(logits, teacher, ids, mask, temperature, loss, True, True)
         ctx.temperature, ctx.held = temperature, _Held(d, loss.grad_scale)
         ctx.save_for_backward(logits, None, mask, saved, teacher, ids)
-        ctx.like = logits.shape, logits.dtype, None
+        ctx.like = _like(logits, None, mask)
         ctx.top = teacher.shape, teacher.dtype, ids.dtype
         return out
 
@@ -346,8 +355,8 @@ class _DistillationLoss(torch.autograd.Function):
         _once("distillation_loss")
         logits, _, mask, saved, teacher, ids = _saved_rows(ctx, "distillation_loss")
         shape, dtype, ids_dtype = ctx.top
-        teacher = _like_forward(teacher, dtype, shape, "distillation_loss")
-        ids = _like_forward(ids, ids_dtype, shape, "distillation_loss")
+        teacher = _like_forward(teacher, dtype, shape, logits.device, "distillation_loss")
+        ids = _like_forward(ids, ids_dtype, shape, logits.device, "distillation_loss")
         d = _distill_backward(logits, teacher, ids, mask, ctx.temperature, saved,
                               _scale(grad_loss), ctx.held.take(), ctx.held.value)
         return (d,) + (None,) * 5
