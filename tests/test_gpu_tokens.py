@@ -9,6 +9,7 @@ each addition on the way, of which a lane makes at most 64, or A / 512 where it 
 a long row, and the lanes' join some ten more."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -845,6 +846,66 @@ def test_another_stream(dev):
         torch.cuda.current_stream(dev).wait_stream(side)
         assert all(torch.equal(p, q) for p, q in zip(got, want)), name
         assert all(torch.equal(p, q) for p, q in zip(top, ppo_amd.top_logits(x, 7)))
+
+
+def test_calls_at_once(dev):
+    """Threads with a stream each, all operators forward and back, and graphs of two
+    losses that replay side by side."""
+    f, x = losses(dev, torch.bfloat16, S=6, T=20, A=9000, K=20)
+
+    def run():
+        out = []
+        for loss in f.values():
+            xg = x.clone().requires_grad_()
+            y = loss(xg)
+            out += [y.detach(), *torch.autograd.grad(y, [xg])]
+        return [*out, *ppo_amd.top_logits(x, 30)]
+
+    want = run()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(8):
+                got = run()
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(n for n, (p, q) in enumerate(zip(got, want)) if not torch.equal(p, q))
+            wrong.append(None)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [None] * 3
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], []
+    for name in ("policy", "distillation"):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            xg = x.clone().requires_grad_()
+            torch.autograd.grad(f[name](xg), [xg])
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                y = f[name](xg)
+                outs.append((y, torch.autograd.grad(y, [xg])[0]))
+        graphs.append(graph)
+        streams.append(stream)
+    names = list(f)
+    for _ in range(4):
+        for y, d in outs:
+            y.detach().fill_(7.0)
+            d.fill_(7.0)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for name, (y, d) in zip(("policy", "distillation"), outs):
+            n = 2 * names.index(name)
+            assert torch.equal(y.detach(), want[n]) and torch.equal(d, want[n + 1])
 
 
 @pytest.mark.parametrize("A", [60, 2500, 30000])
