@@ -491,6 +491,30 @@ def test_preference_loss_of_far_pairs(dev):
     assert abs(float(loss) - math.log(2.0)) < 1e-6
 
 
+@pytest.mark.parametrize("tau", [0.3, 0.7, 1.0, 1.5])
+@pytest.mark.parametrize("A", [40, 900, 20000, 300000])
+def test_preference_of_close_policies(dev, A, tau):
+    """Unlikely actions of policies close to their reference: what is left of the
+    difference is not the rounding of log2(e) / tau, up to u of 80.  With the row's sum
+    in 64 bits a difference is off by the exponentials (2 u each, and again where a
+    part's maximum is taken to the row's), their exponents' roundings (u t each) and its own
+    rounding: u (8 + 4 sum p t + |rel|) with room for the factors."""
+    g = torch.Generator().manual_seed(A)
+    S, T = 4, 3
+    x = -20.0 * tau + torch.randn(S, T, A, generator=g)
+    a = torch.randint(1, A, (S, T), generator=g)
+    x[..., 0] = 0.0
+    x.scatter_(-1, a[..., None], -80.0 * tau)
+    b = bounds(x.view(S * T, A), a.view(-1), tau)
+    ref_ = (b.lp + 0.01 * torch.randn(S * T, generator=g)).float()
+    rel = (b.lp - ref_.double()).view(S, T)
+    err = (U32 * (8 + 4 * b.pt + rel.abs().view(-1))).view(S, T)
+    _, stats = ppo_amd.preference_loss(x.to(dev), a.to(dev), ref_.view(S, T).to(dev), beta=1.0,
+                                       temperature=tau)
+    got = torch.cat([stats["chosen"], stats["rejected"]])
+    assert_within(got, rel.sum(1), err.sum(1) + U32 * rel.sum(1).abs(), "rewards")
+
+
 # --- distillation ------------------------------------------------------------------------------
 
 def distill_case(seed, t, tt, S, T, A, K):

@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
   double sums[1] = {};
   const float inverse = inverse_count(d.weights);
   const T* logits = static_cast<const T*>(rows.logits);
+  const Scale<Stat> scale(rows);
   const Walk<G> walk(rows, order, (int64_t)gridDim.x * kGroups);
   auto dead = [&](int64_t r) {
     if (dlogits) write_zeros<T, G>(dlogits + r * rows.A, rows.A, t);
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
     i = walk.from(i + walk.step, dead);
     const int64_t next = i < rows.n ? walk.row(i) : -1;
     x.take_out(-1, t);
-    Stat st = x.template stat<false>(rows.c);
+    Stat st = x.template stat<false>(scale);
     RowShare share;
     auto finish = [&] {
       const float inv_s = 1.0f / st.s;
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
     };
     if (G > kWave) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      st = block_join<false>(st, rows.c, s_part);
+      st = block_join<false>(st, scale, s_part);
       if (threadIdx.x < kWave) {
         finish();
         if (t == 0) s_row = share;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
       lds_barrier();
       share = s_row;
     } else {
-      st = lanes_join<kTeam, false>(st, rows.c);
+      st = lanes_join<kTeam, false>(st, scale);
       finish();
     }
     share = {shared_by<G>(share.g), shared_by<G>(share.inv_s), shared_by<G>(share.W)};
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
 }
 
 struct DistillJoin {
+  using Sums = Stat;
   static constexpr bool kWholeWave = true;
   Distill d;
   double sums[1];
@@ -331,7 +333,7 @@ struct DistillSplit : DistillTerms {
   __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T* row, float, int, int t,
                                       bool first, int* board) {
     const Entries e = take<T, G>(rows, r, row, board);
-    const Stat x = join_parts<G, false>(parts, r, splits, rows.c);
+    const Stat x = join_parts<G, false>(parts, r, splits, Scale<Stat>(rows));
     const float weight = d.tau * row_weight(d.weights, inverse, r / rows.T);
     inv_s = 1.0f / x.s;
     W = weight * d.grad_scale;

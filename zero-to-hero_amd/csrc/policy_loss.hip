@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
   const float inverse = inverse_count(p.weights);
   if (G > kWave && threadIdx.x < kSums) s_sums[threadIdx.x] = 0.0;
   const T* logits = static_cast<const T*>(rows.logits);
+  const Scale<Stat> scale(rows);
   const Walk<G> walk(rows, order, (int64_t)gridDim.x * kGroups);
   auto dead = [&](int64_t r) {
     if (dlogits) write_zeros<T, G>(dlogits + r * rows.A, rows.A, t);
@@ -118,10 +119,10 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
     const int64_t next = i < rows.n ? walk.row(i) : -1;
     const int next_a = next >= 0 ? rows.action(next) : -1;
     x.take_out(a, t);
-    Stat st = x.template stat<true>(rows.c);
+    Stat st = x.template stat<true>(scale);
     Grad g;
     auto finish = [&](double(&to)[kSums]) {
-      const RowTerms terms = row_terms<true>(st, la, rows.c);
+      const RowTerms terms = row_terms<true>(st, la, scale);
       float gl, ge;
       const RowLoss loss = policy_row(p, in, terms, gl, ge);
       if (t == 0) {
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
       g = row_grad(saved_of(terms, 0.0f), gl * p.grad_scale, ge * p.grad_scale, rows.inv_tau, a);
     };
     if (G > kWave) {
-      st = block_join<true>(st, rows.c, s_part);
+      st = block_join<true>(st, scale, s_part);
       if (threadIdx.x < kWave) {
         finish(s_sums);
         if (t == 0) s_grad = g;
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
       lds_barrier();
       g = s_grad;
     } else {
-      st = lanes_join<G <= kWave ? G : kWave, true>(st, rows.c);
+      st = lanes_join<G <= kWave ? G : kWave, true>(st, scale);
       finish(sums);
     }
     g = shared_by<G>(g);
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(kRowBlock<G>, kRowWaves<G>)
 
 // The same from rows' parts (join_kernel), where a row has several workgroups.
 struct PolicyJoin {
+  using Sums = Stat;
   static constexpr bool kWholeWave = false;
   Policy p;
   double sums[kSums];
@@ -173,7 +175,7 @@ struct PolicyJoin {
   }
   template <bool kEntropy>
   __device__ __forceinline__ void row(const Rows& rows, int64_t r, Stat x, float la, bool first) {
-    const RowTerms t = row_terms<kEntropy>(x, la, rows.c);
+    const RowTerms t = row_terms<kEntropy>(x, la, Scale<Stat>(rows));
     float G, E;
     const RowLoss loss =
         policy_row(p, row_in(p, rows, r, inverse_count(p.weights)), t, G, E);
@@ -218,8 +220,9 @@ struct PolicySplit : GradientTerms {
   template <class T, int G>
   __device__ __forceinline__ Grad row(const Rows& rows, int64_t r, const T* row, float, int a, int t,
                                       bool first, int*) const {
-    const RowTerms terms = row_terms<true>(join_parts<G, true>(parts, r, splits, rows.c),
-                                           action_logit(row, a), rows.c);
+    const Scale<Stat> scale(rows);
+    const RowTerms terms = row_terms<true>(join_parts<G, true>(parts, r, splits, scale),
+                                           action_logit(row, a), scale);
     float gl, ge;
     const RowLoss loss = policy_row(p, row_in(p, rows, r, inverse), terms, gl, ge);
     if (first && t == 0) {

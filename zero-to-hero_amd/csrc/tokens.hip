@@ -37,7 +37,7 @@ Scratch scratch_of(void* workspace, int64_t S, int64_t T, int64_t A, int dtype) 
   s.lengths = reinterpret_cast<int*>(take((size_t)S * sizeof(int)));
   s.sums = reinterpret_cast<double*>(take(sizeof(double) * kSums * kMaxPartials));
   s.parts = reinterpret_cast<Stat*>(take((size_t)(S * T) * row_splits(S * T, A, dtype) *
-                                         sizeof(Stat)));
+                                         sizeof(FineStat)));
   s.bytes = at;
   return s;
 }
@@ -51,12 +51,13 @@ int take_rows(const ppo_token_rows* r, bool actions, Rows& out) {
   if (!r || !dtype_ok(r->dtype) || r->sequences < 0 || r->tokens < 0 || r->A <= 0 ||
       !(r->temperature > 0.0))
     return PPO_ERR_INVALID_ARG;
-  const float c = (float)(1.44269504088896340736 / r->temperature);
+  const double exact = 1.44269504088896340736 / r->temperature;
+  const float c = (float)exact, c_down = (double)c < exact ? c : nextafterf(c, 0.0f);
   const float inv_tau = (float)(1.0 / r->temperature);
   if (!(c > 0.0f) || !(c < INFINITY)) return PPO_ERR_INVALID_ARG;
   if (!sizes_ok(r->sequences, r->tokens, r->A)) return PPO_ERR_TOO_LARGE;
   out = {r->logits, r->actions, r->mask, r->sequences * r->tokens, r->tokens, r->sequences,
-         (int)r->A, r->actions_are_int64, c, inv_tau};
+         (int)r->A, r->actions_are_int64, c, inv_tau, c_down, (float)(exact - (double)c_down)};
   if (out.n == 0) return PPO_OK;
   const uintptr_t size = dtype_size(r->dtype);
   if (!r->logits || (uintptr_t)r->logits % size || (actions && !r->actions))
@@ -178,7 +179,9 @@ int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s,
 namespace {
 
 // What ppo_token_log_probs leaves of a row.
+template <class S>
 struct LogProbs {
+  using Sums = S;
   static constexpr bool kWholeWave = false;
   const float* minus;
   float *log_probs, *entropy;
@@ -189,8 +192,8 @@ struct LogProbs {
     if (entropy) entropy[r] = 0.0f;
   }
   template <bool kEntropy>
-  __device__ __forceinline__ void row(const Rows& rows, int64_t r, Stat x, float la, bool first) {
-    const RowTerms t = row_terms<kEntropy>(x, la, rows.c);
+  __device__ __forceinline__ void row(const Rows& rows, int64_t r, S x, float la, bool first) {
+    const RowTerms t = row_terms<kEntropy>(x, la, Scale<S>(rows));
     if (!first) return;
     log_probs[r] = (float)(minus ? t.lp - (double)minus[r] : t.lp);
     if (entropy) entropy[r] = t.H;
@@ -367,13 +370,17 @@ extern "C" int ppo_token_log_probs(const ppo_token_rows* r, const float* minus, 
   if (!log_probs || (saved && !aligned16(saved))) return PPO_ERR_INVALID_ARG;
   const Scratch s = scratch_of(workspace, rows.S, rows.T, rows.A, r->dtype);
   if (!workspace || !aligned16(workspace) || workspace_bytes < s.bytes) return PPO_ERR_WORKSPACE;
-  const LogProbs emit = {minus, log_probs, entropy, reinterpret_cast<Saved*>(saved)};
   return with_dtype(r->dtype, [&](auto zero) {
     using T = decltype(zero);
     hipStream_t stream = (hipStream_t)stream_ptr;
     const bool again = saved && rows.n * rows.A * (int64_t)sizeof(T) <= kReadAgain;
-    return entropy ? launch_statistics<T, true, true>(rows, s, emit, again, stream)
-                   : launch_statistics<T, false, true>(rows, s, emit, again, stream);
+    auto go = [&](auto sums) {
+      const LogProbs<decltype(sums)> emit = {minus, log_probs, entropy,
+                                             reinterpret_cast<Saved*>(saved)};
+      return entropy ? launch_statistics<T, true, true>(rows, s, emit, again, stream)
+                     : launch_statistics<T, false, true>(rows, s, emit, again, stream);
+    };
+    return minus ? go(FineStat{}) : go(Stat{});
   });
 }
 

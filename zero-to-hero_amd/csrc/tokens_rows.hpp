@@ -16,21 +16,21 @@ using Int = std::integral_constant<int, N>;
 // a time (four and eight are slower: 50304 bf16 69, 72 and 76 us of 4096 rows; of short
 // rows one); the sums follow the running maximum.  `again`: the rows are read again
 // soon, and stay in the caches.
-template <class T, int G, bool kEntropy>
-__device__ __forceinline__ Stat stream_stat(const T* row, int A, int a, float c, int t, int part,
-                                            int splits, bool again) {
+template <class T, int G, bool kEntropy, class S>
+__device__ __forceinline__ S stream_stat(const T* row, int A, int a, const Scale<S>& c, int t,
+                                         int part, int splits, bool again) {
   constexpr int kN = kPer16<T>, kU = G == 16 ? 1 : 2;
   const Cut<T> cut(row, A);
   const v4i* body = reinterpret_cast<const v4i*>(row + cut.head);
   const int per = (cut.nvec + splits - 1) / splits;
   const int end = min(cut.nvec, (part + 1) * per);
   const int b = a - cut.head, va = a >= 0 && b >= 0 ? b / kN : -1;  // the action's chunk
-  Stat x = {kNegInf, 0.0f, 0.0f};
+  S x = {kNegInf, 0.0f, 0.0f};
   if (part == 0 && t < cut.ends) {
     const int col = cut.end_column(t);
     const float l = col == a ? kNegInf : to_f32(row[col]);
     x.m = l;
-    const float d = l == kNegInf ? l : (l - l) * c;  // (NaN and +inf give NaN)
+    const float d = l == kNegInf ? l : l - l;  // (NaN and +inf give NaN)
     x.s = exp2_fast(d);
   }
   for (int i = part * per + t; i < end; i += G * kU) {
@@ -49,12 +49,12 @@ __device__ __forceinline__ Stat stream_stat(const T* row, int A, int a, float c,
     }
     rebase<kEntropy>(x, m, c);
     if (m == kNegInf) m = 0.0f;
-    float s2 = 0.0f;
+    decltype(x.s) s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < kU; ++k)
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
-        const float d = (unpack<T>(w[k], j) - m) * c, e = exp2_fast(d);
+        const float d = c(unpack<T>(w[k], j) - m), e = exp2_fast(d);
         (j & 1 ? s2 : x.s) += e;
         if (kEntropy) x.u = fmaf(e, fmaxf(d, -1e30f), x.u);
       }
@@ -71,9 +71,12 @@ __device__ __forceinline__ float action_logit(const T* row, int a) {
 // One group to a row and the row finished by it (kDirect), or `splits` workgroups to
 // a row that leave their parts.  What bounds it: HBM reads.
 template <class T, int G, bool kEntropy, bool kDirect, class Emit>
-__global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, Stat* parts,
-                                                         int splits, bool again) {
-  __shared__ Stat s_part[4];
+__global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit,
+                                                         typename Emit::Sums* parts, int splits,
+                                                         bool again) {
+  using S = typename Emit::Sums;
+  __shared__ S s_part[4];
+  const Scale<S> c(rows);
   const int t = threadIdx.x % G;
   const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   const int64_t r = kDirect ? group : group / splits;
@@ -86,13 +89,12 @@ __global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, S
   const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
   const int a = rows.actions ? rows.action(r) : -1;
   const float la = kDirect ? action_logit(row, a) : 0.0f;
-  Stat x = stream_stat<T, G, kEntropy>(row, rows.A, a, rows.c, t, part, splits,
-                                                again);
+  S x = stream_stat<T, G, kEntropy>(row, rows.A, a, c, t, part, splits, again);
   if (G > kWave) {
-    x = block_join<kEntropy>(x, rows.c, s_part);
+    x = block_join<kEntropy>(x, c, s_part);
     if (threadIdx.x >= kWave) return;
   } else {
-    x = lanes_join<G <= kWave ? G : kWave, kEntropy>(x, rows.c);
+    x = lanes_join<G <= kWave ? G : kWave, kEntropy>(x, c);
   }
   if constexpr (kDirect)
     emit.template row<kEntropy>(rows, r, x, la, t == 0);
@@ -102,19 +104,19 @@ __global__ void __launch_bounds__(256) statistics_kernel(Rows rows, Emit emit, S
 
 // The parts of row r as one, by every group of lanes that asks for them (groups smaller
 // than a wave have rows of one part).
-template <int G, bool kEntropy>
-__device__ __forceinline__ Stat join_parts(const Stat* parts, int64_t r, int splits, float c) {
+template <int G, bool kEntropy, class S>
+__device__ __forceinline__ S join_parts(const S* parts, int64_t r, int splits, const Scale<S>& c) {
   if (G < kWave) return parts[r];
   const int lane = threadIdx.x & (kWave - 1);
-  const Stat x = lane < splits ? parts[r * splits + lane] : Stat{kNegInf, 0.0f, 0.0f};
+  const S x = lane < splits ? parts[r * splits + lane] : S{kNegInf, 0.0f, 0.0f};
   return lanes_join<kWave, kEntropy>(x, c);
 }
 
 // A wave to a row: its parts joined in the order of their lanes, and the row
 // finished by its lane 0, or by the wave (kWholeWave).
 template <class T, bool kEntropy, class Emit>
-__global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit, const Stat* parts,
-                                                  int splits) {
+__global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit,
+                                                  const typename Emit::Sums* parts, int splits) {
   const int lane = threadIdx.x;
   for (int64_t r = blockIdx.x; r < rows.n; r += gridDim.x) {
     if (!rows.live(r)) {
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(64) join_kernel(Rows rows, Emit emit, const St
     const T* row = static_cast<const T*>(rows.logits) + r * rows.A;
     const int a = rows.actions ? rows.action(r) : -1;
     const float la = action_logit(row, a);
-    const Stat x = join_parts<kWave, kEntropy>(parts, r, splits, rows.c);
+    const auto x = join_parts<kWave, kEntropy>(parts, r, splits, Scale<typename Emit::Sums>(rows));
     if constexpr (Emit::kWholeWave)
       emit.row(rows, r, row, x, lane);
     else
@@ -144,8 +146,8 @@ int launch_parts(const Rows& rows, const Scratch& s, const Emit& emit, bool agai
   splits = row_splits(rows.n, rows.A, sizeof(T) == 4 ? PPO_DTYPE_F32 : PPO_DTYPE_BF16);
   if (!fits_launch(rows.n * splits, 256)) return PPO_ERR_TOO_LARGE;
   hipLaunchKernelGGL((statistics_kernel<T, 256, kEntropy, false, Emit>),
-                     dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit, s.parts,
-                     splits, again);
+                     dim3((unsigned)(rows.n * splits)), dim3(256), 0, stream, rows, emit,
+                     reinterpret_cast<typename Emit::Sums*>(s.parts), splits, again);
   return last_launch_status();
 }
 
@@ -172,7 +174,8 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, bool
   int parts;
   if (const int code = launch_parts<T, kEntropy>(rows, s, emit, again, stream, parts)) return code;
   hipLaunchKernelGGL((join_kernel<T, kEntropy, Emit>), dim3(launch_blocks(rows.n, kMaxPartials)),
-                     dim3(64), 0, stream, rows, emit, s.parts, splits);
+                     dim3(64), 0, stream, rows, emit,
+                     reinterpret_cast<const typename Emit::Sums*>(s.parts), splits);
   return last_launch_status();
 }
 
