@@ -4,7 +4,7 @@
 //   dlogits_j = (G ([j = a] - p_j) - E p_j (log p_j + H)) / temperature,
 // which needs the whole row's sums before its first element: hence registers, or the
 // caches for rows that do not fit.  What bounds it: HBM, one read and one write of the
-// logits (8192 x 131072 bf16 849 us, 5.06 TB/s; 4096 x 32768 with a mask 86, 5.2);
+// logits (8192 x 131072 bf16 839-851 us, 5.1 TB/s; 4096 x 32768 with a mask 86, 5.2);
 // few rows the chain of launches (528 x 500 fp32 16 in a graph).
 #include "tokens_rows.hpp"
 

@@ -1,7 +1,7 @@
 // Token policies: log-probabilities and entropies of the taken actions, their
 // gradient, the preference loss over them, and what all of these operators
 // share on the host: checks, weights, scratch.  What bounds them: HBM, a read of the
-// logits forward (4096 x 50304 bf16, 65% of its rows counting, 54 us, 5.0 TB/s), a read
+// logits forward (4096 x 50304 bf16, 65% of its rows counting, 57 us, 4.7 TB/s), a read
 // and a write backward (95, 7.2 TB/s with part of the read from the caches); few rows
 // the launches (256 x 18 fp32 3.1).
 #include "tokens_rows.hpp"

@@ -10,7 +10,7 @@
 // equal logits) are settled by a radix search for the threshold itself.  What bounds
 // it: HBM reads; a row is in the caches when parts of it are read again (4096 x 32001
 // fp32, K = 64, 116 us, 4.5 TB/s, while a workgroup waits for its bound another one
-// reads); a single row two launches of 7 and 5 us.
+// reads); a single row two launches of 8 and 4 us.
 #include "tokens_rows.hpp"
 
 namespace ppo {
