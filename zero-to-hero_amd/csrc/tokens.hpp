@@ -443,9 +443,9 @@ struct RowRegs {
   }
 
   // The compiler would unpack 16-bit chunks once and keep them so, in twice the
-  // registers, and take many chunks at a time (a row of 256 KB spills half of
-  // itself; 512 x 65536 fp32 69 us, 61 so): for each pass over a chunk it is to take it for changed, and its turn for
-  // coming after `sum`.
+  // registers, and take many chunks at a time (a row of 256 KB spills half of itself; 512 x
+  // 65536 fp32 69 us, 61 so): for each pass over a chunk it is to take it for changed, and
+  // its turn for coming after `sum`.
   __device__ __forceinline__ void turn(int i, float& sum) {
     if (sizeof(T) == 2 || G >= 512) asm volatile("" : "+v"(raw[i]), "+v"(sum));
   }

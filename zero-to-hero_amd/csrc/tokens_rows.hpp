@@ -180,9 +180,10 @@ int launch_statistics(const Rows& rows, const Scratch& s, const Emit& emit, bool
 }
 
 // What a gradient pass asks of a row, by the G lanes of one of its pieces: begin() comes
-// before the first, with all lanes of every wave; row() gives its terms (called by whole groups, so lanes may work together; `first`: the row's first
-// piece, t the lane in its group, board the group's or the wave's share of LDS), masked()
-// is called for a row that does not count, after() when the piece is written (kAfter).
+// before the first, with all lanes of every wave; row() gives its terms (called by whole
+// groups, so lanes may work together; `first`: the row's first piece, t the lane in its
+// group, board the group's or the wave's share of LDS), masked() is called for a row that
+// does not count, after() when the piece is written (kAfter).
 struct GradientTerms {
   static constexpr bool kAfter = false;
   __device__ __forceinline__ void begin() {}
@@ -300,16 +301,6 @@ int launch_gradient(const Rows& rows, const Terms& terms, const float* scale, fl
   return go(Int<256>{});
 }
 
-// How a pass that keeps its rows in registers is laid out: held(lanes, chunks a
-// lane) for the smallest group that holds a row (the last two spill a tenth of it, and
-// are faster all the same: 1024 x 163840 bf16 196 us read twice, 171; 196608 228, 209),
-// or split() where a row does not fit, or the gradients lie otherwise in 16 bytes than the logits (not `alike`), or rows
-// are so few that one workgroup to each takes longer, the more so the larger it is (a row
-// of 131072 bf16 24 us by itself; 32 of them 14 split, 64 17, 128 27 either way; of 50304
-// 100 rows 15 and 16; of 30000 40 rows 13 either way).  Many rows of up to 128 chunks go four
-// to a wave, which then takes their sums' ends together (16384 x 1000 bf16 24 us, 31 one
-// to a wave); none go four to a wave (`least` 64) that need more LDS than that leaves, and
-// of more than 64 chunks none that take entries (`single`).
 // A pass's workgroup, and the waves a SIMD is to hold at least: two workgroups of 512
 // lanes (65536 bf16 218 -> 214 us, 50304 198 -> 187); smaller ones do better with the
 // registers (32768 191 us, 211 with four waves to a SIMD).
@@ -361,6 +352,16 @@ struct Walk {
 inline bool lies_alike(const void* logits, const void* dlogits) {
   return ((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0;
 }
+// How a pass that keeps its rows in registers is laid out: held(lanes, chunks a lane) for
+// the smallest group that holds a row, or split() where a row does not fit, where the
+// gradients lie otherwise in 16 bytes than the logits (not `alike`), or where rows are so few
+// that one workgroup to each takes longer, the more so the larger it is (a row of 131072
+// bf16 24 us by itself; 32 of them 14 split, 64 17, 128 27 either way; of 50304 100 rows 15
+// and 16; of 30000 40 rows 13 either way).  The two largest spill a tenth of their row and
+// are faster all the same (1024 x 163840 bf16 196 us read twice, 171; 196608 228, 209).
+// Many rows of up to 128 chunks go four to a wave, which then takes their sums' ends together
+// (16384 x 1000 bf16 24 us, 31 one to a wave); none do (`least` 64) that need more LDS than
+// that leaves, and of more than 64 chunks none that take entries (kSingle).
 template <bool kSingle, class Held, class Split>
 int with_row_shape(int64_t rows, int64_t chunks, bool alike, int least, Held&& held,
                    Split&& split) {

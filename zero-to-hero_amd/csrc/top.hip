@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
   }
 #pragma unroll
   for (int i = 0; i < kMergeV; ++i)
-    if ((unsigned)(x[i] >> 32) >= bound) append(b, (unsigned)(x[i] >> 32), column_of(x[i]));  // (above 0)
+    if ((unsigned)(x[i] >> 32) >= bound)  // (above 0)
+      append(b, (unsigned)(x[i] >> 32), column_of(x[i]));
   lds_barrier();
   if (b.count > kSorted<1024>) {  // (no two are alike: the K-th by its bits)
     lds_barrier();
