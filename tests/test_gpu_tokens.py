@@ -675,6 +675,27 @@ def test_top_logits_ties_and_values_that_are_not_finite(dev, dtype, A):
     assert bool(same.all())
 
 
+@pytest.mark.parametrize("A", [4100, 20001, 36000, 140001])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_top_logits_of_long_rows(dev, dtype, A):
+    """Rows that a workgroup takes whole, in segments of one round to many, with ties in
+    more segments than are looked at again."""
+    g = torch.Generator(dev).manual_seed(A)
+    x = torch.randn(520, A, device=dev, generator=g).to(TYPES[dtype])
+    x[0] = 0.0
+    x[1] = (torch.arange(A, device=dev) % 7).to(x.dtype)
+    x[2] = -float("inf")
+    x[2, :: A // 7] = 1.0
+    x[3, 5::3] = float("nan")
+    x[4] = torch.arange(A, device=dev).to(x.dtype)
+    x[5, A // 2:] = 9.0
+    want, at = x.float().sort(dim=-1, descending=True, stable=True)
+    for k in (1, 20, 64, 130, 256):
+        v, i = ppo_amd.top_logits(x, k)
+        assert torch.equal(i, at[:, :k]), k
+        assert torch.equal(torch.nan_to_num(v.float(), 7e7), torch.nan_to_num(want[:, :k], 7e7)), k
+
+
 def test_top_logits_that_change_meanwhile(dev):
     """Logits written by another stream during the call: which are found is undefined,
     but every column lies in its row and every value is NaN or was there."""

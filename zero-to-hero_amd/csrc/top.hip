@@ -3,14 +3,15 @@
 // which no two of a row are alike: ties need no care of their own.
 //
 // A workgroup takes a row, or a part of one.  Its lanes keep the largest of what they
-// read, in four segments each; the K-th largest of the lanes' own maxima bounds the K-th
+// read, in up to sixteen segments each; the K-th largest of the lanes' own maxima bounds the K-th
 // largest element from below, so the few segments that reach it (about K of them) are
 // all that is looked at again, and the few elements there that do are sorted, by
 // counting for each how many precede it.  Rows in which too many reach the bound (many
 // equal logits) are settled by a radix search for the threshold itself.  What bounds
 // it: HBM reads; a row is in the caches when parts of it are read again (4096 x 32001
-// fp32, K = 64, 116 us, 4.5 TB/s, while a workgroup waits for its bound another one
-// reads); a single row two launches of 8 and 4 us.
+// fp32, K = 64, 101 us, 5.2 TB/s, while a workgroup waits for its bound another one
+// reads; with segments of eight rounds for two 120, since each one's chunks are lines of
+// their own); a single row two launches of 8 and 4 us.
 #include "tokens_rows.hpp"
 
 namespace ppo {
@@ -20,7 +21,8 @@ constexpr int kMaxK = PPO_TOKEN_MAX_K;
 // Elements that are sorted at most.
 template <int G>
 constexpr int kSorted = G == kWave ? 512 : 2048;
-constexpr int kSegments = 4;
+constexpr int kSegments = 16;
+constexpr int kAgain = 4;  // segments a lane to look at again at most
 
 typedef unsigned long long u64;
 
@@ -41,7 +43,7 @@ struct Board {
   u64 list[kSorted<G>];
   union {
     unsigned best[G];
-    unsigned short again[kSegments * G];  // lane + G segment of segments to look at again
+    unsigned short again[kAgain * G];  // lane + G segment of segments to look at again
     int bins[256];
   };
   unsigned bound;
@@ -123,12 +125,15 @@ struct Part {
   const v4i* body;
   int from;
   Cut<T> cut;
-  int rounds;  // of G chunks a segment
+  int rounds;  // of G chunks a segment: 1, 2, or a multiple of 4
 
   __device__ __forceinline__ Part(const T* row_, int from_, int width)
       : row(row_), from(from_), cut(row_ + from_, width) {
     body = reinterpret_cast<const v4i*>(row + from + cut.head);
-    rounds = (cut.nvec + kSegments * G - 1) / (kSegments * G);
+    const int all = (cut.nvec + G - 1) / G;
+    rounds = all <= kSegments       ? 1
+             : all <= 2 * kSegments ? 2
+                                    : (all + 4 * kSegments - 1) / (4 * kSegments) * 4;
   }
   __device__ __forceinline__ int end_column(int e) const { return from + cut.end_column(e); }
   __device__ __forceinline__ int column(int chunk) const { return from + cut.head + chunk * kN; }
@@ -230,10 +235,10 @@ __device__ void settle(const Part<T, G>& p, Board<G>& b, int K) {
 
 // Part `q` of `parts` of each row; one part: the row's results, else its largest
 // elements to `found` [rows][parts][K], 0 behind the last.
-template <class T, int G>
+template <class T, int G, bool kPast>
 __global__ void __launch_bounds__(G) top_kernel(const T* logits, int A, int K, int parts, int per,
                                                 T* values, int64_t* ids, u64* found) {
-  constexpr int kN = kPer16<T>, kU = 4;
+  constexpr int kN = kPer16<T>;
   __shared__ Board<G> b;
   const int t = threadIdx.x;
   const int64_t r = (int64_t)blockIdx.x / parts;
@@ -242,42 +247,73 @@ __global__ void __launch_bounds__(G) top_kernel(const T* logits, int A, int K, i
   const Part<T, G> p(logits + r * A, from, width);
 
   // (the largest of a segment as a float, and whether a NaN was among them)
-  unsigned best[kSegments], most = 0;
+  unsigned best[kSegments] = {}, most = 0;
   const float end = t < p.cut.ends ? to_f32(p.row[p.end_column(t)]) : kNegInf;
+  const int nvec = p.cut.nvec;
+  // Four chunks of a lane at a time: 4 / kRounds segments, or a quarter of rounds / 4 of one.
+  auto look = [&](auto of_segment) {
+    constexpr int kRounds = decltype(of_segment)::value, kOf = 4 / kRounds;
 #pragma unroll
-  for (int s = 0; s < kSegments; ++s) {
-    float m = kNegInf;
-    bool nan = false;
-    const int first = s * p.rounds * G + t, last = min(p.cut.nvec, (s + 1) * p.rounds * G);
-    for (int i = first; i < last; i += G * kU) {
-      v4i w[kU];
+    for (int s = 0; s < kSegments; s += kOf) {
+      if (s * p.rounds * G >= nvec) break;
+      float m[kOf];
+      bool nan[kOf];
 #pragma unroll
-      for (int k = 0; k < kU; ++k)
-        w[k] = i + k * G < last ? p.body[i + k * G] : no_chunk<T>();
+      for (int c = 0; c < kOf; ++c) {
+        m[c] = kNegInf;
+        nan[c] = false;
+      }
+      const int to = min(nvec, (s + kOf) * p.rounds * G);
+      for (int at = s * p.rounds * G; at < to; at += 4 * G) {
+        v4i w[4];
 #pragma unroll
-      for (int k = 0; k < kU; ++k)
+        for (int k = 0; k < 4; ++k)
+          w[k] = at + k * G + t >= nvec ? no_chunk<T>()
+                 : kPast ? __builtin_nontemporal_load(p.body + at + k * G + t)
+                         : p.body[at + k * G + t];
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          const float l = unpack<T>(w[k], j);
-          m = fmaxf(m, l);
-          nan |= l != l;
+        for (int k = 0; k < 4; ++k) {
+          if (at + k * G >= nvec) break;
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            const float l = unpack<T>(w[k], j);
+            m[k / kRounds] = fmaxf(m[k / kRounds], l);
+            nan[k / kRounds] |= l != l;
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kOf; ++c)
+        if ((s + c) * p.rounds * G + t < nvec) {
+          best[s + c] = nan[c] ? kNanOrder : order_of(m[c]);
+          most = max(most, best[s + c]);
         }
     }
-    best[s] = first < last ? (nan ? kNanOrder : order_of(m)) : 0;
-    most = max(most, best[s]);
-  }
+  };
+  if (p.rounds == 1)
+    look(Int<1>{});
+  else if (p.rounds == 2)
+    look(Int<2>{});
+  else
+    look(Int<4>{});
   const unsigned end_order = t < p.cut.ends ? order_of(end) : 0;
   const unsigned bound = bound_of(b, want, max(most, end_order));
   if (end_order >= bound) append(b, end_order, p.end_column(t));
 #pragma unroll
-  for (int s = 0; s < kSegments; ++s)
-    if (best[s] >= bound) b.again[atomicAdd(&b.items, 1)] = (unsigned short)(s * G + t);
+  for (int s = 0; s < kSegments; ++s) {
+    if (s * p.rounds * G >= nvec) break;
+    if (best[s] >= bound) {
+      const int at = atomicAdd(&b.items, 1);
+      if (at < kAgain * G) b.again[at] = (unsigned short)(s * G + t);
+    }
+  }
   lds_barrier();
-  const int items = b.items * p.rounds;
+  const bool many = b.items > kAgain * G;
+  const int items = many ? 0 : b.items * p.rounds;
   for (int i = t; i < items; i += G) {
     const int item = i / p.rounds, who = b.again[item], s = who / G;
     const int chunk = (s * p.rounds + i - item * p.rounds) * G + who % G;
-    if (chunk >= min(p.cut.nvec, (s + 1) * p.rounds * G)) continue;
+    if (chunk >= nvec) continue;
     const v4i w = p.body[chunk];
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
@@ -286,7 +322,7 @@ __global__ void __launch_bounds__(G) top_kernel(const T* logits, int A, int K, i
     }
   }
   lds_barrier();
-  if (b.count > kSorted<G>) settle(p, b, want);
+  if (many || b.count > kSorted<G>) settle(p, b, want);
   if (parts == 1) {
     ranked<G>(b, K, [&](int rank, u64 e) {
       leave(p.row, e, values + r * K + rank, ids + r * K + rank);
@@ -361,7 +397,10 @@ struct TopPlan {
   int parts, per;
 };
 constexpr int64_t kPartElements = 1 << 16;
-// Bytes of a row that a wave takes by itself (16384 x 2000 bf16 49 -> 31 us; 4096 x 4000
+// Logits of more than the last-level cache holds are read past it (1024 x 200000 bf16, K = 32,
+// 85 -> 76 us; 147 MB of them that lie there 24 -> 27).
+constexpr int64_t kCacheBytes = (int64_t)256 << 20;
+// Bytes of a row that a wave takes by itself (16384 x 2000 bf16 49 -> 25 us; 4096 x 4000
 // fp32 20 -> 22).
 constexpr int64_t kWaveRow = 8192;
 TopPlan plan_of(int64_t rows, int64_t A, int dtype) {
@@ -407,12 +446,14 @@ extern "C" int ppo_token_top(const void* logits, int dtype, int64_t rows, int64_
     using T = decltype(zero);
     const T* in = static_cast<const T*>(logits);
     T* out = static_cast<T*>(values);
+    const bool past = rows * A * dtype_size(dtype) > kCacheBytes;
     // (K of G lanes' maxima: the bound lies close to the K-th element, and few reach it,
     // with more lanes than K)
     auto go = [&](auto lanes) {
       constexpr int G = decltype(lanes)::value;
-      hipLaunchKernelGGL((top_kernel<T, G>), dim3((unsigned)(rows * plan.parts)), dim3(G), 0, stream,
-                         in, (int)A, (int)K, plan.parts, plan.per, out, ids, found);
+      const auto kernel = past ? top_kernel<T, G, true> : top_kernel<T, G, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * plan.parts)), dim3(G), 0, stream, in, (int)A,
+                         (int)K, plan.parts, plan.per, out, ids, found);
       return last_launch_status();
     };
     const int code = plan.parts == 1 && A * dtype_size(dtype) <= kWaveRow && (K <= 48 || A <= 512)
