@@ -893,6 +893,38 @@ def test_another_stream(dev):
         assert all(torch.equal(p, q) for p, q in zip(top, ppo_amd.top_logits(x, 7)))
 
 
+@pytest.mark.parametrize("name", ["policy", "preference", "distillation"])
+def test_gradients_are_the_callers(dev, name):
+    """What a backward pass gives back may be changed, and any incoming gradient will do."""
+    f, x = losses(dev, torch.float32, A=300)
+    f = f[name]
+    xg = x.clone().requires_grad_()
+    y = f(xg)
+    (d,) = torch.autograd.grad(y, [xg], retain_graph=True)
+    want = d.clone()
+    d.zero_()
+    assert torch.equal(torch.autograd.grad(y, [xg])[0], want)
+    y = f(xg)
+    y.backward(retain_graph=True)
+    y.backward()
+    assert torch.allclose(xg.grad, 2 * want, rtol=8 * U32, atol=1e-12)
+    y = f(xg)
+    assert torch.allclose(torch.autograd.grad(y + y, [xg])[0], 2 * want, rtol=8 * U32, atol=1e-12)
+    for s in (0.0, -1.0):
+        (d,) = torch.autograd.grad(f(xg) * s, [xg])
+        assert torch.allclose(d, s * want, rtol=8 * U32, atol=1e-12)
+    live = want.abs().sum(-1) > 0
+    (d,) = torch.autograd.grad(f(xg) * float("nan"), [xg])
+    assert torch.isnan(d[live]).all() and not d[~losses_mask(dev, x)].any()
+    with torch.inference_mode():
+        assert torch.equal(f(x * 1.0), f(x))
+
+
+def losses_mask(dev, x, seed=5):
+    S, T, A = x.shape
+    return policy_case(seed, x.dtype, S, T, A)["mask"].to(dev)
+
+
 def test_calls_at_once(dev):
     """Threads with a stream each, all operators forward and back, and graphs of two
     losses that replay side by side."""
