@@ -74,8 +74,8 @@ def preference(relative, mask, beta, margin, smoothing, average):
 
 def distill_rows(ls, teacher, ids, tau):
     """(row losses, dloss/dz [R, A], q) without the factor tau^2 w / tau; entries with
-    ids < 0 are none."""
-    live = ids >= 0
+    ids < 0 are none, and so is a teacher's -inf."""
+    live = (ids >= 0) & (teacher != -float("inf"))
     t = torch.where(live, teacher / tau, torch.full_like(teacher, -float("inf")))
     some = live.any(1, keepdim=True)
     lq = t - torch.where(some, torch.logsumexp(t, 1, keepdim=True), torch.zeros(len(t), 1).double())

@@ -626,6 +626,30 @@ def test_distillation_edges(dev, A):
         assert float(d.abs().max()) < 64 * U32 / R
 
 
+@pytest.mark.parametrize("A", [30, 1000, 20000, 40000, 300000])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_distillation_of_entries_that_weigh_nothing(dev, A, offset):
+    """A row whose entries are all a teacher's -inf is one without entries: no loss, no
+    gradient, neither with the forward pass nor formed anew, in every layout."""
+    R = 70 if A < 100000 else 4
+    x = at_offset(torch.randn(R, A), dev, offset).requires_grad_()
+    teacher = torch.randn(R, 5, device=dev)
+    ids = torch.randint(0, A, (R, 5), device=dev)
+    ids[1, 3] = ids[1, 0]
+    none = ids.clone()
+    none[1] = -1
+    teacher[1] = -float("inf")
+    runs = []
+    for i in (ids, none):
+        loss = ppo_amd.distillation_loss(x, teacher, i, temperature=2.0)
+        runs.append([loss.detach(), *(torch.autograd.grad(loss * up, [x], retain_graph=True)[0]
+                                      for up in (1.0, -3.0))])
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+    for d in runs[0][1:]:
+        assert not d[1].any() and d[0].any()
+    assert torch.isfinite(runs[0][0])
+
+
 # --- top logits ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", list(TYPES))

@@ -232,6 +232,16 @@ def test_oracle_distillation():
     assert torch.allclose(q.sum(1), (ids >= 0).any(1).double())
 
 
+def test_oracle_distillation_of_entries_that_weigh_nothing():
+    torch.manual_seed(5)
+    ls = ref.log_softmax(torch.randn(3, 8).double())
+    t, ids = torch.randn(3, 2).double(), torch.randint(0, 8, (3, 2))
+    t[1], t[2, 0] = -float("inf"), -float("inf")
+    rows_, d, q = ref.distill_rows(ls, t, ids, 1.4)
+    assert rows_[1] == 0 and not d[1].any() and not q[1].any() and q[2].tolist() == [0.0, 1.0]
+    assert torch.allclose(rows_[2], -ls[2, ids[2, 1]])
+
+
 def test_oracle_weights():
     mask = torch.tensor([[1, 1, 0], [0, 0, 0], [1, 0, 0]], dtype=torch.bool)
     assert torch.allclose(ref.weights(mask), mask.double() / 3)

@@ -106,7 +106,10 @@ __device__ __forceinline__ Entries take_entries(const Teacher& teacher, int64_t 
   gap = lanes_sum<G>(gap);
   const float inv = s == 0.0f ? 0.0f : 1.0f / s;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  for (int k = lane; k < K; k += G) b.q[k] *= inv;
+  for (int k = lane; k < K; k += G) {
+    b.q[k] *= inv;
+    if (s == 0.0f) b.col[k] = -1;  // (entries that all weigh nothing are none)
+  }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   // Entries of one column write its sum, all of them.  Such are rare: only where a column's
   // mark is there already are they looked for, four at a time, and summed.

@@ -565,8 +565,8 @@ def distillation_loss(
 
     teacher_logits [..., K] (fp32, bf16 or fp16, K up to 256) and teacher_ids
     [..., K] (int32 or int64).  An entry with a negative id is none; entries of
-    one id add up; an id from A on gives NaN; a row without entries adds 0 to
-    the loss and counts.  mask, reduction, denominator and grad_scale are
+    one id add up; an id from A on gives NaN; a row without entries, or with
+    none but -inf, adds 0 to the loss, has no gradient and counts.  mask, reduction, denominator and grad_scale are
     token_policy_loss's.  Differentiable once in the student's logits alone."""
     got = _native().distillation_loss(logits, teacher_logits, teacher_ids, mask, temperature,
                                       _lib.TOKEN_REDUCTIONS.get(reduction), denominator,
