@@ -149,7 +149,7 @@ int ppo_token_preference(const float* relative, const uint8_t* mask, int64_t seq
  *   loss = temperature^2 sum_r w_r sum_k q_k (log q_k - log p[id_k])
  * An id may come twice (its entries add up); negative ids are no entries, and a
  * row without entries, or with none but a teacher's -inf, has loss and gradient 0
- * and counts.  An id from A on gives NaN.  rows->actions is not read.  Of `loss`, reduction, denominator and
+ * and counts (NaN where its logits give it).  An id from A on gives NaN.  rows->actions is not read.  Of `loss`, reduction, denominator and
  * grad_scale count.  dlogits and saved may be NULL; backward forms the gradient for
  * any incoming one from saved, as ppo_token_log_probs_backward does.
  */

@@ -650,6 +650,30 @@ def test_distillation_of_entries_that_weigh_nothing(dev, A, offset):
     assert torch.isfinite(runs[0][0])
 
 
+@pytest.mark.parametrize("A", [30, 1000, 20000, 300000])
+@pytest.mark.parametrize("wreck", ["nan", "inf", "-inf"])
+def test_distillation_of_a_wrecked_row_without_entries(dev, A, wreck):
+    """A row that gives NaN (NaN, +inf, nothing but -inf) does so in the loss as in the
+    gradient, also without entries."""
+    R = 70 if A < 100000 else 4
+    x = torch.randn(R, A, device=dev)
+    x[1, slice(None) if wreck == "-inf" else A // 2] = float(wreck)
+    x.requires_grad_()
+    ids = torch.randint(0, A, (R, 3), device=dev)
+    ids[1] = -1
+    teacher = torch.randn(R, 3, device=dev)
+    loss = ppo_amd.distillation_loss(x, teacher, ids)
+    rest = [r for r in range(R) if r != 1]
+    for up in (1.0, 2.0):
+        (d,) = torch.autograd.grad(loss * up, [x], retain_graph=True)
+        assert torch.isnan(d[1]).all() and torch.isfinite(d[rest]).all()
+    assert torch.isnan(loss)
+    with torch.no_grad():
+        assert torch.isnan(ppo_amd.distillation_loss(x, teacher, ids))
+        mask = torch.arange(R, device=dev) != 1
+        assert torch.isfinite(ppo_amd.distillation_loss(x, teacher, ids, mask))
+
+
 # --- top logits ----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", list(TYPES))

@@ -51,10 +51,12 @@ int board_ints(int K) { return 4 * (int)round_up(K, 4) + kMarkWords; }
 // What the entries come to: sum q (1; 0 without entries; NaN with one that is not finite)
 // and the loss but for the student's m and log s:
 //   sum_k q_k (log q_k - log p_k) = c ln 2 (gap + total (m - top)) + log s - log_s.
+// (Without entries 0 times the row's own terms: a row that gives NaN gives it here as in its
+// gradient.)
 struct Entries {
   float total, gap, top, log_s;
   __device__ __forceinline__ float loss(float m, float s_log, float c) const {
-    return total == 0.0f ? 0.0f : fmaf(c * kLn2, gap + (m - top), s_log - log_s);
+    return total == 0.0f ? 0.0f * (m + s_log) : fmaf(c * kLn2, gap + (m - top), s_log - log_s);
   }
 };
 
