@@ -392,6 +392,36 @@ def test_policy_loss_incoming_gradients(dev, A):
         assert all(torch.equal(p, q) for p, q in kept)  # (no later pass writes an earlier one's)
 
 
+@pytest.mark.parametrize("A", [18, 1000, 9000, 40000, 280000])
+def test_policy_loss_far_from_the_reference(dev, A):
+    """The KL term's derivative in log p is -(e^d - 1) however far the reference lies, and
+    finite where it rules out the action that was taken (the loss is infinite there)."""
+    far = torch.tensor([-float("inf"), -1e30, -1e9, -3e4, -200.0, -30.0, -5.0, -1.01, -0.99, -1e-4,
+                        0.0, 0.5, 1.0, 1.5, 20.0])
+    S, T, t = (6 if A < 100000 else 1), 15, torch.float32
+    c = policy_case(A, t, S, T, A)
+    b = bounds(c["x"], c["a"])
+    r = (b.lp + far.repeat(S)).float()
+    old, adv, kc, w = c["old"].double(), c["adv"].double(), 0.3, 1.0 / (S * T)
+    _, kl, _, _, g, _ = ref.policy_terms(b.lp, b.H, old, adv, r.double(), 0.2, 0.2, kc, 0.0)
+    # e^d carries log p's error, d's rounding and two units of expf; of the series 16 in all
+    d, ratio = r.double() - b.lp, torch.exp(b.lp - old)
+    dg = w * (adv * ratio).abs() * (b.e_lp + U32 * (6 + (b.lp - old).abs()))
+    dg = dg + w * kc * (torch.exp(d) * (b.e_lp + U32 * (4 + d.abs().clamp(max=100)))
+                        + 4 * U32 * torch.expm1(d).abs() + 16 * U32 * kl.clamp(max=1.0))
+    want = ref.log_probs_grad(b.ls, c["a"], g * w, 0 * g)
+    bound = b.dlogits(want, g * w, 0 * g, t, dg + 4 * U32 * (g * w).abs())
+    v = lambda u: u.view(S, T).to(dev)  # noqa: E731
+    for offset in (0, 3):
+        xd = at_offset(c["x"].view(S, T, A), dev, offset).requires_grad_()
+        loss, stats = ppo_amd.token_policy_loss(xd, v(c["a"]), v(c["old"]), v(c["adv"]), v(r),
+                                                kl_coef=kc)
+        assert loss == float("inf") and stats["kl"] == float("inf")
+        for up in (1.0, 2.0):
+            (dx,) = torch.autograd.grad(loss, [xd], torch.tensor(up, device=dev), retain_graph=True)
+            assert_within(dx.view(S * T, A), up * want, up * bound, f"{offset} {up}")
+
+
 def test_policy_loss_over_nothing(dev):
     """Masks that leave nothing, and no rows at all: 0, and gradients of 0."""
     f = ppo_amd.token_policy_loss

@@ -33,17 +33,25 @@ struct RowLoss {
   }
 };
 
-// e^d - d - 1: its series where the difference would cancel (to |d| = 1, where the
-// next term is below 2^-28 of the sum).
-__device__ __forceinline__ float kl_estimate(float d) {
-  if (!(fabsf(d) <= 1.0f)) return expf(d) - d - 1.0f;
+// e^d - d - 1 and its derivative e^d - 1: the first's series where the differences would
+// cancel (to |d| = 1, where the next term is below 2^-28 of the sum), and from e^d beyond (a
+// derivative of value + d would lose its 1 in a large -d, and be NaN at d = -inf).
+struct KlEstimate {
+  float value, slope;
+};
+__device__ __forceinline__ KlEstimate kl_estimate(float d) {
+  if (!(fabsf(d) <= 1.0f)) {
+    const float e = expf(d);
+    return {e - d - 1.0f, e - 1.0f};
+  }
   float q = 1.0f / 479001600.0f;
   constexpr float kInv[] = {1.0f / 39916800, 1.0f / 3628800, 1.0f / 362880, 1.0f / 40320,
                             1.0f / 5040,     1.0f / 720,     1.0f / 120,    1.0f / 24,
                             1.0f / 6,        0.5f};
 #pragma unroll
   for (float k : kInv) q = fmaf(d, q, k);
-  return d * d * q;
+  const float v = d * d * q;
+  return {v, v + d};
 }
 
 // A row's inputs beside its logits.
@@ -67,9 +75,9 @@ __device__ __forceinline__ RowLoss policy_row(const Policy& p, const RowIn& in, 
                ratio < p.lo || ratio > p.hi ? 1.0f : 0.0f};
   G = u > v ? 0.0f : -u;
   if (p.ref) {
-    const float d = (float)((double)in.ref - t.lp);
-    o.kl = kl_estimate(d);
-    if (p.kl_coef != 0.0f) G -= p.kl_coef * (o.kl + d);  // (e^d - 1)
+    const KlEstimate kl = kl_estimate((float)((double)in.ref - t.lp));
+    o.kl = kl.value;
+    if (p.kl_coef != 0.0f) G -= p.kl_coef * kl.slope;
   }
   G *= in.w;
   E = -p.entropy_coef * in.w;
