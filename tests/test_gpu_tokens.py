@@ -13,6 +13,7 @@ import threading
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd_ad
 
 import ppo_amd
 from oracle import tokens_oracle as ref
@@ -1300,3 +1301,26 @@ def test_refusals(dev):
     with pytest.raises(_lib.PPOLibraryError):
         top(torch.zeros(1, (1 << 22) + 1, dtype=torch.float16, device=dev), 2)
     assert tokens.top_logits(x[:0], 3)[0].shape == (0, 4, 3)
+
+
+def test_constants_that_ask_for_a_gradient(dev):
+    """Operands in which a loss has no gradient are refused where they ask for one, in
+    either direction, and taken where nothing is differentiated."""
+    x = torch.randn(2, 4, 30, device=dev, requires_grad=True)
+    a = torch.zeros(2, 4, dtype=torch.int64, device=dev)
+    z = torch.zeros(2, 4, device=dev)
+    one = z[:, 0].contiguous()
+    pl, pr = ppo_amd.token_policy_loss, ppo_amd.preference_loss
+    for name, call, v in (("old_log_probs", lambda v: pl(x, a, v, z), z),
+                          ("advantages", lambda v: pl(x, a, z, v), z),
+                          ("advantages", lambda v: pl(x, a, z, v), one),
+                          ("ref_log_probs", lambda v: pl(x, a, z, z, v, kl_coef=0.1), z),
+                          ("ref_log_probs", lambda v: pr(x, a, v), z)):
+        wants = v.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match=f"no gradient in {name}"):
+            call(wants)
+        with torch.no_grad():
+            quiet = call(wants)[0]
+        assert torch.equal(quiet, call(wants.detach())[0].detach())
+        with fwd_ad.dual_level(), pytest.raises(RuntimeError, match=f"no gradient in {name}"):
+            call(fwd_ad.make_dual(v, v))

@@ -107,3 +107,26 @@ def test_registered_operators_compile(dev):
         y = f(x)
         runs.append([y.detach(), *torch.autograd.grad(y, [x])])
     assert all(torch.equal(p, q) for p, q in zip(*runs))
+
+
+def test_registered_constants_that_ask_for_a_gradient(dev):
+    op = torch.ops.ppo_amd
+    x, a, old, adv, mask, teacher, ids = _case(dev)
+    calls = [("old_log_probs", old, lambda v: op.token_policy_loss(
+                  x, a, v, adv, old, mask, 0.2, 0.3, 0.05, 0.01, 1.0, "token", None)),
+             ("advantages", adv, lambda v: op.token_policy_loss(
+                 x, a, old, v, old, mask, 0.2, 0.3, 0.05, 0.01, 1.0, "token", None)),
+             ("ref_log_probs", old, lambda v: op.token_policy_loss(
+                 x, a, old, adv, v, mask, 0.2, 0.3, 0.05, 0.01, 1.0, "token", None)),
+             ("ref_log_probs", old, lambda v: op.preference_loss(
+                 x, a, v, mask, 0.1, 0.05, 0.0, False, 1.0)),
+             ("teacher_logits", teacher, lambda v: op.distillation_loss(
+                 x, v, ids, mask, 2.0, "token", None))]
+    for name, v, call in calls:
+        wants = v.clone().requires_grad_()
+        for f in (call, torch.compile(call, fullgraph=True, backend="aot_eager")):
+            with pytest.raises(RuntimeError, match=f"no gradient in {name}"):
+                f(wants)
+        with torch.no_grad():
+            quiet = call(wants)[0]
+        assert torch.equal(quiet, call(v)[0])

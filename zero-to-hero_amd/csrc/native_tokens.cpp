@@ -61,6 +61,12 @@ PyObject* capture_id(PyObject*, PyObject* index) {
   }
 }
 
+// An operand that has no gradient here: where it asks for one, tokens.py refuses it.
+const Tensor& constant(const Tensor& t) {
+  need(!t._fw_grad(0).defined() && !(at::GradMode::is_enabled() && t.requires_grad()));
+  return t;
+}
+
 // Logits and what every row of them has: actions (int32 or int64; undefined for a
 // distilled row) and a mask (bool or uint8; undefined: every row counts).
 struct Rows {
@@ -100,7 +106,7 @@ struct Rows {
     need(r.sizes() == shape());
     return r;
   }
-  Tensor row_floats(PyObject* o) const { return row_tensor(o, at::kFloat); }
+  Tensor row_constants(PyObject* o) const { return constant(row_tensor(o, at::kFloat)); }
   ppo_token_rows c() const {
     return {logits.const_data_ptr(), ptr(actions), static_cast<const uint8_t*>(ptr(mask)),
             sequences(), tokens(), A(), dtype(),
@@ -341,13 +347,13 @@ struct PolicyNode : public torch::autograd::Function<PolicyNode> {
 PyObject* token_policy_loss(PyObject* const* a) {
   Policy p;
   p.r = Rows(a[0], a[1], a[5], a[10]);
-  p.old = p.r.row_floats(a[2]);
-  p.adv = plain(a[3], at::kFloat, p.r.device());
+  p.old = p.r.row_constants(a[2]);
+  p.adv = constant(plain(a[3], at::kFloat, p.r.device()));
   const at::IntArrayRef rows = p.r.shape();
   p.l.advantages_per_sequence =
       !rows.empty() && p.adv.sizes() == rows.slice(0, rows.size() - 1);
   need(p.l.advantages_per_sequence || p.adv.sizes() == rows);
-  if (a[4] != Py_None) p.ref = p.r.row_floats(a[4]);
+  if (a[4] != Py_None) p.ref = p.r.row_constants(a[4]);
   p.l.clip_low = number(a[6]);
   p.l.clip_high = number(a[7]);
   p.l.kl_coef = finite(a[8]);
@@ -420,7 +426,7 @@ PyObject* preference_loss(PyObject* const* a) {
   Preference p;
   p.r = Rows(a[0], a[1], a[3], a[8]);
   need(p.r.logits.dim() == 3 && p.r.logits.size(0) % 2 == 0);
-  if (a[2] != Py_None) p.ref = p.r.row_floats(a[2]);
+  if (a[2] != Py_None) p.ref = p.r.row_constants(a[2]);
   p.beta = finite(a[4]);
   p.smoothing = number(a[5]);
   need(p.smoothing >= 0.0 && p.smoothing <= 1.0);
@@ -512,13 +518,11 @@ PyObject* distillation_loss(PyObject* const* a) {
   p.r = Rows(a[0], nullptr, a[3], a[4]);
   const at::ScalarType tt = type_of(a[1]), it = type_of(a[2]);
   need(dtype_code(tt) >= 0 && (it == at::kInt || it == at::kLong));
-  p.teacher = plain(a[1], tt, p.r.device());
+  p.teacher = constant(plain(a[1], tt, p.r.device()));
   p.ids = plain(a[2], it, p.r.device());
   const int64_t dim = p.r.logits.dim();
   need(p.teacher.dim() == dim && p.teacher.sizes() == p.ids.sizes() && p.teacher.size(-1) > 0 &&
        p.teacher.sizes().slice(0, dim - 1) == p.r.shape());
-  need(!p.teacher._fw_grad(0).defined() &&
-       !(at::GradMode::is_enabled() && p.teacher.requires_grad()));
   weights_of(a + 5, p.l);
   Tensor loss;
   if (p.r.differentiable()) {

@@ -135,6 +135,13 @@ def _like(logits, actions, mask):
                                                          for t in (actions, mask)))
 
 
+def _check_constants(what: str, **tensors) -> None:
+    """Refuses operands that ask for a gradient which `what` does not form."""
+    for name, t in tensors.items():
+        if _wants_gradient(t):
+            raise RuntimeError(f"{what} has no gradient in {name}: detach it")
+
+
 def _once(what: str) -> None:
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} can be differentiated once: its backward pass has no "
@@ -444,8 +451,8 @@ def token_policy_loss(
     of their means ("sequence"); `denominator` takes the place of the number of
     those tokens or sequences, for a batch in several calls or ranks.
     logits [..., T, A]; actions, old_log_probs, ref_log_probs and mask [..., T];
-    advantages [..., T], or [...] for one a sequence.  Over no tokens the loss
-    is 0.
+    advantages [..., T], or [...] for one a sequence; those three are constants, and
+    refused where they require a gradient.  Over no tokens the loss is 0.
 
     Returns (loss, stats): `loss` is a 0-d tensor to differentiate once in the
     logits, `stats` the same means of the terms, reported values.  The forward
@@ -464,6 +471,8 @@ def token_policy_loss(
     per_sequence = _check_policy(logits, actions, old_log_probs, advantages, ref_log_probs, mask,
                                  clip_low, clip_high, kl_coef, entropy_coef, temperature)
     _check_weights(reduction, denominator, grad_scale)
+    _check_constants("token_policy_loss", old_log_probs=old_log_probs, advantages=advantages,
+                     ref_log_probs=ref_log_probs)
     loss = _loss(reduction, denominator, grad_scale, clip_low, clip_high, kl_coef, entropy_coef,
                  per_sequence)
     args = (logits, actions, old_log_probs, advantages, ref_log_probs, mask, float(temperature),
@@ -509,7 +518,7 @@ def preference_loss(
     rejected ones; actions, ref_log_probs and mask [2 P, T].  A sequence's log
     ratio is the sum (the mean with `average`) of log p[action] - ref_log_probs
     over the tokens that the mask counts, 0 over none; without ref_log_probs
-    they count as 0.  The loss is the mean over pairs of
+    (constants, refused where they require a gradient) they count as 0.  The loss is the mean over pairs of
       -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m),
       m = beta (chosen ratio - rejected ratio) - margin.
 
@@ -523,6 +532,7 @@ def preference_loss(
         return got[0], PreferenceStats(zip(("chosen", "rejected"), got[1]))
     _check_preference(logits, actions, ref_log_probs, mask, beta, label_smoothing, margin,
                       temperature)
+    _check_constants("preference_loss", ref_log_probs=ref_log_probs)
     if _wants_gradient(logits):
         loss, rewards = _PreferenceLoss.apply(logits, actions, ref_log_probs, mask,
                                               float(temperature), beta, margin, label_smoothing,

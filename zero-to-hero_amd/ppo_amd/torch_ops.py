@@ -321,6 +321,13 @@ def _check_scalar(logits: Tensor, scale: Optional[Tensor]) -> None:
             raise ValueError(f"scale must hold one value, got {scale.numel()}")
 
 
+def _refuse_gradients(ctx, what: str, inputs: dict) -> None:
+    """Inputs (index: name) that ask for a gradient which the operator does not form."""
+    for index, name in inputs.items():
+        if ctx.needs_input_grad[index]:
+            raise RuntimeError(f"{what} has no gradient in {name}: detach it")
+
+
 @torch.library.custom_op(f"{_NS}::token_log_probs", mutates_args=(), device_types="cuda")
 def token_log_probs(logits: Tensor, actions: Tensor, mask: Optional[Tensor], temperature: float
                     ) -> tuple[Tensor, Tensor, Tensor]:
@@ -397,6 +404,8 @@ def _token_policy_loss_fake(logits, actions, old_log_probs, advantages, ref_log_
 
 
 def _token_policy_setup(ctx, inputs, output):
+    _refuse_gradients(ctx, "token_policy_loss",
+                      {2: "old_log_probs", 3: "advantages", 4: "ref_log_probs"})
     logits, actions, mask, ctx.temperature = inputs[0], inputs[1], inputs[5], inputs[10]
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(logits, actions, mask, output[1], output[2])
@@ -433,6 +442,7 @@ def _preference_loss_fake(logits, actions, ref_log_probs, mask, beta, label_smoo
 
 
 def _preference_setup(ctx, inputs, output):
+    _refuse_gradients(ctx, "preference_loss", {2: "ref_log_probs"})
     logits, actions, mask, ctx.temperature = inputs[0], inputs[1], inputs[3], inputs[8]
     ctx.mark_non_differentiable(*output[1:])
     ctx.save_for_backward(logits, actions, mask, output[2], output[3])
@@ -485,6 +495,7 @@ def _distillation_loss_backward_fake(logits, teacher_logits, teacher_ids, mask, 
 
 
 def _distillation_setup(ctx, inputs, output):
+    _refuse_gradients(ctx, "distillation_loss", {1: "teacher_logits"})
     logits, teacher, ids, mask, ctx.temperature = inputs[:5]
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(logits, teacher, ids, mask, output[1])
