@@ -26,8 +26,9 @@
  * Logits that another stream writes during a call give undefined results (top's
  * columns lie in their rows all the same).
  *
- * Rows times A up to 2^46, A up to 2^30, rows below 2^24 (2^22 in top; more where a row
- * takes fewer than 256 lanes): PPO_ERR_TOO_LARGE otherwise.
+ * Rows times A up to 2^46, A up to 2^30, rows below 2^24, more where a row takes fewer than
+ * 256 lanes (top: below 2^24, 2^23 and 2^22 for K up to 96, 192 and 256, and below 2^26
+ * of up to 8 KB with K up to 48 or A up to 512): PPO_ERR_TOO_LARGE otherwise.
  */
 #ifndef PPO_TOKENS_H
 #define PPO_TOKENS_H

@@ -726,6 +726,13 @@ def test_top_logits_match_a_stable_sort(dev, shape, dtype):
     assert torch.equal(i.cpu(), wi) and torch.equal(v.cpu().float(), wv)
 
 
+def test_top_logits_of_many_narrow_rows(dev):
+    """More rows than a launch of workgroups holds, by a wave each."""
+    x = torch.randn((1 << 22) + 3, 3, device=dev, dtype=torch.float16)
+    for got, want in zip(ppo_amd.top_logits(x, 2), x.sort(dim=-1, descending=True, stable=True)):
+        assert torch.equal(got, want[:, :2])
+
+
 @pytest.mark.parametrize("A", [40, 3000, 40000, 300000])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_top_logits_ties_and_values_that_are_not_finite(dev, dtype, A):

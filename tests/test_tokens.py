@@ -78,6 +78,14 @@ def test_launches_that_do_not_fit():
                                       ctypes.c_void_p(4100), P, big, None) == 3
 
 
+def test_top_launches_that_do_not_fit():
+    """The limit counts the lanes that a row takes."""
+    lib = _lib.load_tokens()
+    for R, A, K in ((1 << 26, 18, 3), (1 << 24, 3000, 60), (1 << 23, 3000, 100),
+                    (1 << 22, 3000, 200), (1 << 24, 20000, 3)):
+        assert lib.ppo_token_top(P, 1, R, A, K, P, P, None, 0, None) == 3
+
+
 def test_log_probs_arguments():
     lib = _lib.load_tokens()
     f = lib.ppo_token_log_probs

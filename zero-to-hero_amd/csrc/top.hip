@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(1024) top_merge_kernel(const T* logits, int A,
   });
 }
 
-// Parts of a row, so many that few rows fill the chip, of 16 KB at least and of 2^16
-// elements at most.
+// Parts of a row, so many that few rows fill the chip, of 16 KB at least, and below 512
+// rows of about 2^16 elements at most; of more rows one.
 struct TopPlan {
   int parts, per;
 };
@@ -436,7 +436,14 @@ extern "C" int ppo_token_top(const void* logits, int dtype, int64_t rows, int64_
     return PPO_ERR_INVALID_ARG;
   if (K > kMaxK || A > ((int64_t)1 << 22)) return PPO_ERR_TOO_LARGE;
   const TopPlan plan = plan_of(rows, A, dtype);
-  if (!fits_launch(rows * plan.parts, 1024)) return PPO_ERR_TOO_LARGE;
+  // (K of the lanes' maxima: the bound lies close to the K-th element, and few reach it,
+  // with more lanes than K)
+  const int lanes = plan.parts == 1 && A * dtype_size(dtype) <= kWaveRow && (K <= 48 || A <= 512)
+                        ? kWave
+                    : K <= 96  ? 256
+                    : K <= 192 ? 512
+                               : 1024;
+  if (!fits_launch(rows * plan.parts, lanes)) return PPO_ERR_TOO_LARGE;  // (parts: of few rows)
   if (plan.parts > 1 && (!workspace || !aligned16(workspace) ||
                          workspace_bytes < ppo_token_top_workspace_bytes(rows, A, K, dtype)))
     return PPO_ERR_WORKSPACE;
@@ -447,20 +454,17 @@ extern "C" int ppo_token_top(const void* logits, int dtype, int64_t rows, int64_
     const T* in = static_cast<const T*>(logits);
     T* out = static_cast<T*>(values);
     const bool past = rows * A * dtype_size(dtype) > kCacheBytes;
-    // (K of G lanes' maxima: the bound lies close to the K-th element, and few reach it,
-    // with more lanes than K)
-    auto go = [&](auto lanes) {
-      constexpr int G = decltype(lanes)::value;
+    auto go = [&](auto group) {
+      constexpr int G = decltype(group)::value;
       const auto kernel = past ? top_kernel<T, G, true> : top_kernel<T, G, false>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * plan.parts)), dim3(G), 0, stream, in, (int)A,
                          (int)K, plan.parts, plan.per, out, ids, found);
       return last_launch_status();
     };
-    const int code = plan.parts == 1 && A * dtype_size(dtype) <= kWaveRow && (K <= 48 || A <= 512)
-                         ? go(Int<kWave>{})
-                     : K <= 96  ? go(Int<256>{})
-                     : K <= 192 ? go(Int<512>{})
-                                : go(Int<1024>{});
+    const int code = lanes == kWave ? go(Int<kWave>{})
+                     : lanes == 256 ? go(Int<256>{})
+                     : lanes == 512 ? go(Int<512>{})
+                                    : go(Int<1024>{});
     if (code || plan.parts == 1) return code;
     hipLaunchKernelGGL((top_merge_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, stream, in,
                        (int)A, (int)K, plan.parts, out, ids, found);
