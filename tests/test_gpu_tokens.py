@@ -257,6 +257,30 @@ def test_logits_that_are_not_finite(dev, dtype, A):
     assert not dx[ok][(x[ok] == -float("inf")).to(dev) & ~(b.hot > 0).to(dev)].any()
 
 
+@pytest.mark.parametrize("A", [30, 1000, 20000, 300000])
+@pytest.mark.parametrize("low", [-float("inf"), torch.finfo(torch.float32).min])
+def test_entropy_gradients_of_a_scaled_loss_where_nothing_can_be_taken(dev, A, low):
+    """Logits that are left out get a gradient of 0 whatever the incoming one's size; the
+    others' are in proportion (a power of two: the same roundings)."""
+    R, k = (70, 1) if A < 100000 else (4, 16)
+    x, a, g = rows_of(A, torch.float32, R, A)
+    hide = torch.rand(R, A, generator=g) < 0.5
+    hide.scatter_(1, a[:, None], False)
+    x[hide] = low
+    hide, ad, up, z = hide.to(dev), a.to(dev), k * 2.0 ** 34, torch.zeros(R, device=dev)
+    for offset in (0, 3):
+        xd = at_offset(x, dev, offset).requires_grad_()
+        _, H = ppo_amd.token_log_probs(xd, ad, entropy=True)
+        small, big = (torch.autograd.grad(H, [xd], torch.full_like(z, v), retain_graph=True)[0]
+                      for v in (1.0, up))
+        assert not big[hide].any() and torch.equal(big, small * up)
+        old = ppo_amd.token_log_probs(xd.detach(), ad)
+        for scale in (1.0, up):
+            loss, _ = ppo_amd.token_policy_loss(xd, ad, old, z, entropy_coef=1.0, grad_scale=scale)
+            (d,) = torch.autograd.grad(loss, [xd], torch.tensor(up, device=dev))
+            assert torch.isfinite(d).all() and not d[hide].any()
+
+
 def test_actions_outside_the_row(dev):
     for A in (18, 5000, 40000):
         x = torch.randn(66, A, device=dev).requires_grad_()

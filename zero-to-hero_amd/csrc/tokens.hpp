@@ -354,12 +354,14 @@ __device__ __forceinline__ Grad row_grad(const Saved& t, float G, float E, float
   g.da = inv_tau * (G * t.omp - (t.pa == 0.0f ? 0.0f : E * t.pa * (t.lp + t.H)));
   return g;
 }
-// (kC: C is not 0.  An e of 0 has an exponent of -inf, held finite there.)
+// (kC: C is not 0.  An e of 0 has an exponent of -inf, or one that times C may become that:
+// it is held where e has long been 0, and its product with any C of use finite.)
+constexpr float kLeastExponent = -256.0f;
 template <bool kC>
 __device__ __forceinline__ float grad_at(const Grad& g, float c, float l) {
   const float t = (l - g.m) * c;
   const float e = exp2_fast(t);
-  return kC ? e * fmaf(g.C, fmaxf(t, -1e30f), g.B) : e * g.B;
+  return kC ? e * fmaf(g.C, fmaxf(t, kLeastExponent), g.B) : e * g.B;
 }
 
 // ---------------------------------------------------------------------------
