@@ -546,6 +546,21 @@ def test_preference_loss_of_far_pairs(dev):
     assert abs(float(loss) - math.log(2.0)) < 1e-6
 
 
+@pytest.mark.parametrize("A", [40, 20000])
+def test_preference_at_the_largest_temperatures(dev, A):
+    """Nearly uniform rows but for the actions that cannot be taken, up to where
+    log2(e) / temperature is no normal number."""
+    x = torch.randn(4, 3, A, device=dev)
+    x[:, :, 7] = -float("inf")
+    a, z = torch.zeros(4, 3, dtype=torch.int64, device=dev), torch.zeros(4, 3, device=dev)
+    want = -0.1 * 3 * math.log(A - 1)
+    for k in range(48):
+        tau = 1e37 * 1.07 ** k
+        _, stats = ppo_amd.preference_loss(x, a, z, temperature=tau)
+        for reward in (*stats["chosen"], *stats["rejected"]):
+            assert abs(float(reward) - want) <= 8 * U32 * -want, tau
+
+
 @pytest.mark.parametrize("tau", [0.3, 0.7, 1.0, 1.5])
 @pytest.mark.parametrize("A", [40, 900, 20000, 300000])
 def test_preference_of_close_policies(dev, A, tau):

@@ -53,11 +53,13 @@ int take_rows(const ppo_token_rows* r, bool actions, Rows& out) {
     return PPO_ERR_INVALID_ARG;
   const double exact = 1.44269504088896340736 / r->temperature;
   const float c = (float)exact, c_down = (double)c < exact ? c : nextafterf(c, 0.0f);
+  // (what is left underflows at temperatures near the type's largest value)
+  const float c_left = fmaxf((float)(exact - (double)c_down), __FLT_DENORM_MIN__);
   const float inv_tau = (float)(1.0 / r->temperature);
   if (!(c > 0.0f) || !(c < INFINITY)) return PPO_ERR_INVALID_ARG;
   if (!sizes_ok(r->sequences, r->tokens, r->A)) return PPO_ERR_TOO_LARGE;
   out = {r->logits, r->actions, r->mask, r->sequences * r->tokens, r->tokens, r->sequences,
-         (int)r->A, r->actions_are_int64, c, inv_tau, c_down, (float)(exact - (double)c_down)};
+         (int)r->A, r->actions_are_int64, c, inv_tau, c_down, c_left};
   if (out.n == 0) return PPO_OK;
   const uintptr_t size = dtype_size(r->dtype);
   if (!r->logits || (uintptr_t)r->logits % size || (actions && !r->actions))
