@@ -89,9 +89,13 @@ int ppo_token_log_probs_backward(const ppo_token_rows* rows, const float* saved,
 #define PPO_SEQUENCE_MEAN 1  /* 1 / (the sequence's rows that count * sequences
                                 that have any)                                  */
 
+/* Where a denominator and a grad_scale lie: weights are held in fp32. */
+#define PPO_TOKEN_LEAST 1e-30
+#define PPO_TOKEN_MOST 1e30
+
 typedef struct ppo_token_loss {
   double clip_low, clip_high;  /* ratio within [1 - clip_low, 1 + clip_high]     */
-  double kl_coef, entropy_coef;
+  double kl_coef, entropy_coef; /* finite in fp32                                */
   double denominator;          /* > 0: in place of the number of rows (of
                                   sequences) that count; 0: that number          */
   double grad_scale;           /* the gradients are formed for this incoming one */
@@ -150,9 +154,10 @@ int ppo_token_preference(const float* relative, const uint8_t* mask, int64_t seq
  *   loss = temperature^2 sum_r w_r sum_k q_k (log q_k - log p[id_k])
  * An id may come twice (its entries add up); negative ids are no entries, and a
  * row without entries, or with none but a teacher's -inf, has loss and gradient 0
- * and counts (NaN where its logits give it).  An id from A on gives NaN.  rows->actions is not read.  Of `loss`, reduction, denominator and
- * grad_scale count.  dlogits and saved may be NULL; backward forms the gradient for
- * any incoming one from saved, as ppo_token_log_probs_backward does.
+ * and counts (NaN where its logits give it).  An id from A on gives NaN.
+ * rows->actions is not read.  Of `loss`, reduction, denominator and grad_scale
+ * count.  dlogits and saved may be NULL; backward forms the gradient for any
+ * incoming one from saved, as ppo_token_log_probs_backward does.
  */
 #define PPO_TOKEN_MAX_K 256
 int ppo_token_distillation(const ppo_token_rows* rows, const void* teacher, int teacher_dtype,

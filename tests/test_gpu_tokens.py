@@ -1370,3 +1370,24 @@ def test_constants_that_ask_for_a_gradient(dev):
         assert torch.equal(quiet, call(wants.detach())[0].detach())
         with fwd_ad.dual_level(), pytest.raises(RuntimeError, match=f"no gradient in {name}"):
             call(fwd_ad.make_dual(v, v))
+
+
+def test_numbers_that_fp32_does_not_hold(dev):
+    x = torch.randn(2, 4, 30, device=dev)
+    a = torch.zeros(2, 4, dtype=torch.int64, device=dev)
+    z, m = torch.zeros(2, 4, device=dev), torch.ones(2, 4, dtype=torch.bool, device=dev)
+    top = ppo_amd.top_logits(x, 3)
+    for kw in (dict(denominator=1e46), dict(denominator=1e-46), dict(grad_scale=1e39),
+               dict(grad_scale=1e-50)):
+        for mask in (None, m):
+            with pytest.raises(ValueError, match="must be in"):
+                ppo_amd.token_policy_loss(x, a, z, z, mask=mask, **kw)
+            with pytest.raises(ValueError, match="must be in"):
+                ppo_amd.distillation_loss(x, *top, mask, **kw)
+    for kw in (dict(kl_coef=1e39), dict(entropy_coef=-1e39)):
+        with pytest.raises(ValueError, match="_coef must be finite"):
+            ppo_amd.token_policy_loss(x, a, z, z, z, **kw)
+    one = float(ppo_amd.token_policy_loss(x, a, z, z + 1, mask=m, denominator=1.0)[0])
+    for den in (1e-30, 1e-20, 1e20, 1e30):
+        got = float(ppo_amd.token_policy_loss(x, a, z, z + 1, mask=m, denominator=den)[0])
+        assert abs(got * den - one) <= 4 * U32 * abs(one)

@@ -11,7 +11,7 @@ import torch
 
 import ppo_amd
 from oracle import tokens_oracle as ref
-from ppo_amd import _lib
+from ppo_amd import _lib, tokens
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "ppo_tokens.h")
@@ -127,6 +127,33 @@ def test_policy_arguments():
                 dict(scale=float("inf")), dict(red=2), dict(red=-1)):
         assert call(l=loss(**bad)) == 1
     assert call(work=None) == 2 and call(work=ODD) == 2 and call(nbytes=100) == 2
+
+
+UNHELD = [dict(den=1e46), dict(den=1e31), dict(den=1e-46), dict(den=1e-31), dict(scale=1e39),
+          dict(scale=1e31), dict(scale=1e-50), dict(scale=1e-31), dict(kl=1e39), dict(ent=-1e39)]
+
+
+@pytest.mark.parametrize("kw", UNHELD)
+@pytest.mark.parametrize("red", [0, 1])
+@pytest.mark.parametrize("mask", [None, P])
+def test_numbers_that_fp32_does_not_hold(kw, red, mask):
+    """Weights and coefficients that would be infinite or 0 in the kernels, or take a count's
+    place back (a denominator whose inverse is 0)."""
+    lib = _lib.load_tokens()
+    l, big = loss(**kw, red=red), 1 << 40
+    assert lib.ppo_token_policy_loss(rows(mask=mask), P, P, P, l, P, P, P, P, P, big, None) == 1
+    if "den" in kw or "scale" in kw:
+        assert lib.ppo_token_distillation(rows(mask=mask), P, 0, P, 1, 3, l, P, P, P, P, big,
+                                          None) == 1
+        with pytest.raises(ValueError, match="denominator|grad_scale"):
+            tokens._check_weights("token", kw.get("den"), kw.get("scale", 1.0))
+    else:
+        x, a = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64)
+        z = torch.zeros(2)
+        with pytest.MonkeyPatch.context() as m, pytest.raises(ValueError, match="_coef"):
+            m.setattr(tokens, "_require", lambda *args: None)
+            tokens._check_policy(x, a, z, z, z, None, 0.2, 0.2, kw.get("kl", 0.0),
+                                 kw.get("ent", 0.0), 1.0)
 
 
 def test_preference_arguments():

@@ -276,9 +276,9 @@ PyObject* pair(const Tensor& first, PyObject* second) {
   return r.release().ptr();
 }
 
-double positive(PyObject* o) {
+double held(PyObject* o) {
   const double x = number(o);
-  need(x > 0.0 && std::isfinite(x));
+  need(x >= PPO_TOKEN_LEAST && x <= PPO_TOKEN_MOST);
   return x;
 }
 double finite(PyObject* o) {
@@ -286,12 +286,17 @@ double finite(PyObject* o) {
   need(std::isfinite(x));
   return x;
 }
+double coefficient(PyObject* o) {
+  const double x = number(o);
+  need(std::isfinite((float)x));
+  return x;
+}
 
 // reduction, denominator, grad_scale
 void weights_of(PyObject* const* a, ppo_token_loss& l) {
   l.reduction = (int)integer(a[0]);
-  l.denominator = a[1] == Py_None ? 0.0 : positive(a[1]);
-  l.grad_scale = positive(a[2]);
+  l.denominator = a[1] == Py_None ? 0.0 : held(a[1]);
+  l.grad_scale = held(a[2]);
 }
 
 struct Policy {
@@ -356,8 +361,8 @@ PyObject* token_policy_loss(PyObject* const* a) {
   if (a[4] != Py_None) p.ref = p.r.row_constants(a[4]);
   p.l.clip_low = number(a[6]);
   p.l.clip_high = number(a[7]);
-  p.l.kl_coef = finite(a[8]);
-  p.l.entropy_coef = finite(a[9]);
+  p.l.kl_coef = coefficient(a[8]);
+  p.l.entropy_coef = coefficient(a[9]);
   need(p.l.clip_low >= 0.0 && p.l.clip_high >= 0.0);
   need(p.l.kl_coef == 0.0 || p.ref.defined());
   weights_of(a + 11, p.l);

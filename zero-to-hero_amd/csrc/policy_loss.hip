@@ -344,7 +344,7 @@ extern "C" int ppo_token_policy_loss(const ppo_token_rows* r, const float* old_l
   Rows rows;
   if (const int code = take_rows(r, true, rows)) return code;
   if (!loss || !scalars || !(loss->clip_low >= 0.0) || !(loss->clip_high >= 0.0) ||
-      !isfinite(loss->kl_coef) || !isfinite(loss->entropy_coef))
+      !isfinite((float)loss->kl_coef) || !isfinite((float)loss->entropy_coef))
     return PPO_ERR_INVALID_ARG;
   if (loss->kl_coef != 0.0 && !ref_log_probs && rows.n) return PPO_ERR_INVALID_ARG;
   if (rows.n && (!old_log_probs || !advantages)) return PPO_ERR_INVALID_ARG;

@@ -153,8 +153,9 @@ Order take_order(const Rows& rows, Weights& w, const Scratch& s, hipStream_t str
 
 int take_weights(const Rows& rows, const ppo_token_loss* loss, const Scratch& s, Weights& w) {
   const bool sequences = loss->reduction == PPO_SEQUENCE_MEAN;
-  if ((loss->reduction != PPO_TOKEN_MEAN && !sequences) || !(loss->denominator >= 0.0) ||
-      !(loss->grad_scale > 0.0) || !(loss->grad_scale < INFINITY))
+  const auto held = [](double x) { return x >= PPO_TOKEN_LEAST && x <= PPO_TOKEN_MOST; };
+  if ((loss->reduction != PPO_TOKEN_MEAN && !sequences) ||
+      (loss->denominator != 0.0 && !held(loss->denominator)) || !held(loss->grad_scale))
     return PPO_ERR_INVALID_ARG;
   w = {nullptr, nullptr, 0, 0.0f};
   if (loss->denominator > 0.0) w.inverse = (float)(1.0 / loss->denominator);

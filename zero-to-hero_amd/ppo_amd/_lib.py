@@ -226,6 +226,7 @@ def load_layers() -> ctypes.CDLL:
 PPO_TOKEN_SAVED = 8
 PPO_TOKEN_SCALARS = 6
 PPO_TOKEN_MAX_K = 256
+PPO_TOKEN_LEAST, PPO_TOKEN_MOST = 1e-30, 1e30
 TOKEN_SCALAR_NAMES = ("loss", "policy", "kl", "entropy", "approx_kl", "clipfrac")
 TOKEN_REDUCTIONS = {"token": 0, "sequence": 1}
 TOKENS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libppo_tokens.so")

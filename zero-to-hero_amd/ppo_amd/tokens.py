@@ -84,10 +84,11 @@ def _check_weights(reduction, denominator, grad_scale) -> None:
     if reduction not in _lib.TOKEN_REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_lib.TOKEN_REDUCTIONS)}, "
                          f"got {reduction!r}")
-    if denominator is not None and not 0.0 < denominator < math.inf:
-        raise ValueError(f"denominator must be > 0 and finite, got {denominator}")
-    if not 0.0 < grad_scale < math.inf:
-        raise ValueError(f"grad_scale must be > 0 and finite, got {grad_scale}")
+    for value, name in ((1.0 if denominator is None else denominator, "denominator"),
+                        (grad_scale, "grad_scale")):
+        if not _lib.PPO_TOKEN_LEAST <= value <= _lib.PPO_TOKEN_MOST:
+            raise ValueError(f"{name} must be in [{_lib.PPO_TOKEN_LEAST}, "
+                             f"{_lib.PPO_TOKEN_MOST}], got {value}")
 
 
 def _sizes(logits) -> tuple[int, int, int]:
@@ -416,8 +417,8 @@ def _check_policy(logits, actions, old_log_probs, advantages, ref_log_probs, mas
     if not clip_low >= 0.0 or not clip_high >= 0.0:
         raise ValueError(f"clip_low and clip_high must be >= 0, got {clip_low}, {clip_high}")
     for value, name in ((kl_coef, "kl_coef"), (entropy_coef, "entropy_coef")):
-        if not math.isfinite(value):
-            raise ValueError(f"{name} must be finite, got {value}")
+        if not abs(value) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"{name} must be finite in fp32, got {value}")
     if kl_coef != 0.0 and ref_log_probs is None:
         raise ValueError("kl_coef needs ref_log_probs")
     return per_sequence
@@ -449,7 +450,8 @@ def token_policy_loss(
     (clip_high None: clip_low), and the loss their mean over the tokens that
     the mask counts (reduction "token"), or over the sequences that have any,
     of their means ("sequence"); `denominator` takes the place of the number of
-    those tokens or sequences, for a batch in several calls or ranks.
+    those tokens or sequences, for a batch in several calls or ranks (it and
+    grad_scale lie in [1e-30, 1e30]).
     logits [..., T, A]; actions, old_log_probs, ref_log_probs and mask [..., T];
     advantages [..., T], or [...] for one a sequence; those three are constants, and
     refused where they require a gradient.  Over no tokens the loss is 0.
