@@ -165,6 +165,38 @@ def test_log_probs_keep_their_digits_where_one_action_has_all(dev, dtype):
     assert_within(dx[:, 5], omp, bound, "1 - p")
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("R, A", [(1, 1 << 27), (1030, 600001)])
+def test_sums_of_very_wide_rows(dev, R, A, dtype):
+    """The sums of a lane that walks thousands of elements are as good as short ones.  Every
+    element weighs v = 1/2 + 2^-k (1 - 2^-6) but for one in 251, which weighs 1: added one by
+    one to a sum of 2^(23 - k) or more, 32 bits would lose the 2^-k of each, 2^(1 - k) of all."""
+    t = TYPES[dtype]
+    if R > 1000 and t == torch.float32:
+        A //= 2
+    x = torch.full((R, A), 0.25, dtype=t, device=dev)
+    x[:, ::251] = 1.0
+    ones = (A + 250) // 251
+    a = torch.full((R,), 7, device=dev)
+    over = []
+    for k in range(10, 17):
+        z = math.log(0.5 + 2.0 ** -k * (1 - 2.0 ** -6))  # (of v; of 1 it is 0)
+        with torch.no_grad():
+            lp, H = ppo_amd.token_log_probs(x, a, temperature=-0.75 / z, entropy=True)
+        s = ones + (A - ones) * math.exp(z)
+        pt = (A - ones) * math.exp(z) / s * -z
+        # a lane's eight rounds of 9 additions (16 of the entropy's sum) in 32 bits and the
+        # rounding of what 64 bits have summed; the lanes', the workgroup's and the parts'
+        # joins of up to ten additions and a factor of four roundings each
+        n, n_H = 8 * 9 + 1 + 3 * 14, 8 * 16 + 1 + 3 * 14
+        e_s = U32 * (n + 3 * pt)
+        e_lp = U32 * (math.log(s) - 4 * z) + e_s
+        e_H = 2 * U32 * n_H * (1 + pt) + 4 * U32 * pt * (1 - z) + e_s + U32 * (math.log(s) + pt)
+        over += [float((lp.double() - z + math.log(s)).abs().max()) / e_lp,
+                 float((H.double() - math.log(s) - pt).abs().max()) / e_H]
+    assert max(over) <= 1, over
+
+
 def test_log_probs_shapes(dev):
     x = torch.randn(2, 3, 5, 40, device=dev)
     a = torch.randint(0, 40, (2, 3, 5), device=dev)

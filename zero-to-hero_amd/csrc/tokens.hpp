@@ -242,12 +242,15 @@ struct Scale {
 
 // x relative to m, no smaller than its own; parts without elements have m = -inf,
 // s = u = 0.
-template <bool kEntropy, class S>
-__device__ __forceinline__ void rebase(S& x, float m, const Scale<S>& c) {
+__device__ __forceinline__ float fused(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, float b, double c) { return fma(a, (double)b, c); }
+template <bool kEntropy, class X, class S>
+__device__ __forceinline__ void rebase(X& x, float m, const Scale<S>& c) {
+  using U = decltype(x.u);
   const bool none = x.m == kNegInf;
   const float d = c(x.m - m);
   const float f = none ? 0.0f : exp2_fast(d);
-  if (kEntropy) x.u = none || f == 0.0f ? 0.0f : f * fmaf((float)x.s, d, x.u);
+  if (kEntropy) x.u = none || f == 0.0f ? (U)0.0f : f * fused((U)x.s, d, x.u);
   x.s *= f;
   x.m = m;
 }
