@@ -13,9 +13,9 @@ template <int N>
 using Int = std::integral_constant<int, N>;
 
 // What a lane has of a row that it walks, whose length has no bound: the sums of kWalk rounds
-// are formed in 32 bits, those of all rounds in 64 (in 32 alone, 2^27 columns of a weight of
-// 1/2 + 2^-13 are off by 4e-5; with 64 bits in every round log p and the entropy of
-// 4096 x 50304 bf16 take 67.7 us, so 66.2, in 32 bits alone 65.4).
+// are formed in 32 bits, those of more in 64 (in 32 alone, 2^27 columns of a weight of
+// 1/2 + 2^-13 are off by 4e-5; log p and the entropy of 4096 x 50304 bf16 take 65.3 us there,
+// 66.3 so, 67.7 with 64 bits in every round).
 struct Walked {
   float m;
   double s, u;
@@ -74,14 +74,15 @@ __device__ __forceinline__ S stream_stat(const T* row, int A, int a, const Scale
         }
       x.s += s2;
     }
-    if constexpr (kLong) {
+    if (kLong && i < end) {
       rebase<kEntropy>(all, x.m, c);
       all.s += x.s;
       if (kEntropy) all.u += x.u;
       x.s = x.u = 0.0f;
     }
   }
-  if constexpr (kLong) {  // (a lane without chunks may have an end's element)
+  if (kLong && all.s != 0.0) {  // (or NaN)
+    rebase<kEntropy>(all, x.m, c);
     x.s = (decltype(x.s))(all.s + x.s);
     if (kEntropy) x.u = (float)(all.u + x.u);
   }
