@@ -15,7 +15,8 @@
  * that the type allows.  With z = logits / temperature, p = softmax(z) of a row.
  * Statistics, log-probabilities and losses are held in 32 bits or more; a
  * gradient is formed in fp32 and rounded once, to nearest even.  A logit of -inf
- * is an action that cannot be taken: p = 0, no gradient, no part in the entropy.
+ * is an action that cannot be taken: p = 0, no gradient, no part in the entropy (one
+ * that was taken all the same has log p = -inf and, as 1 - p = 1, log p's whole gradient).
  * A row that holds +inf or NaN, or nothing but -inf, gives NaN, and so does a
  * row whose action lies outside [0, A) (it is never dereferenced).
  *

@@ -580,8 +580,8 @@ __device__ __forceinline__ float row_weight(const Weights& w, float inverse, int
   return w.lengths ? inverse / (float)w.lengths[seq] : inverse;
 }
 
-// The rows in the order in which a launch takes them: those that count, then the others,
-// each in their own (null: as they lie, and whether one counts is looked up).  Where a
+// The rows in the order in which a launch takes them: those that count, then the others
+// from the last on (null: as they lie, and whether one counts is looked up).  Where a
 // workgroup has a handful of long rows, taking every so many of the first kind gives
 // all of them as many.
 struct Order {

@@ -383,8 +383,11 @@ inline bool lies_alike(const void* logits, const void* dlogits) {
 // gradients lie otherwise in 16 bytes than the logits (not `alike`), or where rows are so few
 // that one workgroup to each takes longer, the more so the larger it is (a row of 131072
 // bf16 24 us by itself; 32 of them 14 split, 64 17, 128 27 either way; of 50304 100 rows 15
-// and 16; of 30000 40 rows 13 either way).  The two largest spill a tenth of their row and
-// are faster all the same (1024 x 163840 bf16 196 us read twice, 171; 196608 228, 209).
+// and 16; of 30000 40 rows 13 either way).  The two largest spill (of 320 bytes a lane the
+// policy's 80 and the distillation's 156 to 160, of 384 160 to 172 and 236; the policy's in
+// fp16 with the entropy's gradient 348) and are faster all the same (1024 x 163840 bf16 196 us
+// read twice, 171; 196608 228, 209; 196000 fp16 207, 261 with that gradient).  Of 208 and 256
+// bytes the policy's have 12 in scratch, the distillation's 16 and 76.
 // Many rows of up to 128 chunks go four to a wave, which then takes their sums' ends together
 // (16384 x 1000 bf16 24 us, 31 one to a wave); none do (`least` 64) that need more LDS than
 // that leaves, and of more than 64 chunks none that take entries (kSingle).

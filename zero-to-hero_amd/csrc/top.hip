@@ -9,7 +9,7 @@
 // counting for each how many precede it.  Rows in which too many reach the bound (many
 // equal logits) are settled by a radix search for the threshold itself.  What bounds
 // it: HBM reads; a row is in the caches when parts of it are read again (4096 x 32001
-// fp32, K = 64, 101 us, 5.2 TB/s, while a workgroup waits for its bound another one
+// fp32, K = 64, 94 us, 5.5 TB/s, while a workgroup waits for its bound another one
 // reads; with segments of eight rounds for two 120, since each one's chunks are lines of
 // their own); a single row two launches of 8 and 4 us.
 #include "tokens_rows.hpp"
