@@ -41,7 +41,8 @@ __all__ = ["token_log_probs", "token_policy_loss", "preference_loss", "distillat
 
 class TokenStats(dict):
     """token_policy_loss's scalars as 0-d fp32 device tensors: loss, policy, kl,
-    entropy, approx_kl, clipfrac (views of one [6] tensor; no host sync)."""
+    entropy, approx_kl, clipfrac (views of one [6] tensor, whose first element
+    the returned loss is as well; no host sync)."""
 
 
 class PreferenceStats(dict):
